@@ -8,6 +8,7 @@ cusr/kernel/Makefile:77-81):
     cusr_amd/kernel/libcusr_co_fd.so   same kernels, the FD variant's LM ordering by default
     cusr_amd/kernel/batch_lm_ad        CLI with the reference's arguments/blobs (AD ordering)
     cusr_amd/kernel/batch_lm           the same CLI over libcusr_co_fd.so
+    cusr_amd/kernel/libcusr_seq.so     C ABI of include/cusr_seq.h: the sequence operators
     cusr_amd/kernel/kernel_resources.json
                                        per kernel: VGPRs, AGPRs, SGPRs, spills, scratch
                                        bytes per lane, occupancy and static LDS, from the
@@ -32,6 +33,7 @@ BUILD = ROOT / "_build"
 KDIR = ROOT / "kernel"
 LIB = KDIR / "libcusr_co_ad.so"
 LIB_FD = KDIR / "libcusr_co_fd.so"
+LIB_SEQ = KDIR / "libcusr_seq.so"
 CLI = KDIR / "batch_lm_ad"
 CLI_FD = KDIR / "batch_lm"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -52,6 +54,12 @@ DEVICE_FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-ffp-co
                 "-fno-fast-math", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                 "-mllvm", "-structurizecfg-skip-uniform-regions=1",
                 f"-I{REPO / 'include'}", "-Wall", "-Wno-unused-function"]
+
+# The sequence operators have no CPU oracle to match bit for bit: multiply-adds
+# are fused.
+SEQ_FLAGS = [f for f in DEVICE_FLAGS if f != "-ffp-contract=off"
+             and "structurizecfg" not in f and f != "-mllvm"]
+SEQ_SOURCES = ("seq_rotary", "seq_policy_loss", "seq_attention", "seq_attention_grad")
 
 FIT_VARIANTS = [("double", 0, "f64_fwd"), ("double", 1, "f64_rev"),
                 ("float", 0, "f32_fwd"), ("float", 1, "f32_rev")]
@@ -103,6 +111,30 @@ def _run(cmd):
     return err
 
 
+def seq_compiles(bdir: Path):
+    """Compile commands of the sequence operators."""
+    return [[HIPCC, *SEQ_FLAGS, REMARKS, "-x", "hip", "-c", str(CSRC / f"{name}.hip"),
+             "-o", str(bdir / f"{name}.o")] for name in SEQ_SOURCES]
+
+
+def link_shared(target: Path, objs):
+    tmp = target.with_suffix(".so.tmp")
+    _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *objs])
+    os.replace(tmp, target)
+
+
+def build_seq(verbose: bool = False) -> Path:
+    """Compile the sequence operators alone (build() does it too)."""
+    BUILD.mkdir(parents=True, exist_ok=True)
+    compiles = seq_compiles(BUILD)
+    with ThreadPoolExecutor(max_workers=len(compiles)) as ex:
+        for err in ex.map(_run, compiles):
+            if verbose and err.strip():
+                print(err, file=sys.stderr)
+    link_shared(LIB_SEQ, [c[-1] for c in compiles])
+    return LIB_SEQ
+
+
 def build(jobs: int | None = None, verbose: bool = False, defines=(), out: Path | None = None,
           cli: bool = True, src_root: Path | None = None) -> Path:
     """Compile everything; `defines` adds -D flags (tuning variants) and `out`
@@ -142,6 +174,8 @@ def build(jobs: int | None = None, verbose: bool = False, defines=(), out: Path 
     if default:
         compiles.append([HIPCC, *flags, *extra, "-x", "hip", "-DCUSR_DEFAULT_ORDER=1", "-c",
                          str(csrc / "co_lib.hip"), "-o", str(bdir / "co_lib_fd.o")])
+    seq = seq_compiles(bdir) if default else []
+    compiles += seq
     _RES_SINK.clear()
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         for err in ex.map(_run, compiles):
@@ -152,14 +186,14 @@ def build(jobs: int | None = None, verbose: bool = False, defines=(), out: Path 
     res_path = RESOURCES if out is None else Path(out).with_suffix(".resources.json")
     res_path.write_text(json.dumps(table, indent=1, sort_keys=True) + "\n")
     objs = [str(c[c.index("-o") + 1]) for c in compiles]
-    fit_objs = [o for o in objs if "co_lib" not in Path(o).name]
+    seq_objs = [c[-1] for c in seq]
+    fit_objs = [o for o in objs if "co_lib" not in Path(o).name and o not in seq_objs]
     links = [(lib, fit_objs + [str(bdir / "co_lib.o")])]
     if default:
         links.append((LIB_FD, fit_objs + [str(bdir / "co_lib_fd.o")]))
+        links.append((LIB_SEQ, seq_objs))
     for target, lobjs in links:
-        tmp = target.with_suffix(".so.tmp")
-        _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *lobjs])
-        os.replace(tmp, target)
+        link_shared(target, lobjs)
     if cli and default:
         for exe, name in ((CLI, "cusr_co_ad"), (CLI_FD, "cusr_co_fd")):
             _run(["g++", "-O2", "-std=c++17", f"-I{REPO / 'include'}", "-o", str(exe),
@@ -174,5 +208,6 @@ if __name__ == "__main__":
     ap.add_argument("-v", "--verbose", action="store_true")
     ap.add_argument("-D", dest="defines", action="append", default=[])
     ap.add_argument("--out", default=None)
+    ap.add_argument("--seq", action="store_true", help="the sequence operators alone")
     a = ap.parse_args()
-    print(build(a.jobs, a.verbose, a.defines, a.out))
+    print(build_seq(a.verbose) if a.seq else build(a.jobs, a.verbose, a.defines, a.out))

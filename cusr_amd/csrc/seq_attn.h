@@ -1,0 +1,159 @@
+// seq_attn.h -- pieces of the attention kernels (forward, gradient, steps).
+//
+// Rows. A sequence's lq queries and the G heads that share a key head fold
+// into lq * G rows, row r = query r / G, head r % G: the heads of a group read
+// the same keys, so they share tiles, and short sequences fill them better.
+//
+// Products. Scores are formed transposed, S^T = K Q^T, so that a lane of the
+// 32x32 product holds 16 keys of one query: the softmax runs along registers,
+// with one exchange between the wave's halves. The same registers, packed to
+// 16 bits, are the right operand of O^T = V^T P^T: a contraction may take its
+// index in any order, so V's rows are read in the order the lane's keys have
+// (4h..4h+3, 8+4h..8+4h+3 of every 16, h the half). P never passes through LDS.
+#ifndef CUSR_SEQ_ATTN_H
+#define CUSR_SEQ_ATTN_H
+
+#include "seq_common.h"
+
+namespace seq {
+
+struct Attn : SeqAttention {
+    int32_t G;       // query heads per key head
+    float c;         // scale * log2(e): scores in powers of two
+};
+
+__device__ __host__ inline int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
+    return x < lo ? lo : (x > hi ? hi : x);
+}
+
+// A sequence's place: first query and key row, number of queries and keys.
+struct Place { int64_t q0, k0; int lq, lk; };
+
+__device__ inline int64_t offset_at(const int32_t *cu, int b, int64_t t) {
+    return b <= 0 ? 0 : clamp64(cu[b], 0, t);
+}
+
+// Work is handed out in tiles of `rows` rows without a list of tiles: tile
+// slots of sequence b start at floor(cu[b] * fold / rows) + b, which leaves
+// each at least as many as it has tiles and numbers them without gaps for a
+// search. Entry n_seq stands for the rows after the last sequence.
+__device__ __host__ inline int64_t slot_of(int64_t at, int fold, int rows, int b) {
+    return at * fold / rows + b;
+}
+
+// The last b of 0..n_seq with slot_of(b) <= slot: 64 probes at a time, one per
+// lane. Every lane of a wave calls it with the same arguments.
+__device__ inline int find_sequence(const int32_t *cu, int n_seq, int64_t t, int fold, int rows,
+                                    int64_t slot) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = n_seq + 1;
+    while (n > 1) {
+        const int step = (n + 63) / 64;
+        const int i = lane * step;
+        const bool ok = i < n && slot_of(offset_at(cu, lo + i, t), fold, rows, lo + i) <= slot;
+        const int last = __popcll(__ballot(ok)) - 1;
+        if (last <= 0) {          // offsets out of order count as the first
+            n = step < n ? step : n;
+        } else {
+            lo += last * step;
+            n = n - last * step < step ? n - last * step : step;
+        }
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+__device__ inline Place place_of(const Attn &a, int b) {
+    Place p;
+    p.q0 = offset_at(a.cu_q, b, a.tq);
+    if (b >= a.n_seq) {
+        p.lq = (int)(a.tq - p.q0);
+        p.k0 = 0;
+        p.lk = 0;
+        return p;
+    }
+    const int64_t q1 = offset_at(a.cu_q, b + 1, a.tq);
+    p.lq = (int)(q1 > p.q0 ? q1 - p.q0 : 0);
+    p.k0 = clamp64(a.cu_k[b], 0, a.tk);
+    const int64_t k1 = clamp64(a.cu_k[b + 1], p.k0, a.tk);
+    int64_t lk = k1 - p.k0;
+    if (a.k_lens) lk = clamp64(a.k_lens[b], 0, lk);
+    p.lk = (int)lk;
+    return p;
+}
+
+// 16-bit tile rows in LDS: DP elements a row (96 padded to 128), 16-byte
+// chunks permuted within the row so that the transposed reads, which take four
+// rows of 32 bytes at a time, and the row reads, 32 rows of one chunk, spread
+// over the banks.
+template <int DP> struct Tile {
+    static constexpr int stride = DP == 96 ? 128 : DP;      // elements
+    static constexpr int chunks = stride / 8;
+    static __device__ int swz(int row) {
+        return DP == 32 ? 0 : (DP == 64 ? ((row & 3) * 2 + ((row >> 2) & 1)) & 7
+                                        : ((row & 7) * 2 + ((row >> 3) & 1)) & 15);
+    }
+    static __device__ int at(int row, int chunk) {          // element offset
+        return row * stride + ((chunk ^ swz(row)) << 3);
+    }
+    // left operand of a product over the tile's rows: column dt * 32 + lane % 32,
+    // rows k0 + {4h..4h+3, 8+4h..8+4h+3}
+    static __device__ uint4v transposed(const uint16_t *t, int k0, int dt) {
+        const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15;
+        const int col = dt * 32 + (lane & 16) + (i & 3) * 4;
+        const int r0 = k0 + 4 * h + (i >> 2), r1 = r0 + 8;
+        const uint2v lo = read_transposed(t + at(r0, col >> 3) + (col & 7));
+        const uint2v hi = read_transposed(t + at(r1, col >> 3) + (col & 7));
+        uint4v v = {lo[0], lo[1], hi[0], hi[1]};
+        return v;
+    }
+    // left operand over the columns: row r0 + lane % 32, columns 16 c + 8h..+7
+    static __device__ uint4v row(const uint16_t *t, int r0, int c) {
+        const int lane = threadIdx.x & 63;
+        return *(const uint4v *)(t + at(r0 + (lane & 31), 2 * c + (lane >> 5)));
+    }
+};
+
+// Row `r` of a [rows, heads, d] tensor as operand fragments: columns
+// 16 c + 8h .. + 7 for c < DP/16; zero beyond d, and altogether when !ok.
+template <int DP>
+__device__ inline void load_row(uint4v *f, const void *base, int64_t off, int d, bool ok) {
+    const int h = (threadIdx.x & 63) >> 5;
+    const uint16_t *p = (const uint16_t *)base + off;
+#pragma unroll
+    for (int c = 0; c < DP / 16; c++) {
+        uint4v z = {0, 0, 0, 0};
+        f[c] = ok && c * 16 + h * 8 < d ? *(const uint4v *)(p + c * 16 + h * 8) : z;
+    }
+}
+
+// A column of a transposed accumulator (DP values of this lane's row, split
+// between the halves) scaled, packed and stored as 16-byte pieces.
+template <typename T, int DP>
+__device__ inline void store_row(void *base, int64_t off, const float16v *acc, float scale, int d,
+                                 bool ok) {
+    const int h = (threadIdx.x & 63) >> 5;
+    uint16_t *p = (uint16_t *)base + off;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; dt++)
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            uint32_t x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                x[j] = T::pack(acc[dt][8 * g + 2 * j] * scale, acc[dt][8 * g + 2 * j + 1] * scale);
+            // halves hold columns 0-3, 8-11 and 4-7, 12-15: after the exchange
+            // 0-7 and 8-15
+            auto s0 = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+            auto s1 = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+            uint4v v = {s0[0], s1[0], s0[1], s1[1]};
+            const int col = dt * 32 + g * 16 + h * 8;
+            if (ok && col < d) *(uint4v *)(p + col) = v;
+        }
+}
+
+int check_attention(const SeqAttention *a);
+// the head size that the kernels are built for (32, 64, 96, 128)
+inline int padded_head(int d) { return (d + 31) / 32 * 32; }
+
+}  // namespace seq
+#endif

@@ -1,0 +1,514 @@
+"""Sequence operators of a learned proposer of expressions (include/cusr_seq.h).
+
+A pop.bin population is M prefix programs packed end to end: M token sequences.
+A causal model over them proposes expressions, the constant fitter returns
+their losses, and a clipped policy gradient trains the model on those. These
+are that model's operators on the GPU; the reference has no counterpart.
+
+  attention, attention_grad      causal attention over packed sequences with
+                                 grouped heads; single tokens over a cache
+  rotary_table, rotary           rotary positions of q and k in one launch
+  policy_loss, policy_loss_grad  clipped policy loss with a KL term
+
+Tensors are torch CUDA tensors; the work is queued on the current stream of
+their device and the call returns at once. attention, rotary and policy_loss
+take part in autograd when an input requires a gradient. Arguments are checked
+before anything is launched (TypeError, ValueError); a refusal of the library
+raises COError. Import torch before the library is loaded, as for
+co_data_upload_device. There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+import threading
+
+import numpy as np
+import torch
+
+from cusr_amd.kernel.co_inproc import CO_OK, COError, _HERE
+
+SEQ_MAX_HEAD = 128
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+
+# every extern "C" symbol of include/cusr_seq.h
+EXPORTED = ("seq_attention", "seq_attention_workspace", "seq_attention_grad",
+            "seq_attention_grad_workspace", "seq_rotary", "seq_policy_loss",
+            "seq_policy_loss_workspace")
+
+
+class SeqAttention(ctypes.Structure):
+    """cusr_seq.h SeqAttention."""
+    _fields_ = [("struct_size", _I32), ("dtype", _I32), ("n_seq", _I32), ("hq", _I32),
+                ("hkv", _I32), ("d", _I32), ("tq", _I64), ("tk", _I64),
+                ("q_row", _I64), ("q_head", _I64), ("k_row", _I64), ("k_head", _I64),
+                ("v_row", _I64), ("v_head", _I64), ("o_row", _I64), ("o_head", _I64),
+                ("scale", _F), ("reserved", _I32), ("q", _P), ("k", _P), ("v", _P), ("o", _P),
+                ("lse", _P), ("cu_q", _P), ("cu_k", _P), ("k_lens", _P), ("workspace", _P),
+                ("workspace_bytes", _I64)]
+
+
+class SeqAttentionGrad(ctypes.Structure):
+    """cusr_seq.h SeqAttentionGrad."""
+    _fields_ = [("struct_size", _I32), ("reserved", _I32), ("do_row", _I64), ("do_head", _I64),
+                ("dq_row", _I64), ("dq_head", _I64), ("dk_row", _I64), ("dk_head", _I64),
+                ("dv_row", _I64), ("dv_head", _I64), ("d_o", _P), ("dq", _P), ("dk", _P),
+                ("dv", _P)]
+
+
+class SeqRotary(ctypes.Structure):
+    """cusr_seq.h SeqRotary."""
+    _fields_ = [("struct_size", _I32), ("dtype", _I32), ("hq", _I32), ("hkv", _I32), ("d", _I32),
+                ("rot", _I32), ("interleaved", _I32), ("inverse", _I32), ("tokens", _I64),
+                ("table_len", _I64), ("q_row", _I64), ("q_head", _I64), ("k_row", _I64),
+                ("k_head", _I64), ("qo_row", _I64), ("qo_head", _I64), ("ko_row", _I64),
+                ("ko_head", _I64), ("q", _P), ("k", _P), ("q_out", _P), ("k_out", _P),
+                ("positions", _P), ("table", _P)]
+
+
+class SeqPolicyLoss(ctypes.Structure):
+    """cusr_seq.h SeqPolicyLoss."""
+    _fields_ = [("struct_size", _I32), ("dtype", _I32), ("tokens", _I64), ("vocab", _I64),
+                ("row", _I64), ("drow", _I64), ("clip_lo", _F), ("clip_hi", _F),
+                ("kl_coef", _F), ("temperature", _F), ("logits", _P), ("actions", _P),
+                ("logp_old", _P), ("logp_ref", _P), ("advantages", _P), ("weights", _P),
+                ("dloss", _P), ("loss", _P), ("logp", _P), ("dlogits", _P), ("workspace", _P),
+                ("workspace_bytes", _I64)]
+
+
+_lib = None
+_lib_lock = threading.Lock()
+
+
+def lib_path():
+    """libcusr_seq.so next to this module (cusr_amd/build.py output)."""
+    return _HERE / "libcusr_seq.so"
+
+
+def load_library() -> ctypes.CDLL:
+    """Bind libcusr_seq.so once per process; raises when it is not built."""
+    global _lib
+    with _lib_lock:
+        if _lib is None:
+            path = lib_path()
+            if not path.exists():
+                raise FileNotFoundError(f"{path} not built: run python -m cusr_amd.build")
+            lib = ctypes.CDLL(str(path))
+            for name in EXPORTED:
+                fn = getattr(lib, name)
+                fn.restype = ctypes.c_int64 if name.endswith("workspace") else ctypes.c_int
+            for name in ("seq_attention", "seq_rotary", "seq_policy_loss"):
+                getattr(lib, name).argtypes = [_P, _P]
+            lib.seq_attention_grad.argtypes = [_P, _P, _P]
+            for name in ("seq_attention", "seq_attention_grad", "seq_policy_loss"):
+                getattr(lib, name + "_workspace").argtypes = [_P]
+            _lib = lib
+    return _lib
+
+
+def _run(fn, where, device, *structs):
+    """Call an entry point on the device's current stream."""
+    refs = [ctypes.addressof(s) for s in structs]
+    if device.index is None or device.index == torch.cuda.current_device():
+        rc = fn(*refs, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*refs, torch.cuda.current_stream(device).cuda_stream)
+    if rc != CO_OK:
+        raise COError(rc, where)
+
+
+def _workspace(fn, where, struct, device):
+    """Scratch of a call from torch's allocator, on the current stream."""
+    n = fn(ctypes.addressof(struct))
+    if n < 0:
+        raise COError(int(-n if n == -2 else n), where)
+    if n == 0:
+        return None
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    struct.workspace, struct.workspace_bytes = ws.data_ptr(), n
+    return ws
+
+
+def _need(x, name, dtypes, dim, device=None):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor, not {type(x).__name__}")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be on the GPU")
+    if device is not None and x.device != device:
+        raise ValueError(f"{name} is on {x.device}, not on {device}")
+    if x.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, "
+                         f"not {str(x.dtype)[6:]}")
+    if dim is not None and x.dim() != dim:
+        raise ValueError(f"{name} must have {dim} dimensions, not {x.dim()}")
+    return x
+
+
+def _ptr(x):
+    return x.data_ptr() if x is not None and x.numel() else None
+
+
+def _heads16(x):
+    """x as the kernels read it: the last dimension contiguous, rows and heads
+    on 16-byte boundaries; another layout is copied once."""
+    if x.numel() == 0:
+        return x
+    s = x.stride()
+    if s[2] != 1 or s[0] % 8 or s[1] % 8 or x.data_ptr() % 16:
+        return x.contiguous() if x.shape[2] % 8 == 0 and not x.is_contiguous() else x.clone(
+            memory_format=torch.contiguous_format)
+    return x
+
+
+# ------------------------------------------------------------------ attention
+
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _check_attention(q, k, v, cu_q, cu_k, k_lens, scale):
+    _need(q, "q", _HALF, 3)
+    dev = q.device
+    _need(k, "k", (q.dtype,), 3, dev)
+    _need(v, "v", (q.dtype,), 3, dev)
+    hq, d = q.shape[1], q.shape[2]
+    hkv = k.shape[1]
+    if k.shape != v.shape or k.shape[2] != d:
+        raise ValueError(f"k and v must be [rows, heads, {d}] and alike; got {tuple(k.shape)} "
+                         f"and {tuple(v.shape)}")
+    if hkv < 1 or hq < 1 or hq % hkv:
+        raise ValueError(f"query heads ({hq}) must be a multiple of key heads ({hkv})")
+    if d < 8 or d % 8 or d > SEQ_MAX_HEAD:
+        raise ValueError(f"head size must be a multiple of 8 up to {SEQ_MAX_HEAD}, not {d}")
+    _need(cu_q, "cu_q", (torch.int32,), 1, dev)
+    if cu_k is not None:
+        _need(cu_k, "cu_k", (torch.int32,), 1, dev)
+        if cu_k.shape != cu_q.shape:
+            raise ValueError("cu_q and cu_k must have one entry per sequence and one more")
+    if cu_q.numel() < 1:
+        raise ValueError("cu_q must have one entry per sequence and one more")
+    if k_lens is not None:
+        _need(k_lens, "k_lens", (torch.int32,), 1, dev)
+        if k_lens.numel() != cu_q.numel() - 1:
+            raise ValueError("k_lens must have one entry per sequence")
+    if scale is not None and not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+
+
+def _attention_struct(q, k, v, o, lse, cu_q, cu_k, k_lens, scale):
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), o.stride()
+    return SeqAttention(ctypes.sizeof(SeqAttention), _DTYPES[q.dtype], cu_q.numel() - 1,
+                        q.shape[1], k.shape[1], q.shape[2], q.shape[0], k.shape[0],
+                        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1],
+                        scale, 0, _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse),
+                        cu_q.data_ptr(), cu_k.data_ptr(),
+                        None if k_lens is None else k_lens.data_ptr() or None, None, 0)
+
+
+def _attention(q, k, v, cu_q, cu_k, k_lens, scale, return_lse):
+    q, k, v = _heads16(q), _heads16(k), _heads16(v)
+    cu_q = cu_q.contiguous()
+    cu_k = cu_q if cu_k is None else cu_k.contiguous()
+    k_lens = None if k_lens is None else k_lens.contiguous()
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) \
+        if return_lse else None
+    if q.shape[0]:
+        lib = load_library()
+        a = _attention_struct(q, k, v, o, lse, cu_q, cu_k, k_lens, scale)
+        ws = _workspace(lib.seq_attention_workspace, "seq_attention", a, q.device)
+        _run(lib.seq_attention, "seq_attention", q.device, a)
+        del ws
+    return o, lse
+
+
+def attention_grad(do, q, k, v, o, lse, cu_q, cu_k=None, *, k_lens=None, scale=None):
+    """(dq, dk, dv) of attention for the gradient `do` of its output; o and
+    lse are what attention(..., return_lse=True) gave. The same call gives the
+    same bits."""
+    _check_attention(q, k, v, cu_q, cu_k, k_lens, scale)
+    _need(do, "do", (q.dtype,), 3, q.device)
+    _need(o, "o", (q.dtype,), 3, q.device)
+    _need(lse, "lse", (torch.float32,), 2, q.device)
+    if do.shape != q.shape or o.shape != q.shape or lse.shape != (q.shape[1], q.shape[0]):
+        raise ValueError("do and o must be like q, and lse [heads, rows]")
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    q, k, v, o, do = (_heads16(x) for x in (q, k, v, o, do))
+    cu_q, lse = cu_q.contiguous(), lse.contiguous()
+    cu_k = cu_q if cu_k is None else cu_k.contiguous()
+    k_lens = None if k_lens is None else k_lens.contiguous()
+    dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+    if q.shape[0] == 0 or k.shape[0] == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    lib = load_library()
+    a = _attention_struct(q, k, v, o, lse, cu_q, cu_k, k_lens, scale)
+    g = SeqAttentionGrad(ctypes.sizeof(SeqAttentionGrad), 0, *do.stride()[:2], *dq.stride()[:2],
+                         *dk.stride()[:2], *dv.stride()[:2], do.data_ptr(), dq.data_ptr(),
+                         dk.data_ptr(), dv.data_ptr())
+    ws = _workspace(lib.seq_attention_grad_workspace, "seq_attention_grad", a, q.device)
+    _run(lib.seq_attention_grad, "seq_attention_grad", q.device, a, g)
+    del ws
+    return dq, dk, dv
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, k_lens, scale):
+        o, lse = _attention(q, k, v, cu_q, cu_k, k_lens, scale, True)
+        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k, k_lens)
+        ctx.scale = scale
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    def backward(ctx, do, _):
+        q, k, v, o, lse, cu_q, cu_k, k_lens = ctx.saved_tensors
+        return (*attention_grad(do, q, k, v, o, lse, cu_q, cu_k, k_lens=k_lens,
+                                scale=ctx.scale), None, None, None, None)
+
+
+def attention(q, k, v, cu_q, cu_k=None, *, k_lens=None, scale=None, return_lse=False):
+    """Causal attention over packed sequences.
+
+    q [Tq, Hq, D], k and v [Tk, Hkv, D], bfloat16 or float16, D a multiple of 8
+    up to 128, Hq a multiple of Hkv (query head h reads key head h * Hkv // Hq).
+    cu_q int32 [B + 1]: sequence b's queries are rows cu_q[b]:cu_q[b + 1]
+    (cu_q[0] is 0). cu_k (default cu_q) the same for its keys; with k_lens
+    int32 [B] only the first k_lens[b] rows of a segment are keys (a cache with
+    room to spare). Queries are the last of their sequence: query i of lq sees
+    keys 0 .. i + lk - lq, so a newest token alone is a segment of one query.
+    A query that sees no key gives 0. scale defaults to D ** -0.5.
+
+    Returns o like q, or (o, lse) with return_lse: lse fp32 [Hq, Tq], -inf
+    where no key is seen. Probabilities are rounded to the tensors' type for
+    the product with v; sums and statistics are held in fp32."""
+    _check_attention(q, k, v, cu_q, cu_k, k_lens, scale)
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        o, lse = _AttentionFn.apply(q, k, v, cu_q, cu_q if cu_k is None else cu_k, k_lens, scale)
+    else:
+        o, lse = _attention(q, k, v, cu_q, cu_k, k_lens, scale, return_lse)
+    return (o, lse) if return_lse else o
+
+
+# --------------------------------------------------------------------- rotary
+
+SCALINGS = (None, "linear", "base", "parts")
+
+
+def rotary_table(rot, positions, *, base=10000.0, scaling=None, factor=1.0, original=0,
+                 device="cuda"):
+    """Table [positions, rot/2, 2] fp32 of (cos, sin) for rotary: angle of
+    position p and pair i is p * base ** (-2i/rot), formed in float64.
+
+    scaling, for contexts `factor` times the `original` length:
+      "linear"  positions divided by factor
+      "base"    base * factor ** (rot / (rot - 2)): the slowest pair turns
+                factor times slower, the fastest as before
+      "parts"   pairs that turn 32 times or more over `original` positions keep
+                their frequency, those that turn once or less are divided by
+                factor, linearly in between; cos and sin are multiplied by
+                0.1 ln(factor) + 1"""
+    rot, positions = int(rot), int(positions)
+    if rot < 0 or rot % 2 or positions < 0:
+        raise ValueError(f"rot must be even and sizes not negative; got {rot}, {positions}")
+    if scaling not in SCALINGS:
+        raise ValueError(f"scaling must be one of {SCALINGS}, not {scaling!r}")
+    if not (base > 0 and factor > 0 and math.isfinite(base) and math.isfinite(factor)):
+        raise ValueError("base and factor must be positive")
+    if scaling == "parts" and (original < 1 or factor < 1):
+        raise ValueError('scaling "parts" needs the original length and a factor of at least 1')
+    m = 1.0
+    if scaling == "base" and rot > 2:
+        base = base * factor ** (rot / (rot - 2.0))
+    f = np.float64(base) ** (-np.arange(0, rot, 2, dtype=np.float64) / max(rot, 1))
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        turns = original * f / (2.0 * np.pi)
+        keep = np.clip((turns - 1.0) / 31.0, 0.0, 1.0)
+        f = f * (keep + (1.0 - keep) / factor)
+        m = 0.1 * math.log(factor) + 1.0
+    f = torch.from_numpy(np.ascontiguousarray(f)).to(device)
+    a = torch.arange(positions, dtype=torch.float64, device=f.device)[:, None] * f
+    return (torch.stack([a.cos(), a.sin()], dim=-1) * m).float().contiguous()
+
+
+def _rotary(q, k, positions, table, interleaved, inverse, q_out=None, k_out=None):
+    q = q if q.stride(2) == 1 or q.shape[2] < 2 else q.contiguous()
+    if k is not None and k.stride(2) != 1 and k.shape[2] > 1:
+        k = k.contiguous()
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k is not None and k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    positions = positions.to(torch.int32).contiguous()
+    table = table.contiguous()
+    if q.shape[0]:
+        z = (0, 0)
+        r = SeqRotary(ctypes.sizeof(SeqRotary), _DTYPES[q.dtype], q.shape[1],
+                      0 if k is None else k.shape[1], q.shape[2], 2 * table.shape[1],
+                      int(interleaved), int(inverse), q.shape[0], table.shape[0],
+                      *q.stride()[:2], *(z if k is None else k.stride()[:2]),
+                      *q_out.stride()[:2], *(z if k is None else k_out.stride()[:2]),
+                      _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), positions.data_ptr(),
+                      _ptr(table))
+        _run(load_library().seq_rotary, "seq_rotary", q.device, r)
+    return q_out, k_out
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, table, interleaved, inverse):
+        ctx.save_for_backward(positions, table)
+        ctx.how = (interleaved, inverse)
+        q_out, k_out = _rotary(q, k, positions, table, interleaved, inverse)
+        return (q_out, k_out) if k is not None else q_out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        positions, table = ctx.saved_tensors
+        interleaved, inverse = ctx.how
+        dq, dk = _rotary(grads[0], grads[1] if len(grads) > 1 else None, positions, table,
+                         interleaved, not inverse)
+        return dq, dk, None, None, None, None
+
+
+def rotary(q, k, positions, table, *, interleaved=False, inverse=False, inplace=False):
+    """Rotary positions of q [T, Hq, D] and k [T, Hkv, D] (or None) in one
+    launch; float32, bfloat16 or float16. positions int32 or int64 [T]; table
+    from rotary_table. The first rot = 2 * table.shape[1] elements of each head
+    turn in pairs (i, i + rot/2), or (2i, 2i + 1) when interleaved; the rest is
+    copied. inverse turns back, which is the gradient. inplace writes into q
+    and k. A position outside the table gives NaN in its token's turned
+    elements. Returns (q', k'), or q' alone when k is None."""
+    _need(q, "q", tuple(_DTYPES), 3)
+    dev = q.device
+    if k is not None:
+        _need(k, "k", (q.dtype,), 3, dev)
+        if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+            raise ValueError(f"q and k must agree in tokens and head size; got {tuple(q.shape)} "
+                             f"and {tuple(k.shape)}")
+    _need(positions, "positions", (torch.int32, torch.int64), 1, dev)
+    if positions.numel() != q.shape[0]:
+        raise ValueError(f"positions must have {q.shape[0]} entries, not {positions.numel()}")
+    _need(table, "table", (torch.float32,), 3, dev)
+    if table.shape[2] != 2 or 2 * table.shape[1] > q.shape[2]:
+        raise ValueError(f"table must be [positions, rot/2, 2] with rot up to the head size "
+                         f"{q.shape[2]}; got {tuple(table.shape)}")
+    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    if inplace:
+        if grad:
+            raise ValueError("inplace takes no part in autograd")
+        if q.stride(2) != 1 or (k is not None and k.stride(2) != 1):
+            raise ValueError("inplace needs heads that are contiguous")
+        out = _rotary(q, k, positions, table, interleaved, inverse, q, k)
+    elif grad:
+        out = _RotaryFn.apply(q, k, positions, table, bool(interleaved), bool(inverse))
+        return out
+    else:
+        out = _rotary(q, k, positions, table, interleaved, inverse)
+    return out if k is not None else out[0]
+
+
+# ---------------------------------------------------------------- policy loss
+
+def _check_policy(logits, actions, logp_old, advantages, logp_ref, weights, clip, kl_coef,
+                  temperature):
+    _need(logits, "logits", tuple(_DTYPES), 2)
+    T, V = logits.shape
+    dev = logits.device
+    if V < 1:
+        raise ValueError("logits must have at least one column")
+    _need(actions, "actions", (torch.int64, torch.int32), 1, dev)
+    named = [("logp_old", logp_old), ("advantages", advantages)]
+    named += [(n, x) for n, x in (("logp_ref", logp_ref), ("weights", weights)) if x is not None]
+    for name, x in named:
+        _need(x, name, (torch.float32,), 1, dev)
+    for name, x in named + [("actions", actions)]:
+        if x.numel() != T:
+            raise ValueError(f"{name} must have {T} entries, not {x.numel()}")
+    lo, hi = (float(c) for c in clip)
+    if not (lo >= 0 and hi >= 0):
+        raise ValueError(f"clip must be two widths of at least 0; got {clip}")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError("temperature must be positive")
+    if not math.isfinite(kl_coef):
+        raise ValueError("kl_coef must be finite")
+    return lo, hi
+
+
+def _policy(logits, actions, logp_old, advantages, logp_ref, weights, clip, kl_coef, temperature,
+            dloss, grad):
+    T, V = logits.shape
+    if V > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    actions = actions.to(torch.int64).contiguous()
+    logp_old, advantages = logp_old.contiguous(), advantages.contiguous()
+    logp_ref = None if logp_ref is None else logp_ref.contiguous()
+    weights = torch.full((T,), 1.0 / max(T, 1), device=logits.device) if weights is None \
+        else weights.contiguous()
+    loss = torch.empty((), dtype=torch.float32, device=logits.device)
+    logp = torch.empty(T, dtype=torch.float32, device=logits.device)
+    dlogits = torch.empty((T, V), dtype=logits.dtype, device=logits.device) if grad else None
+    lib = load_library()
+    p = SeqPolicyLoss(ctypes.sizeof(SeqPolicyLoss), _DTYPES[logits.dtype], T, V,
+                      logits.stride(0), V, *clip, float(kl_coef), float(temperature),
+                      _ptr(logits), _ptr(actions), _ptr(logp_old), _ptr(logp_ref),
+                      _ptr(advantages), _ptr(weights), _ptr(dloss), loss.data_ptr(), _ptr(logp),
+                      _ptr(dlogits), None, 0)
+    ws = _workspace(lib.seq_policy_loss_workspace, "seq_policy_loss", p, logits.device)
+    _run(lib.seq_policy_loss, "seq_policy_loss", logits.device, p)
+    del ws
+    return loss, logp, dlogits
+
+
+class _PolicyFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, actions, logp_old, advantages, logp_ref, weights, clip, kl_coef,
+                temperature):
+        ctx.save_for_backward(logits, actions, logp_old, advantages, logp_ref, weights)
+        ctx.how = (clip, kl_coef, temperature)
+        loss, logp, _ = _policy(logits, actions, logp_old, advantages, logp_ref, weights, clip,
+                                kl_coef, temperature, None, False)
+        ctx.mark_non_differentiable(logp)
+        return loss, logp
+
+    @staticmethod
+    def backward(ctx, dloss, _):
+        # one pass over the logits: the sums are formed again, not stored
+        dlogits = _policy(*ctx.saved_tensors, *ctx.how, dloss.float().contiguous(), True)[2]
+        return (dlogits,) + (None,) * 8
+
+
+def policy_loss(logits, actions, logp_old, advantages, *, logp_ref=None, weights=None,
+                clip=(0.2, 0.2), kl_coef=0.0, temperature=1.0):
+    """Clipped policy loss with a KL term: (loss, logp).
+
+    logits [T, V] float32, bfloat16 or float16 (-inf: a symbol that is not
+    allowed there); actions [T] the tokens taken; logp_old, advantages and
+    logp_ref (or None) float32 [T]; weights float32 [T], 1/T each by default.
+    With z = logits / temperature, logp = z[action] - logsumexp z and
+    ratio = exp(logp - logp_old), the loss is the weighted sum over tokens of
+        -min(ratio A, clip(ratio, 1 - clip[0], 1 + clip[1]) A)
+        + kl_coef (exp(logp_ref - logp) - (logp_ref - logp) - 1).
+    A token of weight 0 is not read: logp 0, gradient 0. An action whose
+    logit is -inf has logp -inf and no gradient; one outside the vocabulary
+    gives NaN. logp carries no gradient. Sums are held in fp32 or more."""
+    lo_hi = _check_policy(logits, actions, logp_old, advantages, logp_ref, weights, clip,
+                          kl_coef, temperature)
+    args = (logits, actions, logp_old, advantages, logp_ref, weights, lo_hi, kl_coef, temperature)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _PolicyFn.apply(*args)
+    return _policy(*args, None, False)[:2]
+
+
+def policy_loss_grad(logits, actions, logp_old, advantages, *, logp_ref=None, weights=None,
+                     clip=(0.2, 0.2), kl_coef=0.0, temperature=1.0):
+    """policy_loss and its gradient in one pass: (loss, logp, dlogits), dlogits
+    like logits."""
+    lo_hi = _check_policy(logits, actions, logp_old, advantages, logp_ref, weights, clip,
+                          kl_coef, temperature)
+    return _policy(logits, actions, logp_old, advantages, logp_ref, weights, lo_hi, kl_coef,
+                   temperature, None, True)
