@@ -29,51 +29,270 @@ __device__ inline Term policy_term(const SeqPolicyLoss &p, int64_t t, float logp
     return r;
 }
 
+// 16 bytes of a row: 8 values of a 16-bit type, 4 of fp32
+template <typename T> struct Vec;
+template <> struct Vec<__bf16> {
+    static constexpr int n = 8;
+    static __device__ float get(const uint4v &v, int j) {
+        return j & 1 ? Bf16::hi(v[j / 2]) : Bf16::lo(v[j / 2]);
+    }
+    static __device__ uint4v pack(const float *f) {
+        return {Bf16::pack(f[0], f[1]), Bf16::pack(f[2], f[3]), Bf16::pack(f[4], f[5]),
+                Bf16::pack(f[6], f[7])};
+    }
+};
+template <> struct Vec<_Float16> {
+    static constexpr int n = 8;
+    static __device__ float get(const uint4v &v, int j) {
+        return j & 1 ? Fp16::hi(v[j / 2]) : Fp16::lo(v[j / 2]);
+    }
+    static __device__ uint4v pack(const float *f) {
+        return {Fp16::pack(f[0], f[1]), Fp16::pack(f[2], f[3]), Fp16::pack(f[4], f[5]),
+                Fp16::pack(f[6], f[7])};
+    }
+};
+template <> struct Vec<float> {
+    static constexpr int n = 4;
+    static __device__ float get(const uint4v &v, int j) { return __uint_as_float(v[j]); }
+    static __device__ uint4v pack(const float *f) {
+        return {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                __float_as_uint(f[3])};
+    }
+};
+
+// Running maximum m and sum of exp2((x - m) k) of a thread.
+struct Running {
+    float m = neg_inf(), s = 0.0f;
+    template <int N> __device__ void add(const float *x, float k) {
+        float c = x[0];
+#pragma unroll
+        for (int j = 1; j < N; j++) c = fmaxf(c, x[j]);
+        const float mn = fmaxf(m, c), m0 = mn == neg_inf() ? 0.0f : mn;
+        s *= exp2_fast((m - m0) * k);
+#pragma unroll
+        for (int j = 0; j < N; j++) s += exp2_fast((x[j] - m0) * k);
+        m = mn;
+    }
+};
+
+// The maximum and the sum of a block's running pairs, in one order, on every
+// thread. red holds 2 * waves floats.
+template <int WAVES>
+__device__ inline void block_softmax(Running r, float k, float *red, float &m0, float &sum) {
+    float m = r.m;
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const int w = threadIdx.x >> 6;
+    if (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) red[w] = m;
+        __syncthreads();
+        m = red[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; i++) m = fmaxf(m, red[i]);
+    }
+    m0 = m == neg_inf() ? 0.0f : m;
+    // a thread without a finite value has r.m = -inf and s = 0 (or NaN)
+    float s = r.s * (r.m == neg_inf() ? 1.0f : exp2_fast((r.m - m0) * k));
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+    if (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) red[WAVES + w] = s;
+        __syncthreads();
+        s = red[WAVES];
+#pragma unroll
+        for (int i = 1; i < WAVES; i++) s += red[WAVES + i];
+    }
+    sum = s;
+}
+
+// What a row's gradient needs: dlogits_j = gs * exp2((x_j - m0) k), plus g at
+// the action.
+struct RowGrad { float g, gs; };
 template <typename T>
-__global__ __launch_bounds__(256) void policy_rows(SeqPolicyLoss p, float *terms) {
+__device__ inline RowGrad finish_row(const SeqPolicyLoss &p, int64_t t, int64_t act, float xa,
+                                     float w, float m0, float sum, float &term, float &logp) {
+    const float inv_t = 1.0f / p.temperature;
+    logp = xa == neg_inf() ? neg_inf() : (xa - m0) * inv_t - logf(sum);
+    const Term q = policy_term(p, t, logp);
+    term = w * q.loss;
+    RowGrad r;
+    r.g = logp == neg_inf() ? 0.0f : w * q.slope * inv_t;
+    if (p.dloss) r.g *= *p.dloss;
+    r.gs = r.g == 0.0f ? 0.0f : -r.g / sum;
+    return r;
+}
+
+// A row per block, any size, stride and alignment: reads the row once for the
+// sums and, for the gradient, once more.
+template <typename T>
+__global__ __launch_bounds__(1024) void policy_stream(SeqPolicyLoss p, double *terms) {
+    constexpr int N = Vec<T>::n;
     const int64_t t = blockIdx.x;
     const T *x = (const T *)p.logits + t * p.row;
     T *dx = p.dlogits ? (T *)p.dlogits + t * p.drow : nullptr;
     const float w = p.weights[t];
     if (w == 0.0f) {
-        if (threadIdx.x == 0) { p.logp[t] = 0.0f; terms[t] = 0.0f; }
-        if (dx) for (int64_t j = threadIdx.x; j < p.vocab; j += 256) dx[j] = (T)0.0f;
+        if (threadIdx.x == 0) { p.logp[t] = 0.0f; terms[t] = 0.0; }
+        if (dx) for (int64_t j = threadIdx.x; j < p.vocab; j += 1024) dx[j] = (T)0.0f;
         return;
     }
-    const float inv_t = 1.0f / p.temperature;
-    __shared__ float red[8];
-    float m = neg_inf();
-    for (int64_t j = threadIdx.x; j < p.vocab; j += 256) m = fmaxf(m, (float)x[j]);
-    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float m0 = m == neg_inf() ? 0.0f : m;
-    float sum = 0.0f;
-    for (int64_t j = threadIdx.x; j < p.vocab; j += 256)
-        sum += exp2_fast(((float)x[j] - m0) * inv_t * kLog2e);
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    if ((threadIdx.x & 63) == 0) red[4 + (threadIdx.x >> 6)] = sum;
-    __syncthreads();
-    sum = (red[4] + red[5]) + (red[6] + red[7]);
-    const int64_t a = p.actions[t];
-    const bool in = a >= 0 && a < p.vocab;
-    const float xa = in ? (float)x[a] : __builtin_nanf("");
-    const float logp = xa == neg_inf() ? neg_inf() : (xa - m0) * inv_t - logf(sum);
-    const Term term = policy_term(p, t, logp);
-    if (threadIdx.x == 0) { p.logp[t] = logp; terms[t] = w * term.loss; }
-    if (!dx) return;
-    float g = logp == neg_inf() ? 0.0f : w * term.slope * inv_t;
-    if (p.dloss) g *= *p.dloss;
-    const float gs = g == 0.0f ? 0.0f : -g / sum;
-    for (int64_t j = threadIdx.x; j < p.vocab; j += 256) {
-        const float e = exp2_fast(((float)x[j] - m0) * inv_t * kLog2e);
-        dx[j] = (T)((j == a ? g : 0.0f) + gs * e);
+    __shared__ float red[32];
+    const float k = kLog2e / p.temperature;
+    Running r;
+    // whole 16-byte pieces between the row's first and last aligned address
+    const int64_t head = (int64_t)((-(uintptr_t)x & 15) / sizeof(T));
+    const int64_t pieces = p.vocab > head ? (p.vocab - head) / N : 0;
+    for (int64_t i = threadIdx.x; i < pieces; i += 1024) {
+        const uint4v v = *(const uint4v *)(x + head + i * N);
+        float f[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) f[j] = Vec<T>::get(v, j);
+        r.add<N>(f, k);
     }
+    const int64_t edge = p.vocab - pieces * N;        // values outside the pieces
+    for (int64_t i = threadIdx.x; i < edge; i += 1024) {
+        const float f = (float)x[i < head ? i : pieces * N + i];
+        r.add<1>(&f, k);
+    }
+    float m0, sum, term, logp;
+    block_softmax<16>(r, k, red, m0, sum);
+    const int64_t a = p.actions[t];
+    const float xa = a >= 0 && a < p.vocab ? (float)x[a] : __builtin_nanf("");
+    const RowGrad g = finish_row<T>(p, t, a, xa, w, m0, sum, term, logp);
+    if (threadIdx.x == 0) { p.logp[t] = logp; terms[t] = term; }
+    if (dx)
+        for (int64_t j = threadIdx.x; j < p.vocab; j += 1024)
+            dx[j] = (T)((j == a ? g.g : 0.0f) + g.gs * exp2_fast(((float)x[j] - m0) * k));
 }
 
-// the tokens' terms in one fixed order
-__global__ __launch_bounds__(1024) void policy_sum(const float *terms, int64_t n, float *loss) {
+// A row per block of THREADS, kept in registers as NV pieces of 16 bytes a
+// thread: read once, written once. Pieces are the aligned ones inside the row;
+// the few values before and after them go one to a thread.
+template <typename T, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS) void policy_row(SeqPolicyLoss p, double *terms) {
+    constexpr int N = Vec<T>::n, WAVES = THREADS / 64;
+    const int64_t t = blockIdx.x;
+    const T *x = (const T *)p.logits + t * p.row;
+    T *dx = (T *)p.dlogits + t * p.drow;
+    const int V = (int)p.vocab, tid = (int)threadIdx.x;
+    const int head = min(V, (int)((-(uintptr_t)x & 15) / sizeof(T)));
+    const int pieces = (V - head) / N, edge = V - pieces * N;
+    const int je = tid < head ? tid : pieces * N + tid;     // this thread's edge value
+    const uint4v *x4 = (const uint4v *)(x + head);
+    uint4v *d4 = (uint4v *)(dx + head);
+    const float w = p.weights[t];
+    if (w == 0.0f) {
+        if (tid == 0) { p.logp[t] = 0.0f; terms[t] = 0.0; }
+        const uint4v z = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            if (i * THREADS + tid < pieces) (d4 + i * THREADS)[tid] = z;
+        if (tid < edge) dx[je] = (T)0.0f;
+        return;
+    }
+    const float k = kLog2e / p.temperature;
+    uint4v v[NV];
+    const float ninf[8] = {neg_inf(), neg_inf(), neg_inf(), neg_inf(),
+                           neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+    const uint4v none = Vec<T>::pack(ninf);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        v[i] = none;
+        if (i * THREADS + tid < pieces) v[i] = (x4 + i * THREADS)[tid];
+    }
+    const float xe = tid < edge ? (float)x[je] : neg_inf();
+    const int64_t a = p.actions[t];
+    const float xa = a >= 0 && a < V ? (float)x[a] : __builtin_nanf("");
+    __shared__ float red[2 * WAVES];
+    Running r;
+    r.add<1>(&xe, k);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        float f[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) f[j] = Vec<T>::get(v[i], j);
+        r.add<N>(f, k);
+    }
+    float m0, sum, term, logp;
+    block_softmax<WAVES>(r, k, red, m0, sum);
+    const RowGrad g = finish_row<T>(p, t, a, xa, w, m0, sum, term, logp);
+    if (tid == 0) { p.logp[t] = logp; terms[t] = term; }
+    const int act = a >= 0 && a < V ? (int)a : -1;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int j0 = head + (i * THREADS + tid) * N;
+        float f[N];
+        // the unpacked values of the first pass are not to be kept: twice the registers
+        asm volatile("" : "+v"(v[i]));
+#pragma unroll
+        for (int j = 0; j < N; j++) f[j] = g.gs * exp2_fast((Vec<T>::get(v[i], j) - m0) * k);
+        if (act >= j0 && act < j0 + N)
+#pragma unroll
+            for (int j = 0; j < N; j++) f[j] += j0 + j == act ? g.g : 0.0f;
+        if (i * THREADS + tid < pieces) (d4 + i * THREADS)[tid] = Vec<T>::pack(f);
+    }
+    if (tid < edge) dx[je] = (T)((je == act ? g.g : 0.0f) + g.gs * exp2_fast((xe - m0) * k));
+}
+
+// Few symbols: a block takes R rows through LDS, in 16-byte pieces when they
+// lie end to end (`joined`); a thread owns a row. A thread starts its row at a column of
+// its own, so that rows of a power-of-two length spread over the banks.
+template <typename T, int R>
+__global__ __launch_bounds__(R) void policy_symbols(SeqPolicyLoss p, bool joined, double *terms) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    __shared__ double red[R / 64];
+    constexpr int N = Vec<T>::n;
+    const int V = (int)p.vocab;
+    const int64_t t0 = (int64_t)blockIdx.x * R;
+    const int rows = (int)(p.tokens - t0 < R ? p.tokens - t0 : R);
+    const T *x = (const T *)p.logits + t0 * p.row;
+    T *row = (T *)lds;
+    const int n = rows * V, pieces = joined ? n / N : 0;
+    for (int i = threadIdx.x; i < pieces; i += R) ((uint4v *)lds)[i] = ((const uint4v *)x)[i];
+    for (int i = pieces * N + threadIdx.x; i < n; i += R) row[i] = x[(i / V) * p.row + i % V];
+    __syncthreads();
+    const int64_t t = t0 + threadIdx.x;
+    float term = 0.0f;
+    if ((int)threadIdx.x < rows) {
+        T *y = row + threadIdx.x * V;
+        const float w = p.weights[t];
+        const int j1 = (int)threadIdx.x % V;
+        if (w == 0.0f) {
+            p.logp[t] = 0.0f;
+            for (int i = 0, j = j1; i < V; i++, j = j + 1 == V ? 0 : j + 1) y[j] = (T)0.0f;
+        } else {
+            const float k = kLog2e / p.temperature;
+            float m = neg_inf(), sum = 0.0f, logp;
+            for (int i = 0, j = j1; i < V; i++, j = j + 1 == V ? 0 : j + 1)
+                m = fmaxf(m, (float)y[j]);
+            const float m0 = m == neg_inf() ? 0.0f : m;
+            for (int i = 0, j = j1; i < V; i++, j = j + 1 == V ? 0 : j + 1)
+                sum += exp2_fast(((float)y[j] - m0) * k);
+            const int64_t a = p.actions[t];
+            const float xa = a >= 0 && a < V ? (float)y[a] : __builtin_nanf("");
+            const RowGrad g = finish_row<T>(p, t, a, xa, w, m0, sum, term, logp);
+            p.logp[t] = logp;
+            if (p.dlogits)
+                for (int i = 0, j = j1; i < V; i++, j = j + 1 == V ? 0 : j + 1)
+                    y[j] = (T)((j == a ? g.g : 0.0f) +
+                               g.gs * exp2_fast(((float)y[j] - m0) * k));
+        }
+    }
+    double s = term;
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = red[0];
+        for (int i = 1; i < R / 64; i++) s += red[i];
+        terms[blockIdx.x] = s;
+    }
+    if (!p.dlogits) return;
+    T *dx = (T *)p.dlogits + t0 * p.drow;
+    for (int i = threadIdx.x; i < pieces; i += R) ((uint4v *)dx)[i] = ((const uint4v *)lds)[i];
+    for (int i = pieces * N + threadIdx.x; i < n; i += R) dx[(i / V) * p.drow + i % V] = row[i];
+}
+
+// the blocks' terms in one fixed order, in 64 bits
+__global__ __launch_bounds__(1024) void policy_sum(const double *terms, int64_t n, float *loss) {
     __shared__ double red[16];
     double s = 0.0;
     for (int64_t i = threadIdx.x; i < n; i += 1024) s += terms[i];
@@ -87,6 +306,13 @@ __global__ __launch_bounds__(1024) void policy_sum(const float *terms, int64_t n
     }
 }
 
+// Rows of a policy_symbols block: 256 while they fit 32 KB of LDS, fewer
+// beyond; 0: too long a row.
+int symbol_rows(const SeqPolicyLoss &p) {
+    const int64_t bytes = p.vocab * (p.dtype == SEQ_FP32 ? 4 : 2);
+    return bytes <= 128 ? 256 : (bytes <= 256 ? 128 : (bytes <= 512 ? 64 : 0));
+}
+
 int check_policy(const SeqPolicyLoss *p) {
     if (!p || p->struct_size != (int32_t)sizeof(SeqPolicyLoss)) return CO_ERR_NULLARG;
     if (p->tokens < 0 || p->vocab < 1) return CO_ERR_NULLARG;
@@ -95,11 +321,42 @@ int check_policy(const SeqPolicyLoss *p) {
     return CO_OK;
 }
 
+template <typename T, int THREADS, int NV>
+void launch_row(const SeqPolicyLoss &p, double *terms, hipStream_t s) {
+    policy_row<T, THREADS, NV><<<dim3((unsigned)p.tokens), THREADS, 0, s>>>(p, terms);
+}
+
+// Launches the rows' kernel; returns the number of terms it leaves.
 template <typename T>
-int launch_policy(const SeqPolicyLoss &p, hipStream_t s) {
-    float *terms = (float *)p.workspace;
-    policy_rows<T><<<dim3((unsigned)p.tokens), 256, 0, s>>>(p, terms);
-    return launch_status();
+int64_t launch_policy(const SeqPolicyLoss &p, double *terms, hipStream_t s) {
+    constexpr int N = Vec<T>::n;
+    const int rows = symbol_rows(p);
+    if (rows) {
+        const int64_t blocks = (p.tokens + rows - 1) / rows;
+        const dim3 grid((unsigned)blocks);
+        const bool joined = p.row == p.vocab && !((uintptr_t)p.logits & 15) &&
+                            (!p.dlogits || (p.drow == p.vocab && !((uintptr_t)p.dlogits & 15)));
+        const size_t lds = (size_t)rows * p.vocab * sizeof(T);
+        if (rows == 256) policy_symbols<T, 256><<<grid, 256, lds, s>>>(p, joined, terms);
+        else if (rows == 128) policy_symbols<T, 128><<<grid, 128, lds, s>>>(p, joined, terms);
+        else policy_symbols<T, 64><<<grid, 64, lds, s>>>(p, joined, terms);
+        return blocks;
+    }
+    const int64_t n = (p.vocab + N - 1) / N;       // no row has more pieces
+    const bool same = p.dlogits && !(((uintptr_t)p.logits ^ (uintptr_t)p.dlogits) & 15) &&
+                      (p.row - p.drow) % N == 0;
+    if (!same || n > 1024 * 16) policy_stream<T><<<dim3((unsigned)p.tokens), 1024, 0, s>>>(p, terms);
+    else if (n <= 64 * 2) launch_row<T, 64, 2>(p, terms, s);
+    else if (n <= 256 * 1) launch_row<T, 256, 1>(p, terms, s);
+    else if (n <= 256 * 2) launch_row<T, 256, 2>(p, terms, s);
+    else if (n <= 256 * 4) launch_row<T, 256, 4>(p, terms, s);
+    else if (n <= 256 * 8) launch_row<T, 256, 8>(p, terms, s);
+    else if (n <= 1024 * 4) launch_row<T, 1024, 4>(p, terms, s);
+    else if (n <= 1024 * 6) launch_row<T, 1024, 6>(p, terms, s);
+    else if (n <= 1024 * 8) launch_row<T, 1024, 8>(p, terms, s);
+    else if (n <= 1024 * 12) launch_row<T, 1024, 12>(p, terms, s);
+    else launch_row<T, 1024, 16>(p, terms, s);
+    return p.tokens;
 }
 
 }  // namespace seq
@@ -107,7 +364,7 @@ int launch_policy(const SeqPolicyLoss &p, hipStream_t s) {
 extern "C" int64_t seq_policy_loss_workspace(const SeqPolicyLoss *p) {
     const int rc = seq::check_policy(p);
     if (rc != CO_OK) return rc > 0 ? -rc : rc;
-    return 4 * p->tokens;
+    return 8 * p->tokens;
 }
 
 extern "C" int seq_policy_loss(const SeqPolicyLoss *p, void *stream) {
@@ -116,18 +373,21 @@ extern "C" int seq_policy_loss(const SeqPolicyLoss *p, void *stream) {
     if (!p->loss) return CO_ERR_NULLARG;
     if (!(p->temperature > 0.0f)) return CO_ERR_DATA;
     hipStream_t s = (hipStream_t)stream;
+    double *ws = (double *)p->workspace;
+    int64_t terms = 0;
     if (p->tokens) {
         if (!p->logits || !p->actions || !p->logp_old || !p->advantages || !p->weights ||
             !p->logp || !p->workspace)
             return CO_ERR_NULLARG;
-        if (p->workspace_bytes < 4 * p->tokens) return CO_ERR_DATA;
+        if (p->workspace_bytes < 8 * p->tokens) return CO_ERR_DATA;
         switch (p->dtype) {
-            case SEQ_FP32: rc = seq::launch_policy<float>(*p, s); break;
-            case SEQ_BF16: rc = seq::launch_policy<__bf16>(*p, s); break;
-            default: rc = seq::launch_policy<_Float16>(*p, s); break;
+            case SEQ_FP32: terms = seq::launch_policy<float>(*p, ws, s); break;
+            case SEQ_BF16: terms = seq::launch_policy<__bf16>(*p, ws, s); break;
+            default: terms = seq::launch_policy<_Float16>(*p, ws, s); break;
         }
+        rc = seq::launch_status();
         if (rc != CO_OK) return rc;
     }
-    seq::policy_sum<<<1, 1024, 0, s>>>((const float *)p->workspace, p->tokens, p->loss);
+    seq::policy_sum<<<1, 1024, 0, s>>>(ws, terms, p->loss);
     return seq::launch_status();
 }
