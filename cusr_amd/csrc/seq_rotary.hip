@@ -10,6 +10,7 @@ namespace seq {
 
 template <typename T> __device__ inline float load1(const T *p) { return (float)*p; }
 
+// Any size, stride and alignment: a thread per pair or copied element.
 template <typename T>
 __global__ __launch_bounds__(256) void rotary_kernel(SeqRotary r) {
     const int heads = r.hq + r.hkv, half = r.rot / 2;
@@ -43,8 +44,108 @@ __global__ __launch_bounds__(256) void rotary_kernel(SeqRotary r) {
     }
 }
 
+// 16-byte pieces: N values of T
+template <typename T> struct Piece {
+    static constexpr int n = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(n)));
+};
+
+// A thread owns one piece's place in the head (in the half layout, the piece
+// and its partner half a turn further) of one token and runs over `per` heads
+// of q and k with the same cosines and sines. Needs 16-byte rows and heads and
+// pairs that fill pieces.
+template <typename T, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_pieces(SeqRotary r, int items, int per) {
+    constexpr int N = Piece<T>::n, P = INTERLEAVED ? N / 2 : N;    // pairs of a thread
+    typedef typename Piece<T>::vec vec;
+    const int tokens = 256 / items;
+    const int slot = (int)threadIdx.x / items, e = (int)threadIdx.x % items;
+    const int64_t t = (int64_t)blockIdx.x * tokens + slot;
+    if (slot >= tokens || t >= r.tokens) return;
+    const int half = r.rot / 2, turning = half / P;      // pieces that turn
+    const int h0 = (int)blockIdx.y * per, h1 = min(h0 + per, r.hq + r.hkv);
+    const bool turn = e < turning;
+    float c[P], s[P];
+    if (turn) {
+        const int64_t pos = r.positions[t];
+        const bool in = pos >= 0 && pos < r.table_len;
+        const float4v *cs = (const float4v *)(r.table + (pos * half + e * P) * 2);
+#pragma unroll
+        for (int j = 0; j < P; j += 2) {
+            const float nan = __builtin_nanf("");
+            float4v v = {nan, nan, nan, nan};
+            if (in) v = cs[j / 2];
+            c[j] = v[0]; c[j + 1] = v[2];
+            s[j] = r.inverse ? -v[1] : v[1];
+            s[j + 1] = r.inverse ? -v[3] : v[3];
+        }
+    }
+    // first element of the piece, and of its partner
+    const int ia = turn ? e * (INTERLEAVED ? N : P) : r.rot + (e - turning) * N;
+    const int ib = ia + half;
+#pragma unroll 4
+    for (int h = h0; h < h1; h++) {
+        const bool is_q = h < r.hq;
+        const T *x = is_q ? (const T *)r.q + t * r.q_row + h * r.q_head
+                          : (const T *)r.k + t * r.k_row + (h - r.hq) * r.k_head;
+        T *y = is_q ? (T *)r.q_out + t * r.qo_row + h * r.qo_head
+                    : (T *)r.k_out + t * r.ko_row + (h - r.hq) * r.ko_head;
+        vec a = *(const vec *)(x + ia);
+        if (!turn) {
+            *(vec *)(y + ia) = a;
+        } else if (INTERLEAVED) {
+            vec o;
+#pragma unroll
+            for (int j = 0; j < P; j++) {
+                const float u = (float)a[2 * j], w = (float)a[2 * j + 1];
+                o[2 * j] = (T)(u * c[j] - w * s[j]);
+                o[2 * j + 1] = (T)(w * c[j] + u * s[j]);
+            }
+            *(vec *)(y + ia) = o;
+        } else {
+            const vec b = *(const vec *)(x + ib);
+            vec oa, ob;
+#pragma unroll
+            for (int j = 0; j < P; j++) {
+                const float u = (float)a[j], w = (float)b[j];
+                oa[j] = (T)(u * c[j] - w * s[j]);
+                ob[j] = (T)(w * c[j] + u * s[j]);
+            }
+            *(vec *)(y + ia) = oa;
+            *(vec *)(y + ib) = ob;
+        }
+    }
+}
+
+bool off(const void *p, int64_t row, int64_t head, int n) {
+    return ((uintptr_t)p & 15) || row % n || head % n;
+}
+
+// Whether every piece lies on a 16-byte boundary, and pairs fill pieces.
+bool in_pieces(const SeqRotary &r, int n) {
+    const int turned = r.interleaved ? r.rot : r.rot / 2;
+    if (turned % n || r.d % n || r.d / n > 256 || ((uintptr_t)r.table & 15)) return false;
+    if (r.hq && (off(r.q, r.q_row, r.q_head, n) || off(r.q_out, r.qo_row, r.qo_head, n)))
+        return false;
+    return !(r.hkv && (off(r.k, r.k_row, r.k_head, n) || off(r.k_out, r.ko_row, r.ko_head, n)));
+}
+
 template <typename T>
 int launch_rotary(const SeqRotary &r, hipStream_t s) {
+    constexpr int N = Piece<T>::n;
+    if (in_pieces(r, N)) {
+        const int items = (r.interleaved ? r.rot : r.rot / 2) / N + (r.d - r.rot) / N;
+        const int heads = r.hq + r.hkv, tokens = 256 / items;
+        const int64_t blocks = (r.tokens + tokens - 1) / tokens;
+        // A thread takes as many heads as leave 4 blocks per compute unit: the
+        // table is read once for them; few tokens spread over heads instead.
+        int per = 1;
+        while (per < heads && blocks * ((heads + 2 * per - 1) / (2 * per)) >= 1024) per *= 2;
+        const dim3 grid((unsigned)blocks, (unsigned)((heads + per - 1) / per));
+        if (r.interleaved) rotary_pieces<T, true><<<grid, 256, 0, s>>>(r, items, per);
+        else rotary_pieces<T, false><<<grid, 256, 0, s>>>(r, items, per);
+        return launch_status();
+    }
     const int64_t n = r.tokens * (r.hq + r.hkv) * (r.d - r.rot / 2);
     int64_t blocks = (n + 255) / 256;
     if (blocks > 65536) blocks = 65536;
