@@ -4,6 +4,15 @@
 
 namespace seq {
 
+// A row's output from its unscaled sum, and its lse. No visible key: l is 0.
+template <typename T, int DP>
+__device__ inline void store_out(const Attn &a, int64_t t, int head, const float16v *o, float m,
+                                 float l, bool ok) {
+    store_row<T, DP>(a.o, t * a.o_row + head * a.o_head, o, l == 0.0f ? 0.0f : 1.0f / l, a.d, ok);
+    if (a.lse && ok && (threadIdx.x & 63) < 32)
+        a.lse[head * a.tq + t] = l == 0.0f ? neg_inf() : m * a.scale + logf(l);
+}
+
 // One wave owns a tile of 32 rows of one key head and runs over the keys 32 at
 // a time with a running maximum and sum. K comes straight from memory as the
 // left operand; V passes through the wave's own LDS tile to be transposed.
@@ -81,14 +90,217 @@ __global__ __launch_bounds__(256) void attn_wave(Attn a, int64_t slots) {
                 o[dt] = T::mfma(Tile<DP>::transposed(vt, kc * 16, dt), pb, o[dt]);
         }
     }
-    l = add_halves(l);
-    store_row<T, DP>(a.o, (p.q0 + qi) * a.o_row + head * a.o_head, o, l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l), a.d, ok);
-    if (a.lse && ok && h == 0)
-        a.lse[head * a.tq + p.q0 + qi] = l == 0.0f ? neg_inf() : m * a.scale + logf(l);
+    store_out<T, DP>(a, p.q0 + qi, head, o, m, add_halves(l), ok);
+}
+
+// Few rows over many keys (single tokens over a cache). A sequence's keys are
+// cut into chunks, one wave to a chunk, key head and tile of 32 rows; each
+// leaves its maximum, sum and unscaled output, and attn_join adds them up. The
+// next 32 keys are loaded while the present ones are worked on: eight waves a
+// compute unit keep 128 KB in flight. Chunks are slots over the key rows, as
+// tiles are over the query rows.
+struct Step {
+    int chunk;          // keys of a chunk, a multiple of 32
+    int tiles;          // row tiles of a slot that have room in the partials
+    int64_t slots;
+    float *o, *ml;      // [slot][hkv][tiles * 32][DP], [slot][hkv][tiles * 32][2]
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
+    __shared__ __align__(16) uint16_t lds[4][32 * Tile<DP>::stride];
+    uint16_t *vt = lds[threadIdx.x >> 6];
+    constexpr int CH = DP / 8;               // 16-byte pieces of a row
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int64_t item = blockIdx.x * 4ll + (threadIdx.x >> 6);
+    const int64_t slot = item / a.hkv;
+    const int hk = (int)(item % a.hkv);
+    if (slot >= st.slots) return;
+    const int b = find_sequence(a.cu_k, a.n_seq, a.tk, 1, st.chunk, slot);
+    // the rows after the last sequence see no key: entry n_seq, chunk 0
+    const Place p = place_of(a, b);
+    const int64_t c64 = slot - slot_of(offset_at(a.cu_k, b, a.tk), 1, st.chunk, b);
+    const int64_t rows = (int64_t)p.lq * a.G;
+    if (c64 < 0 || rows == 0) return;
+    const int chunks = (p.lk + st.chunk - 1) / st.chunk;
+    const bool split = chunks > 1 && rows <= st.tiles * 32;
+    if (c64 >= (split ? chunks : 1)) return;
+    const int key0 = split ? (int)c64 * st.chunk : 0;
+    const int key1 = split && key0 + st.chunk < p.lk ? key0 + st.chunk : p.lk;
+    const uint16_t *kp = (const uint16_t *)a.k + p.k0 * a.k_row + hk * a.k_head;
+    const uint16_t *vp = (const uint16_t *)a.v + p.k0 * a.v_row + hk * a.v_head;
+
+    // a sequence with more rows than the partials have room for is not split
+    for (int64_t tile = blockIdx.y; tile * 32 < rows; tile += st.tiles) {
+        const int64_t row = tile * 32 + (lane & 31);
+        const bool ok = row < rows;
+        const int qi = ok ? (int)(row / a.G) : 0, g = ok ? (int)(row % a.G) : 0;
+        const int head = hk * a.G + g;
+        const int lim = ok ? qi + p.lk - p.lq : -1;
+        uint4v q[DP / 16], k[DP / 16], v[DP / 16];
+        load_row<DP>(q, a.q, (p.q0 + qi) * a.q_row + head * a.q_head, a.d, ok);
+        const int64_t last_row = tile * 32 + 31 < rows ? tile * 32 + 31 : rows - 1;
+        const int seen = (int)(last_row / a.G) + p.lk - p.lq + 1;
+        const int end = key1 < seen ? key1 : seen;
+        auto fetch = [&](int k0) {
+            const int kr = k0 + (lane & 31);
+            load_row<DP>(k, kp, (int64_t)kr * a.k_row, a.d, kr < end);
+#pragma unroll
+            for (int j = 0; j < DP / 16; j++) {
+                const int i = lane + 64 * j, r = k0 + i / CH, ch = i % CH;
+                const uint4v z = {0, 0, 0, 0};
+                v[j] = r < end && ch * 8 < a.d
+                           ? *(const uint4v *)(vp + (int64_t)r * a.v_row + ch * 8) : z;
+            }
+        };
+        float16v o[DP / 32] = {};
+        float m = neg_inf(), l = 0.0f;
+        fetch(key0);
+        for (int k0 = key0; k0 < end; k0 += 32) {
+            float16v s = {};
+#pragma unroll
+            for (int c = 0; c < DP / 16; c++) s = T::mfma(k[c], q[c], s);
+            wave_sync();
+#pragma unroll
+            for (int j = 0; j < DP / 16; j++) {
+                const int i = lane + 64 * j;
+                *(uint4v *)(vt + Tile<DP>::at(i / CH, i % CH)) = v[j];
+            }
+            if (k0 + 32 < end) fetch(k0 + 32);
+            float mx = neg_inf();
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int key = k0 + 8 * (r / 4) + 4 * h + r % 4;
+                s[r] = key <= lim && key < end ? s[r] : neg_inf();
+                mx = fmaxf(mx, s[r]);
+            }
+            const float mn = fmaxf(m, max_halves(mx));
+            const float m0 = mn == neg_inf() ? 0.0f : mn;
+            const float alpha = exp2_fast((m - m0) * a.c);
+            float sum = 0.0f;
+            uint32_t pk[8];
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const float p0 = exp2_fast((s[r] - m0) * a.c);
+                const float p1 = exp2_fast((s[r + 1] - m0) * a.c);
+                sum += p0 + p1;
+                pk[r / 2] = T::pack(p0, p1);
+            }
+            l = l * alpha + sum;
+            m = mn;
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; dt++) o[dt] *= alpha;
+            wave_sync();
+#pragma unroll
+            for (int kc = 0; kc < 2; kc++) {
+                const uint4v pb = {pk[4 * kc], pk[4 * kc + 1], pk[4 * kc + 2], pk[4 * kc + 3]};
+#pragma unroll
+                for (int dt = 0; dt < DP / 32; dt++)
+                    o[dt] = T::mfma(Tile<DP>::transposed(vt, kc * 16, dt), pb, o[dt]);
+            }
+        }
+        l = add_halves(l);
+        if (split) {
+            const int64_t pr = ((slot * a.hkv + hk) * st.tiles + tile) * 32 + (lane & 31);
+            if (ok) {
+#pragma unroll
+                for (int dt = 0; dt < DP / 32; dt++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float4v f = {o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2],
+                                           o[dt][4 * j + 3]};
+                        *(float4v *)(st.o + pr * DP + dt * 32 + 8 * j + 4 * h) = f;
+                    }
+                if (h == 0) {
+                    st.ml[2 * pr] = m;
+                    st.ml[2 * pr + 1] = l;
+                }
+            }
+        } else {
+            store_out<T, DP>(a, p.q0 + qi, head, o, m, l, ok);
+        }
+    }
+}
+
+// Joins the chunks of a split sequence: a wave to a row of the output, which
+// has one owner and one order of summation.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_join(Attn a, Step st) {
+    const int lane = threadIdx.x & 63;
+    const int64_t item = blockIdx.x * 4ll + (threadIdx.x >> 6);
+    if (item >= a.tq * a.hq) return;
+    const int64_t t = item / a.hq;
+    const int head = (int)(item % a.hq), hk = head / a.G;
+    const int b = sequence_of_row(a.cu_q, a.n_seq, a.tq, t);
+    const Place p = place_of(a, b);
+    const int chunks = (p.lk + st.chunk - 1) / st.chunk;
+    const int64_t rows = (int64_t)p.lq * a.G;
+    if (chunks <= 1 || rows > st.tiles * 32 || t < p.q0 || t >= p.q0 + p.lq) return;
+    const int64_t row = (t - p.q0) * a.G + head % a.G;
+    const int64_t slot0 = slot_of(offset_at(a.cu_k, b, a.tk), 1, st.chunk, b);
+    const int64_t stride = (int64_t)a.hkv * st.tiles * 32;
+    const int64_t pr = slot0 * stride + (int64_t)hk * st.tiles * 32 + row;
+    float m = neg_inf();
+    for (int c = lane; c < chunks; c += 64) m = fmaxf(m, st.ml[2 * (pr + c * stride)]);
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float m0 = m == neg_inf() ? 0.0f : m;
+    float l = 0.0f;
+    for (int c = lane; c < chunks; c += 64) {
+        const float *x = st.ml + 2 * (pr + c * stride);
+        l += x[1] * exp2_fast((x[0] - m0) * a.c);
+    }
+    for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+    float acc[2] = {0.0f, 0.0f};
+#pragma unroll 8
+    for (int c = 0; c < chunks; c++) {
+        const float w = exp2_fast((st.ml[2 * (pr + c * stride)] - m0) * a.c);
+        const float *x = st.o + (pr + c * stride) * DP;
+        for (int e = 0; e < (DP + 63) / 64; e++)
+            if (lane + 64 * e < DP) acc[e] += w * x[lane + 64 * e];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    typename T::elem *out = (typename T::elem *)a.o + t * a.o_row + head * a.o_head;
+    for (int e = 0; e < (DP + 63) / 64; e++)
+        if (lane + 64 * e < a.d) out[lane + 64 * e] = (typename T::elem)(acc[e] * inv);
+    if (a.lse && lane == 0)
+        a.lse[head * a.tq + t] = l == 0.0f ? neg_inf() : m * a.scale + logf(l);
+}
+
+// Whether a call is few rows over many keys, and its chunks. At most 256 rows
+// a sequence on average, and at least four keys a query and 128 a sequence:
+// then the keys decide. Chunks leave about 4096 waves, of 256 to 512 keys:
+// longer ones leave waves idle at the end, shorter ones more to join.
+bool plan_step(const Attn &a, Step &st) {
+    if (a.n_seq == 0 || a.tq * a.G > 256ll * a.n_seq || a.tk < 4 * a.tq ||
+        a.tk < 128ll * a.n_seq)
+        return false;
+    st.tiles = (int)((a.tq * a.G + 32ll * a.n_seq - 1) / (32ll * a.n_seq));
+    st.chunk = a.tk * a.hkv * st.tiles / 512 >= 4096 ? 512 : 256;
+    st.slots = slot_of(a.tk, 1, st.chunk, a.n_seq) + 1;
+    return true;
+}
+int64_t step_rows(const Attn &a, const Step &st) { return st.slots * a.hkv * st.tiles * 32; }
+int64_t step_bytes(const Attn &a, const Step &st) {
+    return a.tk <= st.chunk ? 0 : step_rows(a, st) * (padded_head(a.d) + 2) * 4;
 }
 
 template <typename T, int DP>
-int launch_wave(const Attn &a, hipStream_t s) {
+int launch_step(const Attn &a, Step st, hipStream_t s) {
+    st.o = (float *)a.workspace;
+    st.ml = st.o + step_rows(a, st) * DP;
+    const dim3 grid((unsigned)((st.slots * a.hkv + 3) / 4), (unsigned)st.tiles);
+    attn_step<T, DP><<<grid, 256, 0, s>>>(a, st);
+    if (a.tk > st.chunk) {
+        if (hipGetLastError() != hipSuccess) return CO_ERR_CUDA;
+        attn_join<T, DP><<<dim3((unsigned)((a.tq * a.hq + 3) / 4)), 256, 0, s>>>(a, st);
+    }
+    return launch_status();
+}
+
+template <typename T, int DP>
+int launch_head(const Attn &a, hipStream_t s) {
+    Step st;
+    if (plan_step(a, st)) return launch_step<T, DP>(a, st, s);
     const int64_t slots = slot_of(a.tq, a.G, 32, a.n_seq) + 1;
     const int64_t blocks = (slots * a.hkv + 3) / 4;
     attn_wave<T, DP><<<dim3((unsigned)blocks), 256, 0, s>>>(a, slots);
@@ -98,10 +310,10 @@ int launch_wave(const Attn &a, hipStream_t s) {
 template <typename T>
 int launch_forward(const Attn &a, hipStream_t s) {
     switch (padded_head(a.d)) {
-        case 32: return launch_wave<T, 32>(a, s);
-        case 64: return launch_wave<T, 64>(a, s);
-        case 96: return launch_wave<T, 96>(a, s);
-        default: return launch_wave<T, 128>(a, s);
+        case 32: return launch_head<T, 32>(a, s);
+        case 64: return launch_head<T, 64>(a, s);
+        case 96: return launch_head<T, 96>(a, s);
+        default: return launch_head<T, 128>(a, s);
     }
 }
 
@@ -134,7 +346,10 @@ int check_attention_data(const SeqAttention *a) {
 
 extern "C" int64_t seq_attention_workspace(const SeqAttention *a) {
     const int rc = seq::check_attention(a);
-    return rc == CO_OK ? 0 : (rc > 0 ? -rc : rc);
+    if (rc != CO_OK) return rc > 0 ? -rc : rc;
+    const seq::Attn x = seq::make_attn(a);
+    seq::Step st;
+    return seq::plan_step(x, st) ? seq::step_bytes(x, st) : 0;
 }
 
 extern "C" int seq_attention(const SeqAttention *sa, void *stream) {
@@ -143,10 +358,10 @@ extern "C" int seq_attention(const SeqAttention *sa, void *stream) {
     if (sa->tq == 0) return CO_OK;
     rc = seq::check_attention_data(sa);
     if (rc != CO_OK) return rc;
-    seq::Attn a;
-    static_cast<SeqAttention &>(a) = *sa;
-    a.G = a.hq / a.hkv;
-    a.c = a.scale * seq::kLog2e;
+    const seq::Attn a = seq::make_attn(sa);
+    const int64_t need = seq_attention_workspace(sa);
+    if (need && !a.workspace) return CO_ERR_NULLARG;
+    if (need > a.workspace_bytes || ((uintptr_t)a.workspace & 15)) return CO_ERR_DATA;
     hipStream_t s = (hipStream_t)stream;
     return a.dtype == SEQ_BF16 ? seq::launch_forward<seq::Bf16>(a, s)
                                : seq::launch_forward<seq::Fp16>(a, s);

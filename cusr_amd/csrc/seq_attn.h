@@ -62,6 +62,18 @@ __device__ inline int find_sequence(const int32_t *cu, int n_seq, int64_t t, int
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
+// The sequence of query row t (n_seq: none): the last whose offset is not
+// beyond it. Empty sequences share their offset with the next.
+__device__ inline int sequence_of_row(const int32_t *cu, int n_seq, int64_t tq, int64_t t) {
+    int lo = 0, hi = n_seq;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (offset_at(cu, mid, tq) <= t) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
 __device__ inline Place place_of(const Attn &a, int b) {
     Place p;
     p.q0 = offset_at(a.cu_q, b, a.tq);
@@ -149,6 +161,14 @@ __device__ inline void store_row(void *base, int64_t off, const float16v *acc, f
             const int col = dt * 32 + g * 16 + h * 8;
             if (ok && col < d) *(uint4v *)(p + col) = v;
         }
+}
+
+inline Attn make_attn(const SeqAttention *s) {
+    Attn a;
+    static_cast<SeqAttention &>(a) = *s;
+    a.G = a.hq / a.hkv;
+    a.c = a.scale * kLog2e;
+    return a;
 }
 
 int check_attention(const SeqAttention *a);
