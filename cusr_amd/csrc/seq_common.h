@@ -29,6 +29,13 @@ __device__ inline float neg_inf() { return -__builtin_inff(); }
 // 2^x: one v_exp_f32 (results below 2^-126 flush to 0)
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// largest of three: one instruction, and no step to quiet a NaN before it
+__device__ inline float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 // larger of the two halves' values, in both lanes of (l, l + 32)
 __device__ inline float max_halves(float x) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

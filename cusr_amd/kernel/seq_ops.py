@@ -192,8 +192,8 @@ def _check_attention(q, k, v, cu_q, cu_k, k_lens, scale):
         _need(k_lens, "k_lens", (torch.int32,), 1, dev)
         if k_lens.numel() != cu_q.numel() - 1:
             raise ValueError("k_lens must have one entry per sequence")
-    if scale is not None and not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if scale is not None and not 0.0 < scale <= 1e30:
+        raise ValueError(f"scale must be positive, not {scale}")
 
 
 def _attention_struct(q, k, v, o, lse, cu_q, cu_k, k_lens, scale):

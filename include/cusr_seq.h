@@ -47,7 +47,7 @@ extern "C" {
  * cu_q[0] is 0. Queries are the last ones of the keys: query i of lq sees
  * keys 0 .. i + lk - lq. A query that sees no key, and a query row in no
  * sequence, give o = 0 and lse = -inf. Offsets out of order or out of range
- * are clamped into the tensors.
+ * are clamped into the tensors. scale is positive.
  *
  * lse (may be null for the forward) [hq, tq] fp32: log of the sum of
  * exp(scale q.k) over the visible keys. */
@@ -113,8 +113,8 @@ int seq_rotary(const SeqRotary *r, void *stream);
  *   l = -min(ratio A, clip(ratio, 1 - clip_lo, 1 + clip_hi) A)
  *       + kl_coef (exp(logp_ref - logp) - (logp_ref - logp) - 1),
  *   loss = sum over tokens of weight * l.
- * logp_ref null: no KL term. A token of weight 0 takes no part: its logits
- * are not read, logp = 0, its gradient row is 0. A row whose action has the
+ * logp_ref null: no KL term. A token of weight 0 takes no part,
+ * whatever its logits: logp = 0, its gradient row is 0. A row whose action has the
  * logit -inf has logp = -inf, ratio 0 and no gradient (and with a KL term an
  * infinite loss). An action outside the vocabulary gives logp = NaN.
  * dlogits (may be null: loss and logp alone) [tokens, vocab] like logits,

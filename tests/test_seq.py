@@ -148,7 +148,7 @@ def test_library_refusals():
             setattr(a, n, 4096)
         for n in ("q_row", "k_row", "v_row", "o_row"):
             setattr(a, n, 256)
-        a.workspace_bytes = 1 << 20
+        a.workspace_bytes, a.scale = 1 << 20, 0.125
         for n, x in kw.items():
             setattr(a, n, x)
         return a
