@@ -95,15 +95,17 @@ __global__ __launch_bounds__(256) void attn_wave(Attn a, int64_t slots) {
 
 // Long sequences: a block of WAVES waves owns WAVES * 32 rows of one key head;
 // 64 keys at a time pass through LDS for all of them, the next 64 on their way
-// in registers meanwhile. Two waves a SIMD, so that one's softmax runs beside
-// the other's matrix instructions. The sums are rescaled only when some row's
-// maximum has grown by more than 2^8: a lower reference is as exact, since
-// numerator and denominator share it, and 2^8 is far from any overflow.
+// there meanwhile. Two waves a SIMD, so that one's softmax runs beside the
+// other's matrix instructions; the vector instructions of the softmax and the
+// matrix instructions take about as long, so addresses are kept out of the loop.
+// The sums are rescaled only when some row's maximum has grown by more than 2^8:
+// a lower reference is as exact, since numerator and denominator share it, and
+// 2^8 is far from any overflow.
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int64_t slots) {
-    constexpr int KB = 64, CH = DP / 8, ROWS = WAVES * 32, THREADS = WAVES * 64;
-    constexpr int NP = (KB * CH + THREADS - 1) / THREADS;     // pieces a thread moves
-    __shared__ __align__(16) uint16_t lds[2][2][KB * Tile<DP>::stride];   // [buffer][k, v]
+    typedef KeyTiles<DP, 64, WAVES> Keys;
+    constexpr int KB = 64, ROWS = WAVES * 32, STRIDE = Keys::STRIDE;
+    __shared__ __align__(256) unsigned char lds[2 * Keys::BYTES];
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int64_t slot = blockIdx.x / a.hkv;
     const int hk = (int)(blockIdx.x % a.hkv);
@@ -130,88 +132,71 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int64_t slot
     const int64_t w0 = tile * ROWS + wave * 32;
     const int wave_keys = w0 < rows ? seen_by(w0 + 31) : 0;
     const int all_keys = w0 + 31 < rows ? seen_by(w0) : 0;
-    const uint16_t *kp = (const uint16_t *)a.k + p.k0 * a.k_row + hk * a.k_head;
-    const uint16_t *vp = (const uint16_t *)a.v + p.k0 * a.v_row + hk * a.v_head;
+    const Keys tiles(a, p, hk, keys);
+    const uint32_t lds0 = lds_address(lds);
+    const typename Tile<DP>::Rows kr = Tile<DP>::rows(lds0);
+    const typename Tile<DP>::Columns vc = Tile<DP>::columns(lds0 + Keys::BYTES / 2);
 
-    uint4v kn[NP], vn[NP];
-    auto fetch = [&](int k0) {
-#pragma unroll
-        for (int j = 0; j < NP; j++) {
-            const int i = threadIdx.x + THREADS * j, r = k0 + i / CH, ch = i % CH;
-            const bool in = i < KB * CH && r < keys && ch * 8 < a.d;
-            const uint4v z = {0, 0, 0, 0};
-            kn[j] = in ? *(const uint4v *)(kp + (int64_t)r * a.k_row + ch * 8) : z;
-            vn[j] = in ? *(const uint4v *)(vp + (int64_t)r * a.v_row + ch * 8) : z;
-        }
-    };
-    auto stash = [&](int buf) {
-#pragma unroll
-        for (int j = 0; j < NP; j++) {
-            const int i = threadIdx.x + THREADS * j;
-            if (KB * CH % THREADS == 0 || i < KB * CH) {
-                *(uint4v *)(lds[buf][0] + Tile<DP>::at(i / CH, i % CH)) = kn[j];
-                *(uint4v *)(lds[buf][1] + Tile<DP>::at(i / CH, i % CH)) = vn[j];
-            }
-        }
-    };
     float16v o[DP / 32] = {};
     float m = neg_inf(), l = 0.0f;
-    if (keys > 0) {
-        fetch(0);
-        stash(0);
-    }
-    for (int k0 = 0, buf = 0; k0 < keys; k0 += KB, buf ^= 1) {
-        __syncthreads();
-        if (k0 + KB < keys) fetch(k0 + KB);
-        if (k0 < wave_keys) {
-            const uint16_t *kt = lds[buf][0], *vt = lds[buf][1];
-            float16v s[2] = {};
+    // 64 keys from k0, in buffer `buf`
+    auto work = [&](auto buf, int k0) {
+        constexpr uint32_t B = decltype(buf)::value * Keys::BYTES;
+        wait_copies<0>();
+        block_barrier();
+        if (k0 + KB < keys) tiles.copy(k0 + KB, lds0 + (Keys::BYTES - B));
+        if (k0 >= wave_keys) return;
+        float16v s[2] = {};
 #pragma unroll
-            for (int c = 0; c < DP / 16; c++)
+        for (int c = 0; c < DP / 16; c++)
 #pragma unroll
-                for (int u = 0; u < 2; u++)
-                    s[u] = T::mfma(Tile<DP>::row(kt, u * 32, c), q[c], s[u]);
-            if (k0 + KB > all_keys)
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (k0 + u * 32 + 8 * (r / 4) + 4 * h + r % 4 > lim) s[u][r] = neg_inf();
-            float mx = max3(s[0][0], s[0][1], s[1][0]);
-            mx = fmaxf(mx, s[1][1]);
-#pragma unroll
-            for (int r = 2; r < 16; r += 2) mx = max3(max3(mx, s[0][r], s[0][r + 1]), s[1][r], s[1][r + 1]);
-            mx = max_halves(mx);
-            if (__any((mx - m) * a.c > 8.0f)) {
-                const float mn = fmaxf(m, mx), m0 = mn == neg_inf() ? 0.0f : mn;
-                const float alpha = exp2_fast((m - m0) * a.c);
-                l *= alpha;
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; dt++) o[dt] *= alpha;
-                m = mn;
-            }
-            const float mc = m == neg_inf() ? 0.0f : m * a.c;
-            float sum[2] = {0.0f, 0.0f};
+            for (int u = 0; u < 2; u++)
+                s[u] = T::mfma(Tile<DP>::row(kr.c[c], B + u * 32 * STRIDE), q[c], s[u]);
+        if (k0 + KB > all_keys)
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int kc = 0; kc < 2; kc++) {
-                    uint4v pb;
+                for (int r = 0; r < 16; r++)
+                    if (k0 + u * 32 + 8 * (r / 4) + 4 * h + r % 4 > lim) s[u][r] = neg_inf();
+        float mx = fmaxf(max3(s[0][0], s[0][1], s[1][0]), s[1][1]);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float p0 = exp2_fast(__builtin_fmaf(s[u][8 * kc + 2 * j], a.c, -mc));
-                        const float p1 = exp2_fast(__builtin_fmaf(s[u][8 * kc + 2 * j + 1], a.c, -mc));
-                        sum[0] += p0;
-                        sum[1] += p1;
-                        pb[j] = T::pack(p0, p1);
-                    }
+        for (int r = 2; r < 16; r += 2)
+            mx = max3(max3(mx, s[0][r], s[0][r + 1]), s[1][r], s[1][r + 1]);
+        mx = max_halves(mx);
+        if (__any((mx - m) * a.c > 8.0f)) {
+            const float mn = fmaxf(m, mx), m0 = mn == neg_inf() ? 0.0f : mn;
+            const float alpha = exp2_fast((m - m0) * a.c);
+            l *= alpha;
 #pragma unroll
-                    for (int dt = 0; dt < DP / 32; dt++)
-                        o[dt] = T::mfma(Tile<DP>::transposed(vt, u * 32 + kc * 16, dt), pb, o[dt]);
-                }
-            l += sum[0] + sum[1];
+            for (int dt = 0; dt < DP / 32; dt++) o[dt] *= alpha;
+            m = mn;
         }
-        if (k0 + KB < keys) stash(buf ^ 1);
+        const float mc = m == neg_inf() ? 0.0f : m * a.c;
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int kc = 0; kc < 2; kc++) {
+                uint4v pb;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float p0 = exp2_fast(__builtin_fmaf(s[u][8 * kc + 2 * j], a.c, -mc));
+                    const float p1 = exp2_fast(__builtin_fmaf(s[u][8 * kc + 2 * j + 1], a.c, -mc));
+                    sum[0] += p0;
+                    sum[1] += p1;
+                    pb[j] = T::pack(p0, p1);
+                }
+#pragma unroll
+                for (int dt = 0; dt < DP / 32; dt++)
+                    o[dt] = T::mfma(Tile<DP>::transposed(vc, dt, B + (u * 32 + kc * 16) * STRIDE), pb,
+                                    o[dt]);
+            }
+        l += sum[0] + sum[1];
+    };
+    if (keys > 0) tiles.copy(0, lds0);
+    for (int k0 = 0; k0 < keys; k0 += 2 * KB) {
+        work(Const<0>{}, k0);
+        if (k0 + KB < keys) work(Const<1>{}, k0 + KB);
     }
     store_out<T, DP>(a, p.q0 + qi, head, o, m, add_halves(l), ok);
 }

@@ -12,7 +12,8 @@ namespace seq {
 
 struct AttnGrad : Attn {
     SeqAttentionGrad g;
-    float *delta;            // [hq, tq]
+    // lse in powers of two [hq, tq] and +inf, then delta [hq, tq] and 0
+    float *stat;
 };
 
 template <typename T>
@@ -23,6 +24,20 @@ __device__ inline float dot_row(const uint4v *x, const uint4v *y, int n) {
         for (int j = 0; j < 4; j++)
             s += T::lo(x[c][j]) * T::lo(y[c][j]) + T::hi(x[c][j]) * T::hi(y[c][j]);
     return s;
+}
+
+// The rows' statistics for the kernel that owns keys; one thread adds the
+// values that stand for rows beyond a tile's last.
+__device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float delta, bool ok) {
+    const int64_t n = a.tq * a.hq;
+    if (ok && (threadIdx.x & 63) < 32) {
+        a.stat[at] = lse2;
+        a.stat[n + 1 + at] = delta;
+        if (at == 0) {
+            a.stat[n] = __builtin_inff();
+            a.stat[2 * n + 1] = 0.0f;
+        }
+    }
 }
 
 // A wave owns 32 rows: delta, then dQ^T = sum over keys of K^T dS^T.
@@ -54,7 +69,7 @@ __global__ __launch_bounds__(256) void attn_grad_q(AttnGrad a, int64_t slots) {
         load_row<DP>(dO, a.g.d_o, t * a.g.do_row + head * a.g.do_head, a.d, ok);
         delta = add_halves(dot_row<T>(o, dO, DP / 16));
         lse2 = ok ? a.lse[head * a.tq + t] * kLog2e : 0.0f;
-        if (ok && h == 0) a.delta[head * a.tq + t] = delta;
+        put_stat(a, head * a.tq + t, lse2, delta, ok);
     }
     load_row<DP>(q, a.q, t * a.q_row + head * a.q_head, a.d, ok);
     const int64_t last_row = tile * 32 + 31 < rows ? tile * 32 + 31 : rows - 1;
@@ -146,8 +161,9 @@ __global__ __launch_bounds__(256) void attn_grad_kv(AttnGrad a, int64_t slots) {
             *(uint4v *)(ot + Tile<DP>::at(lane & 31, 2 * c + h)) = dO[c];
         }
         if (h == 0) {
-            stat[lane] = rok ? a.lse[head * a.tq + t] * kLog2e : 0.0f;
-            stat[32 + lane] = rok ? a.delta[head * a.tq + t] : 0.0f;
+            const int64_t n = a.tq * a.hq, at = rok ? head * a.tq + t : n;
+            stat[lane] = a.stat[at];
+            stat[32 + lane] = a.stat[n + 1 + at];
             ((int *)stat)[64 + lane] = rok ? qi + p.lk - p.lq : -1;
         }
         float16v s = {}, dp = {};
@@ -184,16 +200,303 @@ __global__ __launch_bounds__(256) void attn_grad_kv(AttnGrad a, int64_t slots) {
     store_row<T, DP>(a.g.dv, kr * a.g.dv_row + hk * a.g.dv_head, dv, 1.0f, a.d, ok);
 }
 
+// Long sequences, rows: a block of WAVES waves owns 32 rows a wave of one key
+// head; keys and values pass through LDS 64 at a time, as in the forward.
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, int64_t slots) {
+    typedef KeyTiles<DP, 64, WAVES> Keys;
+    constexpr int KB = 64, ROWS = WAVES * 32, STRIDE = Keys::STRIDE;
+    __shared__ __align__(256) unsigned char lds[2 * Keys::BYTES];
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+    const int64_t slot = blockIdx.x / a.hkv;
+    const int hk = (int)(blockIdx.x % a.hkv);
+    if (slot >= slots) return;
+    const int b = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, ROWS, slot);
+    const Place p = place_of(a, b);
+    const int64_t rows = (int64_t)p.lq * a.G;
+    const int64_t tile = (rows + ROWS - 1) / ROWS - 1 - (slot - slot_of(p.q0, a.G, ROWS, b));
+    if (tile < 0 || tile * ROWS >= rows) return;
+    const int64_t row = tile * ROWS + wave * 32 + (lane & 31);
+    const bool ok = row < rows;
+    const int qi = ok ? (int)(row / a.G) : 0, g = ok ? (int)(row % a.G) : 0;
+    const int head = hk * a.G + g;
+    const int lim = ok ? qi + p.lk - p.lq : -1;
+    const int64_t t = p.q0 + qi;
+    uint4v q[DP / 16], dO[DP / 16];
+    float delta, lse2;
+    load_row<DP>(dO, a.g.d_o, t * a.g.do_row + head * a.g.do_head, a.d, ok);
+    load_row<DP>(q, a.o, t * a.o_row + head * a.o_head, a.d, ok);
+    delta = add_halves(dot_row<T>(q, dO, DP / 16));
+    lse2 = ok ? a.lse[head * a.tq + t] * kLog2e : 0.0f;
+    put_stat(a, head * a.tq + t, lse2, delta, ok);
+    load_row<DP>(q, a.q, t * a.q_row + head * a.q_head, a.d, ok);
+    auto seen_by = [&](int64_t r) {
+        return (int)((r < rows ? r : rows - 1) / a.G) + p.lk - p.lq + 1;
+    };
+    const int keys = seen_by(tile * ROWS + ROWS - 1);
+    const int64_t w0 = tile * ROWS + wave * 32;
+    const int wave_keys = w0 < rows ? seen_by(w0 + 31) : 0;
+    const int all_keys = w0 + 31 < rows ? seen_by(w0) : 0;
+    const Keys tiles(a, p, hk, keys);
+    const uint32_t lds0 = lds_address(lds);
+    const typename Tile<DP>::Rows kr = Tile<DP>::rows(lds0);
+    const typename Tile<DP>::Columns kc_ = Tile<DP>::columns(lds0);
+
+    float16v dq[DP / 32] = {};
+    auto work = [&](auto buf, int k0) {
+        constexpr uint32_t B = decltype(buf)::value * Keys::BYTES, V = B + Keys::BYTES / 2;
+        wait_copies<0>();
+        block_barrier();
+        if (k0 + KB < keys) tiles.copy(k0 + KB, lds0 + (Keys::BYTES - B));
+        if (k0 >= wave_keys) return;
+        const bool edge = k0 + KB > all_keys;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float16v s = {}, dp = {};
+#pragma unroll
+            for (int c = 0; c < DP / 16; c++) {
+                s = T::mfma(Tile<DP>::row(kr.c[c], B + u * 32 * STRIDE), q[c], s);
+                dp = T::mfma(Tile<DP>::row(kr.c[c], V + u * 32 * STRIDE), dO[c], dp);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float pr = exp2_fast(__builtin_fmaf(s[r], a.c, -lse2));
+                dp[r] = pr * (dp[r] - delta);
+            }
+            if (edge)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (k0 + u * 32 + 8 * (r / 4) + 4 * h + r % 4 > lim) dp[r] = 0.0f;
+#pragma unroll
+            for (int kc = 0; kc < 2; kc++) {
+                uint4v pb;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    pb[j] = T::pack(dp[8 * kc + 2 * j], dp[8 * kc + 2 * j + 1]);
+#pragma unroll
+                for (int dt = 0; dt < DP / 32; dt++)
+                    dq[dt] = T::mfma(Tile<DP>::transposed(kc_, dt, B + (u * 32 + kc * 16) * STRIDE),
+                                     pb, dq[dt]);
+            }
+        }
+    };
+    if (keys > 0) tiles.copy(0, lds0);
+    for (int k0 = 0; k0 < keys; k0 += 2 * KB) {
+        work(Const<0>{}, k0);
+        if (k0 + KB < keys) work(Const<1>{}, k0 + KB);
+    }
+    store_row<T, DP>(a.g.dq, t * a.g.dq_row + head * a.g.dq_head, dq, a.scale, a.d, ok);
+}
+
+// Long sequences, keys: a block owns 128 keys of one key head, a wave 32 of them
+// and every other tile of 32 rows; a wave has both gradients of its keys and the
+// keys in registers and their values in LDS (registers for those too would
+// spill). The two waves that share keys add up at the end: with four waves a
+// block's longest run over the rows would last twice as long, with 256 keys a
+// block too few blocks would be left to share the work out (5 sequences of 700 to
+// 4,801: half the compute units idle). Rows pass through LDS 64 at a time,
+// copied there past the registers one tile ahead of their use. Rows beyond the
+// last repeat it with lse +inf, which makes their P and dS 0.
+template <typename T, int DP>
+__global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int64_t slots) {
+    constexpr int RB = 64, KEYS = 128, STRIDE = Tile<DP>::stride * 2;         // bytes
+    constexpr int PER = RB * STRIDE / 1024;             // copies of 1 KB a tile of q or do
+    constexpr int COPIES = 2 * PER / 8;                 // of a wave
+    constexpr uint32_t TILE = RB * STRIDE, BUF = 2 * TILE + 512;   // q, do, lse and delta
+    constexpr uint32_t BYTES = 2 * BUF + KEYS * STRIDE, SUMS = 4 * 2 * 32 * DP * 4;
+    __shared__ __align__(256) unsigned char lds[BYTES > SUMS ? BYTES : SUMS];
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kx = wave & 3, rx = wave >> 2;
+    const int64_t slot = blockIdx.x / a.hkv;
+    const int hk = (int)(blockIdx.x % a.hkv);
+    if (slot >= slots) return;
+    const int b = find_sequence(a.cu_k, a.n_seq, a.tk, 1, KEYS, slot);
+    const int64_t s0 = offset_at(a.cu_k, b, a.tk);
+    const int64_t s1 = b >= a.n_seq ? a.tk : clamp64(a.cu_k[b + 1], s0, a.tk);
+    const int64_t tile = slot - slot_of(s0, 1, KEYS, b);
+    if (tile < 0 || tile * KEYS >= s1 - s0) return;
+    const Place p = b >= a.n_seq ? Place{0, s0, 0, 0} : place_of(a, b);
+    const int base = (int)(s0 - p.k0);                  // key number of the segment's first row
+    const int key0 = (int)(tile * KEYS) + base;         // of the block
+    const int wkey0 = key0 + kx * 32;                   // of the wave
+    const int key = wkey0 + (lane & 31);
+    const bool live = key >= 0 && key < p.lk;
+    uint4v k[DP / 16];
+    float16v dk[DP / 32] = {}, dv[DP / 32] = {};
+    load_row<DP>(k, a.k, (p.k0 + key) * a.k_row + hk * a.k_head, a.d, live);
+    uint16_t *vl = (uint16_t *)(lds + 2 * BUF) + kx * 32 * Tile<DP>::stride;
+    if (rx == 0) {
+        uint4v v[DP / 16];
+        load_row<DP>(v, a.v, (p.k0 + key) * a.v_row + hk * a.v_head, a.d, live);
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++)
+            *(uint4v *)(vl + Tile<DP>::at(lane & 31, 2 * c + h)) = v[c];
+    }
+    const int rows = key0 < p.lk ? p.lq * a.G : 0;
+    const int shift = p.lk - p.lq;
+    auto first_row = [&](int key) {      // of the tile of 32 with a row that sees the key
+        return (int)((int64_t)(key - shift > 0 ? key - shift : 0) * a.G / 32 * 32);
+    };
+    const int start = first_row(key0);
+    const int wave_start = wkey0 < p.lk ? first_row(wkey0) : rows;
+    const uint32_t lds0 = lds_address(lds);
+    // One tile's copies: this wave's share of q and do, and two waves' statistics.
+    // When the group's heads divide 32 rows, a whole tile's rows lie at the same
+    // lane offsets from an address of the wave.
+    const int row_l = wave % PER * (1024 / STRIDE) + lane * 16 / STRIDE;    // in the tile
+    const int ch_l = (lane * 16 % STRIDE / 16) ^ Tile<DP>::swz(row_l);
+    const int col_l = ch_l * 8 < a.d ? ch_l * 8 : 0;
+    const int64_t q_most = a.q_row * 64 + a.q_head * a.G, o_most = a.g.do_row * 64 + a.g.do_head * a.G;
+    const bool plain = 32 % a.G == 0 && a.q_row >= 0 && a.q_head >= 0 && a.g.do_row >= 0 &&
+                       a.g.do_head >= 0 && q_most < 1 << 30 && o_most < 1 << 30;
+    const uint32_t q_off = 2 * (uint32_t)(row_l / a.G * a.q_row + row_l % a.G * a.q_head + col_l);
+    const uint32_t o_off = 2 * (uint32_t)(row_l / a.G * a.g.do_row + row_l % a.G * a.g.do_head + col_l);
+    const uint16_t *q0p = (const uint16_t *)a.q + p.q0 * a.q_row + (int64_t)hk * a.G * a.q_head;
+    const uint16_t *o0p = (const uint16_t *)a.g.d_o + p.q0 * a.g.do_row +
+                          (int64_t)hk * a.G * a.g.do_head;
+    auto copy = [&](int r0, uint32_t buf) {
+        const bool whole = plain && r0 + RB <= rows;
+#pragma unroll
+        for (int x = 0; x < COPIES; x++) {
+            const int idx = wave + x * 8;
+            const bool is_q = idx < PER;
+            const int more = (idx % PER - wave % PER) * (1024 / STRIDE);    // 0 or 32 rows
+            const uint16_t *from = is_q ? q0p : o0p;
+            const int64_t row_step = is_q ? a.q_row : a.g.do_row;
+            if (whole) {
+                copy_to_lds16(from + (r0 + more) / a.G * row_step, is_q ? q_off : o_off,
+                              buf + idx * 1024);
+            } else {
+                const int row = min(r0 + more + row_l, rows - 1);
+                copy_to_lds16(from + row / a.G * row_step +
+                                  row % a.G * (is_q ? a.q_head : a.g.do_head) + col_l,
+                              buf + idx * 1024);
+            }
+        }
+        if (kx == 0) {
+            const int row = r0 + rx * 32 + (lane & 31);
+            const int64_t at = ((int64_t)(hk * a.G) + row % a.G) * a.tq + p.q0 + row / a.G;
+            // past the rows: the workspace's +inf and 0
+            copy_to_lds4(a.stat + (row < rows ? at : a.tq * a.hq) + h * (a.tq * a.hq + 1),
+                         buf + 2 * TILE + rx * 256);
+        }
+    };
+    const typename Tile<DP>::Rows qr = Tile<DP>::rows(lds0 + rx * (TILE / 2));
+    const typename Tile<DP>::Columns qc = Tile<DP>::columns(lds0 + rx * (TILE / 2));
+    // from a row's address in q to the same row and column of this wave's values
+    const uint32_t to_v = lds_address(vl) - (lds0 + rx * (TILE / 2));
+    const uint32_t stat = lds0 + 2 * TILE + rx * 256 + 16 * h;
+    auto work = [&](auto buf, int r0) {
+        constexpr uint32_t B = decltype(buf)::value * BUF;
+        // this tile has landed for every wave, and none reads the one before it
+        wait_copies<0>();
+        block_barrier();
+        if (r0 + RB < rows) copy(r0 + RB, lds0 + (BUF - B));
+        const int rw = r0 + rx * 32;                     // this wave's rows
+        if (rw < wave_start || rw >= rows) return;
+        float16v s = {}, dp = {};
+        uint32_t vd = to_v;
+        asm volatile("" : "+s"(vd));     // V's addresses are formed here, not kept
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) s = T::mfma(Tile<DP>::row(qr.c[c], B), k[c], s);
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++)
+            dp = T::mfma(Tile<DP>::row(qr.c[c], B + TILE), Tile<DP>::row(qr.c[c] + vd, 0), dp);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4v l4 = __builtin_bit_cast(float4v, Tile<DP>::row(stat, B + 32 * i));
+            const float4v e4 = __builtin_bit_cast(float4v, Tile<DP>::row(stat, B + 128 + 32 * i));
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int r = 4 * i + j;
+                const float pr = exp2_fast(__builtin_fmaf(s[r], a.c, -l4[j]));
+                s[r] = pr;
+                dp[r] = pr * (dp[r] - e4[j]);
+            }
+        }
+        // rows before the keys' last do not all see them (and rows that see no
+        // key at all have lse -inf)
+        if (rw / a.G + shift < wkey0 + 31)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (key > (rw + 8 * (r / 4) + 4 * h + r % 4) / a.G + shift) s[r] = dp[r] = 0.0f;
+#pragma unroll
+        for (int kc = 0; kc < 2; kc++) {
+            uint4v pb, db;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                pb[j] = T::pack(s[8 * kc + 2 * j], s[8 * kc + 2 * j + 1]);
+                db[j] = T::pack(dp[8 * kc + 2 * j], dp[8 * kc + 2 * j + 1]);
+            }
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; dt++) {
+                dv[dt] = T::mfma(Tile<DP>::transposed(qc, dt, B + TILE + kc * 16 * STRIDE), pb, dv[dt]);
+                dk[dt] = T::mfma(Tile<DP>::transposed(qc, dt, B + kc * 16 * STRIDE), db, dk[dt]);
+            }
+        }
+    };
+    if (start < rows) copy(start, lds0);
+    for (int r0 = start; r0 < rows; r0 += 2 * RB) {
+        work(Const<0>{}, r0);
+        if (r0 + RB < rows) work(Const<1>{}, r0 + RB);
+    }
+    // no copy is on its way and no wave reads a tile: the LDS takes the second
+    // halves' sums
+    wait_copies<0>();
+    block_barrier();
+    float4v *sums = (float4v *)lds + kx * (2 * DP / 8 * 64) + lane;
+    if (rx == 1)
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; dt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float4v x = {dk[dt][4 * j], dk[dt][4 * j + 1], dk[dt][4 * j + 2],
+                                   dk[dt][4 * j + 3]};
+                const float4v y = {dv[dt][4 * j], dv[dt][4 * j + 1], dv[dt][4 * j + 2],
+                                   dv[dt][4 * j + 3]};
+                sums[(dt * 4 + j) * 64] = x;
+                sums[(DP / 8 + dt * 4 + j) * 64] = y;
+            }
+    __syncthreads();
+    if (rx == 1) return;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; dt++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float4v x = sums[(dt * 4 + j) * 64], y = sums[(DP / 8 + dt * 4 + j) * 64];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                // a column that is not a key's: zeros
+                dk[dt][4 * j + e] = live ? dk[dt][4 * j + e] + x[e] : 0.0f;
+                dv[dt][4 * j + e] = live ? dv[dt][4 * j + e] + y[e] : 0.0f;
+            }
+        }
+    const int64_t kr = s0 + tile * KEYS + kx * 32 + (lane & 31);
+    store_row<T, DP>(a.g.dk, kr * a.g.dk_row + hk * a.g.dk_head, dk, a.scale, a.d, kr < s1);
+    store_row<T, DP>(a.g.dv, kr * a.g.dv_row + hk * a.g.dv_head, dv, 1.0f, a.d, kr < s1);
+}
+
 template <typename T, int DP>
 int launch_grad(const AttnGrad &a, hipStream_t s) {
+    const int64_t n = a.n_seq ? a.n_seq : 1;
     if (a.tq) {
-        const int64_t slots = slot_of(a.tq, a.G, 32, a.n_seq) + 1;
-        attn_grad_q<T, DP><<<dim3((unsigned)((slots * a.hkv + 3) / 4)), 256, 0, s>>>(a, slots);
+        if (a.tq * a.G >= 256 * n) {
+            const int64_t slots = slot_of(a.tq, a.G, 256, a.n_seq) + 1;
+            attn_grad_q_tiles<T, DP, 8><<<dim3((unsigned)(slots * a.hkv)), 512, 0, s>>>(a, slots);
+        } else {
+            const int64_t slots = slot_of(a.tq, a.G, 32, a.n_seq) + 1;
+            attn_grad_q<T, DP><<<dim3((unsigned)((slots * a.hkv + 3) / 4)), 256, 0, s>>>(a, slots);
+        }
         if (hipGetLastError() != hipSuccess) return CO_ERR_CUDA;
     }
     if (a.tk) {
-        const int64_t slots = slot_of(a.tk, 1, 32, a.n_seq) + 1;
-        attn_grad_kv<T, DP><<<dim3((unsigned)((slots * a.hkv + 3) / 4)), 256, 0, s>>>(a, slots);
+        if (a.tk >= 128 * n) {
+            const int64_t slots = slot_of(a.tk, 1, 128, a.n_seq) + 1;
+            attn_grad_kv_tiles<T, DP><<<dim3((unsigned)(slots * a.hkv)), 512, 0, s>>>(a, slots);
+        } else {
+            const int64_t slots = slot_of(a.tk, 1, 32, a.n_seq) + 1;
+            attn_grad_kv<T, DP><<<dim3((unsigned)((slots * a.hkv + 3) / 4)), 256, 0, s>>>(a, slots);
+        }
     }
     return launch_status();
 }
@@ -214,7 +517,7 @@ int check_attention_data(const SeqAttention *a);
 
 extern "C" int64_t seq_attention_grad_workspace(const SeqAttention *a) {
     const int rc = seq::check_attention(a);
-    return rc == CO_OK ? 4 * a->hq * a->tq : (rc > 0 ? -rc : rc);
+    return rc == CO_OK ? 8 * (a->hq * a->tq + 1) : (rc > 0 ? -rc : rc);
 }
 
 extern "C" int seq_attention_grad(const SeqAttention *sa, const SeqAttentionGrad *g,
@@ -233,13 +536,13 @@ extern "C" int seq_attention_grad(const SeqAttention *sa, const SeqAttentionGrad
     if ((g->do_row | g->do_head | g->dq_row | g->dq_head | g->dk_row | g->dk_head | g->dv_row |
          g->dv_head) & 7)
         return CO_ERR_DATA;
-    if (sa->workspace_bytes < 4 * sa->hq * sa->tq) return CO_ERR_DATA;
+    if (sa->workspace_bytes < 8 * (sa->hq * sa->tq + 1)) return CO_ERR_DATA;
     seq::AttnGrad a;
     static_cast<SeqAttention &>(a) = *sa;
     a.G = a.hq / a.hkv;
     a.c = a.scale * seq::kLog2e;
     a.g = *g;
-    a.delta = (float *)sa->workspace;
+    a.stat = (float *)sa->workspace;
     hipStream_t s = (hipStream_t)stream;
     return a.dtype == SEQ_BF16 ? seq::launch_grad_head<seq::Bf16>(a, s)
                                : seq::launch_grad_head<seq::Fp16>(a, s);

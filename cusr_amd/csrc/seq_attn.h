@@ -93,6 +93,40 @@ __device__ inline Place place_of(const Attn &a, int b) {
     return p;
 }
 
+typedef __attribute__((address_space(3))) const uint16_t *lds_ptr;
+typedef __attribute__((address_space(3))) const uint4v *lds_ptr4;
+__device__ inline uint32_t lds_address(const void *p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+
+// Copies from memory to LDS past the registers: 16 (or 4) bytes a lane, to
+// `to` + 16 (4) lane; `to` is the same for the wave. The second form adds a
+// lane's offset to an address of the wave, which costs no vector instruction.
+// Copies count as loads: wait_copies<N> waits until at most the wave's last N
+// loads are on their way. Written in assembly because the compiler, which cannot
+// tell the buffers apart, would wait for the newest copy before every LDS read;
+// there is no output register, and its own waits only grow longer by the extra
+// loads.
+__device__ inline void copy_to_lds16(const void *from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
+}
+__device__ inline void copy_to_lds16(const void *wave_from, uint32_t lane_offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(lane_offset), "s"(wave_from)
+                 : "memory");
+}
+__device__ inline void copy_to_lds4(const void *from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
+}
+template <int N> __device__ inline void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
+}
+
+// Barrier of the block that no memory access of the program moves across.
+__device__ inline void block_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
 // 16-bit tile rows in LDS: DP elements a row (96 padded to 128), 16-byte
 // chunks permuted within the row so that the transposed reads, which take four
 // rows of 32 bytes at a time, and the row reads, 32 rows of one chunk, spread
@@ -118,10 +152,94 @@ template <int DP> struct Tile {
         uint4v v = {lo[0], lo[1], hi[0], hi[1]};
         return v;
     }
+    // The same two reads by LDS byte address, for the inner loops. A lane keeps
+    // one address for each column (rows) or 32 columns (transposed); rows and
+    // buffers are constants in the instruction, so a read costs no arithmetic.
+    // `at` is a multiple of 16 rows in bytes, and a tile starts on 256 bytes.
+    struct Rows { uint32_t c[DP / 16]; };
+    static __device__ Rows rows(uint32_t tile) {
+        const int lane = threadIdx.x & 63;
+        Rows r;
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) r.c[c] = tile + 2 * at(lane & 31, 2 * c + (lane >> 5));
+        return r;
+    }
+    static __device__ uint4v row(uint32_t address, uint32_t at) {
+        return *(lds_ptr4)(uintptr_t)(address + at);
+    }
+    struct Columns { uint32_t lo[DP / 32], hi[DP / 32]; };
+    static __device__ Columns columns(uint32_t tile) {
+        const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15;
+        Columns x;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; dt++) {
+            const int col = dt * 32 + (lane & 16) + (i & 3) * 4, r = 4 * h + (i >> 2);
+            x.lo[dt] = tile + 2 * (at(r, col >> 3) + (col & 7));
+            x.hi[dt] = tile + 2 * (at(r + 8, col >> 3) + (col & 7));
+        }
+        return x;
+    }
+    static __device__ uint4v transposed(const Columns &x, int dt, uint32_t at) {
+        const uint2v a = read_transposed((lds_ptr)(uintptr_t)(x.lo[dt] + at));
+        const uint2v b = read_transposed((lds_ptr)(uintptr_t)(x.hi[dt] + at));
+        uint4v v = {a[0], a[1], b[0], b[1]};
+        return v;
+    }
     // left operand over the columns: row r0 + lane % 32, columns 16 c + 8h..+7
     static __device__ uint4v row(const uint16_t *t, int r0, int c) {
         const int lane = threadIdx.x & 63;
         return *(const uint4v *)(t + at(r0 + (lane & 31), 2 * c + (lane >> 5)));
+    }
+};
+
+// Tiles of KB keys and their values on their way to LDS, for a block of WAVES
+// waves. Whole tiles take their addresses from the wave's registers alone; the
+// last one repeats its last key.
+template <int DP, int KB, int WAVES> struct KeyTiles {
+    static constexpr int STRIDE = Tile<DP>::stride * 2;          // bytes of a row in LDS
+    static constexpr int PER = KB * STRIDE / 1024;               // copies of k, and of v
+    static constexpr int ROWS = 1024 / STRIDE;                   // rows of a copy
+    static constexpr int COPIES = 2 * PER / WAVES;               // of a wave
+    static_assert(COPIES >= 1 && 2 * PER % WAVES == 0 && (PER % WAVES == 0 || PER * 2 == WAVES), "");
+    static constexpr uint32_t BYTES = 2 * KB * STRIDE;           // k, then v
+    const char *k, *v;
+    int64_t k_step, v_step;
+    int keys, wave, row, col;                                    // this lane's first row, column
+    uint32_t k_off, v_off;
+    bool plain;
+
+    __device__ KeyTiles(const Attn &a, const Place &p, int hk, int keys_) {
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int lane = threadIdx.x & 63;
+        k = (const char *)a.k + 2 * (p.k0 * a.k_row + hk * a.k_head);
+        v = (const char *)a.v + 2 * (p.k0 * a.v_row + hk * a.v_head);
+        k_step = 2 * a.k_row;
+        v_step = 2 * a.v_row;
+        keys = keys_;
+        row = wave % PER * ROWS + lane * 16 / STRIDE;
+        const int ch = (lane * 16 % STRIDE / 16) ^ Tile<DP>::swz(row);
+        col = ch * 8 < a.d ? ch * 16 : 0;
+        // a lane's offset within a tile has 32 bits
+        plain = k_step >= 0 && k_step < 1 << 25 && v_step >= 0 && v_step < 1 << 25;
+        k_off = (uint32_t)(row * k_step) + col;
+        v_off = (uint32_t)(row * v_step) + col;
+    }
+    __device__ void copy(int k0, uint32_t to) const {
+#pragma unroll
+        for (int x = 0; x < COPIES; x++) {
+            const int idx = wave + x * WAVES, part = idx % PER;
+            const bool is_k = idx < PER;
+            const int r = k0 + (part - wave % PER) * ROWS;
+            const uint32_t at = to + idx * 1024;
+            const char *from = is_k ? k : v;
+            const int64_t step = is_k ? k_step : v_step;
+            if (plain && k0 + KB <= keys) {
+                copy_to_lds16(from + r * step, is_k ? k_off : v_off, at);
+            } else {
+                const int mine = r + row < keys ? r + row : keys - 1;
+                copy_to_lds16(from + mine * step + col, at);
+            }
+        }
     }
 };
 

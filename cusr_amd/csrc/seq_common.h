@@ -21,6 +21,8 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
+template <int N> struct Const { static constexpr int value = N; };
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -92,9 +94,12 @@ __device__ inline void wave_sync() {
 // 4 x 16 block of 16-bit values in LDS, transposed on the way to registers:
 // lane i of each group of 16 gives the address of row i / 4, columns
 // 4 (i % 4) .. + 3, and gets column i, rows 0..3.
-__device__ inline uint2v read_transposed(const uint16_t *p) {
+__device__ inline uint2v read_transposed(__attribute__((address_space(3))) const uint16_t *p) {
     typedef __attribute__((address_space(3))) short4v *lds4;
     return __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p));
+}
+__device__ inline uint2v read_transposed(const uint16_t *p) {
+    return read_transposed((__attribute__((address_space(3))) const uint16_t *)p);
 }
 
 inline int launch_status() {
