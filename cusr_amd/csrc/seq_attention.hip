@@ -133,6 +133,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int64_t slot
     const int wave_keys = w0 < rows ? seen_by(w0 + 31) : 0;
     const int all_keys = w0 + 31 < rows ? seen_by(w0) : 0;
     const Keys tiles(a, p, hk, keys);
+    landed(q);
     const uint32_t lds0 = lds_address(lds);
     const typename Tile<DP>::Rows kr = Tile<DP>::rows(lds0);
     const typename Tile<DP>::Columns vc = Tile<DP>::columns(lds0 + Keys::BYTES / 2);
@@ -158,10 +159,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int64_t slot
 #pragma unroll
                 for (int r = 0; r < 16; r++)
                     if (k0 + u * 32 + 8 * (r / 4) + 4 * h + r % 4 > lim) s[u][r] = neg_inf();
-        float mx = fmaxf(max3(s[0][0], s[0][1], s[1][0]), s[1][1]);
+        float top[4] = {s[0][0], s[0][8], s[1][0], s[1][8]};     // four chains of eight
 #pragma unroll
-        for (int r = 2; r < 16; r += 2)
-            mx = max3(max3(mx, s[0][r], s[0][r + 1]), s[1][r], s[1][r + 1]);
+        for (int r = 1; r < 7; r += 2)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                top[i] = max3(top[i], s[i / 2][i % 2 * 8 + r], s[i / 2][i % 2 * 8 + r + 1]);
+        float mx = max3(max3(top[0], top[1], s[0][7]), max3(top[2], top[3], s[1][7]),
+                        fmaxf(s[0][15], s[1][15]));
         mx = max_halves(mx);
         if (__any((mx - m) * a.c > 8.0f)) {
             const float mn = fmaxf(m, mx), m0 = mn == neg_inf() ? 0.0f : mn;

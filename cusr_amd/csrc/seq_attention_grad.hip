@@ -238,6 +238,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, i
     const int wave_keys = w0 < rows ? seen_by(w0 + 31) : 0;
     const int all_keys = w0 + 31 < rows ? seen_by(w0) : 0;
     const Keys tiles(a, p, hk, keys);
+    landed(q);
+    landed(dO);
     const uint32_t lds0 = lds_address(lds);
     const typename Tile<DP>::Rows kr = Tile<DP>::rows(lds0);
     const typename Tile<DP>::Columns kc_ = Tile<DP>::columns(lds0);
@@ -303,7 +305,7 @@ __global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int64_t
     constexpr int PER = RB * STRIDE / 1024;             // copies of 1 KB a tile of q or do
     constexpr int COPIES = 2 * PER / 8;                 // of a wave
     constexpr uint32_t TILE = RB * STRIDE, BUF = 2 * TILE + 512;   // q, do, lse and delta
-    constexpr uint32_t BYTES = 2 * BUF + KEYS * STRIDE, SUMS = 4 * 2 * 32 * DP * 4;
+    constexpr uint32_t BYTES = 2 * BUF + 2 * KEYS * STRIDE, SUMS = 4 * 2 * 32 * DP * 4;
     __shared__ __align__(256) unsigned char lds[BYTES > SUMS ? BYTES : SUMS];
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kx = wave & 3, rx = wave >> 2;
@@ -321,16 +323,17 @@ __global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int64_t
     const int wkey0 = key0 + kx * 32;                   // of the wave
     const int key = wkey0 + (lane & 31);
     const bool live = key >= 0 && key < p.lk;
-    uint4v k[DP / 16];
     float16v dk[DP / 32] = {}, dv[DP / 32] = {};
-    load_row<DP>(k, a.k, (p.k0 + key) * a.k_row + hk * a.k_head, a.d, live);
-    uint16_t *vl = (uint16_t *)(lds + 2 * BUF) + kx * 32 * Tile<DP>::stride;
-    if (rx == 0) {
-        uint4v v[DP / 16];
-        load_row<DP>(v, a.v, (p.k0 + key) * a.v_row + hk * a.v_head, a.d, live);
+    // this wave's keys, and 128 rows further their values
+    uint16_t *kl = (uint16_t *)(lds + 2 * BUF) + kx * 32 * Tile<DP>::stride;
+    {
+        uint4v x[DP / 16];               // one of the two waves brings the keys, one the values
+        const void *from = rx ? a.v : a.k;
+        const int64_t step = rx ? a.v_row : a.k_row, head = rx ? a.v_head : a.k_head;
+        load_row<DP>(x, from, (p.k0 + key) * step + hk * head, a.d, live);
 #pragma unroll
         for (int c = 0; c < DP / 16; c++)
-            *(uint4v *)(vl + Tile<DP>::at(lane & 31, 2 * c + h)) = v[c];
+            *(uint4v *)(kl + rx * KEYS * Tile<DP>::stride + Tile<DP>::at(lane & 31, 2 * c + h)) = x[c];
     }
     const int rows = key0 < p.lk ? p.lq * a.G : 0;
     const int shift = p.lk - p.lq;
@@ -355,21 +358,23 @@ __global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int64_t
     const uint16_t *o0p = (const uint16_t *)a.g.d_o + p.q0 * a.g.do_row +
                           (int64_t)hk * a.G * a.g.do_head;
     auto copy = [&](int r0, uint32_t buf) {
-        const bool whole = plain && r0 + RB <= rows;
+        if (plain && r0 + RB <= rows) {
 #pragma unroll
-        for (int x = 0; x < COPIES; x++) {
-            const int idx = wave + x * 8;
-            const bool is_q = idx < PER;
-            const int more = (idx % PER - wave % PER) * (1024 / STRIDE);    // 0 or 32 rows
-            const uint16_t *from = is_q ? q0p : o0p;
-            const int64_t row_step = is_q ? a.q_row : a.g.do_row;
-            if (whole) {
-                copy_to_lds16(from + (r0 + more) / a.G * row_step, is_q ? q_off : o_off,
-                              buf + idx * 1024);
-            } else {
-                const int row = min(r0 + more + row_l, rows - 1);
-                copy_to_lds16(from + row / a.G * row_step +
-                                  row % a.G * (is_q ? a.q_head : a.g.do_head) + col_l,
+            for (int x = 0; x < COPIES; x++) {
+                const int idx = wave + x * 8;
+                const int t = (r0 + (idx % PER - wave % PER) * (1024 / STRIDE)) / a.G;
+                copy_to_lds16(idx < PER ? q0p + t * a.q_row : o0p + t * a.g.do_row,
+                              idx < PER ? q_off : o_off, buf + idx * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < COPIES; x++) {
+                const int idx = wave + x * 8;
+                const int row =
+                    min(r0 + (idx % PER - wave % PER) * (1024 / STRIDE) + row_l, rows - 1);
+                const int t = row / a.G, g = row % a.G;
+                copy_to_lds16((idx < PER ? q0p + t * a.q_row + g * a.q_head
+                                         : o0p + t * a.g.do_row + g * a.g.do_head) + col_l,
                               buf + idx * 1024);
             }
         }
@@ -383,25 +388,26 @@ __global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int64_t
     };
     const typename Tile<DP>::Rows qr = Tile<DP>::rows(lds0 + rx * (TILE / 2));
     const typename Tile<DP>::Columns qc = Tile<DP>::columns(lds0 + rx * (TILE / 2));
-    // from a row's address in q to the same row and column of this wave's values
-    const uint32_t to_v = lds_address(vl) - (lds0 + rx * (TILE / 2));
+    // from a row's address in q to the same row and column of this wave's keys
+    const uint32_t to_k = lds_address(kl) - (lds0 + rx * (TILE / 2));
     const uint32_t stat = lds0 + 2 * TILE + rx * 256 + 16 * h;
     auto work = [&](auto buf, int r0) {
         constexpr uint32_t B = decltype(buf)::value * BUF;
         // this tile has landed for every wave, and none reads the one before it
         wait_copies<0>();
         block_barrier();
-        if (r0 + RB < rows) copy(r0 + RB, lds0 + (BUF - B));
+        if (r0 > start) copy(r0 - RB, lds0 + (BUF - B));
         const int rw = r0 + rx * 32;                     // this wave's rows
         if (rw < wave_start || rw >= rows) return;
         float16v s = {}, dp = {};
-        uint32_t vd = to_v;
-        asm volatile("" : "+s"(vd));     // V's addresses are formed here, not kept
+        uint32_t kd = to_k;
+        asm volatile("" : "+s"(kd));     // the keys' addresses are formed here, not kept
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) s = T::mfma(Tile<DP>::row(qr.c[c], B), k[c], s);
-#pragma unroll
-        for (int c = 0; c < DP / 16; c++)
-            dp = T::mfma(Tile<DP>::row(qr.c[c], B + TILE), Tile<DP>::row(qr.c[c] + vd, 0), dp);
+        for (int c = 0; c < DP / 16; c++) {
+            const uint32_t ka = qr.c[c] + kd;
+            s = T::mfma(Tile<DP>::row(qr.c[c], B), Tile<DP>::row(ka, 0), s);
+            dp = T::mfma(Tile<DP>::row(qr.c[c], B + TILE), Tile<DP>::row(ka, KEYS * STRIDE), dp);
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float4v l4 = __builtin_bit_cast(float4v, Tile<DP>::row(stat, B + 32 * i));
@@ -416,10 +422,15 @@ __global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int64_t
         }
         // rows before the keys' last do not all see them (and rows that see no
         // key at all have lse -inf)
-        if (rw / a.G + shift < wkey0 + 31)
+        if (rw / a.G + shift < wkey0 + 31) {
+            const float inv = 1.0f / (float)a.G;
 #pragma unroll
-            for (int r = 0; r < 16; r++)
-                if (key > (rw + 8 * (r / 4) + 4 * h + r % 4) / a.G + shift) s[r] = dp[r] = 0.0f;
+            for (int r = 0; r < 16; r++) {
+                const int lim = divide(rw + 8 * (r / 4) + 4 * h + r % 4, a.G, inv) + shift;
+                s[r] = key > lim ? 0.0f : s[r];
+                dp[r] = key > lim ? 0.0f : dp[r];
+            }
+        }
 #pragma unroll
         for (int kc = 0; kc < 2; kc++) {
             uint4v pb, db;
@@ -435,10 +446,16 @@ __global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int64_t
             }
         }
     };
-    if (start < rows) copy(start, lds0);
-    for (int r0 = start; r0 < rows; r0 += 2 * RB) {
-        work(Const<0>{}, r0);
-        if (r0 + RB < rows) work(Const<1>{}, r0 + RB);
+    // From the last rows to the first: blocks of one sequence start at rows of
+    // their own but end at the same one, so those that run together read the same
+    // rows at the same time and find them in the L2.
+    const int last = start + (rows - 1 - start) / RB * RB;
+    if (start < rows) {
+        copy(last, lds0);
+        for (int r0 = last; r0 >= start; r0 -= 2 * RB) {
+            work(Const<0>{}, r0);
+            if (r0 - RB >= start) work(Const<1>{}, r0 - RB);
+        }
     }
     // no copy is on its way and no wave reads a tile: the LDS takes the second
     // halves' sums

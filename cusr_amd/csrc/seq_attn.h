@@ -26,6 +26,16 @@ __device__ __host__ inline int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
     return x < lo ? lo : (x > hi ? hi : x);
 }
 
+// x / n for 0 <= x < 2^31, n >= 1, without a branch: the quotient by a float
+// reciprocal `inv` is off by at most a few hundred for large x, so the remainder,
+// taken exactly, corrects it once by its own quotient and once by one.
+__device__ inline int divide(int x, int n, float inv) {
+    int q = (int)((float)x * inv);
+    q += (int)((float)(x - q * n) * inv);
+    const int r = x - q * n;
+    return q + (r >= n) - (r < 0);
+}
+
 // A sequence's place: first query and key row, number of queries and keys.
 struct Place { int64_t q0, k0; int lq, lk; };
 
@@ -124,6 +134,22 @@ template <int N> __device__ inline void wait_copies() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
 }
 
+// Waits here for loads of operands that a loop uses. At their first use the
+// compiler would wait in the loop, each time round, for every copy under way.
+template <int N> __device__ inline void landed(uint4v (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+v"(x[i]));
+}
+// Order of a block of straight code: N times M matrix instructions, then R LDS
+// reads. Left to itself the compiler, short of registers, puts every read right
+// before the product that waits for it.
+template <int N, int M, int R> __device__ inline void interleave() {
+    if constexpr (N > 0) {
+        if constexpr (M > 0) __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+        if constexpr (R > 0) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+        interleave<N - 1, M, R>();
+    }
+}
 // Barrier of the block that no memory access of the program moves across.
 __device__ inline void block_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
@@ -225,20 +251,22 @@ template <int DP, int KB, int WAVES> struct KeyTiles {
         v_off = (uint32_t)(row * v_step) + col;
     }
     __device__ void copy(int k0, uint32_t to) const {
+        const bool whole = plain && k0 + KB <= keys;
+        if (whole) {
+#pragma unroll
+            for (int x = 0; x < COPIES; x++) {
+                const int idx = wave + x * WAVES, r = k0 + (idx % PER - wave % PER) * ROWS;
+                copy_to_lds16(idx < PER ? k + r * k_step : v + r * v_step,
+                              idx < PER ? k_off : v_off, to + idx * 1024);
+            }
+            return;
+        }
 #pragma unroll
         for (int x = 0; x < COPIES; x++) {
-            const int idx = wave + x * WAVES, part = idx % PER;
-            const bool is_k = idx < PER;
-            const int r = k0 + (part - wave % PER) * ROWS;
-            const uint32_t at = to + idx * 1024;
-            const char *from = is_k ? k : v;
-            const int64_t step = is_k ? k_step : v_step;
-            if (plain && k0 + KB <= keys) {
-                copy_to_lds16(from + r * step, is_k ? k_off : v_off, at);
-            } else {
-                const int mine = r + row < keys ? r + row : keys - 1;
-                copy_to_lds16(from + mine * step + col, at);
-            }
+            const int idx = wave + x * WAVES, r = k0 + (idx % PER - wave % PER) * ROWS + row;
+            const int mine = r < keys ? r : keys - 1;
+            copy_to_lds16((idx < PER ? k + mine * k_step : v + mine * v_step) + col,
+                          to + idx * 1024);
         }
     }
 };
