@@ -6,64 +6,61 @@ namespace seq {
 
 // A row's output from its unscaled sum, and its lse. No visible key: l is 0.
 template <typename T, int DP>
-__device__ inline void store_out(const Attn &a, int64_t t, int head, const float16v *o, float m,
+__device__ inline void store_out(const Attn &a, int t, int head, const float16v *o, float m,
                                  float l, bool ok) {
     store_row<T, DP>(a.o, t * a.o_row + head * a.o_head, o, l == 0.0f ? 0.0f : 1.0f / l, a.d, ok);
     if (a.lse && ok && (threadIdx.x & 63) < 32)
         a.lse[head * a.tq + t] = l == 0.0f ? neg_inf() : m * a.scale + logf(l);
 }
 
-// One wave owns a tile of 32 rows of one key head and runs over the keys 32 at
-// a time with a running maximum and sum. K comes straight from memory as the
-// left operand; V passes through the wave's own LDS tile to be transposed.
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_wave(Attn a, int64_t slots) {
-    __shared__ __align__(16) uint16_t lds[4][32 * Tile<DP>::stride];
-    uint16_t *vt = lds[threadIdx.x >> 6];
+// A wave's tile of 32 rows over the keys key0 .. key1-1, 32 at a time with a
+// running maximum and sum. AHEAD: the next 32 keys are loaded while the present
+// ones are worked on, at the price of their registers. K comes straight from memory as the left operand; V passes
+// through the wave's own LDS tile to be transposed.
+struct Row { int t, head; bool ok; };
+template <typename T, int DP, bool AHEAD>
+__device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, int key0, int key1,
+                               uint16_t *vt, float16v *o, float &m, float &l) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    const int64_t item = blockIdx.x * 4ll + (threadIdx.x >> 6);
-    const int64_t slot = item / a.hkv;
-    const int hk = (int)(item % a.hkv);
-    if (slot >= slots) return;
-    const int b = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, 32, slot);
-    const Place p = place_of(a, b);
-    const int64_t tile = slot - slot_of(p.q0, a.G, 32, b);
-    const int64_t rows = (int64_t)p.lq * a.G;
-    if (tile < 0 || tile * 32 >= rows) return;
-    const int64_t row = tile * 32 + (lane & 31);
+    const int rows = p.lq * a.G, row = tile * 32 + (lane & 31);
+    const float inv = 1.0f / (float)a.G;
     const bool ok = row < rows;
-    const int qi = ok ? (int)(row / a.G) : 0, g = ok ? (int)(row % a.G) : 0;
-    const int head = hk * a.G + g;
-    const int lim = ok ? qi + p.lk - p.lq : -1;      // last visible key
-    uint4v q[DP / 16];
+    const int qi = divide(ok ? row : 0, a.G, inv);
+    const int head = hk * a.G + (ok ? row - qi * a.G : 0);
+    const int lim = ok ? qi + p.lk - p.lq : -1;          // last visible key
+    const int seen = divide(min(tile * 32 + 31, rows - 1), a.G, inv) + p.lk - p.lq + 1;
+    const int end = min(key1, seen);
+    const uint16_t *kp = (const uint16_t *)a.k + p.k0 * a.k_row + hk * a.k_head;
+    const uint16_t *vp = (const uint16_t *)a.v + p.k0 * a.v_row + hk * a.v_head;
+    uint4v q[DP / 16], k[DP / 16], v[DP / 16];
+    // keys beyond the last repeat it: their scores are masked
+    auto fetch = [&](int k0) {
+        const int r = min(k0 + (lane & 31), end - 1);
+        load_row<DP>(k, kp, r * a.k_row, a.d, true);
+        load_row<DP>(v, vp, r * a.v_row, a.d, true);
+    };
+    if (key0 < end) fetch(key0);
     load_row<DP>(q, a.q, (p.q0 + qi) * a.q_row + head * a.q_head, a.d, ok);
-
-    const int64_t last_row = tile * 32 + 31 < rows ? tile * 32 + 31 : rows - 1;
-    const int keys = (int)(last_row / a.G) + p.lk - p.lq + 1;   // visible to the tile
-    float16v o[DP / 32] = {};
-    float m = neg_inf(), l = 0.0f;
-    for (int k0 = 0; k0 < keys; k0 += 32) {
-        // V: 32 rows to LDS, rows beyond the keys as zeros
-        wave_sync();
-        for (int i = lane; i < 32 * (DP / 8); i += 64) {
-            const int r = i / (DP / 8), ch = i % (DP / 8);
-            uint4v z = {0, 0, 0, 0};
-            if (k0 + r < keys && ch * 8 < a.d)
-                z = *(const uint4v *)((const uint16_t *)a.v + (p.k0 + k0 + r) * a.v_row +
-                                      hk * a.v_head + ch * 8);
-            *(uint4v *)(vt + Tile<DP>::at(r, ch)) = z;
-        }
-        uint4v k[DP / 16];
-        const int kr = k0 + (lane & 31);
-        load_row<DP>(k, a.k, (p.k0 + kr) * a.k_row + hk * a.k_head, a.d, kr < keys);
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; dt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
+    m = neg_inf();
+    l = 0.0f;
+    for (int k0 = key0; k0 < end; k0 += 32) {
         float16v s = {};
 #pragma unroll
         for (int c = 0; c < DP / 16; c++) s = T::mfma(k[c], q[c], s);
+        wave_sync();
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++)
+            *(uint4v *)(vt + Tile<DP>::at(lane & 31, 2 * c + h)) = v[c];
+        if (AHEAD && k0 + 32 < end) fetch(k0 + 32);
         float mx = neg_inf();
 #pragma unroll
         for (int r = 0; r < 16; r++) {
             const int key = k0 + 8 * (r / 4) + 4 * h + r % 4;
-            s[r] = key <= lim ? s[r] : neg_inf();
+            s[r] = key <= lim && key < end ? s[r] : neg_inf();
             mx = fmaxf(mx, s[r]);
         }
         const float mn = fmaxf(m, max_halves(mx));
@@ -73,7 +70,8 @@ __global__ __launch_bounds__(256) void attn_wave(Attn a, int64_t slots) {
         uint32_t pk[8];
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-            const float p0 = exp2_fast((s[r] - m0) * a.c), p1 = exp2_fast((s[r + 1] - m0) * a.c);
+            const float p0 = exp2_fast((s[r] - m0) * a.c);
+            const float p1 = exp2_fast((s[r + 1] - m0) * a.c);
             sum += p0 + p1;
             pk[r / 2] = T::pack(p0, p1);
         }
@@ -89,8 +87,36 @@ __global__ __launch_bounds__(256) void attn_wave(Attn a, int64_t slots) {
             for (int dt = 0; dt < DP / 32; dt++)
                 o[dt] = T::mfma(Tile<DP>::transposed(vt, kc * 16, dt), pb, o[dt]);
         }
+        if (!AHEAD && k0 + 32 < end) fetch(k0 + 32);
     }
-    store_out<T, DP>(a, p.q0 + qi, head, o, m, add_halves(l), ok);
+    l = add_halves(l);
+    return {p.q0 + qi, head, ok};
+}
+
+// Short sequences: a wave owns up to 128 rows of a sequence and key head, in
+// tiles of 32: most waves then have a sequence to themselves, and few slots are
+// empty. What bounds it is memory, and before that the chain of loads from the
+// slot to the rows.
+constexpr int kShortRows = 128;
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attn_wave(Attn a, int slots) {
+    __shared__ __align__(16) uint16_t lds[4][32 * Tile<DP>::stride];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint16_t *vt = lds[wave];
+    const int item = blockIdx.x * 4 + wave;
+    const int slot = item / a.hkv, hk = item - slot * a.hkv;
+    if (slot >= slots) return;
+    const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, kShortRows, slot);
+    const int b = f.b;
+    const Place p = place_of(a, b, f.start, f.end);
+    const int first = (slot - slot_of(p.q0, a.G, kShortRows, b)) * (kShortRows / 32);
+    if (first < 0) return;
+    for (int tile = first; tile < first + kShortRows / 32 && tile * 32 < p.lq * a.G; tile++) {
+        float16v o[DP / 32];
+        float m, l;
+        const Row r = run_rows<T, DP, false>(a, p, hk, tile, 0, p.lk, vt, o, m, l);
+        store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok);
+    }
 }
 
 // Long sequences: a block of WAVES waves owns WAVES * 32 rows of one key head;
@@ -102,34 +128,35 @@ __global__ __launch_bounds__(256) void attn_wave(Attn a, int64_t slots) {
 // a lower reference is as exact, since numerator and denominator share it, and
 // 2^8 is far from any overflow.
 template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int64_t slots) {
+__global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int slots) {
     typedef KeyTiles<DP, 64, WAVES> Keys;
     constexpr int KB = 64, ROWS = WAVES * 32, STRIDE = Keys::STRIDE;
     __shared__ __align__(256) unsigned char lds[2 * Keys::BYTES];
-    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
-    const int64_t slot = blockIdx.x / a.hkv;
-    const int hk = (int)(blockIdx.x % a.hkv);
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int slot = (int)blockIdx.x / a.hkv, hk = (int)blockIdx.x - slot * a.hkv;
     if (slot >= slots) return;
-    const int b = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, ROWS, slot);
-    const Place p = place_of(a, b);
-    const int64_t rows = (int64_t)p.lq * a.G;
+    const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, ROWS, slot);
+    const int b = f.b;
+    const Place p = place_of(a, b, f.start, f.end);
+    const int rows = p.lq * a.G;
     // the last tiles, which see most keys, go first
-    const int64_t tile = (rows + ROWS - 1) / ROWS - 1 - (slot - slot_of(p.q0, a.G, ROWS, b));
+    const int tile = (rows + ROWS - 1) / ROWS - 1 - (slot - slot_of(p.q0, a.G, ROWS, b));
     if (tile < 0 || tile * ROWS >= rows) return;
-    const int64_t row = tile * ROWS + wave * 32 + (lane & 31);
+    const int row = tile * ROWS + wave * 32 + (lane & 31);
     const bool ok = row < rows;
-    const int qi = ok ? (int)(row / a.G) : 0, g = ok ? (int)(row % a.G) : 0;
+    const int qi = ok ? row / a.G : 0, g = ok ? row % a.G : 0;
     const int head = hk * a.G + g;
     const int lim = ok ? qi + p.lk - p.lq : -1;
     uint4v q[DP / 16];
     load_row<DP>(q, a.q, (p.q0 + qi) * a.q_row + head * a.q_head, a.d, ok);
     // keys that the block's rows see, that this wave's see, and that each of
     // this wave's rows sees
-    auto seen_by = [&](int64_t r) {
-        return (int)((r < rows ? r : rows - 1) / a.G) + p.lk - p.lq + 1;
+    auto seen_by = [&](int r) {
+        return min(r, rows - 1) / a.G + p.lk - p.lq + 1;
     };
     const int keys = seen_by(tile * ROWS + ROWS - 1);
-    const int64_t w0 = tile * ROWS + wave * 32;
+    const int w0 = tile * ROWS + wave * 32;
     const int wave_keys = w0 < rows ? seen_by(w0 + 31) : 0;
     const int all_keys = w0 + 31 < rows ? seen_by(w0) : 0;
     const Keys tiles(a, p, hk, keys);
@@ -208,14 +235,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int64_t slot
 
 // Few rows over many keys (single tokens over a cache). A sequence's keys are
 // cut into chunks, one wave to a chunk, key head and tile of 32 rows; each
-// leaves its maximum, sum and unscaled output, and attn_join adds them up. The
-// next 32 keys are loaded while the present ones are worked on: eight waves a
-// compute unit keep 128 KB in flight. Chunks are slots over the key rows, as
+// leaves its maximum, sum and unscaled output, and attn_join adds them up. With
+// the next 32 keys always on their way, eight waves a compute unit keep 128 KB
+// in flight. Chunks are slots over the key rows, as
 // tiles are over the query rows.
 struct Step {
     int chunk;          // keys of a chunk, a multiple of 32
     int tiles;          // row tiles of a slot that have room in the partials
-    int64_t slots;
+    int slots;
     float *o, *ml;      // [slot][hkv][tiles * 32][DP], [slot][hkv][tiles * 32][2]
 };
 
@@ -223,114 +250,44 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
     __shared__ __align__(16) uint16_t lds[4][32 * Tile<DP>::stride];
     uint16_t *vt = lds[threadIdx.x >> 6];
-    constexpr int CH = DP / 8;               // 16-byte pieces of a row
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    const int64_t item = blockIdx.x * 4ll + (threadIdx.x >> 6);
-    const int64_t slot = item / a.hkv;
-    const int hk = (int)(item % a.hkv);
+    const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int slot = item / a.hkv, hk = item - slot * a.hkv;
     if (slot >= st.slots) return;
-    const int b = find_sequence(a.cu_k, a.n_seq, a.tk, 1, st.chunk, slot);
+    const Found f = find_sequence(a.cu_k, a.n_seq, a.tk, 1, st.chunk, slot);
+    const int b = f.b;
     // the rows after the last sequence see no key: entry n_seq, chunk 0
     const Place p = place_of(a, b);
-    const int64_t c64 = slot - slot_of(offset_at(a.cu_k, b, a.tk), 1, st.chunk, b);
-    const int64_t rows = (int64_t)p.lq * a.G;
-    if (c64 < 0 || rows == 0) return;
+    const int chunk = slot - slot_of(f.start, 1, st.chunk, b);
+    const int rows = p.lq * a.G;
+    if (chunk < 0 || rows == 0) return;
     const int chunks = (p.lk + st.chunk - 1) / st.chunk;
     const bool split = chunks > 1 && rows <= st.tiles * 32;
-    if (c64 >= (split ? chunks : 1)) return;
-    const int key0 = split ? (int)c64 * st.chunk : 0;
+    if (chunk >= (split ? chunks : 1)) return;
+    const int key0 = split ? chunk * st.chunk : 0;
     const int key1 = split && key0 + st.chunk < p.lk ? key0 + st.chunk : p.lk;
-    const uint16_t *kp = (const uint16_t *)a.k + p.k0 * a.k_row + hk * a.k_head;
-    const uint16_t *vp = (const uint16_t *)a.v + p.k0 * a.v_row + hk * a.v_head;
-
     // a sequence with more rows than the partials have room for is not split
-    for (int64_t tile = blockIdx.y; tile * 32 < rows; tile += st.tiles) {
-        const int64_t row = tile * 32 + (lane & 31);
-        const bool ok = row < rows;
-        const int qi = ok ? (int)(row / a.G) : 0, g = ok ? (int)(row % a.G) : 0;
-        const int head = hk * a.G + g;
-        const int lim = ok ? qi + p.lk - p.lq : -1;
-        uint4v q[DP / 16], k[DP / 16], v[DP / 16];
-        load_row<DP>(q, a.q, (p.q0 + qi) * a.q_row + head * a.q_head, a.d, ok);
-        const int64_t last_row = tile * 32 + 31 < rows ? tile * 32 + 31 : rows - 1;
-        const int seen = (int)(last_row / a.G) + p.lk - p.lq + 1;
-        const int end = key1 < seen ? key1 : seen;
-        auto fetch = [&](int k0) {
-            const int kr = k0 + (lane & 31);
-            load_row<DP>(k, kp, (int64_t)kr * a.k_row, a.d, kr < end);
-#pragma unroll
-            for (int j = 0; j < DP / 16; j++) {
-                const int i = lane + 64 * j, r = k0 + i / CH, ch = i % CH;
-                const uint4v z = {0, 0, 0, 0};
-                v[j] = r < end && ch * 8 < a.d
-                           ? *(const uint4v *)(vp + (int64_t)r * a.v_row + ch * 8) : z;
-            }
-        };
-        float16v o[DP / 32] = {};
-        float m = neg_inf(), l = 0.0f;
-        fetch(key0);
-        for (int k0 = key0; k0 < end; k0 += 32) {
-            float16v s = {};
-#pragma unroll
-            for (int c = 0; c < DP / 16; c++) s = T::mfma(k[c], q[c], s);
-            wave_sync();
-#pragma unroll
-            for (int j = 0; j < DP / 16; j++) {
-                const int i = lane + 64 * j;
-                *(uint4v *)(vt + Tile<DP>::at(i / CH, i % CH)) = v[j];
-            }
-            if (k0 + 32 < end) fetch(k0 + 32);
-            float mx = neg_inf();
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int key = k0 + 8 * (r / 4) + 4 * h + r % 4;
-                s[r] = key <= lim && key < end ? s[r] : neg_inf();
-                mx = fmaxf(mx, s[r]);
-            }
-            const float mn = fmaxf(m, max_halves(mx));
-            const float m0 = mn == neg_inf() ? 0.0f : mn;
-            const float alpha = exp2_fast((m - m0) * a.c);
-            float sum = 0.0f;
-            uint32_t pk[8];
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                const float p0 = exp2_fast((s[r] - m0) * a.c);
-                const float p1 = exp2_fast((s[r + 1] - m0) * a.c);
-                sum += p0 + p1;
-                pk[r / 2] = T::pack(p0, p1);
-            }
-            l = l * alpha + sum;
-            m = mn;
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; dt++) o[dt] *= alpha;
-            wave_sync();
-#pragma unroll
-            for (int kc = 0; kc < 2; kc++) {
-                const uint4v pb = {pk[4 * kc], pk[4 * kc + 1], pk[4 * kc + 2], pk[4 * kc + 3]};
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; dt++)
-                    o[dt] = T::mfma(Tile<DP>::transposed(vt, kc * 16, dt), pb, o[dt]);
-            }
+    for (int tile = blockIdx.y; tile * 32 < rows; tile += st.tiles) {
+        float16v o[DP / 32];
+        float m, l;
+        const Row r = run_rows<T, DP, true>(a, p, hk, tile, key0, key1, vt, o, m, l);
+        if (!split) {
+            store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok);
+            continue;
         }
-        l = add_halves(l);
-        if (split) {
-            const int64_t pr = ((slot * a.hkv + hk) * st.tiles + tile) * 32 + (lane & 31);
-            if (ok) {
+        const int64_t pr = (((int64_t)slot * a.hkv + hk) * st.tiles + tile) * 32 + (lane & 31);
+        if (!r.ok) continue;
 #pragma unroll
-                for (int dt = 0; dt < DP / 32; dt++)
+        for (int dt = 0; dt < DP / 32; dt++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float4v f = {o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2],
-                                           o[dt][4 * j + 3]};
-                        *(float4v *)(st.o + pr * DP + dt * 32 + 8 * j + 4 * h) = f;
-                    }
-                if (h == 0) {
-                    st.ml[2 * pr] = m;
-                    st.ml[2 * pr + 1] = l;
-                }
+            for (int j = 0; j < 4; j++) {
+                const float4v f = {o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2],
+                                   o[dt][4 * j + 3]};
+                *(float4v *)(st.o + pr * DP + dt * 32 + 8 * j + 4 * h) = f;
             }
-        } else {
-            store_out<T, DP>(a, p.q0 + qi, head, o, m, l, ok);
+        if (h == 0) {
+            st.ml[2 * pr] = m;
+            st.ml[2 * pr + 1] = l;
         }
     }
 }
@@ -340,16 +297,15 @@ __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void attn_join(Attn a, Step st) {
     const int lane = threadIdx.x & 63;
-    const int64_t item = blockIdx.x * 4ll + (threadIdx.x >> 6);
+    const int item = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (item >= a.tq * a.hq) return;
-    const int64_t t = item / a.hq;
-    const int head = (int)(item % a.hq), hk = head / a.G;
+    const int t = item / a.hq, head = item - t * a.hq, hk = head / a.G;
     const int b = sequence_of_row(a.cu_q, a.n_seq, a.tq, t);
     const Place p = place_of(a, b);
     const int chunks = (p.lk + st.chunk - 1) / st.chunk;
-    const int64_t rows = (int64_t)p.lq * a.G;
+    const int rows = p.lq * a.G;
     if (chunks <= 1 || rows > st.tiles * 32 || t < p.q0 || t >= p.q0 + p.lq) return;
-    const int64_t row = (t - p.q0) * a.G + head % a.G;
+    const int row = (t - p.q0) * a.G + head % a.G;
     const int64_t slot0 = slot_of(offset_at(a.cu_k, b, a.tk), 1, st.chunk, b);
     const int64_t stride = (int64_t)a.hkv * st.tiles * 32;
     const int64_t pr = slot0 * stride + (int64_t)hk * st.tiles * 32 + row;
@@ -392,7 +348,9 @@ bool plan_step(const Attn &a, Step &st) {
     st.slots = slot_of(a.tk, 1, st.chunk, a.n_seq) + 1;
     return true;
 }
-int64_t step_rows(const Attn &a, const Step &st) { return st.slots * a.hkv * st.tiles * 32; }
+int64_t step_rows(const Attn &a, const Step &st) {
+    return (int64_t)st.slots * a.hkv * st.tiles * 32;
+}
 int64_t step_bytes(const Attn &a, const Step &st) {
     return a.tk <= st.chunk ? 0 : step_rows(a, st) * (padded_head(a.d) + 2) * 4;
 }
@@ -401,7 +359,7 @@ template <typename T, int DP>
 int launch_step(const Attn &a, Step st, hipStream_t s) {
     st.o = (float *)a.workspace;
     st.ml = st.o + step_rows(a, st) * DP;
-    const dim3 grid((unsigned)((st.slots * a.hkv + 3) / 4), (unsigned)st.tiles);
+    const dim3 grid((unsigned)((st.slots * (int64_t)a.hkv + 3) / 4), (unsigned)st.tiles);
     attn_step<T, DP><<<grid, 256, 0, s>>>(a, st);
     if (a.tk > st.chunk) {
         if (hipGetLastError() != hipSuccess) return CO_ERR_CUDA;
@@ -412,7 +370,7 @@ int launch_step(const Attn &a, Step st, hipStream_t s) {
 
 template <typename T, int DP, int WAVES>
 int launch_tiles(const Attn &a, hipStream_t s) {
-    const int64_t slots = slot_of(a.tq, a.G, WAVES * 32, a.n_seq) + 1;
+    const int slots = slot_of(a.tq, a.G, WAVES * 32, a.n_seq) + 1;
     attn_tiles<T, DP, WAVES><<<dim3((unsigned)(slots * a.hkv)), WAVES * 64, 0, s>>>(a, slots);
     return launch_status();
 }
@@ -424,8 +382,8 @@ int launch_head(const Attn &a, hipStream_t s) {
     const int64_t rows = a.n_seq ? a.tq * a.G / a.n_seq : 0;      // of a sequence, on average
     if (rows >= 256) return launch_tiles<T, DP, 8>(a, s);
     if (rows >= 96) return launch_tiles<T, DP, 4>(a, s);
-    const int64_t slots = slot_of(a.tq, a.G, 32, a.n_seq) + 1;
-    const int64_t blocks = (slots * a.hkv + 3) / 4;
+    const int slots = slot_of(a.tq, a.G, kShortRows, a.n_seq) + 1;
+    const int64_t blocks = (slots * (int64_t)a.hkv + 3) / 4;
     attn_wave<T, DP><<<dim3((unsigned)blocks), 256, 0, s>>>(a, slots);
     return launch_status();
 }
@@ -449,7 +407,9 @@ int check_attention(const SeqAttention *a) {
     if (a->n_seq < 0 || a->tq < 0 || a->tk < 0 || a->hkv < 1 || a->hq < 1 || a->d < 1)
         return CO_ERR_NULLARG;
     if (a->d % 8 || a->d > SEQ_MAX_HEAD || a->hq % a->hkv || a->n_seq > 1 << 28 ||
-        a->tq * a->hq > SEQ_MAX_ROWS || a->tk > SEQ_MAX_ROWS || a->hq > 1 << 15)
+        a->tq > SEQ_MAX_ROWS / a->hq || a->tk > SEQ_MAX_ROWS || a->hq > 1 << 15 ||
+        // the most waves that a launch has: a slot for 32 rows of either kind
+        (a->tq / 32 * (a->hq / a->hkv) + a->tk / 32 + a->n_seq + 2) * a->hkv > SEQ_MAX_ROWS)
         return CO_ERR_BOUNDS;
     if ((a->dtype != SEQ_BF16 && a->dtype != SEQ_FP16) || !(a->scale > 0.0f) ||
         a->scale > 1e30f)

@@ -42,7 +42,7 @@ __device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float
 
 // A wave owns 32 rows: delta, then dQ^T = sum over keys of K^T dS^T.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_grad_q(AttnGrad a, int64_t slots) {
+__global__ __launch_bounds__(256) void attn_grad_q(AttnGrad a, int slots) {
     __shared__ __align__(16) uint16_t lds[4][32 * Tile<DP>::stride];
     uint16_t *kt = lds[threadIdx.x >> 6];
     const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -50,14 +50,15 @@ __global__ __launch_bounds__(256) void attn_grad_q(AttnGrad a, int64_t slots) {
     const int64_t slot = item / a.hkv;
     const int hk = (int)(item % a.hkv);
     if (slot >= slots) return;
-    const int b = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, 32, slot);
-    const Place p = place_of(a, b);
-    const int64_t tile = slot - slot_of(p.q0, a.G, 32, b);
-    const int64_t rows = (int64_t)p.lq * a.G;
+    const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, 32, slot);
+    const int b = f.b;
+    const Place p = place_of(a, b, f.start, f.end);
+    const int tile = slot - slot_of(p.q0, a.G, 32, b);
+    const int rows = p.lq * a.G;
     if (tile < 0 || tile * 32 >= rows) return;
-    const int64_t row = tile * 32 + (lane & 31);
+    const int row = tile * 32 + (lane & 31);
     const bool ok = row < rows;
-    const int qi = ok ? (int)(row / a.G) : 0, g = ok ? (int)(row % a.G) : 0;
+    const int qi = ok ? row / a.G : 0, g = ok ? row % a.G : 0;
     const int head = hk * a.G + g;
     const int lim = ok ? qi + p.lk - p.lq : -1;
     const int64_t t = p.q0 + qi;
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(256) void attn_grad_q(AttnGrad a, int64_t slots) {
 // Slots are tiles of the key rows 0..tk-1, whatever sequence they belong to:
 // entry n_seq covers the rows after the last sequence.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_grad_kv(AttnGrad a, int64_t slots) {
+__global__ __launch_bounds__(256) void attn_grad_kv(AttnGrad a, int slots) {
     __shared__ __align__(16) uint16_t lds[4][2 * 32 * Tile<DP>::stride + 192];
     uint16_t *qt = lds[threadIdx.x >> 6], *ot = qt + 32 * Tile<DP>::stride;
     float *stat = (float *)(ot + 32 * Tile<DP>::stride);     // lse, delta, limit of 32 rows
@@ -125,10 +126,9 @@ __global__ __launch_bounds__(256) void attn_grad_kv(AttnGrad a, int64_t slots) {
     const int64_t slot = item / a.hkv;
     const int hk = (int)(item % a.hkv);
     if (slot >= slots) return;
-    const int b = find_sequence(a.cu_k, a.n_seq, a.tk, 1, 32, slot);
-    const int64_t s0 = offset_at(a.cu_k, b, a.tk);
-    const int64_t s1 = b >= a.n_seq ? a.tk : clamp64(a.cu_k[b + 1], s0, a.tk);
-    const int64_t tile = slot - slot_of(s0, 1, 32, b);
+    const Found f = find_sequence(a.cu_k, a.n_seq, a.tk, 1, 32, slot);
+    const int b = f.b, s0 = f.start, s1 = max(f.end, s0);
+    const int tile = slot - slot_of(s0, 1, 32, b);
     if (tile < 0 || tile * 32 >= s1 - s0) return;
     // rows of segment 0 before its start belong to no sequence
     const Place p = b >= a.n_seq ? Place{0, s0, 0, 0} : place_of(a, b);
@@ -140,15 +140,15 @@ __global__ __launch_bounds__(256) void attn_grad_kv(AttnGrad a, int64_t slots) {
     load_row<DP>(k, a.k, kr * a.k_row + hk * a.k_head, a.d, live);
     load_row<DP>(v, a.v, kr * a.v_row + hk * a.v_head, a.d, live);
     float16v dk[DP / 32] = {}, dv[DP / 32] = {};
-    const int64_t rows = (int64_t)p.lq * a.G;
+    const int rows = p.lq * a.G;
     const int key0 = (int)(tile * 32 + (s0 - p.k0));
     // the first query that sees a key of the tile
     int64_t r0 = (int64_t)(key0 - (p.lk - p.lq) > 0 ? key0 - (p.lk - p.lq) : 0) * a.G / 32 * 32;
     if (key0 >= p.lk) r0 = rows;
     for (; r0 < rows; r0 += 32) {
-        const int64_t row = r0 + (lane & 31);
+        const int row = r0 + (lane & 31);
         const bool rok = row < rows;
-        const int qi = rok ? (int)(row / a.G) : 0, g = rok ? (int)(row % a.G) : 0;
+        const int qi = rok ? row / a.G : 0, g = rok ? row % a.G : 0;
         const int head = hk * a.G + g;
         const int64_t t = p.q0 + qi;
         uint4v q[DP / 16], dO[DP / 16];
@@ -203,22 +203,23 @@ __global__ __launch_bounds__(256) void attn_grad_kv(AttnGrad a, int64_t slots) {
 // Long sequences, rows: a block of WAVES waves owns 32 rows a wave of one key
 // head; keys and values pass through LDS 64 at a time, as in the forward.
 template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, int64_t slots) {
+__global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, int slots) {
     typedef KeyTiles<DP, 64, WAVES> Keys;
     constexpr int KB = 64, ROWS = WAVES * 32, STRIDE = Keys::STRIDE;
     __shared__ __align__(256) unsigned char lds[2 * Keys::BYTES];
-    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
-    const int64_t slot = blockIdx.x / a.hkv;
-    const int hk = (int)(blockIdx.x % a.hkv);
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int slot = (int)blockIdx.x / a.hkv, hk = (int)blockIdx.x - slot * a.hkv;
     if (slot >= slots) return;
-    const int b = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, ROWS, slot);
-    const Place p = place_of(a, b);
-    const int64_t rows = (int64_t)p.lq * a.G;
-    const int64_t tile = (rows + ROWS - 1) / ROWS - 1 - (slot - slot_of(p.q0, a.G, ROWS, b));
+    const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, ROWS, slot);
+    const int b = f.b;
+    const Place p = place_of(a, b, f.start, f.end);
+    const int rows = p.lq * a.G;
+    const int tile = (rows + ROWS - 1) / ROWS - 1 - (slot - slot_of(p.q0, a.G, ROWS, b));
     if (tile < 0 || tile * ROWS >= rows) return;
-    const int64_t row = tile * ROWS + wave * 32 + (lane & 31);
+    const int row = tile * ROWS + wave * 32 + (lane & 31);
     const bool ok = row < rows;
-    const int qi = ok ? (int)(row / a.G) : 0, g = ok ? (int)(row % a.G) : 0;
+    const int qi = ok ? row / a.G : 0, g = ok ? row % a.G : 0;
     const int head = hk * a.G + g;
     const int lim = ok ? qi + p.lk - p.lq : -1;
     const int64_t t = p.q0 + qi;
@@ -230,11 +231,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, i
     lse2 = ok ? a.lse[head * a.tq + t] * kLog2e : 0.0f;
     put_stat(a, head * a.tq + t, lse2, delta, ok);
     load_row<DP>(q, a.q, t * a.q_row + head * a.q_head, a.d, ok);
-    auto seen_by = [&](int64_t r) {
-        return (int)((r < rows ? r : rows - 1) / a.G) + p.lk - p.lq + 1;
+    auto seen_by = [&](int r) {
+        return min(r, rows - 1) / a.G + p.lk - p.lq + 1;
     };
     const int keys = seen_by(tile * ROWS + ROWS - 1);
-    const int64_t w0 = tile * ROWS + wave * 32;
+    const int w0 = tile * ROWS + wave * 32;
     const int wave_keys = w0 < rows ? seen_by(w0 + 31) : 0;
     const int all_keys = w0 + 31 < rows ? seen_by(w0) : 0;
     const Keys tiles(a, p, hk, keys);
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, i
 // copied there past the registers one tile ahead of their use. Rows beyond the
 // last repeat it with lse +inf, which makes their P and dS 0.
 template <typename T, int DP>
-__global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int64_t slots) {
+__global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int slots) {
     constexpr int RB = 64, KEYS = 128, STRIDE = Tile<DP>::stride * 2;         // bytes
     constexpr int PER = RB * STRIDE / 1024;             // copies of 1 KB a tile of q or do
     constexpr int COPIES = 2 * PER / 8;                 // of a wave
@@ -309,17 +310,15 @@ __global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int64_t
     __shared__ __align__(256) unsigned char lds[BYTES > SUMS ? BYTES : SUMS];
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kx = wave & 3, rx = wave >> 2;
-    const int64_t slot = blockIdx.x / a.hkv;
-    const int hk = (int)(blockIdx.x % a.hkv);
+    const int slot = (int)blockIdx.x / a.hkv, hk = (int)blockIdx.x - slot * a.hkv;
     if (slot >= slots) return;
-    const int b = find_sequence(a.cu_k, a.n_seq, a.tk, 1, KEYS, slot);
-    const int64_t s0 = offset_at(a.cu_k, b, a.tk);
-    const int64_t s1 = b >= a.n_seq ? a.tk : clamp64(a.cu_k[b + 1], s0, a.tk);
-    const int64_t tile = slot - slot_of(s0, 1, KEYS, b);
+    const Found f = find_sequence(a.cu_k, a.n_seq, a.tk, 1, KEYS, slot);
+    const int b = f.b, s0 = f.start, s1 = max(f.end, s0);
+    const int tile = slot - slot_of(s0, 1, KEYS, b);
     if (tile < 0 || tile * KEYS >= s1 - s0) return;
     const Place p = b >= a.n_seq ? Place{0, s0, 0, 0} : place_of(a, b);
-    const int base = (int)(s0 - p.k0);                  // key number of the segment's first row
-    const int key0 = (int)(tile * KEYS) + base;         // of the block
+    const int base = s0 - p.k0;                  // key number of the segment's first row
+    const int key0 = tile * KEYS + base;         // of the block
     const int wkey0 = key0 + kx * 32;                   // of the wave
     const int key = wkey0 + (lane & 31);
     const bool live = key >= 0 && key < p.lk;

@@ -22,8 +22,8 @@ struct Attn : SeqAttention {
     float c;         // scale * log2(e): scores in powers of two
 };
 
-__device__ __host__ inline int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
-    return x < lo ? lo : (x > hi ? hi : x);
+__device__ inline int clamp_to(int x, int lo, int64_t hi) {
+    return x < lo ? lo : (x > hi ? (int)hi : x);
 }
 
 // x / n for 0 <= x < 2^31, n >= 1, without a branch: the quotient by a float
@@ -36,45 +36,93 @@ __device__ inline int divide(int x, int n, float inv) {
     return q + (r >= n) - (r < 0);
 }
 
-// A sequence's place: first query and key row, number of queries and keys.
-struct Place { int64_t q0, k0; int lq, lk; };
+// Rows, query rows times heads among them, number less than 2^31 (the entry
+// checks it), so places and tiles have 32 bits; only addresses have 64.
 
-__device__ inline int64_t offset_at(const int32_t *cu, int b, int64_t t) {
-    return b <= 0 ? 0 : clamp64(cu[b], 0, t);
+// A sequence's place: first query and key row, number of queries and keys.
+struct Place { int q0, k0, lq, lk; };
+
+__device__ inline int offset_at(const int32_t *cu, int b, int64_t t) {
+    return b <= 0 ? 0 : clamp_to(cu[b], 0, t);
 }
 
 // Work is handed out in tiles of `rows` rows without a list of tiles: tile
 // slots of sequence b start at floor(cu[b] * fold / rows) + b, which leaves
 // each at least as many as it has tiles and numbers them without gaps for a
 // search. Entry n_seq stands for the rows after the last sequence.
-__device__ __host__ inline int64_t slot_of(int64_t at, int fold, int rows, int b) {
-    return at * fold / rows + b;
+__device__ __host__ inline int slot_of(int64_t at, int fold, int rows, int b) {
+    return (int)((uint32_t)at * (uint32_t)fold / (uint32_t)rows) + b;
 }
 
-// The last b of 0..n_seq with slot_of(b) <= slot: 64 probes at a time, one per
-// lane. Every lane of a wave calls it with the same arguments.
-__device__ inline int find_sequence(const int32_t *cu, int n_seq, int64_t t, int fold, int rows,
-                                    int64_t slot) {
+// A slot's sequence: the last b of 0..n_seq with slot_of(b) <= slot, and the
+// offsets of it and the next (the tensor's end after n_seq). 64 probes at a time,
+// one per lane: first around the place that the slot would have if all sequences
+// were of one length, then, when that does not enclose it, over all of them. Each
+// round waits for a load, so the last one also brings the offsets. Every lane of a
+// wave calls it with the same arguments.
+struct Found { int b, start, end; };
+__device__ inline Found find_sequence(const int32_t *cu, int n_seq, int64_t t, int fold, int rows,
+                                      int slot) {
     const int lane = threadIdx.x & 63;
-    int lo = 0, n = n_seq + 1;
-    while (n > 1) {
-        const int step = (n + 63) / 64;
-        const int i = lane * step;
-        const bool ok = i < n && slot_of(offset_at(cu, lo + i, t), fold, rows, lo + i) <= slot;
-        const int last = __popcll(__ballot(ok)) - 1;
-        if (last <= 0) {          // offsets out of order count as the first
-            n = step < n ? step : n;
-        } else {
-            lo += last * step;
-            n = n - last * step < step ? n - last * step : step;
+    int lo = 0, n = n_seq + 1, step = (n + 63) / 64;
+    const int slots = slot_of(t, fold, rows, n_seq) + 1;
+    if (step > 1) {
+        // sequences of like lengths lie within a fraction of n of the guess
+        const int narrow = (n + 2047) / 2048;
+        const int guess = (int)((float)slot / (float)slots * (float)n) - 32 * narrow;
+        const int i = min(max(guess, 0), n - 64 * narrow) + lane * narrow;
+        const uint64_t ok = __ballot(slot_of(offset_at(cu, i, t), fold, rows, i) <= slot);
+        // the first holds and the last does not, or there is none after it
+        const int last = __popcll(ok) - 1;
+        const int first = __builtin_amdgcn_readfirstlane(i);
+        if (last >= 0 && (last < 63 || first + 64 * narrow >= n)) {
+            lo = first + last * narrow;
+            n = min(narrow, n - lo);
+            step = (n + 63) / 64;
         }
     }
-    return __builtin_amdgcn_readfirstlane(lo);
+    for (;;) {
+        const int i = lane * step;
+        const int at = offset_at(cu, min(lo + i, n_seq), t);
+        const bool ok = i < n && slot_of(at, fold, rows, lo + i) <= slot;
+        const int last = max(__popcll(__ballot(ok)) - 1, 0);   // offsets out of order: the first
+        if (step == 1) {
+            Found f;
+            f.b = __builtin_amdgcn_readfirstlane(lo + last);
+            f.start = __builtin_amdgcn_readlane(at, last);
+            // the next offset is the next lane's, unless this is the last lane
+            f.end = f.b >= n_seq ? (int)t
+                                 : (last < 63 ? __builtin_amdgcn_readlane(at, last + 1)
+                                              : offset_at(cu, f.b + 1, t));
+            return f;
+        }
+        lo += last * step;
+        n = min(n - last * step, step);
+        step = (n + 63) / 64;
+    }
+}
+
+__device__ inline Place place_of(const Attn &a, int b, int q0, int q1) {
+    Place p;
+    p.q0 = q0;
+    p.lq = q1 > q0 ? q1 - q0 : 0;
+    p.k0 = p.lk = 0;
+    if (b >= a.n_seq) return p;          // the rows after the last sequence: no keys
+    int k1 = q1;
+    if (a.cu_k == a.cu_q && a.tk == a.tq) {
+        p.k0 = q0;
+    } else {
+        p.k0 = clamp_to(a.cu_k[b], 0, a.tk);
+        k1 = clamp_to(a.cu_k[b + 1], p.k0, a.tk);
+    }
+    p.lk = max(k1 - p.k0, 0);
+    if (a.k_lens) p.lk = clamp_to(a.k_lens[b], 0, p.lk);
+    return p;
 }
 
 // The sequence of query row t (n_seq: none): the last whose offset is not
 // beyond it. Empty sequences share their offset with the next.
-__device__ inline int sequence_of_row(const int32_t *cu, int n_seq, int64_t tq, int64_t t) {
+__device__ inline int sequence_of_row(const int32_t *cu, int n_seq, int64_t tq, int t) {
     int lo = 0, hi = n_seq;
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -83,24 +131,9 @@ __device__ inline int sequence_of_row(const int32_t *cu, int n_seq, int64_t tq, 
     }
     return lo;
 }
-
 __device__ inline Place place_of(const Attn &a, int b) {
-    Place p;
-    p.q0 = offset_at(a.cu_q, b, a.tq);
-    if (b >= a.n_seq) {
-        p.lq = (int)(a.tq - p.q0);
-        p.k0 = 0;
-        p.lk = 0;
-        return p;
-    }
-    const int64_t q1 = offset_at(a.cu_q, b + 1, a.tq);
-    p.lq = (int)(q1 > p.q0 ? q1 - p.q0 : 0);
-    p.k0 = clamp64(a.cu_k[b], 0, a.tk);
-    const int64_t k1 = clamp64(a.cu_k[b + 1], p.k0, a.tk);
-    int64_t lk = k1 - p.k0;
-    if (a.k_lens) lk = clamp64(a.k_lens[b], 0, lk);
-    p.lk = (int)lk;
-    return p;
+    return place_of(a, b, offset_at(a.cu_q, b, a.tq),
+                    b >= a.n_seq ? (int)a.tq : offset_at(a.cu_q, b + 1, a.tq));
 }
 
 typedef __attribute__((address_space(3))) const uint16_t *lds_ptr;
@@ -277,11 +310,18 @@ template <int DP>
 __device__ inline void load_row(uint4v *f, const void *base, int64_t off, int d, bool ok) {
     const int h = (threadIdx.x & 63) >> 5;
     const uint16_t *p = (const uint16_t *)base + off;
+    const uint4v z = {0, 0, 0, 0};
+    if (d == DP) {                       // the same for all: no test for each piece
 #pragma unroll
-    for (int c = 0; c < DP / 16; c++) {
-        uint4v z = {0, 0, 0, 0};
-        f[c] = ok && c * 16 + h * 8 < d ? *(const uint4v *)(p + c * 16 + h * 8) : z;
+        for (int c = 0; c < DP / 16; c++) f[c] = z;
+        if (ok)
+#pragma unroll
+            for (int c = 0; c < DP / 16; c++) f[c] = *(const uint4v *)(p + c * 16 + h * 8);
+        return;
     }
+#pragma unroll
+    for (int c = 0; c < DP / 16; c++)
+        f[c] = ok && c * 16 + h * 8 < d ? *(const uint4v *)(p + c * 16 + h * 8) : z;
 }
 
 // A column of a transposed accumulator (DP values of this lane's row, split
@@ -305,7 +345,7 @@ __device__ inline void store_row(void *base, int64_t off, const float16v *acc, f
             auto s1 = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
             uint4v v = {s0[0], s1[0], s0[1], s1[1]};
             const int col = dt * 32 + g * 16 + h * 8;
-            if (ok && col < d) *(uint4v *)(p + col) = v;
+            if (d == DP ? ok : ok && col < d) *(uint4v *)(p + col) = v;
         }
 }
 
