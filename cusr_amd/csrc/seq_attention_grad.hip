@@ -40,164 +40,187 @@ __device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float
     }
 }
 
-// A wave owns 32 rows: delta, then dQ^T = sum over keys of K^T dS^T.
+// Short sequences: a wave owns up to 128 rows of a sequence and key head, and
+// every so many tiles of 32 of its keys; most have a sequence to themselves, read
+// it once (the second part finds it in the caches, or, when it is one tile, in
+// the registers) and need no statistics from another kernel. First the rows:
+// delta, then dQ^T = sum over keys of K^T dS^T, from S^T. Then the keys:
+// dV^T = dO^T P and dK^T = Q^T dS, from S formed the other way round: the same
+// registers are the left or the right operand.
+constexpr int kShortRows = 128;
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_grad_q(AttnGrad a, int slots) {
-    __shared__ __align__(16) uint16_t lds[4][32 * Tile<DP>::stride];
-    uint16_t *kt = lds[threadIdx.x >> 6];
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_grad_short(AttnGrad a, int slots) {
+    constexpr int C = DP / 16, S = Tile<DP>::stride;
+    __shared__ __align__(16) uint16_t lds[4][2 * 32 * S];
+    __shared__ __align__(16) float stats[4][3][kShortRows];     // lse, delta, last visible key
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    const int64_t item = blockIdx.x * 4ll + (threadIdx.x >> 6);
-    const int64_t slot = item / a.hkv;
-    const int hk = (int)(item % a.hkv);
+    uint16_t *ta = lds[wave], *tb = ta + 32 * S;
+    float *lses = stats[wave][0], *deltas = stats[wave][1];
+    int *lims = (int *)stats[wave][2];
+    const int item = blockIdx.x * 4 + wave;
+    const int slot = item / a.hkv, hk = item - slot * a.hkv;
     if (slot >= slots) return;
-    const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, 32, slot);
-    const int b = f.b;
-    const Place p = place_of(a, b, f.start, f.end);
-    const int tile = slot - slot_of(p.q0, a.G, 32, b);
-    const int rows = p.lq * a.G;
-    if (tile < 0 || tile * 32 >= rows) return;
-    const int row = tile * 32 + (lane & 31);
-    const bool ok = row < rows;
-    const int qi = ok ? row / a.G : 0, g = ok ? row % a.G : 0;
-    const int head = hk * a.G + g;
-    const int lim = ok ? qi + p.lk - p.lq : -1;
-    const int64_t t = p.q0 + qi;
-    uint4v q[DP / 16], dO[DP / 16];
-    float delta, lse2;
-    {
-        uint4v o[DP / 16];
-        load_row<DP>(o, a.o, t * a.o_row + head * a.o_head, a.d, ok);
-        load_row<DP>(dO, a.g.d_o, t * a.g.do_row + head * a.g.do_head, a.d, ok);
-        delta = add_halves(dot_row<T>(o, dO, DP / 16));
-        lse2 = ok ? a.lse[head * a.tq + t] * kLog2e : 0.0f;
-        put_stat(a, head * a.tq + t, lse2, delta, ok);
-    }
-    load_row<DP>(q, a.q, t * a.q_row + head * a.q_head, a.d, ok);
-    const int64_t last_row = tile * 32 + 31 < rows ? tile * 32 + 31 : rows - 1;
-    const int keys = (int)(last_row / a.G) + p.lk - p.lq + 1;
-    float16v dq[DP / 32] = {};
-    for (int k0 = 0; k0 < keys; k0 += 32) {
-        const int kr = k0 + (lane & 31);
-        uint4v k[DP / 16], v[DP / 16];
-        load_row<DP>(k, a.k, (p.k0 + kr) * a.k_row + hk * a.k_head, a.d, kr < keys);
-        load_row<DP>(v, a.v, (p.k0 + kr) * a.v_row + hk * a.v_head, a.d, kr < keys);
-        wave_sync();
-#pragma unroll
-        for (int c = 0; c < DP / 16; c++)
-            *(uint4v *)(kt + Tile<DP>::at(lane & 31, 2 * c + h)) = k[c];
-        float16v s = {}, dp = {};
-#pragma unroll
-        for (int c = 0; c < DP / 16; c++) s = T::mfma(k[c], q[c], s);
-#pragma unroll
-        for (int c = 0; c < DP / 16; c++) dp = T::mfma(v[c], dO[c], dp);
-        uint32_t pk[8];
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            float ds[2];
-            for (int j = 0; j < 2; j++) {
-                const int key = k0 + 8 * (r / 4) + 4 * h + (r + j) % 4;
-                const float pr = exp2_fast(s[r + j] * a.c - lse2);
-                ds[j] = key <= lim ? pr * (dp[r + j] - delta) : 0.0f;
-            }
-            pk[r / 2] = T::pack(ds[0], ds[1]);
+    const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, kShortRows, slot);
+    const Place p = place_of(a, f.b, f.start, f.end);
+    const int rows = p.lq * a.G, tiles = (rows + 31) / 32;
+    const int mine = slot - slot_of(f.start, a.G, kShortRows, f.b);
+    const int shares = max((rows + kShortRows - 1) / kShortRows, 1);
+    if (mine < 0 || mine >= shares) return;
+    // the key rows of the segment, of which p.lk are keys
+    const bool same = a.cu_k == a.cu_q && a.tk == a.tq;
+    const int s0 = same ? f.start : offset_at(a.cu_k, f.b, a.tk);
+    const int s1 = same ? f.end : (f.b >= a.n_seq ? (int)a.tk
+                                                  : max(offset_at(a.cu_k, f.b + 1, a.tk), s0));
+    const int shift = p.lk - p.lq;
+    const float inv = 1.0f / (float)a.G;
+    const uint16_t *kp = (const uint16_t *)a.k + p.k0 * a.k_row + hk * a.k_head;
+    const uint16_t *vp = (const uint16_t *)a.v + p.k0 * a.v_row + hk * a.v_head;
+    uint4v q[C], dO[C], k[C], v[C];
+    struct { int t, head, lim; bool ok; } r;
+    auto row_of = [&](int tile) {
+        const int row = tile * 32 + (lane & 31);
+        r.ok = row < rows;
+        const int qi = divide(r.ok ? row : 0, a.G, inv);
+        r.t = p.q0 + qi;
+        r.head = hk * a.G + (r.ok ? row - qi * a.G : 0);
+        r.lim = r.ok ? qi + shift : -1;
+    };
+    auto load_rows = [&]() {
+        load_row<DP>(q, a.q, r.t * a.q_row + r.head * a.q_head, a.d, r.ok);
+        load_row<DP>(dO, a.g.d_o, r.t * a.g.do_row + r.head * a.g.do_head, a.d, r.ok);
+    };
+    // statistics of this lane's row, to LDS at `at`
+    auto put_stats = [&](int at, float &lse2, float &delta) {
+        uint4v o[C];
+        load_row<DP>(o, a.o, r.t * a.o_row + r.head * a.o_head, a.d, r.ok);
+        lse2 = r.ok ? a.lse[r.head * a.tq + r.t] * kLog2e : 0.0f;
+        delta = add_halves(dot_row<T>(o, dO, C));
+        if (h == 0) {
+            lses[at + lane] = lse2;
+            deltas[at + lane] = delta;
+            lims[at + lane] = r.lim;
         }
-        wave_sync();
+    };
+
+    for (int tile = mine * 4; tile < mine * 4 + 4 && tile < tiles; tile++) {
+        row_of(tile);
+        const int end = divide(min(tile * 32 + 31, rows - 1), a.G, inv) + shift + 1;
+        auto load_keys = [&](int k0) {       // beyond the last, the last again: masked
+            const int i = min(k0 + (lane & 31), end - 1);
+            load_row<DP>(k, kp, i * a.k_row, a.d, true);
+            load_row<DP>(v, vp, i * a.v_row, a.d, true);
+        };
+        load_rows();
+        if (end > 0) load_keys(0);
+        float lse2, delta;
+        put_stats((tile & 3) * 32, lse2, delta);
+        float16v dq[DP / 32] = {};
+        for (int k0 = 0; k0 < end; k0 += 32) {
+            if (k0) load_keys(k0);
+            wave_sync();
 #pragma unroll
-        for (int kc = 0; kc < 2; kc++) {
-            const uint4v pb = {pk[4 * kc], pk[4 * kc + 1], pk[4 * kc + 2], pk[4 * kc + 3]};
+            for (int c = 0; c < C; c++) *(uint4v *)(ta + Tile<DP>::at(lane & 31, 2 * c + h)) = k[c];
+            float16v s = {}, dp = {};
+#pragma unroll
+            for (int c = 0; c < C; c++) s = T::mfma(k[c], q[c], s);
+#pragma unroll
+            for (int c = 0; c < C; c++) dp = T::mfma(v[c], dO[c], dp);
+            uint32_t pk[8];
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                float ds[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int key = k0 + 8 * (i / 4) + 4 * h + (i + j) % 4;
+                    const float pr = exp2_fast(__builtin_fmaf(s[i + j], a.c, -lse2));
+                    ds[j] = key <= r.lim ? pr * (dp[i + j] - delta) : 0.0f;
+                }
+                pk[i / 2] = T::pack(ds[0], ds[1]);
+            }
+            wave_sync();
+#pragma unroll
+            for (int kc = 0; kc < 2; kc++) {
+                const uint4v pb = {pk[4 * kc], pk[4 * kc + 1], pk[4 * kc + 2], pk[4 * kc + 3]};
+#pragma unroll
+                for (int dt = 0; dt < DP / 32; dt++)
+                    dq[dt] = T::mfma(Tile<DP>::transposed(ta, kc * 16, dt), pb, dq[dt]);
+            }
+        }
+        store_row<T, DP>(a.g.dq, r.t * a.g.dq_row + r.head * a.g.dq_head, dq, a.scale, a.d, r.ok);
+    }
+
+    const bool kept = tiles == 1 && s1 - s0 <= 32 && s0 == p.k0 && p.lk > 0;
+    for (int kt = mine; kt * 32 < s1 - s0; kt += shares) {
+        const int kr = s0 + kt * 32 + (lane & 31);               // this lane's key row
+        const int key0 = kt * 32 + s0 - p.k0, key = key0 + (lane & 31);
+        const bool live = kr < s1 && key >= 0 && key < p.lk;
+        float16v dk[DP / 32] = {}, dv[DP / 32] = {};
+        if (key0 < p.lk) {
+            if (!kept) {
+                load_row<DP>(k, kp, key * a.k_row, a.d, live);
+                load_row<DP>(v, vp, key * a.v_row, a.d, live);
+            }
+            for (int tile = max(key0 - shift, 0) * a.G / 32; tile < tiles; tile++) {
+                int at = (tile & 3) * 32;
+                if (!kept) {
+                    row_of(tile);
+                    load_rows();
+                }
+                wave_sync();
+                if (shares > 1) {            // the rows may be another wave's
+                    float x, y;
+                    put_stats(at = 0, x, y);
+                }
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    *(uint4v *)(ta + Tile<DP>::at(lane & 31, 2 * c + h)) = q[c];
+                    *(uint4v *)(tb + Tile<DP>::at(lane & 31, 2 * c + h)) = dO[c];
+                }
+                float16v s = {}, dp = {};
+#pragma unroll
+                for (int c = 0; c < C; c++) s = T::mfma(q[c], k[c], s);
+#pragma unroll
+                for (int c = 0; c < C; c++) dp = T::mfma(dO[c], v[c], dp);
+                wave_sync();
+                uint32_t pp[8], pd[8];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float4v l4 = *(const float4v *)(lses + at + 8 * i + 4 * h);
+                    const float4v e4 = *(const float4v *)(deltas + at + 8 * i + 4 * h);
+                    const uint4v m4 = *(const uint4v *)(lims + at + 8 * i + 4 * h);
+                    float pr[4], ds[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const bool see = key <= (int)m4[j];
+                        pr[j] = see ? exp2_fast(__builtin_fmaf(s[4 * i + j], a.c, -l4[j])) : 0.0f;
+                        ds[j] = see ? pr[j] * (dp[4 * i + j] - e4[j]) : 0.0f;
+                    }
+                    pp[2 * i] = T::pack(pr[0], pr[1]);
+                    pp[2 * i + 1] = T::pack(pr[2], pr[3]);
+                    pd[2 * i] = T::pack(ds[0], ds[1]);
+                    pd[2 * i + 1] = T::pack(ds[2], ds[3]);
+                }
+#pragma unroll
+                for (int kc = 0; kc < 2; kc++) {
+                    const uint4v pb = {pp[4 * kc], pp[4 * kc + 1], pp[4 * kc + 2], pp[4 * kc + 3]};
+                    const uint4v db = {pd[4 * kc], pd[4 * kc + 1], pd[4 * kc + 2], pd[4 * kc + 3]};
+#pragma unroll
+                    for (int dt = 0; dt < DP / 32; dt++) {
+                        dv[dt] = T::mfma(Tile<DP>::transposed(tb, kc * 16, dt), pb, dv[dt]);
+                        dk[dt] = T::mfma(Tile<DP>::transposed(ta, kc * 16, dt), db, dk[dt]);
+                    }
+                }
+            }
+        }
+        if (!live)                           // a row that is no key's: zeros
 #pragma unroll
             for (int dt = 0; dt < DP / 32; dt++)
-                dq[dt] = T::mfma(Tile<DP>::transposed(kt, kc * 16, dt), pb, dq[dt]);
-        }
+#pragma unroll
+                for (int i = 0; i < 16; i++) dk[dt][i] = dv[dt][i] = 0.0f;
+        store_row<T, DP>(a.g.dk, kr * a.g.dk_row + hk * a.g.dk_head, dk, a.scale, a.d, kr < s1);
+        store_row<T, DP>(a.g.dv, kr * a.g.dv_row + hk * a.g.dv_head, dv, 1.0f, a.d, kr < s1);
     }
-    store_row<T, DP>(a.g.dq, t * a.g.dq_row + head * a.g.dq_head, dq, a.scale, a.d, ok);
-}
-
-// A wave owns 32 keys of one key head and sums over the rows that see them.
-// Slots are tiles of the key rows 0..tk-1, whatever sequence they belong to:
-// entry n_seq covers the rows after the last sequence.
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_grad_kv(AttnGrad a, int slots) {
-    __shared__ __align__(16) uint16_t lds[4][2 * 32 * Tile<DP>::stride + 192];
-    uint16_t *qt = lds[threadIdx.x >> 6], *ot = qt + 32 * Tile<DP>::stride;
-    float *stat = (float *)(ot + 32 * Tile<DP>::stride);     // lse, delta, limit of 32 rows
-    const int lane = threadIdx.x & 63, h = lane >> 5;
-    const int64_t item = blockIdx.x * 4ll + (threadIdx.x >> 6);
-    const int64_t slot = item / a.hkv;
-    const int hk = (int)(item % a.hkv);
-    if (slot >= slots) return;
-    const Found f = find_sequence(a.cu_k, a.n_seq, a.tk, 1, 32, slot);
-    const int b = f.b, s0 = f.start, s1 = max(f.end, s0);
-    const int tile = slot - slot_of(s0, 1, 32, b);
-    if (tile < 0 || tile * 32 >= s1 - s0) return;
-    // rows of segment 0 before its start belong to no sequence
-    const Place p = b >= a.n_seq ? Place{0, s0, 0, 0} : place_of(a, b);
-    const int key = (int)(tile * 32 + (s0 - p.k0)) + (lane & 31);   // in the sequence
-    const bool ok = tile * 32 + (lane & 31) < s1 - s0;
-    const bool live = ok && key >= 0 && key < p.lk;
-    const int64_t kr = s0 + tile * 32 + (lane & 31);
-    uint4v k[DP / 16], v[DP / 16];
-    load_row<DP>(k, a.k, kr * a.k_row + hk * a.k_head, a.d, live);
-    load_row<DP>(v, a.v, kr * a.v_row + hk * a.v_head, a.d, live);
-    float16v dk[DP / 32] = {}, dv[DP / 32] = {};
-    const int rows = p.lq * a.G;
-    const int key0 = (int)(tile * 32 + (s0 - p.k0));
-    // the first query that sees a key of the tile
-    int64_t r0 = (int64_t)(key0 - (p.lk - p.lq) > 0 ? key0 - (p.lk - p.lq) : 0) * a.G / 32 * 32;
-    if (key0 >= p.lk) r0 = rows;
-    for (; r0 < rows; r0 += 32) {
-        const int row = r0 + (lane & 31);
-        const bool rok = row < rows;
-        const int qi = rok ? row / a.G : 0, g = rok ? row % a.G : 0;
-        const int head = hk * a.G + g;
-        const int64_t t = p.q0 + qi;
-        uint4v q[DP / 16], dO[DP / 16];
-        load_row<DP>(q, a.q, t * a.q_row + head * a.q_head, a.d, rok);
-        load_row<DP>(dO, a.g.d_o, t * a.g.do_row + head * a.g.do_head, a.d, rok);
-        wave_sync();
-#pragma unroll
-        for (int c = 0; c < DP / 16; c++) {
-            *(uint4v *)(qt + Tile<DP>::at(lane & 31, 2 * c + h)) = q[c];
-            *(uint4v *)(ot + Tile<DP>::at(lane & 31, 2 * c + h)) = dO[c];
-        }
-        if (h == 0) {
-            const int64_t n = a.tq * a.hq, at = rok ? head * a.tq + t : n;
-            stat[lane] = a.stat[at];
-            stat[32 + lane] = a.stat[n + 1 + at];
-            ((int *)stat)[64 + lane] = rok ? qi + p.lk - p.lq : -1;
-        }
-        float16v s = {}, dp = {};
-#pragma unroll
-        for (int c = 0; c < DP / 16; c++) s = T::mfma(q[c], k[c], s);
-#pragma unroll
-        for (int c = 0; c < DP / 16; c++) dp = T::mfma(dO[c], v[c], dp);
-        wave_sync();
-        uint32_t pp[8], pd[8];
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            float pr[2], ds[2];
-            for (int j = 0; j < 2; j++) {
-                const int i = 8 * (r / 4) + 4 * h + (r + j) % 4;
-                const bool see = live && key <= ((const int *)stat)[64 + i];
-                pr[j] = see ? exp2_fast(s[r + j] * a.c - stat[i]) : 0.0f;
-                ds[j] = see ? pr[j] * (dp[r + j] - stat[32 + i]) : 0.0f;
-            }
-            pp[r / 2] = T::pack(pr[0], pr[1]);
-            pd[r / 2] = T::pack(ds[0], ds[1]);
-        }
-#pragma unroll
-        for (int kc = 0; kc < 2; kc++) {
-            const uint4v pb = {pp[4 * kc], pp[4 * kc + 1], pp[4 * kc + 2], pp[4 * kc + 3]};
-            const uint4v db = {pd[4 * kc], pd[4 * kc + 1], pd[4 * kc + 2], pd[4 * kc + 3]};
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; dt++) {
-                dv[dt] = T::mfma(Tile<DP>::transposed(ot, kc * 16, dt), pb, dv[dt]);
-                dk[dt] = T::mfma(Tile<DP>::transposed(qt, kc * 16, dt), db, dk[dt]);
-            }
-        }
-    }
-    store_row<T, DP>(a.g.dk, kr * a.g.dk_row + hk * a.g.dk_head, dk, a.scale, a.d, ok);
-    store_row<T, DP>(a.g.dv, kr * a.g.dv_row + hk * a.g.dv_head, dv, 1.0f, a.d, ok);
 }
 
 // Long sequences, rows: a block of WAVES waves owns 32 rows a wave of one key
@@ -492,28 +515,25 @@ __global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int slo
     store_row<T, DP>(a.g.dv, kr * a.g.dv_row + hk * a.g.dv_head, dv, 1.0f, a.d, kr < s1);
 }
 
+// At fewer than 128 keys a sequence a block of the long kernels would mostly
+// wait for itself.
+bool short_sequences(const Attn &a) { return a.tk < 128ll * a.n_seq || a.n_seq == 0; }
+
 template <typename T, int DP>
 int launch_grad(const AttnGrad &a, hipStream_t s) {
-    const int64_t n = a.n_seq ? a.n_seq : 1;
+    if (short_sequences(a)) {
+        const int slots = slot_of(a.tq, a.G, kShortRows, a.n_seq) + 1;
+        const dim3 grid((unsigned)((slots * (int64_t)a.hkv + 3) / 4));
+        attn_grad_short<T, DP><<<grid, 256, 0, s>>>(a, slots);
+        return launch_status();
+    }
     if (a.tq) {
-        if (a.tq * a.G >= 256 * n) {
-            const int64_t slots = slot_of(a.tq, a.G, 256, a.n_seq) + 1;
-            attn_grad_q_tiles<T, DP, 8><<<dim3((unsigned)(slots * a.hkv)), 512, 0, s>>>(a, slots);
-        } else {
-            const int64_t slots = slot_of(a.tq, a.G, 32, a.n_seq) + 1;
-            attn_grad_q<T, DP><<<dim3((unsigned)((slots * a.hkv + 3) / 4)), 256, 0, s>>>(a, slots);
-        }
+        const int slots = slot_of(a.tq, a.G, 256, a.n_seq) + 1;
+        attn_grad_q_tiles<T, DP, 8><<<dim3((unsigned)(slots * a.hkv)), 512, 0, s>>>(a, slots);
         if (hipGetLastError() != hipSuccess) return CO_ERR_CUDA;
     }
-    if (a.tk) {
-        if (a.tk >= 128 * n) {
-            const int64_t slots = slot_of(a.tk, 1, 128, a.n_seq) + 1;
-            attn_grad_kv_tiles<T, DP><<<dim3((unsigned)(slots * a.hkv)), 512, 0, s>>>(a, slots);
-        } else {
-            const int64_t slots = slot_of(a.tk, 1, 32, a.n_seq) + 1;
-            attn_grad_kv<T, DP><<<dim3((unsigned)((slots * a.hkv + 3) / 4)), 256, 0, s>>>(a, slots);
-        }
-    }
+    const int slots = slot_of(a.tk, 1, 128, a.n_seq) + 1;
+    attn_grad_kv_tiles<T, DP><<<dim3((unsigned)(slots * a.hkv)), 512, 0, s>>>(a, slots);
     return launch_status();
 }
 
