@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 import threading
 
 import numpy as np
@@ -77,6 +78,20 @@ class SeqPolicyLoss(ctypes.Structure):
                 ("workspace_bytes", _I64)]
 
 
+def _packer(structure):
+    """A ctypes structure's layout as a struct.Struct: a call packs its
+    arguments in one step, several times faster than filling the structure."""
+    codes = {_I32: "i", _I64: "q", _F: "f", _P: "P"}
+    p = struct.Struct("".join(codes[t] for _, t in structure._fields_))
+    assert p.size == ctypes.sizeof(structure)
+    return p.pack, p.size
+
+
+_pack_attention, _SIZE_ATTENTION = _packer(SeqAttention)
+_pack_attention_grad, _SIZE_ATTENTION_GRAD = _packer(SeqAttentionGrad)
+_pack_rotary, _SIZE_ROTARY = _packer(SeqRotary)
+_pack_policy, _SIZE_POLICY = _packer(SeqPolicyLoss)
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -89,6 +104,8 @@ def lib_path():
 def load_library() -> ctypes.CDLL:
     """Bind libcusr_seq.so once per process; raises when it is not built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lib_lock:
         if _lib is None:
             path = lib_path()
@@ -108,27 +125,27 @@ def load_library() -> ctypes.CDLL:
 
 
 def _run(fn, where, device, *structs):
-    """Call an entry point on the device's current stream."""
-    refs = [ctypes.addressof(s) for s in structs]
-    if device.index is None or device.index == torch.cuda.current_device():
-        rc = fn(*refs, torch.cuda.current_stream(device).cuda_stream)
+    """Call an entry point with packed structures on the device's current
+    stream (torch.cuda.current_stream without its wrapper object)."""
+    if device == torch.cuda.current_device():
+        rc = fn(*structs, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*refs, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*structs, torch._C._cuda_getCurrentRawStream(device))
     if rc != CO_OK:
         raise COError(rc, where)
 
 
-def _workspace(fn, where, struct, device):
-    """Scratch of a call from torch's allocator, on the current stream."""
-    n = fn(ctypes.addressof(struct))
-    if n < 0:
-        raise COError(int(-n if n == -2 else n), where)
-    if n == 0:
-        return None
+def _workspace(fn, where, packed, device):
+    """(pointer, bytes, owner) of a call's scratch, from torch's allocator on
+    the current stream."""
+    n = fn(packed)
+    if n <= 0:
+        if n:
+            raise COError(int(-n if n == -2 else n), where)
+        return None, 0, None
     ws = torch.empty(n, dtype=torch.uint8, device=device)
-    struct.workspace, struct.workspace_bytes = ws.data_ptr(), n
-    return ws
+    return ws.data_ptr(), n, ws
 
 
 def _need(x, name, dtypes, dim, device=None):
@@ -147,19 +164,40 @@ def _need(x, name, dtypes, dim, device=None):
 
 
 def _ptr(x):
-    return x.data_ptr() if x is not None and x.numel() else None
+    return 0 if x is None else x.data_ptr()
 
 
 def _heads16(x):
     """x as the kernels read it: the last dimension contiguous, rows and heads
     on 16-byte boundaries; another layout is copied once."""
-    if x.numel() == 0:
+    s0, s1, s2 = x.stride()
+    if s2 == 1 and not (s0 | s1) & 7 and not x.data_ptr() & 15:
         return x
-    s = x.stride()
-    if s[2] != 1 or s[0] % 8 or s[1] % 8 or x.data_ptr() % 16:
+    if x.numel():
         return x.contiguous() if x.shape[2] % 8 == 0 and not x.is_contiguous() else x.clone(
             memory_format=torch.contiguous_format)
     return x
+
+
+def _plain_attention(q, k, v, cu_q, cu_k, k_lens):
+    """Whether the common checks hold; _check_attention says which does not."""
+    try:
+        _, hq, d = q.shape
+        _, hkv, dk = k.shape
+        n, dev, dt = cu_q.shape[0], q.get_device(), q.dtype
+        return (dev >= 0 and q.is_cuda and dt in _HALF and k.dtype is dt and v.dtype is dt
+                and k.shape == v.shape and d == dk and hkv > 0 and hq > 0 and hq % hkv == 0
+                and d & 7 == 0 and 8 <= d <= SEQ_MAX_HEAD and k.get_device() == dev
+                and v.get_device() == dev and cu_q.dtype is torch.int32 and cu_q.dim() == 1
+                and n > 0 and cu_q.get_device() == dev
+                and (cu_k is None or cu_k is cu_q
+                     or (cu_k.dtype is torch.int32 and cu_k.shape == cu_q.shape
+                         and cu_k.get_device() == dev))
+                and (k_lens is None
+                     or (k_lens.dtype is torch.int32 and k_lens.dim() == 1
+                         and k_lens.shape[0] == n - 1 and k_lens.get_device() == dev)))
+    except (AttributeError, ValueError, TypeError, IndexError):
+        return False
 
 
 # ------------------------------------------------------------------ attention
@@ -168,6 +206,8 @@ _HALF = (torch.bfloat16, torch.float16)
 
 
 def _check_attention(q, k, v, cu_q, cu_k, k_lens, scale):
+    if _plain_attention(q, k, v, cu_q, cu_k, k_lens) and (scale is None or 0.0 < scale <= 1e30):
+        return
     _need(q, "q", _HALF, 3)
     dev = q.device
     _need(k, "k", (q.dtype,), 3, dev)
@@ -196,14 +236,13 @@ def _check_attention(q, k, v, cu_q, cu_k, k_lens, scale):
         raise ValueError(f"scale must be positive, not {scale}")
 
 
-def _attention_struct(q, k, v, o, lse, cu_q, cu_k, k_lens, scale):
+def _attention_args(q, k, v, o, lse, cu_q, cu_k, k_lens, scale):
     qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), o.stride()
-    return SeqAttention(ctypes.sizeof(SeqAttention), _DTYPES[q.dtype], cu_q.numel() - 1,
-                        q.shape[1], k.shape[1], q.shape[2], q.shape[0], k.shape[0],
-                        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1],
-                        scale, 0, _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse),
-                        cu_q.data_ptr(), cu_k.data_ptr(),
-                        None if k_lens is None else k_lens.data_ptr() or None, None, 0)
+    tq, hq, d = q.shape
+    return (_SIZE_ATTENTION, _DTYPES[q.dtype], cu_q.shape[0] - 1, hq, k.shape[1], d, tq,
+            k.shape[0], qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], scale, 0,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), cu_q.data_ptr(),
+            cu_k.data_ptr(), _ptr(k_lens))
 
 
 def _attention(q, k, v, cu_q, cu_k, k_lens, scale, return_lse):
@@ -211,14 +250,17 @@ def _attention(q, k, v, cu_q, cu_k, k_lens, scale, return_lse):
     cu_q = cu_q.contiguous()
     cu_k = cu_q if cu_k is None else cu_k.contiguous()
     k_lens = None if k_lens is None else k_lens.contiguous()
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) \
         if return_lse else None
     if q.shape[0]:
-        lib = load_library()
-        a = _attention_struct(q, k, v, o, lse, cu_q, cu_k, k_lens, scale)
-        ws = _workspace(lib.seq_attention_workspace, "seq_attention", a, q.device)
-        _run(lib.seq_attention, "seq_attention", q.device, a)
+        lib, dev = load_library(), q.get_device()
+        args = _attention_args(q, k, v, o, lse, cu_q, cu_k, k_lens, scale)
+        packed = _pack_attention(*args, 0, 0)
+        ptr, n, ws = _workspace(lib.seq_attention_workspace, "seq_attention", packed, q.device)
+        if n:
+            packed = _pack_attention(*args, ptr, n)
+        _run(lib.seq_attention, "seq_attention", dev, packed)
         del ws
     return o, lse
 
@@ -238,16 +280,18 @@ def attention_grad(do, q, k, v, o, lse, cu_q, cu_k=None, *, k_lens=None, scale=N
     cu_q, lse = cu_q.contiguous(), lse.contiguous()
     cu_k = cu_q if cu_k is None else cu_k.contiguous()
     k_lens = None if k_lens is None else k_lens.contiguous()
-    dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+    dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
     if q.shape[0] == 0 or k.shape[0] == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     lib = load_library()
-    a = _attention_struct(q, k, v, o, lse, cu_q, cu_k, k_lens, scale)
-    g = SeqAttentionGrad(ctypes.sizeof(SeqAttentionGrad), 0, *do.stride()[:2], *dq.stride()[:2],
-                         *dk.stride()[:2], *dv.stride()[:2], do.data_ptr(), dq.data_ptr(),
-                         dk.data_ptr(), dv.data_ptr())
-    ws = _workspace(lib.seq_attention_grad_workspace, "seq_attention_grad", a, q.device)
-    _run(lib.seq_attention_grad, "seq_attention_grad", q.device, a, g)
+    args = _attention_args(q, k, v, o, lse, cu_q, cu_k, k_lens, scale)
+    ptr, n, ws = _workspace(lib.seq_attention_grad_workspace, "seq_attention_grad",
+                            _pack_attention(*args, 0, 0), q.device)
+    packed = _pack_attention(*args, ptr or 0, n)
+    g = _pack_attention_grad(_SIZE_ATTENTION_GRAD, 0, *do.stride()[:2], *dq.stride()[:2],
+                             *dk.stride()[:2], *dv.stride()[:2], do.data_ptr(), dq.data_ptr(),
+                             dk.data_ptr(), dv.data_ptr())
+    _run(lib.seq_attention_grad, "seq_attention_grad", q.get_device(), packed, g)
     del ws
     return dq, dk, dv
 
@@ -336,25 +380,32 @@ def rotary_table(rot, positions, *, base=10000.0, scaling=None, factor=1.0, orig
 
 
 def _rotary(q, k, positions, table, interleaved, inverse, q_out=None, k_out=None):
-    q = q if q.stride(2) == 1 or q.shape[2] < 2 else q.contiguous()
-    if k is not None and k.stride(2) != 1 and k.shape[2] > 1:
-        k = k.contiguous()
+    tokens, hq, d = q.shape
+    qs = q.stride()
+    if qs[2] != 1 and d > 1:
+        q = q.contiguous()
+        qs = q.stride()
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if k is not None and k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    positions = positions.to(torch.int32).contiguous()
-    table = table.contiguous()
-    if q.shape[0]:
-        z = (0, 0)
-        r = SeqRotary(ctypes.sizeof(SeqRotary), _DTYPES[q.dtype], q.shape[1],
-                      0 if k is None else k.shape[1], q.shape[2], 2 * table.shape[1],
-                      int(interleaved), int(inverse), q.shape[0], table.shape[0],
-                      *q.stride()[:2], *(z if k is None else k.stride()[:2]),
-                      *q_out.stride()[:2], *(z if k is None else k_out.stride()[:2]),
-                      _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), positions.data_ptr(),
-                      _ptr(table))
-        _run(load_library().seq_rotary, "seq_rotary", q.device, r)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    hkv, ks, kos = 0, (0, 0), (0, 0)
+    if k is not None:
+        hkv, ks = k.shape[1], k.stride()
+        if ks[2] != 1 and d > 1:
+            k = k.contiguous()
+            ks = k.stride()
+        if k_out is None:
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        kos = k_out.stride()
+    if positions.dtype is not torch.int32:
+        positions = positions.to(torch.int32)
+    positions, table = positions.contiguous(), table.contiguous()
+    if tokens:
+        qos = q_out.stride()
+        r = _pack_rotary(_SIZE_ROTARY, _DTYPES[q.dtype], hq, hkv, d, 2 * table.shape[1],
+                         bool(interleaved), bool(inverse), tokens, table.shape[0], qs[0], qs[1],
+                         ks[0], ks[1], qos[0], qos[1], kos[0], kos[1], q.data_ptr(), _ptr(k),
+                         q_out.data_ptr(), _ptr(k_out), positions.data_ptr(), table.data_ptr())
+        _run(load_library().seq_rotary, "seq_rotary", q.get_device(), r)
     return q_out, k_out
 
 
@@ -383,6 +434,42 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, inplace=
     copied. inverse turns back, which is the gradient. inplace writes into q
     and k. A position outside the table gives NaN in its token's turned
     elements. Returns (q', k'), or q' alone when k is None."""
+    if not _plain_rotary(q, k, positions, table):
+        _check_rotary(q, k, positions, table)
+    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    if inplace:
+        if grad:
+            raise ValueError("inplace takes no part in autograd")
+        if q.stride(2) != 1 or (k is not None and k.stride(2) != 1):
+            raise ValueError("inplace needs heads that are contiguous")
+        out = _rotary(q, k, positions, table, interleaved, inverse, q, k)
+    elif grad:
+        return _RotaryFn.apply(q, k, positions, table, bool(interleaved), bool(inverse))
+    else:
+        out = _rotary(q, k, positions, table, interleaved, inverse)
+    return out if k is not None else out[0]
+
+
+def _plain_rotary(q, k, positions, table):
+    """Whether the common checks hold; _check_rotary says which does not."""
+    try:
+        tokens, _, d = q.shape
+        n, half, two = table.shape
+        dev, dt = q.get_device(), q.dtype
+        return (dev >= 0 and q.is_cuda and dt in _DTYPES and two == 2 and 2 * half <= d
+                and table.dtype is torch.float32 and table.get_device() == dev
+                and positions.dtype in _INTS and positions.dim() == 1
+                and positions.shape[0] == tokens and positions.get_device() == dev
+                and (k is None or (k.dtype is dt and k.dim() == 3 and k.shape[0] == tokens
+                                   and k.shape[2] == d and k.get_device() == dev)))
+    except (AttributeError, ValueError, TypeError, IndexError):
+        return False
+
+
+_INTS = (torch.int32, torch.int64)
+
+
+def _check_rotary(q, k, positions, table):
     _need(q, "q", tuple(_DTYPES), 3)
     dev = q.device
     if k is not None:
@@ -397,25 +484,33 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, inplace=
     if table.shape[2] != 2 or 2 * table.shape[1] > q.shape[2]:
         raise ValueError(f"table must be [positions, rot/2, 2] with rot up to the head size "
                          f"{q.shape[2]}; got {tuple(table.shape)}")
-    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
-    if inplace:
-        if grad:
-            raise ValueError("inplace takes no part in autograd")
-        if q.stride(2) != 1 or (k is not None and k.stride(2) != 1):
-            raise ValueError("inplace needs heads that are contiguous")
-        out = _rotary(q, k, positions, table, interleaved, inverse, q, k)
-    elif grad:
-        out = _RotaryFn.apply(q, k, positions, table, bool(interleaved), bool(inverse))
-        return out
-    else:
-        out = _rotary(q, k, positions, table, interleaved, inverse)
-    return out if k is not None else out[0]
 
 
 # ---------------------------------------------------------------- policy loss
 
+def _plain_policy(logits, actions, given, maybe):
+    """Whether the common checks hold; _check_policy says which does not."""
+    try:
+        T, V = logits.shape
+        dev = logits.get_device()
+        if not (dev >= 0 and logits.is_cuda and V > 0 and logits.dtype in _DTYPES
+                and actions.dtype in _INTS and actions.shape == (T,)
+                and actions.get_device() == dev):
+            return False
+        for x in given + tuple(x for x in maybe if x is not None):
+            if x.dtype is not torch.float32 or x.shape != (T,) or x.get_device() != dev:
+                return False
+        return True
+    except (AttributeError, ValueError, TypeError):
+        return False
+
+
 def _check_policy(logits, actions, logp_old, advantages, logp_ref, weights, clip, kl_coef,
                   temperature):
+    lo, hi = (float(c) for c in clip)
+    if (_plain_policy(logits, actions, (logp_old, advantages), (logp_ref, weights))
+            and lo >= 0 and hi >= 0 and 0 < temperature < math.inf and math.isfinite(kl_coef)):
+        return lo, hi
     _need(logits, "logits", tuple(_DTYPES), 2)
     T, V = logits.shape
     dev = logits.device
@@ -429,7 +524,6 @@ def _check_policy(logits, actions, logp_old, advantages, logp_ref, weights, clip
     for name, x in named + [("actions", actions)]:
         if x.numel() != T:
             raise ValueError(f"{name} must have {T} entries, not {x.numel()}")
-    lo, hi = (float(c) for c in clip)
     if not (lo >= 0 and hi >= 0):
         raise ValueError(f"clip must be two widths of at least 0; got {clip}")
     if not (temperature > 0 and math.isfinite(temperature)):
@@ -444,7 +538,9 @@ def _policy(logits, actions, logp_old, advantages, logp_ref, weights, clip, kl_c
     T, V = logits.shape
     if V > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
-    actions = actions.to(torch.int64).contiguous()
+    if actions.dtype is not torch.int64:
+        actions = actions.to(torch.int64)
+    actions = actions.contiguous()
     logp_old, advantages = logp_old.contiguous(), advantages.contiguous()
     logp_ref = None if logp_ref is None else logp_ref.contiguous()
     weights = torch.full((T,), 1.0 / max(T, 1), device=logits.device) if weights is None \
@@ -453,13 +549,14 @@ def _policy(logits, actions, logp_old, advantages, logp_ref, weights, clip, kl_c
     logp = torch.empty(T, dtype=torch.float32, device=logits.device)
     dlogits = torch.empty((T, V), dtype=logits.dtype, device=logits.device) if grad else None
     lib = load_library()
-    p = SeqPolicyLoss(ctypes.sizeof(SeqPolicyLoss), _DTYPES[logits.dtype], T, V,
-                      logits.stride(0), V, *clip, float(kl_coef), float(temperature),
-                      _ptr(logits), _ptr(actions), _ptr(logp_old), _ptr(logp_ref),
-                      _ptr(advantages), _ptr(weights), _ptr(dloss), loss.data_ptr(), _ptr(logp),
-                      _ptr(dlogits), None, 0)
-    ws = _workspace(lib.seq_policy_loss_workspace, "seq_policy_loss", p, logits.device)
-    _run(lib.seq_policy_loss, "seq_policy_loss", logits.device, p)
+    args = (_SIZE_POLICY, _DTYPES[logits.dtype], T, V, logits.stride(0), V, *clip, kl_coef,
+            temperature, logits.data_ptr(), actions.data_ptr(), logp_old.data_ptr(),
+            _ptr(logp_ref), advantages.data_ptr(), weights.data_ptr(), _ptr(dloss),
+            loss.data_ptr(), logp.data_ptr(), _ptr(dlogits))
+    ptr, n, ws = _workspace(lib.seq_policy_loss_workspace, "seq_policy_loss",
+                            _pack_policy(*args, 0, 0), logits.device)
+    _run(lib.seq_policy_loss, "seq_policy_loss", logits.get_device(),
+         _pack_policy(*args, ptr or 0, n))
     del ws
     return loss, logp, dlogits
 
