@@ -8,15 +8,19 @@ namespace seq {
 template <typename T, int DP>
 __device__ inline void store_out(const Attn &a, int t, int head, const float16v *o, float m,
                                  float l, bool ok) {
-    store_row<T, DP>(a.o, t * a.o_row + head * a.o_head, o, l == 0.0f ? 0.0f : 1.0f / l, a.d, ok);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    store_row<T, DP>(a.o, t * a.o_row + head * a.o_head, o, inv, a.d, ok);
+    if (a.o_low)
+        store_row<T, DP, true>(a.o_low, ((int64_t)t * a.hq + head) * a.d, o, inv, a.d, ok);
     if (a.lse && ok && (threadIdx.x & 63) < 32)
         a.lse[head * a.tq + t] = l == 0.0f ? neg_inf() : m * a.scale + logf(l);
 }
 
 // A wave's tile of 32 rows over the keys key0 .. key1-1, 32 at a time with a
-// running maximum and sum. AHEAD: the next 32 keys are loaded while the present
-// ones are worked on, at the price of their registers. K comes straight from memory as the left operand; V passes
-// through the wave's own LDS tile to be transposed.
+// running maximum and sum. K comes straight from memory as the left operand; V
+// passes through the wave's own LDS tile to be transposed. AHEAD: the next 32 keys
+// are loaded while the present ones are worked on, V in registers too; without it
+// V goes to LDS past the registers, which leaves room for more waves.
 struct Row { int t, head; bool ok; };
 template <typename T, int DP, bool AHEAD>
 __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, int key0, int key1,
@@ -36,8 +40,11 @@ __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, 
     // keys beyond the last repeat it: their scores are masked
     auto fetch = [&](int k0) {
         const int r = min(k0 + (lane & 31), end - 1);
+        if (!AHEAD)
+            copy_tile<DP>(vp, a.d, lds_address(vt),
+                          [&](int i) { return min(k0 + i, end - 1) * a.v_row; });
         load_row<DP>(k, kp, r * a.k_row, a.d, true);
-        load_row<DP>(v, vp, r * a.v_row, a.d, true);
+        if (AHEAD) load_row<DP>(v, vp, r * a.v_row, a.d, true);
     };
     if (key0 < end) fetch(key0);
     load_row<DP>(q, a.q, (p.q0 + qi) * a.q_row + head * a.q_head, a.d, ok);
@@ -51,10 +58,12 @@ __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, 
         float16v s = {};
 #pragma unroll
         for (int c = 0; c < DP / 16; c++) s = T::mfma(k[c], q[c], s);
-        wave_sync();
+        if (AHEAD) {
+            wave_sync();
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++)
-            *(uint4v *)(vt + Tile<DP>::at(lane & 31, 2 * c + h)) = v[c];
+            for (int c = 0; c < DP / 16; c++)
+                *(uint4v *)(vt + Tile<DP>::at(lane & 31, 2 * c + h)) = v[c];
+        }
         if (AHEAD && k0 + 32 < end) fetch(k0 + 32);
         float mx = neg_inf();
 #pragma unroll
@@ -79,7 +88,8 @@ __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, 
         m = mn;
 #pragma unroll
         for (int dt = 0; dt < DP / 32; dt++) o[dt] *= alpha;
-        wave_sync();
+        if (AHEAD) wave_sync();
+        else wait_copies<0>();
 #pragma unroll
         for (int kc = 0; kc < 2; kc++) {
             const uint4v pb = {pk[4 * kc], pk[4 * kc + 1], pk[4 * kc + 2], pk[4 * kc + 3]};
@@ -100,7 +110,7 @@ __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, 
 constexpr int kShortRows = 128;
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attn_wave(Attn a, int slots) {
-    __shared__ __align__(16) uint16_t lds[4][32 * Tile<DP>::stride];
+    __shared__ __align__(256) uint16_t lds[4][32 * Tile<DP>::stride];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint16_t *vt = lds[wave];
     const int item = blockIdx.x * 4 + wave;
@@ -329,8 +339,13 @@ __global__ __launch_bounds__(256) void attn_join(Attn a, Step st) {
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     typename T::elem *out = (typename T::elem *)a.o + t * a.o_row + head * a.o_head;
+    typename T::elem *low = (typename T::elem *)a.o_low + (int64_t)item * a.d;
     for (int e = 0; e < (DP + 63) / 64; e++)
-        if (lane + 64 * e < a.d) out[lane + 64 * e] = (typename T::elem)(acc[e] * inv);
+        if (lane + 64 * e < a.d) {
+            const float x = acc[e] * inv;
+            out[lane + 64 * e] = (typename T::elem)x;
+            if (a.o_low) low[lane + 64 * e] = (typename T::elem)(x - (float)(typename T::elem)x);
+        }
     if (a.lse && lane == 0)
         a.lse[head * a.tq + t] = l == 0.0f ? neg_inf() : m * a.scale + logf(l);
 }
@@ -422,7 +437,8 @@ int check_attention_data(const SeqAttention *a) {
     if (!a->cu_q || !a->cu_k || !a->q || !a->o || (a->tk && (!a->k || !a->v)))
         return CO_ERR_NULLARG;
     if (misaligned(a->q, a->q_row, a->q_head) || misaligned(a->k, a->k_row, a->k_head) ||
-        misaligned(a->v, a->v_row, a->v_head) || misaligned(a->o, a->o_row, a->o_head))
+        misaligned(a->v, a->v_row, a->v_head) || misaligned(a->o, a->o_row, a->o_head) ||
+        ((uintptr_t)a->o_low & 15))
         return CO_ERR_DATA;
     return CO_OK;
 }

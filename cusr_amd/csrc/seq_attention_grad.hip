@@ -41,21 +41,24 @@ __device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float
 }
 
 // Short sequences: a wave owns up to 128 rows of a sequence and key head, and
-// every so many tiles of 32 of its keys; most have a sequence to themselves, read
-// it once (the second part finds it in the caches, or, when it is one tile, in
-// the registers) and need no statistics from another kernel. First the rows:
-// delta, then dQ^T = sum over keys of K^T dS^T, from S^T. Then the keys:
-// dV^T = dO^T P and dK^T = Q^T dS, from S formed the other way round: the same
-// registers are the left or the right operand.
+// every so many tiles of 32 of its keys; most have a sequence to themselves and
+// need no statistics from another kernel. First the rows: delta = sum of P dP,
+// which needs no o, then dQ^T = sum over keys of K^T dS^T, from S^T. Then the
+// keys: dV^T = dO^T P and dK^T = Q^T dS, from S formed the other way round: the
+// same tiles are the left or the right operand. The side that is summed over
+// passes through LDS, past the registers. What bounds it is memory, and before
+// that the chain of loads from the slot to the rows, so registers are kept few.
 constexpr int kShortRows = 128;
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_grad_short(AttnGrad a, int slots) {
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : (DP == 96 ? 2 : 1))
+void attn_grad_short(AttnGrad a, int slots) {
     constexpr int C = DP / 16, S = Tile<DP>::stride;
-    __shared__ __align__(16) uint16_t lds[4][2 * 32 * S];
+    __shared__ __align__(256) uint16_t lds[4][2][32 * S];
     __shared__ __align__(16) float stats[4][3][kShortRows];     // lse, delta, last visible key
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    uint16_t *ta = lds[wave], *tb = ta + 32 * S;
+    const uint16_t *ta = lds[wave][0], *tb = lds[wave][1];
+    const uint32_t ta_at = lds_address(ta), tb_at = lds_address(tb);
     float *lses = stats[wave][0], *deltas = stats[wave][1];
     int *lims = (int *)stats[wave][2];
     const int item = blockIdx.x * 4 + wave;
@@ -76,113 +79,131 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_grad_short(AttnGra
     const float inv = 1.0f / (float)a.G;
     const uint16_t *kp = (const uint16_t *)a.k + p.k0 * a.k_row + hk * a.k_head;
     const uint16_t *vp = (const uint16_t *)a.v + p.k0 * a.v_row + hk * a.v_head;
-    uint4v q[C], dO[C], k[C], v[C];
-    struct { int t, head, lim; bool ok; } r;
-    auto row_of = [&](int tile) {
-        const int row = tile * 32 + (lane & 31);
-        r.ok = row < rows;
-        const int qi = divide(r.ok ? row : 0, a.G, inv);
-        r.t = p.q0 + qi;
-        r.head = hk * a.G + (r.ok ? row - qi * a.G : 0);
-        r.lim = r.ok ? qi + shift : -1;
-    };
-    auto load_rows = [&]() {
-        load_row<DP>(q, a.q, r.t * a.q_row + r.head * a.q_head, a.d, r.ok);
-        load_row<DP>(dO, a.g.d_o, r.t * a.g.do_row + r.head * a.g.do_head, a.d, r.ok);
-    };
-    // statistics of this lane's row, to LDS at `at`
-    auto put_stats = [&](int at, float &lse2, float &delta) {
-        uint4v o[C];
-        load_row<DP>(o, a.o, r.t * a.o_row + r.head * a.o_head, a.d, r.ok);
-        lse2 = r.ok ? a.lse[r.head * a.tq + r.t] * kLog2e : 0.0f;
-        delta = add_halves(dot_row<T>(o, dO, C));
-        if (h == 0) {
-            lses[at + lane] = lse2;
-            deltas[at + lane] = delta;
-            lims[at + lane] = r.lim;
-        }
-    };
+    const uint16_t *qp = (const uint16_t *)a.q + p.q0 * a.q_row + hk * a.G * a.q_head;
+    const uint16_t *dop = (const uint16_t *)a.g.d_o + p.q0 * a.g.do_row + hk * a.G * a.g.do_head;
 
     for (int tile = mine * 4; tile < mine * 4 + 4 && tile < tiles; tile++) {
-        row_of(tile);
         const int end = divide(min(tile * 32 + 31, rows - 1), a.G, inv) + shift + 1;
-        auto load_keys = [&](int k0) {       // beyond the last, the last again: masked
-            const int i = min(k0 + (lane & 31), end - 1);
-            load_row<DP>(k, kp, i * a.k_row, a.d, true);
-            load_row<DP>(v, vp, i * a.v_row, a.d, true);
+        auto copy_keys = [&](int k0) {       // beyond the last, the last again: masked
+            copy_tile<DP>(kp, a.d, ta_at, [&](int i) { return min(k0 + i, end - 1) * a.k_row; });
+            copy_tile<DP>(vp, a.d, tb_at, [&](int i) { return min(k0 + i, end - 1) * a.v_row; });
         };
-        load_rows();
-        if (end > 0) load_keys(0);
-        float lse2, delta;
-        put_stats((tile & 3) * 32, lse2, delta);
+        if (end > 0) copy_keys(0);
+        const int row = tile * 32 + (lane & 31);
+        const bool ok = row < rows;
+        const int qi = divide(ok ? row : 0, a.G, inv), g = ok ? row - qi * a.G : 0;
+        const int lim = ok ? qi + shift : -1;
+        uint4v q[C], dO[C];
+        load_row<DP>(q, qp, qi * a.q_row + g * a.q_head, a.d, ok);
+        load_row<DP>(dO, dop, qi * a.g.do_row + g * a.g.do_head, a.d, ok);
+        const float lse2 = ok ? a.lse[(hk * a.G + g) * a.tq + p.q0 + qi] * kLog2e : 0.0f;
+        float delta = 0.0f;
         float16v dq[DP / 32] = {};
-        for (int k0 = 0; k0 < end; k0 += 32) {
-            if (k0) load_keys(k0);
-            wave_sync();
+        // P and P dP of 32 keys, from the tiles; unseen keys give 0
+        auto products = [&](int k0, float16v &s, float16v &dp) {
+            s = dp = float16v{};
 #pragma unroll
-            for (int c = 0; c < C; c++) *(uint4v *)(ta + Tile<DP>::at(lane & 31, 2 * c + h)) = k[c];
-            float16v s = {}, dp = {};
+            for (int c = 0; c < C; c++) s = T::mfma(Tile<DP>::row(ta, 0, c), q[c], s);
 #pragma unroll
-            for (int c = 0; c < C; c++) s = T::mfma(k[c], q[c], s);
+            for (int c = 0; c < C; c++) dp = T::mfma(Tile<DP>::row(tb, 0, c), dO[c], dp);
 #pragma unroll
-            for (int c = 0; c < C; c++) dp = T::mfma(v[c], dO[c], dp);
-            uint32_t pk[8];
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                float ds[2];
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int key = k0 + 8 * (i / 4) + 4 * h + (i + j) % 4;
-                    const float pr = exp2_fast(__builtin_fmaf(s[i + j], a.c, -lse2));
-                    ds[j] = key <= r.lim ? pr * (dp[i + j] - delta) : 0.0f;
-                }
-                pk[i / 2] = T::pack(ds[0], ds[1]);
+            for (int i = 0; i < 16; i++) {
+                const int key = k0 + 8 * (i / 4) + 4 * h + i % 4;
+                s[i] = key <= lim ? exp2_fast(__builtin_fmaf(s[i], a.c, -lse2)) : 0.0f;
+                dp[i] = key <= lim ? s[i] * dp[i] : 0.0f;
             }
-            wave_sync();
+        };
+        auto add = [&](const float16v &s, const float16v &dp) {
 #pragma unroll
             for (int kc = 0; kc < 2; kc++) {
-                const uint4v pb = {pk[4 * kc], pk[4 * kc + 1], pk[4 * kc + 2], pk[4 * kc + 3]};
+                uint4v pb;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int i = 8 * kc + 2 * j;
+                    pb[j] = T::pack(dp[i] - s[i] * delta, dp[i + 1] - s[i + 1] * delta);
+                }
 #pragma unroll
                 for (int dt = 0; dt < DP / 32; dt++)
                     dq[dt] = T::mfma(Tile<DP>::transposed(ta, kc * 16, dt), pb, dq[dt]);
             }
+        };
+        float16v s, dp;
+        for (int k0 = 0; k0 < end; k0 += 32) {
+            if (k0) copy_keys(k0);
+            wait_copies<0>();
+            products(k0, s, dp);
+#pragma unroll
+            for (int i = 0; i < 16; i++) delta += dp[i];
         }
-        store_row<T, DP>(a.g.dq, r.t * a.g.dq_row + r.head * a.g.dq_head, dq, a.scale, a.d, r.ok);
+        delta = add_halves(delta);
+        if (end > 0 && end <= 32) {
+            add(s, dp);
+        } else {                             // once more, with delta
+            for (int k0 = 0; k0 < end; k0 += 32) {
+                copy_keys(k0);
+                wait_copies<0>();
+                products(k0, s, dp);
+                add(s, dp);
+            }
+        }
+        const int64_t t = p.q0 + qi, head = hk * a.G + g;
+        store_row<T, DP>(a.g.dq, t * a.g.dq_row + head * a.g.dq_head, dq, a.scale, a.d, ok);
+        if (h == 0) {
+            lses[(tile & 3) * 32 + lane] = lse2;
+            deltas[(tile & 3) * 32 + lane] = delta;
+            lims[(tile & 3) * 32 + lane] = lim;
+        }
     }
 
-    const bool kept = tiles == 1 && s1 - s0 <= 32 && s0 == p.k0 && p.lk > 0;
     for (int kt = mine; kt * 32 < s1 - s0; kt += shares) {
         const int kr = s0 + kt * 32 + (lane & 31);               // this lane's key row
         const int key0 = kt * 32 + s0 - p.k0, key = key0 + (lane & 31);
         const bool live = kr < s1 && key >= 0 && key < p.lk;
         float16v dk[DP / 32] = {}, dv[DP / 32] = {};
         if (key0 < p.lk) {
-            if (!kept) {
-                load_row<DP>(k, kp, key * a.k_row, a.d, live);
-                load_row<DP>(v, vp, key * a.v_row, a.d, live);
-            }
+            uint4v k[C], v[C];
+            load_row<DP>(k, kp, key * a.k_row, a.d, live);
+            load_row<DP>(v, vp, key * a.v_row, a.d, live);
             for (int tile = max(key0 - shift, 0) * a.G / 32; tile < tiles; tile++) {
                 int at = (tile & 3) * 32;
-                if (!kept) {
-                    row_of(tile);
-                    load_rows();
+                // rows beyond the last repeat it: their last visible key is -1
+                auto row_at = [&](int i, int64_t step, int64_t head) {
+                    const int row = min(tile * 32 + i, rows - 1), qi = divide(row, a.G, inv);
+                    return qi * step + (row - qi * a.G) * head;
+                };
+                copy_tile<DP>(qp, a.d, ta_at, [&](int i) { return row_at(i, a.q_row, a.q_head); });
+                copy_tile<DP>(dop, a.d, tb_at,
+                              [&](int i) { return row_at(i, a.g.do_row, a.g.do_head); });
+                if (shares > 1) {
+                    // the rows may be another wave's: delta from o, and what its
+                    // type rounded away if that is kept
+                    const int row = tile * 32 + (lane & 31);
+                    const bool ok = row < rows;
+                    const int qi = divide(ok ? row : 0, a.G, inv), g = ok ? row - qi * a.G : 0;
+                    const int64_t t = p.q0 + qi, head = hk * a.G + g;
+                    uint4v x[C], y[C];
+                    load_row<DP>(x, a.o, t * a.o_row + head * a.o_head, a.d, ok);
+                    load_row<DP>(y, dop, qi * a.g.do_row + g * a.g.do_head, a.d, ok);
+                    float delta = dot_row<T>(x, y, C);
+                    if (a.o_low) {
+                        load_row<DP>(x, a.o_low, (t * a.hq + head) * a.d, a.d, ok);
+                        delta += dot_row<T>(x, y, C);
+                    }
+                    delta = add_halves(delta);
+                    at = 0;
+                    wave_sync();
+                    if (h == 0) {
+                        lses[lane] = ok ? a.lse[head * a.tq + t] * kLog2e : 0.0f;
+                        deltas[lane] = delta;
+                        lims[lane] = ok ? qi + shift : -1;
+                    }
                 }
-                wave_sync();
-                if (shares > 1) {            // the rows may be another wave's
-                    float x, y;
-                    put_stats(at = 0, x, y);
-                }
-#pragma unroll
-                for (int c = 0; c < C; c++) {
-                    *(uint4v *)(ta + Tile<DP>::at(lane & 31, 2 * c + h)) = q[c];
-                    *(uint4v *)(tb + Tile<DP>::at(lane & 31, 2 * c + h)) = dO[c];
-                }
+                wait_copies<0>();
                 float16v s = {}, dp = {};
 #pragma unroll
-                for (int c = 0; c < C; c++) s = T::mfma(q[c], k[c], s);
+                for (int c = 0; c < C; c++) s = T::mfma(Tile<DP>::row(ta, 0, c), k[c], s);
 #pragma unroll
-                for (int c = 0; c < C; c++) dp = T::mfma(dO[c], v[c], dp);
-                wave_sync();
+                for (int c = 0; c < C; c++) dp = T::mfma(Tile<DP>::row(tb, 0, c), v[c], dp);
                 uint32_t pp[8], pd[8];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -250,7 +271,12 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, i
     float delta, lse2;
     load_row<DP>(dO, a.g.d_o, t * a.g.do_row + head * a.g.do_head, a.d, ok);
     load_row<DP>(q, a.o, t * a.o_row + head * a.o_head, a.d, ok);
-    delta = add_halves(dot_row<T>(q, dO, DP / 16));
+    delta = dot_row<T>(q, dO, DP / 16);
+    if (a.o_low) {
+        load_row<DP>(q, a.o_low, ((int64_t)t * a.hq + head) * a.d, a.d, ok);
+        delta += dot_row<T>(q, dO, DP / 16);
+    }
+    delta = add_halves(delta);
     lse2 = ok ? a.lse[head * a.tq + t] * kLog2e : 0.0f;
     put_stat(a, head * a.tq + t, lse2, delta, ok);
     load_row<DP>(q, a.q, t * a.q_row + head * a.q_head, a.d, ok);
@@ -567,6 +593,7 @@ extern "C" int seq_attention_grad(const SeqAttention *sa, const SeqAttentionGrad
     if ((sa->tq && (!sa->lse || !g->d_o || !g->dq || !sa->workspace)) ||
         (sa->tk && (!g->dk || !g->dv)))
         return CO_ERR_NULLARG;
+    if ((uintptr_t)sa->o_low & 15) return CO_ERR_DATA;
     if (((uintptr_t)g->d_o | (uintptr_t)g->dq | (uintptr_t)g->dk | (uintptr_t)g->dv) & 15)
         return CO_ERR_DATA;
     if ((g->do_row | g->do_head | g->dq_row | g->dq_head | g->dk_row | g->dk_head | g->dv_row |

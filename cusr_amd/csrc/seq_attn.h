@@ -325,8 +325,9 @@ __device__ inline void load_row(uint4v *f, const void *base, int64_t off, int d,
 }
 
 // A column of a transposed accumulator (DP values of this lane's row, split
-// between the halves) scaled, packed and stored as 16-byte pieces.
-template <typename T, int DP>
+// between the halves) scaled, packed and stored as 16-byte pieces. LOW: what the
+// packing rounds away instead.
+template <typename T, int DP, bool LOW = false>
 __device__ inline void store_row(void *base, int64_t off, const float16v *acc, float scale, int d,
                                  bool ok) {
     const int h = (threadIdx.x & 63) >> 5;
@@ -337,8 +338,12 @@ __device__ inline void store_row(void *base, int64_t off, const float16v *acc, f
         for (int g = 0; g < 2; g++) {
             uint32_t x[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                x[j] = T::pack(acc[dt][8 * g + 2 * j] * scale, acc[dt][8 * g + 2 * j + 1] * scale);
+            for (int j = 0; j < 4; j++) {
+                const float u = acc[dt][8 * g + 2 * j] * scale;
+                const float w = acc[dt][8 * g + 2 * j + 1] * scale;
+                x[j] = T::pack(u, w);
+                if (LOW) x[j] = T::pack(u - T::lo(x[j]), w - T::hi(x[j]));
+            }
             // halves hold columns 0-3, 8-11 and 4-7, 12-15: after the exchange
             // 0-7 and 8-15
             auto s0 = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
@@ -347,6 +352,22 @@ __device__ inline void store_row(void *base, int64_t off, const float16v *acc, f
             const int col = dt * 32 + g * 16 + h * 8;
             if (d == DP ? ok : ok && col < d) *(uint4v *)(p + col) = v;
         }
+}
+
+// 32 rows of a tensor to a wave's LDS tile, past the registers: row_offset(i)
+// is row i's element offset from `base`. Columns beyond d repeat the first.
+template <int DP, typename F>
+__device__ inline void copy_tile(const void *base, int d, uint32_t to, F row_offset) {
+    constexpr int STRIDE = Tile<DP>::stride * 2, ROWS = 1024 / STRIDE;
+    const int lane = threadIdx.x & 63;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the tile's last reads are done
+#pragma unroll
+    for (int x = 0; x < 32 / ROWS; x++) {
+        const int r = x * ROWS + lane * 16 / STRIDE;
+        const int ch = (lane * 16 % STRIDE / 16) ^ Tile<DP>::swz(r);
+        copy_to_lds16((const uint16_t *)base + row_offset(r) + (ch * 8 < d ? ch * 8 : 0),
+                      to + x * 1024);
+    }
 }
 
 inline Attn make_attn(const SeqAttention *s) {

@@ -46,7 +46,7 @@ class SeqAttention(ctypes.Structure):
                 ("q_row", _I64), ("q_head", _I64), ("k_row", _I64), ("k_head", _I64),
                 ("v_row", _I64), ("v_head", _I64), ("o_row", _I64), ("o_head", _I64),
                 ("scale", _F), ("reserved", _I32), ("q", _P), ("k", _P), ("v", _P), ("o", _P),
-                ("lse", _P), ("cu_q", _P), ("cu_k", _P), ("k_lens", _P), ("workspace", _P),
+                ("lse", _P), ("o_low", _P), ("cu_q", _P), ("cu_k", _P), ("k_lens", _P), ("workspace", _P),
                 ("workspace_bytes", _I64)]
 
 
@@ -236,13 +236,13 @@ def _check_attention(q, k, v, cu_q, cu_k, k_lens, scale):
         raise ValueError(f"scale must be positive, not {scale}")
 
 
-def _attention_args(q, k, v, o, lse, cu_q, cu_k, k_lens, scale):
+def _attention_args(q, k, v, o, lse, low, cu_q, cu_k, k_lens, scale):
     qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), o.stride()
     tq, hq, d = q.shape
     return (_SIZE_ATTENTION, _DTYPES[q.dtype], cu_q.shape[0] - 1, hq, k.shape[1], d, tq,
             k.shape[0], qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], scale, 0,
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), cu_q.data_ptr(),
-            cu_k.data_ptr(), _ptr(k_lens))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), _ptr(low),
+            cu_q.data_ptr(), cu_k.data_ptr(), _ptr(k_lens))
 
 
 def _attention(q, k, v, cu_q, cu_k, k_lens, scale, return_lse):
@@ -253,9 +253,15 @@ def _attention(q, k, v, cu_q, cu_k, k_lens, scale, return_lse):
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) \
         if return_lse else None
+    low, n_seq = None, cu_q.shape[0] - 1
+    if return_lse and (k.shape[0] >= 128 * n_seq
+                       or q.shape[0] * q.shape[1] > 64 * n_seq * k.shape[1]):
+        # The gradient of sequences this long takes sum(o * do) from o: it gets the
+        # part of o that o's type rounds away. Shorter ones form the sum anew.
+        low = lse.o_low = torch.empty_like(o)
     if q.shape[0]:
         lib, dev = load_library(), q.get_device()
-        args = _attention_args(q, k, v, o, lse, cu_q, cu_k, k_lens, scale)
+        args = _attention_args(q, k, v, o, lse, low, cu_q, cu_k, k_lens, scale)
         packed = _pack_attention(*args, 0, 0)
         ptr, n, ws = _workspace(lib.seq_attention_workspace, "seq_attention", packed, q.device)
         if n:
@@ -268,7 +274,9 @@ def _attention(q, k, v, cu_q, cu_k, k_lens, scale, return_lse):
 def attention_grad(do, q, k, v, o, lse, cu_q, cu_k=None, *, k_lens=None, scale=None):
     """(dq, dk, dv) of attention for the gradient `do` of its output; o and
     lse are what attention(..., return_lse=True) gave. The same call gives the
-    same bits."""
+    same bits. lse comes with an attribute o_low where it helps: what o's type
+    rounded away of it. A copy of lse without it gives gradients of long
+    sequences that are off by up to half as much again."""
     _check_attention(q, k, v, cu_q, cu_k, k_lens, scale)
     _need(do, "do", (q.dtype,), 3, q.device)
     _need(o, "o", (q.dtype,), 3, q.device)
@@ -276,6 +284,10 @@ def attention_grad(do, q, k, v, o, lse, cu_q, cu_k=None, *, k_lens=None, scale=N
     if do.shape != q.shape or o.shape != q.shape or lse.shape != (q.shape[1], q.shape[0]):
         raise ValueError("do and o must be like q, and lse [heads, rows]")
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    low = getattr(lse, "o_low", None)
+    if low is not None and (low.shape != q.shape or low.dtype != q.dtype
+                            or low.device != q.device or not low.is_contiguous()):
+        raise ValueError("lse.o_low does not belong to this call")
     q, k, v, o, do = (_heads16(x) for x in (q, k, v, o, do))
     cu_q, lse = cu_q.contiguous(), lse.contiguous()
     cu_k = cu_q if cu_k is None else cu_k.contiguous()
@@ -284,7 +296,7 @@ def attention_grad(do, q, k, v, o, lse, cu_q, cu_k=None, *, k_lens=None, scale=N
     if q.shape[0] == 0 or k.shape[0] == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     lib = load_library()
-    args = _attention_args(q, k, v, o, lse, cu_q, cu_k, k_lens, scale)
+    args = _attention_args(q, k, v, o, lse, low, cu_q, cu_k, k_lens, scale)
     ptr, n, ws = _workspace(lib.seq_attention_grad_workspace, "seq_attention_grad",
                             _pack_attention(*args, 0, 0), q.device)
     packed = _pack_attention(*args, ptr or 0, n)
@@ -300,14 +312,17 @@ class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, k_lens, scale):
         o, lse = _attention(q, k, v, cu_q, cu_k, k_lens, scale, True)
-        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k, k_lens)
+        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k, k_lens, getattr(lse, "o_low", None))
         ctx.scale = scale
         ctx.mark_non_differentiable(lse)
         return o, lse
 
     @staticmethod
     def backward(ctx, do, _):
-        q, k, v, o, lse, cu_q, cu_k, k_lens = ctx.saved_tensors
+        q, k, v, o, lse, cu_q, cu_k, k_lens, low = ctx.saved_tensors
+        if low is not None:
+            lse = lse.detach()
+            lse.o_low = low
         return (*attention_grad(do, q, k, v, o, lse, cu_q, cu_k, k_lens=k_lens,
                                 scale=ctx.scale), None, None, None, None)
 

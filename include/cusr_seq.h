@@ -50,7 +50,10 @@ extern "C" {
  * are clamped into the tensors. scale is positive.
  *
  * lse (may be null for the forward) [hq, tq] fp32: log of the sum of
- * exp(scale q.k) over the visible keys. */
+ * exp(scale q.k) over the visible keys. o_low (may be null): what rounding o to
+ * its type took away, itself rounded to it. A gradient needs sum(o * d_o) of each
+ * row; from o alone its error is that of o's rounding and goes into every key of
+ * the row alike. */
 typedef struct SeqAttention {
     int32_t struct_size;
     int32_t dtype;
@@ -62,6 +65,7 @@ typedef struct SeqAttention {
     const void *q, *k, *v;
     void *o;
     float *lse;
+    void *o_low;              /* null, or [tq, hq, d], contiguous */
     const int32_t *cu_q, *cu_k, *k_lens;
     void *workspace;          /* seq_attention_workspace bytes, 256-aligned */
     int64_t workspace_bytes;
@@ -72,7 +76,7 @@ typedef struct SeqAttention {
 int64_t seq_attention_workspace(const SeqAttention *a);
 int seq_attention(const SeqAttention *a, void *stream);
 
-/* Gradient of seq_attention: a's q, k, v, o, lse and offsets as the forward
+/* Gradient of seq_attention: a's q, k, v, o, lse, o_low and offsets as the forward
  * call had them; d_o is the gradient of o. dq, dk, dv as q, k, v. Rows of dk and dv
  * that no query sees are 0. No atomics: the same call gives the same bits. */
 typedef struct SeqAttentionGrad {
