@@ -109,7 +109,7 @@ __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, 
 // slot to the rows.
 constexpr int kShortRows = 128;
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attn_wave(Attn a, int slots) {
+__global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void attn_wave(Attn a, int slots) {
     __shared__ __align__(256) uint16_t lds[4][32 * Tile<DP>::stride];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint16_t *vt = lds[wave];

@@ -50,15 +50,15 @@ __device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float
 // that the chain of loads from the slot to the rows, so registers are kept few.
 constexpr int kShortRows = 128;
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 64 ? 3 : (DP == 96 ? 2 : 1))
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1)
 void attn_grad_short(AttnGrad a, int slots) {
     constexpr int C = DP / 16, S = Tile<DP>::stride;
-    __shared__ __align__(256) uint16_t lds[4][2][32 * S];
+    __shared__ __align__(256) uint16_t lds[4][4][32 * S];
     __shared__ __align__(16) float stats[4][3][kShortRows];     // lse, delta, last visible key
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const uint16_t *ta = lds[wave][0], *tb = lds[wave][1];
-    const uint32_t ta_at = lds_address(ta), tb_at = lds_address(tb);
+    const uint32_t lds_at = lds_address(ta), ta_at = lds_at, tb_at = lds_at + 64 * S;
     float *lses = stats[wave][0], *deltas = stats[wave][1];
     int *lims = (int *)stats[wave][2];
     const int item = blockIdx.x * 4 + wave;
@@ -81,6 +81,27 @@ void attn_grad_short(AttnGrad a, int slots) {
     const uint16_t *vp = (const uint16_t *)a.v + p.k0 * a.v_row + hk * a.v_head;
     const uint16_t *qp = (const uint16_t *)a.q + p.q0 * a.q_row + hk * a.G * a.q_head;
     const uint16_t *dop = (const uint16_t *)a.g.d_o + p.q0 * a.g.do_row + hk * a.G * a.g.do_head;
+
+    // rows of a tile to the pair of LDS tiles `at`; beyond the last row, the last
+    // again: their last visible key is -1
+    auto copy_rows = [&](int tile, uint32_t at) {
+        auto row_at = [&](int i, int64_t step, int64_t head) {
+            const int row = min(tile * 32 + i, rows - 1), qi = divide(row, a.G, inv);
+            return qi * step + (row - qi * a.G) * head;
+        };
+        copy_tile<DP>(qp, a.d, at, [&](int i) { return row_at(i, a.q_row, a.q_head); });
+        copy_tile<DP>(dop, a.d, at + 64 * S, [&](int i) { return row_at(i, a.g.do_row, a.g.do_head); });
+    };
+    // the first row tile that sees a key of tile kt; the keys' part, kt by kt and
+    // tile by tile, has its next tile on the way while it works on one, and its
+    // first from here on
+    auto first_tile = [&](int kt) {
+        const int key0 = kt * 32 + s0 - p.k0;
+        return kt * 32 < s1 - s0 && key0 < p.lk ? max(key0 - shift, 0) * a.G / 32 : tiles;
+    };
+    int next = first_tile(mine);
+    uint32_t pair = 2;                       // the LDS tiles that the keys' part reads next
+    if (next < tiles) copy_rows(next, lds_at + pair * 64 * S);
 
     for (int tile = mine * 4; tile < mine * 4 + 4 && tile < tiles; tile++) {
         const int end = divide(min(tile * 32 + 31, rows - 1), a.G, inv) + shift + 1;
@@ -164,16 +185,8 @@ void attn_grad_short(AttnGrad a, int slots) {
             uint4v k[C], v[C];
             load_row<DP>(k, kp, key * a.k_row, a.d, live);
             load_row<DP>(v, vp, key * a.v_row, a.d, live);
-            for (int tile = max(key0 - shift, 0) * a.G / 32; tile < tiles; tile++) {
+            for (int tile = next; tile < tiles; tile++) {
                 int at = (tile & 3) * 32;
-                // rows beyond the last repeat it: their last visible key is -1
-                auto row_at = [&](int i, int64_t step, int64_t head) {
-                    const int row = min(tile * 32 + i, rows - 1), qi = divide(row, a.G, inv);
-                    return qi * step + (row - qi * a.G) * head;
-                };
-                copy_tile<DP>(qp, a.d, ta_at, [&](int i) { return row_at(i, a.q_row, a.q_head); });
-                copy_tile<DP>(dop, a.d, tb_at,
-                              [&](int i) { return row_at(i, a.g.do_row, a.g.do_head); });
                 if (shares > 1) {
                     // the rows may be another wave's: delta from o, and what its
                     // type rounded away if that is kept
@@ -199,11 +212,15 @@ void attn_grad_short(AttnGrad a, int slots) {
                     }
                 }
                 wait_copies<0>();
+                const uint16_t *tq = lds[wave][pair], *to = lds[wave][pair + 1];
+                pair ^= 2;
+                next = tile + 1 < tiles ? tile + 1 : first_tile(kt + shares);
+                if (next < tiles) copy_rows(next, lds_at + pair * 64 * S);
                 float16v s = {}, dp = {};
 #pragma unroll
-                for (int c = 0; c < C; c++) s = T::mfma(Tile<DP>::row(ta, 0, c), k[c], s);
+                for (int c = 0; c < C; c++) s = T::mfma(Tile<DP>::row(tq, 0, c), k[c], s);
 #pragma unroll
-                for (int c = 0; c < C; c++) dp = T::mfma(Tile<DP>::row(tb, 0, c), v[c], dp);
+                for (int c = 0; c < C; c++) dp = T::mfma(Tile<DP>::row(to, 0, c), v[c], dp);
                 uint32_t pp[8], pd[8];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -228,8 +245,8 @@ void attn_grad_short(AttnGrad a, int slots) {
                     const uint4v db = {pd[4 * kc], pd[4 * kc + 1], pd[4 * kc + 2], pd[4 * kc + 3]};
 #pragma unroll
                     for (int dt = 0; dt < DP / 32; dt++) {
-                        dv[dt] = T::mfma(Tile<DP>::transposed(tb, kc * 16, dt), pb, dv[dt]);
-                        dk[dt] = T::mfma(Tile<DP>::transposed(ta, kc * 16, dt), db, dk[dt]);
+                        dv[dt] = T::mfma(Tile<DP>::transposed(to, kc * 16, dt), pb, dv[dt]);
+                        dk[dt] = T::mfma(Tile<DP>::transposed(tq, kc * 16, dt), db, dk[dt]);
                     }
                 }
             }

@@ -160,7 +160,7 @@ extern "C" int seq_rotary(const SeqRotary *r, void *stream) {
     if (r->tokens < 0 || r->hq < 0 || r->hkv < 0 || r->d < 1 || r->table_len < 0)
         return CO_ERR_NULLARG;
     if (r->rot < 0 || r->rot > r->d || r->rot % 2 || r->tokens > SEQ_MAX_ROWS ||
-        r->hq > 65535 || r->hkv > 65535 || r->d > 65535)
+        r->hq > 32767 || r->hkv > 32767 || r->d > 65535)
         return CO_ERR_BOUNDS;
     if (r->dtype < SEQ_FP32 || r->dtype > SEQ_FP16) return CO_ERR_DATA;
     if (r->tokens == 0 || r->hq + r->hkv == 0) return CO_OK;
