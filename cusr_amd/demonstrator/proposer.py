@@ -187,10 +187,18 @@ class Proposer:
 
 
 class Trainer:
-    """Clipped policy gradient with a KL term to the starting parameters."""
+    """Clipped policy gradient with a KL term to the starting parameters.
 
-    def __init__(self, proposer, *, rate=3e-3, clip=0.2, kl_coef=0.01, epochs=4):
+    top: the share of a population, by reward, that is learnt from. A search
+    wants the best program rather than a good mean, so it learns from the best
+    few, by how far they pass the last of them; 1 learns from all, by how far
+    they pass the mean."""
+
+    def __init__(self, proposer, *, rate=3e-3, clip=0.2, kl_coef=0.01, epochs=4, top=1.0):
+        if not 0.0 < top <= 1.0:
+            raise ValueError("top must be a share of the population")
         self.p, self.clip, self.kl_coef, self.epochs = proposer, clip, kl_coef, epochs
+        self.top = top
         self.start = {k: v.detach().clone() for k, v in proposer.parameters.items()}
         self.opt = torch.optim.Adam(list(proposer.parameters.values()), lr=rate)
 
@@ -206,10 +214,12 @@ class Trainer:
         """Reinforce a population by its programs' rewards [M]; returns the
         loss of each epoch."""
         r = torch.as_tensor(rewards, dtype=torch.float32, device=self.p.device)
-        advantage = ((r - r.mean()) / (r.std() + 1e-6))[pop.sequence]
+        least = r.mean() if self.top == 1.0 else torch.quantile(r, 1.0 - self.top)
+        used = torch.ones_like(r) if self.top == 1.0 else (r >= least).float()
+        advantage = ((r - least) / (r[used > 0].std(unbiased=False) + 1e-6))[pop.sequence]
         old, ref = self.p.log_probabilities(pop), self._reference(pop)
-        # every program counts alike, whatever its length
-        weights = (1.0 / pop.lengths.float() / len(pop.lengths))[pop.sequence]
+        # every program that is learnt from counts alike, whatever its length
+        weights = (used / pop.lengths.float() / used.sum())[pop.sequence]
         losses = []
         for _ in range(self.epochs):
             loss, _ = seq_ops.policy_loss(self.p.logits(pop), pop.symbols, old, advantage,
@@ -236,7 +246,7 @@ def search(X, y, *, rounds=10, population=1024, max_iter=10, seed=0, proposer=No
     best reward."""
     X, y = np.asarray(X, np.float64), np.asarray(y, np.float64)
     p = proposer or Proposer(X.shape[1], seed=seed)
-    tr = trainer or Trainer(p)
+    tr = trainer or Trainer(p, top=0.1, kl_coef=0.05)
     lm = backend or KernelLM(max_iter=max_iter)
     g = torch.Generator(device=p.device).manual_seed(seed)
     rng = np.random.default_rng(seed)

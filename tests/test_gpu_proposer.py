@@ -26,6 +26,8 @@ def test_symbols_and_rewards():
     assert r.tolist() == [1.0, 0.5, 0.0, 0.0]
     with pytest.raises(ValueError):
         pr.Proposer(2, width=100, heads=3, device="cpu")
+    with pytest.raises(ValueError):
+        pr.Trainer(None, top=0.0)
 
 
 @gpu
@@ -65,8 +67,8 @@ def test_single_tokens_agree_with_packed_sequences():
     at = steps[pop.sequence, pop.positions.long()].masked_fill(~pop.allowed, float("-inf"))
     a, b = packed.log_softmax(1), at.log_softmax(1)
     # a layer's bfloat16 roundings (eight of 2^-8 a layer, relative) on logits of order 1
-    assert float((a - b)[pop.allowed].abs().max()) <= 2 * 8 * 2.0 ** -8 * float(
-        packed[pop.allowed].abs().max().clamp(min=1.0))
+    far, size = (x[pop.allowed].abs().max().item() for x in (a - b, packed))
+    assert far <= 2 * 8 * 2.0 ** -8 * max(size, 1.0)
     lp = p.log_probabilities(pop)
     want = a.gather(1, pop.symbols[:, None])[:, 0]
     assert torch.allclose(lp, want, atol=1e-4)

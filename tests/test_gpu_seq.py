@@ -218,6 +218,67 @@ def test_attention_autograd(ops):
     assert all(torch.equal(x.grad, w) for x, w in zip(a, want))
 
 
+def test_attention_gradient_is_as_good_as_its_type(ops):
+    """The row sums that the gradient needs are not those of the rounded output:
+    over many values the error is that of rounding P, dS and the result, about
+    sqrt(2) roundings of the type, with delta's part (as large again) gone."""
+    for lens, hq, hkv in (([30] * 40, 4, 4), ([50, 61] * 10, 4, 2), ([700, 300], 4, 2),
+                          ([40] * 12, 16, 1)):
+        c = cu(lens)
+        q, k, v, do = (normal((sum(lens), h, 64), BF, i + 3, 1.5 if i == 0 else 1.0)
+                       for i, h in enumerate((hq, hkv, hkv, hq)))
+        o, lse = ops.attention(q, k, v, c, return_lse=True)
+        got = ops.attention_grad(do, q, k, v, o, lse, c)
+        r = ref.attention(q, k, v, c, c, do=do)
+        for n, g in zip(("dq", "dk", "dv"), got):
+            want = r[n]
+            rms = lambda x: float(x.square().mean().sqrt())  # noqa: E731
+            off = rms(g.cpu().double() - want) / rms(want)
+            rounded = rms(want.to(BF).double() - want) / rms(want)
+            _say(f"  {lens[:2]} {n}: error {off:.5f}, of rounding alone {rounded:.5f}")
+            assert off <= 1.75 * rounded, (lens[:2], n)
+
+
+def test_graph_replays(ops):
+    """Attention, its gradient, rotary positions and the policy loss captured in
+    a graph, replayed on changed inputs with eager work in between."""
+    lens = [70, 3, 200, 31]
+    c, T = cu(lens), sum(lens)
+    table, pos = ops.rotary_table(64, 256), torch.arange(T, device=DEV) % 200
+    q, k, v, do = (normal((T, h, 64), BF, i) for i, h in enumerate((4, 2, 2, 4)))
+    pc = policy_case(T, 40, BF, 3, forbidden=0.2)
+    step = [normal((4, 4, 64), BF, 7), torch.tensor([70, 3, 200, 31], dtype=torch.int32,
+                                                    device=DEV)]
+
+    def work():
+        a, b = ops.rotary(q, k, pos, table)
+        o, lse = ops.attention(a, b, v, c, return_lse=True)
+        g = ops.attention_grad(do, a, b, v, o, lse, c)
+        s = ops.attention(step[0], b, v, torch.arange(5, dtype=torch.int32, device=DEV), c,
+                          k_lens=step[1])
+        return (o, *g, s, *ops.policy_loss_grad(**pc, kl_coef=0.1))
+
+    work()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for i in range(4):
+        q.copy_(normal(q.shape, BF, 50 + i))
+        do.copy_(normal(do.shape, BF, 60 + i))
+        pc["advantages"].copy_(normal(pc["advantages"].shape, F32, 70 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in out]
+        want = work()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
 def test_attention_offsets_out_of_range(ops):
     """Offsets beyond the tensors or out of order stay inside them."""
     q, k, v = (normal((50, h, 64), BF, i) for i, h in enumerate((4, 2, 2)))
