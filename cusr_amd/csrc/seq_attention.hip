@@ -198,12 +198,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int slots) {
                     if (k0 + u * 32 + 8 * (r / 4) + 4 * h + r % 4 > lim) s[u][r] = neg_inf();
         float top[4] = {s[0][0], s[0][8], s[1][0], s[1][8]};     // four chains of eight
 #pragma unroll
-        for (int r = 1; r < 7; r += 2)
+        for (int r = 1; r < 8; r++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                top[i] = max3(top[i], s[i / 2][i % 2 * 8 + r], s[i / 2][i % 2 * 8 + r + 1]);
-        float mx = max3(max3(top[0], top[1], s[0][7]), max3(top[2], top[3], s[1][7]),
-                        fmaxf(s[0][15], s[1][15]));
+            for (int i = 0; i < 4; i++) top[i] = max2(top[i], s[i / 2][i % 2 * 8 + r]);
+        float mx = max2(max2(top[0], top[1]), max2(top[2], top[3]));
         mx = max_halves(mx);
         if (__any((mx - m) * a.c > 8.0f)) {
             const float mn = fmaxf(m, mx), m0 = mn == neg_inf() ? 0.0f : mn;

@@ -155,7 +155,8 @@ __device__ inline void copy_to_lds16(const void *from, uint32_t to) {
                  :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
 }
 __device__ inline void copy_to_lds16(const void *wave_from, uint32_t lane_offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+    // five states between a vector instruction that wrote the address and its use
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                  :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(lane_offset), "s"(wave_from)
                  : "memory");
 }

@@ -31,11 +31,11 @@ __device__ inline float neg_inf() { return -__builtin_inff(); }
 // 2^x: one v_exp_f32 (results below 2^-126 flush to 0)
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// largest of three: one instruction, and no step to quiet a NaN before it
-__device__ inline float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
+// larger of two, as the middle one of them and infinity: unlike fmaxf it needs no
+// instruction before it to quiet a NaN of a matrix product, and unlike assembly it
+// waits for the product
+__device__ inline float max2(float a, float b) {
+    return __builtin_amdgcn_fmed3f(a, b, __builtin_inff());
 }
 
 // larger of the two halves' values, in both lanes of (l, l + 32)
