@@ -261,8 +261,8 @@ void attn_grad_short(AttnGrad a, int slots) {
     }
 }
 
-// Long sequences, rows: a block of WAVES waves owns 32 rows a wave of one key
-// head; keys and values pass through LDS 64 at a time, as in the forward.
+// Long sequences, rows: a block of four waves owns 128 rows of one key head; keys
+// and values pass through LDS 64 at a time, as in the forward.
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, int slots) {
     typedef KeyTiles<DP, 64, WAVES> Keys;
@@ -357,25 +357,28 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, i
     store_row<T, DP>(a.g.dq, t * a.g.dq_row + head * a.g.dq_head, dq, a.scale, a.d, ok);
 }
 
-// Long sequences, keys: a block owns 128 keys of one key head, a wave 32 of them
-// and every other tile of 32 rows; a wave has both gradients of its keys and the
-// keys in registers and their values in LDS (registers for those too would
-// spill). The two waves that share keys add up at the end: with four waves a
-// block's longest run over the rows would last twice as long, with 256 keys a
-// block too few blocks would be left to share the work out (5 sequences of 700 to
-// 4,801: half the compute units idle). Rows pass through LDS 64 at a time,
-// copied there past the registers one tile ahead of their use. Rows beyond the
-// last repeat it with lse +inf, which makes their P and dS 0.
-template <typename T, int DP>
-__global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int slots) {
-    constexpr int RB = 64, KEYS = 128, STRIDE = Tile<DP>::stride * 2;         // bytes
+// Long sequences, keys: a block owns KX * 32 keys of one key head, a wave 32 of
+// them and every other tile of 32 rows. Both gradients of its keys are in the
+// wave's registers; keys and values are in LDS, since with them in registers too
+// no operand could be read ahead of its product and each product waited for its
+// own. The two waves that share keys add up at the end: with one, a block's
+// longest run over the rows would last twice as long, and the longest run is what
+// few sequences wait for. Rows pass through LDS 64 at a time, copied there past
+// the registers one tile ahead of their use. Rows beyond the last repeat it with
+// lse +inf, which makes their P and dS 0. Bound by the matrix cores, 48 % busy,
+// and the waits of eight waves at one barrier: 32 heads of 128 over 8, five
+// sequences of 700 to 4,801 in about 0.6 ms, 1 PFLOP/s.
+template <typename T, int DP, int KX>
+__global__ __launch_bounds__(KX * 128, KX == 4 || DP <= 64 ? 2 : 1) void attn_grad_kv_tiles(AttnGrad a, int slots) {
+    constexpr int RB = 64, KEYS = KX * 32, WAVES = KX * 2;
+    constexpr int STRIDE = Tile<DP>::stride * 2;        // bytes
     constexpr int PER = RB * STRIDE / 1024;             // copies of 1 KB a tile of q or do
-    constexpr int COPIES = 2 * PER / 8;                 // of a wave
+    constexpr int COPIES = 2 * PER / WAVES;                 // of a wave
     constexpr uint32_t TILE = RB * STRIDE, BUF = 2 * TILE + 512;   // q, do, lse and delta
-    constexpr uint32_t BYTES = 2 * BUF + 2 * KEYS * STRIDE, SUMS = 4 * 2 * 32 * DP * 4;
+    constexpr uint32_t BYTES = 2 * BUF + 2 * KEYS * STRIDE, SUMS = KX * 2 * 32 * DP * 4;
     __shared__ __align__(256) unsigned char lds[BYTES > SUMS ? BYTES : SUMS];
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kx = wave & 3, rx = wave >> 2;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kx = wave % KX, rx = wave / KX;
     const int slot = (int)blockIdx.x / a.hkv, hk = (int)blockIdx.x - slot * a.hkv;
     if (slot >= slots) return;
     const Found f = find_sequence(a.cu_k, a.n_seq, a.tk, 1, KEYS, slot);
@@ -426,7 +429,7 @@ __global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int slo
         if (plain && r0 + RB <= rows) {
 #pragma unroll
             for (int x = 0; x < COPIES; x++) {
-                const int idx = wave + x * 8;
+                const int idx = wave + x * WAVES;
                 const int t = (r0 + (idx % PER - wave % PER) * (1024 / STRIDE)) / a.G;
                 copy_to_lds16(idx < PER ? q0p + t * a.q_row : o0p + t * a.g.do_row,
                               idx < PER ? q_off : o_off, buf + idx * 1024);
@@ -434,7 +437,7 @@ __global__ __launch_bounds__(512, 2) void attn_grad_kv_tiles(AttnGrad a, int slo
         } else {
 #pragma unroll
             for (int x = 0; x < COPIES; x++) {
-                const int idx = wave + x * 8;
+                const int idx = wave + x * WAVES;
                 const int row =
                     min(r0 + (idx % PER - wave % PER) * (1024 / STRIDE) + row_l, rows - 1);
                 const int t = row / a.G, g = row % a.G;
@@ -571,12 +574,24 @@ int launch_grad(const AttnGrad &a, hipStream_t s) {
         return launch_status();
     }
     if (a.tq) {
-        const int slots = slot_of(a.tq, a.G, 256, a.n_seq) + 1;
-        attn_grad_q_tiles<T, DP, 8><<<dim3((unsigned)(slots * a.hkv)), 512, 0, s>>>(a, slots);
+        const int slots = slot_of(a.tq, a.G, 128, a.n_seq) + 1;
+        attn_grad_q_tiles<T, DP, 4><<<dim3((unsigned)(slots * a.hkv)), 256, 0, s>>>(a, slots);
         if (hipGetLastError() != hipSuccess) return CO_ERR_CUDA;
     }
+    // Blocks of 64 keys where 128 would not fill the chip once (one sequence of 2,000,
+    // 32 heads of 128 over 8: 263 against 289 us with the rows' part), and for heads up
+    // to 64, whose registers and LDS leave room for three a compute unit (16 sequences
+    // of 300, 8 heads: 32 against 39 us); wider heads have room for one and need all
+    // eight waves (two of 6,000: 2.0 against 2.5 ms).
     const int slots = slot_of(a.tk, 1, 128, a.n_seq) + 1;
-    attn_grad_kv_tiles<T, DP><<<dim3((unsigned)(slots * a.hkv)), 512, 0, s>>>(a, slots);
+    if constexpr (DP > 64) {
+        if (slots * a.hkv > 256) {
+            attn_grad_kv_tiles<T, DP, 4><<<dim3((unsigned)(slots * a.hkv)), 512, 0, s>>>(a, slots);
+            return launch_status();
+        }
+    }
+    const int more = slot_of(a.tk, 1, 64, a.n_seq) + 1;
+    attn_grad_kv_tiles<T, DP, 2><<<dim3((unsigned)(more * a.hkv)), 256, 0, s>>>(a, more);
     return launch_status();
 }
 

@@ -59,6 +59,9 @@ PACKED = [
     ([1025, 40], 2, 1, 128, BF),
     ([33, 95], 7, 1, 64, BF),
     ([900, 333, 1], 8, 8, 128, FP),
+    ([200] * 40, 8, 8, 128, BF),           # enough blocks of 128 keys to fill the chip
+    ([130, 300, 1] * 14, 16, 8, 96, FP),
+    ([128, 0, 129, 193] * 9, 6, 6, 64, BF),
 ]
 
 
