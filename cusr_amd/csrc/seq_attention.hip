@@ -351,16 +351,20 @@ __global__ __launch_bounds__(256) void attn_join(Attn a, Step st) {
         a.lse[head * a.tq + t] = l == 0.0f ? neg_inf() : m * a.scale + logf(l);
 }
 
-// Whether a call is few rows over many keys, and its chunks. At most 256 rows
-// a sequence on average, and at least four keys a query and 128 a sequence:
-// then the keys decide. Chunks leave about 4096 waves, of 256 to 512 keys:
-// longer ones leave waves idle at the end, shorter ones more to join.
+// Whether a call is few rows over many keys, and its chunks. At most 256 rows a
+// sequence on average, and at least four keys a query: then the keys decide. Fewer
+// than 512 keys are as soon read by the waves that the rows have (256 sequences of
+// 200 keys, 32 heads over 8: 36 against 63 us; 64 of 4,000: 250 against 222 us; one
+// of 4,000: 195 against 24 us), unless there are hardly any waves. Chunks of 512
+// keys, or as few as 128 as long as that leaves less than a wave per compute unit
+// (8 sequences of 4,000: 512 40 us, 256 45 us; one: 38 and 24 us).
 bool plan_step(const Attn &a, Step &st) {
-    if (a.n_seq == 0 || a.tq * a.G > 256ll * a.n_seq || a.tk < 4 * a.tq ||
-        a.tk < 128ll * a.n_seq)
-        return false;
+    if (a.n_seq == 0 || a.tq * a.G > 256ll * a.n_seq || a.tk < 4 * a.tq) return false;
     st.tiles = (int)((a.tq * a.G + 32ll * a.n_seq - 1) / (32ll * a.n_seq));
-    st.chunk = a.tk * a.hkv * st.tiles / 512 >= 4096 ? 512 : 256;
+    const int64_t waves = (int64_t)a.n_seq * a.hkv * st.tiles;
+    if (a.tk < (waves < 256 ? 256ll : 512ll) * a.n_seq) return false;
+    st.chunk = 512;
+    while (st.chunk > 128 && a.tk * a.hkv * st.tiles / st.chunk < 256) st.chunk /= 2;
     st.slots = slot_of(a.tk, 1, st.chunk, a.n_seq) + 1;
     return true;
 }
@@ -396,7 +400,8 @@ int launch_head(const Attn &a, hipStream_t s) {
     Step st;
     if (plan_step(a, st)) return launch_step<T, DP>(a, st, s);
     const int64_t rows = a.n_seq ? a.tq * a.G / a.n_seq : 0;      // of a sequence, on average
-    // Tiles shared by four waves from 96 rows on; below, two of the waves would idle.
+    // Tiles shared by four waves from 96 rows on; below, two of the waves would idle
+    // (4 heads of 64, sequences of 32: 43 against 85 us, 64: alike, 96: 79 against 69 us).
     if (rows >= 96) return launch_tiles<T, DP, 4>(a, s);
     const int slots = slot_of(a.tq, a.G, kShortRows, a.n_seq) + 1;
     const int64_t blocks = (slots * (int64_t)a.hkv + 3) / 4;

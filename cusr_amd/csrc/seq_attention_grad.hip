@@ -561,9 +561,13 @@ __global__ __launch_bounds__(KX * 128, KX == 4 || DP <= 64 ? 2 : 1) void attn_gr
     store_row<T, DP>(a.g.dv, kr * a.g.dv_row + hk * a.g.dv_head, dv, 1.0f, a.d, kr < s1);
 }
 
-// At fewer than 128 keys a sequence a block of the long kernels would mostly
-// wait for itself.
-bool short_sequences(const Attn &a) { return a.tk < 128ll * a.n_seq || a.n_seq == 0; }
+// Below these keys a sequence, on average, blocks of the long kernels mostly wait
+// for themselves; above, a wave alone takes longer (4 heads of 64: sequences of 96
+// 200 against 281 us, of 128 303 against 297 us; heads of 128, with half the waves:
+// of 64 193 against 309 us, of 100 612 against 457 us).
+bool short_sequences(const Attn &a) {
+    return a.tk < (padded_head(a.d) <= 64 ? 128ll : 80ll) * a.n_seq || a.n_seq == 0;
+}
 
 template <typename T, int DP>
 int launch_grad(const AttnGrad &a, hipStream_t s) {
