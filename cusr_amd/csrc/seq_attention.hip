@@ -252,9 +252,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int slots) {
 // tiles are over the query rows.
 struct Step {
     int chunk;          // keys of a chunk, a multiple of 32
-    int tiles;          // row tiles of a slot that have room in the partials
+    int tiles;          // row tiles of a slot
+    int rows;           // rows of a slot that have room in the partials
     int slots;
-    float *o, *ml;      // [slot][hkv][tiles * 32][DP], [slot][hkv][tiles * 32][2]
+    float *o, *ml;      // [slot][hkv][rows][DP], [slot][hkv][rows][2]
 };
 
 template <typename T, int DP>
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
     const int rows = p.lq * a.G;
     if (chunk < 0 || rows == 0) return;
     const int chunks = (p.lk + st.chunk - 1) / st.chunk;
-    const bool split = chunks > 1 && rows <= st.tiles * 32;
+    const bool split = chunks > 1 && rows <= st.rows;
     if (chunk >= (split ? chunks : 1)) return;
     const int key0 = split ? chunk * st.chunk : 0;
     const int key1 = split && key0 + st.chunk < p.lk ? key0 + st.chunk : p.lk;
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
             store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok);
             continue;
         }
-        const int64_t pr = (((int64_t)slot * a.hkv + hk) * st.tiles + tile) * 32 + (lane & 31);
+        const int64_t pr = ((int64_t)slot * a.hkv + hk) * st.rows + tile * 32 + (lane & 31);
         if (!r.ok) continue;
 #pragma unroll
         for (int dt = 0; dt < DP / 32; dt++)
@@ -315,11 +316,11 @@ __global__ __launch_bounds__(256) void attn_join(Attn a, Step st) {
     const Place p = place_of(a, b);
     const int chunks = (p.lk + st.chunk - 1) / st.chunk;
     const int rows = p.lq * a.G;
-    if (chunks <= 1 || rows > st.tiles * 32 || t < p.q0 || t >= p.q0 + p.lq) return;
+    if (chunks <= 1 || rows > st.rows || t < p.q0 || t >= p.q0 + p.lq) return;
     const int row = (t - p.q0) * a.G + head % a.G;
     const int64_t slot0 = slot_of(offset_at(a.cu_k, b, a.tk), 1, st.chunk, b);
-    const int64_t stride = (int64_t)a.hkv * st.tiles * 32;
-    const int64_t pr = slot0 * stride + (int64_t)hk * st.tiles * 32 + row;
+    const int64_t stride = (int64_t)a.hkv * st.rows;
+    const int64_t pr = slot0 * stride + (int64_t)hk * st.rows + row;
     float m = neg_inf();
     for (int c = lane; c < chunks; c += 64) m = fmaxf(m, st.ml[2 * (pr + c * stride)]);
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -366,10 +367,13 @@ bool plan_step(const Attn &a, Step &st) {
     st.chunk = 512;
     while (st.chunk > 128 && a.tk * a.hkv * st.tiles / st.chunk < 256) st.chunk /= 2;
     st.slots = slot_of(a.tk, 1, st.chunk, a.n_seq) + 1;
+    // room for twice the average: a sequence of more rows is not split
+    const int64_t twice = (2 * a.tq * a.G + a.n_seq - 1) / a.n_seq;
+    st.rows = (int)(twice < 32ll * st.tiles ? (twice + 3) / 4 * 4 : 32ll * st.tiles);
     return true;
 }
 int64_t step_rows(const Attn &a, const Step &st) {
-    return (int64_t)st.slots * a.hkv * st.tiles * 32;
+    return (int64_t)st.slots * a.hkv * st.rows;
 }
 int64_t step_bytes(const Attn &a, const Step &st) {
     return a.tk <= st.chunk ? 0 : step_rows(a, st) * (padded_head(a.d) + 2) * 4;

@@ -26,6 +26,7 @@ import threading
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from cusr_amd.kernel.co_inproc import CO_OK, COError, _HERE
 
@@ -318,6 +319,7 @@ class _AttentionFn(torch.autograd.Function):
         return o, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do, _):
         q, k, v, o, lse, cu_q, cu_k, k_lens, low = ctx.saved_tensors
         if low is not None:
@@ -340,7 +342,9 @@ def attention(q, k, v, cu_q, cu_k=None, *, k_lens=None, scale=None, return_lse=F
     A query that sees no key gives 0. scale defaults to D ** -0.5.
 
     Returns o like q, or (o, lse) with return_lse: lse fp32 [Hq, Tq], -inf
-    where no key is seen. Probabilities are rounded to the tensors' type for
+    where no key is seen. A key or value that is not finite, in a place that a
+    query does not see, is kept from it beyond its sequence's length, but reaches
+    queries up to 94 places before its own within it. Probabilities are rounded to the tensors' type for
     the product with v; sums and statistics are held in fp32."""
     _check_attention(q, k, v, cu_q, cu_k, k_lens, scale)
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
@@ -433,6 +437,7 @@ class _RotaryFn(torch.autograd.Function):
         return (q_out, k_out) if k is not None else q_out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         positions, table = ctx.saved_tensors
         interleaved, inverse = ctx.how
@@ -588,6 +593,7 @@ class _PolicyFn(torch.autograd.Function):
         return loss, logp
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss, _):
         # one pass over the logits: the sums are formed again, not stored
         dlogits = _policy(*ctx.saved_tensors, *ctx.how, dloss.float().contiguous(), True)[2]

@@ -47,7 +47,9 @@ extern "C" {
  * cu_q[0] is 0. Queries are the last ones of the keys: query i of lq sees
  * keys 0 .. i + lk - lq. A query that sees no key, and a query row in no
  * sequence, give o = 0 and lse = -inf. Offsets out of order or out of range
- * are clamped into the tensors. scale is positive.
+ * are clamped into the tensors. scale is positive. Within a sequence's keys a
+ * value that is not finite also reaches queries that do not see it, up to 94
+ * places before it (a masked probability is a 0 in a matrix product).
  *
  * lse (may be null for the forward) [hq, tq] fp32: log of the sum of
  * exp(scale q.k) over the visible keys. o_low (may be null): what rounding o to

@@ -313,6 +313,42 @@ def test_attention_offsets_out_of_range(ops):
     assert not any(bool(x[40:].any()) for x in g)
 
 
+def test_nothing_to_do(ops):
+    """No tokens, no keys, no sequences."""
+    for T, K in ((0, 0), (0, 5), (7, 0)):
+        q, k = normal((T, 4, 64), BF, 1), normal((K, 2, 64), BF, 2)
+        cq, ck = cu([T]), cu([K])
+        o, lse = ops.attention(q, k, k, cq, ck, return_lse=True)
+        assert o.shape == q.shape and not bool(o.any())
+        g = ops.attention_grad(q, q, k, k, o, lse, cq, ck)
+        assert [x.shape for x in g] == [q.shape, k.shape, k.shape]
+        assert not any(bool(x.any()) for x in g)
+    q, k = normal((9, 4, 64), BF, 1), normal((9, 2, 64), BF, 2)
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+    o, lse = ops.attention(q, k, k, none, return_lse=True)
+    assert not bool(o.any()) and bool((lse == float("-inf")).all())
+    assert not any(bool(x.any()) for x in ops.attention_grad(q, q, k, k, o, lse, none))
+    table, pos = ops.rotary_table(64, 9), torch.zeros(0, dtype=torch.int64, device=DEV)
+    assert ops.rotary(q[:0], None, pos, table).shape == (0, 4, 64)
+    f = torch.zeros(0, device=DEV)
+    loss, logp, dx = ops.policy_loss_grad(torch.zeros(0, 7, device=DEV), pos, f, f)
+    assert float(loss) == 0.0 and logp.shape == (0,) and dx.shape == (0, 7)
+
+
+def test_attention_uneven_rows_over_a_cache(ops):
+    """Most sequences bring one query, one brings many: more rows than a split has
+    room for, beside splits."""
+    lq, lk = [1] * 11 + [200, 1], [900] * 11 + [1500, 2000]
+    q, do = (normal((sum(lq), 8, 64), BF, i) for i in (1, 2))
+    k, v = (normal((sum(lk), 2, 64), BF, i) for i in (3, 4))
+    cq, ck = cu(lq), cu(lk)
+    o, lse = ops.attention(q, k, v, cq, ck, return_lse=True)
+    g = ops.attention_grad(do, q, k, v, o, lse, cq, ck)
+    r = ref.attention(q, k, v, cq, ck, do=do)
+    for n, x in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *g)):
+        check(n, x, r[n], r[n + "_tol"])
+
+
 def test_attention_rows_past_32_bits(ops):
     """A cache whose element offsets pass 2^31: the last segment is read where
     it lies."""
