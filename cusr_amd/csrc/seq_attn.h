@@ -174,29 +174,21 @@ template <int N> __device__ inline void landed(uint4v (&x)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++) asm volatile("" : "+v"(x[i]));
 }
-// Order of a block of straight code: N times M matrix instructions, then R LDS
-// reads. Left to itself the compiler, short of registers, puts every read right
-// before the product that waits for it.
-template <int N, int M, int R> __device__ inline void interleave() {
-    if constexpr (N > 0) {
-        if constexpr (M > 0) __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
-        if constexpr (R > 0) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
-        interleave<N - 1, M, R>();
-    }
-}
 // Barrier of the block that no memory access of the program moves across.
 __device__ inline void block_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
-// 16-bit tile rows in LDS: DP elements a row (96 padded to 128), 16-byte
-// chunks permuted within the row so that the transposed reads, which take four
-// rows of 32 bytes at a time, and the row reads, 32 rows of one chunk, spread
-// over the banks.
+// 16-bit tile rows in LDS: DP elements a row (96 padded to 128), the row's 16-byte
+// pieces permuted by the row's place among 16.
 template <int DP> struct Tile {
     static constexpr int stride = DP == 96 ? 128 : DP;      // elements
     static constexpr int chunks = stride / 8;
+    // The LDS serves 256 bytes at a time. A transposed read of half a wave takes 64
+    // bytes of each of four rows in turn: they have to lie in different quarters. A row
+    // read takes one piece of 16 rows: they have to lie in different pieces.
     static __device__ int swz(int row) {
-        return DP == 32 ? 0 : (DP == 64 ? ((row & 3) * 2 + ((row >> 2) & 1)) & 7
-                                        : ((row & 7) * 2 + ((row >> 3) & 1)) & 15);
+        return DP == 32   ? row >> 2 & 3
+               : DP == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3)
+                          : (row & 3) << 2 | (row >> 2 & 3);
     }
     static __device__ int at(int row, int chunk) {          // element offset
         return row * stride + ((chunk ^ swz(row)) << 3);
