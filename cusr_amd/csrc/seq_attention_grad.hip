@@ -45,9 +45,13 @@ __device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float
 // need no statistics from another kernel. First the rows: delta = sum of P dP,
 // which needs no o, then dQ^T = sum over keys of K^T dS^T, from S^T. Then the
 // keys: dV^T = dO^T P and dK^T = Q^T dS, from S formed the other way round: the
-// same tiles are the left or the right operand. The side that is summed over
-// passes through LDS, past the registers. What bounds it is memory, and before
-// that the chain of loads from the slot to the rows, so registers are kept few.
+// same tiles are the left or the right operand. What is read passes through LDS,
+// past the registers. What bounds it is the chain of loads from the slot to the
+// rows beside vector instructions (half the time) with two waves a SIMD, hence
+// the path of its own for up to 64 rows and keys, in which few loads wait for
+// others: 8,192 sequences of 3 to 63, 8 heads of 64, take 0.60 ms (3.2 TB/s), on
+// the general path 0.73; stores of 32 bytes of each row instead of whole rows
+// took 0.02 more.
 constexpr int kShortRows = 128;
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1)
@@ -57,8 +61,7 @@ void attn_grad_short(AttnGrad a, int slots) {
     __shared__ __align__(16) float stats[4][3][kShortRows];     // lse, delta, last visible key
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    const uint16_t *ta = lds[wave][0], *tb = lds[wave][1];
-    const uint32_t lds_at = lds_address(ta), ta_at = lds_at, tb_at = lds_at + 64 * S;
+    const uint32_t lds_at = lds_address(lds[wave][0]);
     float *lses = stats[wave][0], *deltas = stats[wave][1];
     int *lims = (int *)stats[wave][2];
     const int item = blockIdx.x * 4 + wave;
@@ -80,111 +83,259 @@ void attn_grad_short(AttnGrad a, int slots) {
     const uint16_t *kp = (const uint16_t *)a.k + p.k0 * a.k_row + hk * a.k_head;
     const uint16_t *vp = (const uint16_t *)a.v + p.k0 * a.v_row + hk * a.v_head;
     const uint16_t *qp = (const uint16_t *)a.q + p.q0 * a.q_row + hk * a.G * a.q_head;
+    uint16_t *dqp = (uint16_t *)a.g.dq + p.q0 * a.g.dq_row + hk * a.G * a.g.dq_head;
     const uint16_t *dop = (const uint16_t *)a.g.d_o + p.q0 * a.g.do_row + hk * a.G * a.g.do_head;
 
-    // rows of a tile to the pair of LDS tiles `at`; beyond the last row, the last
-    // again: their last visible key is -1
-    auto copy_rows = [&](int tile, uint32_t at) {
-        auto row_at = [&](int i, int64_t step, int64_t head) {
-            const int row = min(tile * 32 + i, rows - 1), qi = divide(row, a.G, inv);
-            return qi * step + (row - qi * a.G) * head;
-        };
-        copy_tile<DP>(qp, a.d, at, [&](int i) { return row_at(i, a.q_row, a.q_head); });
-        copy_tile<DP>(dop, a.d, at + 64 * S, [&](int i) { return row_at(i, a.g.do_row, a.g.do_head); });
+    // tiles to LDS tiles, past the registers. Beyond the last row or key, the last
+    // again: it is masked, by its last visible key -1
+    auto row_at = [&](int i, int64_t step, int64_t head) {
+        const int row = min(i, rows - 1), qi = divide(row, a.G, inv);
+        return qi * step + (row - qi * a.G) * head;
     };
-    // the first row tile that sees a key of tile kt; the keys' part, kt by kt and
-    // tile by tile, has its next tile on the way while it works on one, and its
-    // first from here on
-    auto first_tile = [&](int kt) {
-        const int key0 = kt * 32 + s0 - p.k0;
-        return kt * 32 < s1 - s0 && key0 < p.lk ? max(key0 - shift, 0) * a.G / 32 : tiles;
+    auto copy_q = [&](int tile, int to) {
+        copy_tile<DP>(qp, a.d, lds_at + to * 64 * S,
+                      [&](int i) { return row_at(tile * 32 + i, a.q_row, a.q_head); });
     };
-    int next = first_tile(mine);
-    uint32_t pair = 2;                       // the LDS tiles that the keys' part reads next
-    if (next < tiles) copy_rows(next, lds_at + pair * 64 * S);
+    auto copy_do = [&](int tile, int to) {
+        copy_tile<DP>(dop, a.d, lds_at + to * 64 * S,
+                      [&](int i) { return row_at(tile * 32 + i, a.g.do_row, a.g.do_head); });
+    };
+    auto copy_keys = [&](int k0, int end, int tk, int tv) {
+        copy_tile<DP>(kp, a.d, lds_at + tk * 64 * S,
+                      [&](int i) { return min(k0 + i, end - 1) * a.k_row; });
+        copy_tile<DP>(vp, a.d, lds_at + tv * 64 * S,
+                      [&](int i) { return min(k0 + i, end - 1) * a.v_row; });
+    };
+    // keys that a tile of rows sees
+    auto seen_by = [&](int tile) {
+        return divide(min(tile * 32 + 31, rows - 1), a.G, inv) + shift + 1;
+    };
 
-    for (int tile = mine * 4; tile < mine * 4 + 4 && tile < tiles; tile++) {
-        const int end = divide(min(tile * 32 + 31, rows - 1), a.G, inv) + shift + 1;
-        auto copy_keys = [&](int k0) {       // beyond the last, the last again: masked
-            copy_tile<DP>(kp, a.d, ta_at, [&](int i) { return min(k0 + i, end - 1) * a.k_row; });
-            copy_tile<DP>(vp, a.d, tb_at, [&](int i) { return min(k0 + i, end - 1) * a.v_row; });
-        };
-        if (end > 0) copy_keys(0);
+    // a tile of rows: this lane's, and their sums
+    uint4v q[C], dO[C];
+    int lim;
+    float lse2, delta;
+    float16v dq[DP / 32];
+    auto begin_rows = [&](int tile, bool load) {
         const int row = tile * 32 + (lane & 31);
         const bool ok = row < rows;
         const int qi = divide(ok ? row : 0, a.G, inv), g = ok ? row - qi * a.G : 0;
-        const int lim = ok ? qi + shift : -1;
-        uint4v q[C], dO[C];
-        load_row<DP>(q, qp, qi * a.q_row + g * a.q_head, a.d, ok);
-        load_row<DP>(dO, dop, qi * a.g.do_row + g * a.g.do_head, a.d, ok);
-        const float lse2 = ok ? a.lse[(hk * a.G + g) * a.tq + p.q0 + qi] * kLog2e : 0.0f;
-        float delta = 0.0f;
-        float16v dq[DP / 32] = {};
-        // P and P dP of 32 keys, from the tiles; unseen keys give 0
-        auto products = [&](int k0, float16v &s, float16v &dp) {
-            s = dp = float16v{};
-#pragma unroll
-            for (int c = 0; c < C; c++) s = T::mfma(Tile<DP>::row(ta, 0, c), q[c], s);
-#pragma unroll
-            for (int c = 0; c < C; c++) dp = T::mfma(Tile<DP>::row(tb, 0, c), dO[c], dp);
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int key = k0 + 8 * (i / 4) + 4 * h + i % 4;
-                s[i] = key <= lim ? exp2_fast(__builtin_fmaf(s[i], a.c, -lse2)) : 0.0f;
-                dp[i] = key <= lim ? s[i] * dp[i] : 0.0f;
-            }
-        };
-        auto add = [&](const float16v &s, const float16v &dp) {
-#pragma unroll
-            for (int kc = 0; kc < 2; kc++) {
-                uint4v pb;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int i = 8 * kc + 2 * j;
-                    pb[j] = T::pack(dp[i] - s[i] * delta, dp[i + 1] - s[i + 1] * delta);
-                }
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; dt++)
-                    dq[dt] = T::mfma(Tile<DP>::transposed(ta, kc * 16, dt), pb, dq[dt]);
-            }
-        };
-        float16v s, dp;
-        for (int k0 = 0; k0 < end; k0 += 32) {
-            if (k0) copy_keys(k0);
-            wait_copies<0>();
-            products(k0, s, dp);
-#pragma unroll
-            for (int i = 0; i < 16; i++) delta += dp[i];
+        lim = ok ? qi + shift : -1;
+        if (load) {
+            load_row<DP>(q, qp, qi * a.q_row + g * a.q_head, a.d, ok);
+            load_row<DP>(dO, dop, qi * a.g.do_row + g * a.g.do_head, a.d, ok);
         }
-        delta = add_halves(delta);
-        if (end > 0 && end <= 32) {
-            add(s, dp);
-        } else {                             // once more, with delta
-            for (int k0 = 0; k0 < end; k0 += 32) {
-                copy_keys(k0);
-                wait_copies<0>();
-                products(k0, s, dp);
-                add(s, dp);
-            }
-        }
-        const int64_t t = p.q0 + qi, head = hk * a.G + g;
-        store_row<T, DP>(a.g.dq, t * a.g.dq_row + head * a.g.dq_head, dq, a.scale, a.d, ok);
+        lse2 = ok ? a.lse[(hk * a.G + g) * a.tq + p.q0 + qi] * kLog2e : 0.0f;
+        delta = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; dt++) dq[dt] = float16v{};
+    };
+    auto end_rows = [&](int tile, int free) {
+        store_tile<T, DP>(dqp, dq, a.scale, a.d, rows - tile * 32, lds[wave][free], [&](int i) {
+            return row_at(tile * 32 + i, a.g.dq_row, a.g.dq_head);
+        });
         if (h == 0) {
             lses[(tile & 3) * 32 + lane] = lse2;
             deltas[(tile & 3) * 32 + lane] = delta;
             lims[(tile & 3) * 32 + lane] = lim;
         }
+    };
+    auto products = [&](int k0, int tk, int tv, float16v &s, float16v &dp) {
+        s = dp = float16v{};
+#pragma unroll
+        for (int c = 0; c < C; c++) s = T::mfma(Tile<DP>::row(lds[wave][tk], 0, c), q[c], s);
+#pragma unroll
+        for (int c = 0; c < C; c++) dp = T::mfma(Tile<DP>::row(lds[wave][tv], 0, c), dO[c], dp);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int key = k0 + 8 * (i / 4) + 4 * h + i % 4;
+            s[i] = key <= lim ? exp2_fast(__builtin_fmaf(s[i], a.c, -lse2)) : 0.0f;
+            dp[i] = key <= lim ? s[i] * dp[i] : 0.0f;
+        }
+    };
+    auto add = [&](int tk, const float16v &s, const float16v &dp) {
+#pragma unroll
+        for (int kc = 0; kc < 2; kc++) {
+            uint4v pb;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int i = 8 * kc + 2 * j;
+                pb[j] = T::pack(dp[i] - s[i] * delta, dp[i + 1] - s[i + 1] * delta);
+            }
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; dt++)
+                dq[dt] = T::mfma(Tile<DP>::transposed(lds[wave][tk], kc * 16, dt), pb, dq[dt]);
+        }
+    };
+
+    // a tile of keys: this lane's, and their sums
+    uint4v k[C], v[C];
+    int key;
+    float16v dk[DP / 32], dv[DP / 32];
+    auto begin_keys = [&](int kt) {
+        key = kt * 32 + s0 - p.k0 + (lane & 31);
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; dt++) dk[dt] = dv[dt] = float16v{};
+    };
+    auto load_keys = [&](int kt) {
+        const int at = kt * 32 + s0 - p.k0 + (lane & 31);
+        const bool live = s0 + kt * 32 + (lane & 31) < s1 && at >= 0 && at < p.lk;
+        load_row<DP>(k, kp, at * a.k_row, a.d, live);
+        load_row<DP>(v, vp, at * a.v_row, a.d, live);
+    };
+    // adds the rows in the LDS tiles q and dO, statistics from `at` on
+    auto add_rows = [&](const uint16_t *tq, const uint16_t *to, int at) {
+        float16v s = {}, dp = {};
+#pragma unroll
+        for (int c = 0; c < C; c++) s = T::mfma(Tile<DP>::row(tq, 0, c), k[c], s);
+#pragma unroll
+        for (int c = 0; c < C; c++) dp = T::mfma(Tile<DP>::row(to, 0, c), v[c], dp);
+        uint32_t pp[8], pd[8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4v l4 = *(const float4v *)(lses + at + 8 * i + 4 * h);
+            const float4v e4 = *(const float4v *)(deltas + at + 8 * i + 4 * h);
+            const uint4v m4 = *(const uint4v *)(lims + at + 8 * i + 4 * h);
+            float pr[4], ds[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool see = key <= (int)m4[j];
+                pr[j] = see ? exp2_fast(__builtin_fmaf(s[4 * i + j], a.c, -l4[j])) : 0.0f;
+                ds[j] = see ? pr[j] * (dp[4 * i + j] - e4[j]) : 0.0f;
+            }
+            pp[2 * i] = T::pack(pr[0], pr[1]);
+            pp[2 * i + 1] = T::pack(pr[2], pr[3]);
+            pd[2 * i] = T::pack(ds[0], ds[1]);
+            pd[2 * i + 1] = T::pack(ds[2], ds[3]);
+        }
+#pragma unroll
+        for (int kc = 0; kc < 2; kc++) {
+            const uint4v pb = {pp[4 * kc], pp[4 * kc + 1], pp[4 * kc + 2], pp[4 * kc + 3]};
+            const uint4v db = {pd[4 * kc], pd[4 * kc + 1], pd[4 * kc + 2], pd[4 * kc + 3]};
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; dt++) {
+                dv[dt] = T::mfma(Tile<DP>::transposed(to, kc * 16, dt), pb, dv[dt]);
+                dk[dt] = T::mfma(Tile<DP>::transposed(tq, kc * 16, dt), db, dk[dt]);
+            }
+        }
+    };
+    auto end_keys = [&](int kt, int free_k, int free_v) {
+        const int n = s1 - s0 - kt * 32;
+        if (n <= (lane & 31) || key < 0 || key >= p.lk)      // a row that is no key's: zeros
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; dt++) dk[dt] = dv[dt] = float16v{};
+        store_tile<T, DP>((uint16_t *)a.g.dk + hk * a.g.dk_head, dk, a.scale, a.d, n,
+                          lds[wave][free_k], [&](int i) { return (s0 + kt * 32 + i) * a.g.dk_row; });
+        store_tile<T, DP>((uint16_t *)a.g.dv + hk * a.g.dv_head, dv, 1.0f, a.d, n,
+                          lds[wave][free_v], [&](int i) { return (s0 + kt * 32 + i) * a.g.dv_row; });
+    };
+
+    // Up to 64 rows and keys, the first 32 rows with up to 32 keys: each tile comes
+    // from memory once or twice, and what comes next is on its way meanwhile. K
+    // is in LDS tiles 0 and 1, V in 2 and 3; then the first rows in 1 and 3, the
+    // second in 0 and 2.
+    if (rows > 0 && rows <= 64 && s1 - s0 <= 64 && s0 == p.k0 && seen_by(0) > 0 && seen_by(0) <= 32) {
+        // this lane's row of an LDS tile, zero beyond d, where the tile repeats columns
+        auto row_of = [&](uint4v *f, int t) {
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                f[c] = Tile<DP>::row(lds[wave][t], 0, c);
+                if (a.d < DP && c * 16 + h * 8 >= a.d) f[c] = uint4v{0, 0, 0, 0};
+            }
+        };
+        float16v s, dp;
+        for (int tile = tiles - 1; tile >= 0; tile--) {
+            const int end = seen_by(tile);
+            if (tile == tiles - 1) copy_keys(0, end, 0, 2);
+            if (tile == 1 && end > 32) copy_keys(32, end, 1, 3);
+            if (tile == 0 && tiles == 1) copy_q(0, 1), copy_do(0, 3);
+            begin_rows(tile, tile == 1);
+            wait_copies<0>();
+            if (tile == 0) {
+                row_of(q, 1);
+                row_of(dO, 3);
+            }
+            products(0, 0, 2, s, dp);
+#pragma unroll
+            for (int i = 0; i < 16; i++) delta += dp[i];
+            if (end > 32) {
+                float16v s1, dp1;
+                products(32, 1, 3, s1, dp1);
+#pragma unroll
+                for (int i = 0; i < 16; i++) delta += dp1[i];
+                delta = add_halves(delta);
+                add(1, s1, dp1);
+            } else {
+                delta = add_halves(delta);
+            }
+            add(0, s, dp);
+            if (tile == 1) {
+                end_rows(1, 3);
+                copy_q(0, 1);
+                copy_do(0, 3);
+            } else {
+                row_of(k, 0);
+                row_of(v, 2);
+                end_rows(0, 2);
+                if (tiles == 2) copy_q(1, 0), copy_do(1, 2);
+            }
+        }
+        wave_sync();
+        for (int kt = 0; kt * 32 < s1 - s0; kt++) {
+            begin_keys(kt);
+            for (int tile = kt; tile < tiles; tile++) {
+                if (tile == 1) wait_copies<0>();
+                add_rows(lds[wave][1 - tile], lds[wave][3 - tile], tile * 32);
+            }
+            if (kt == 0 && s1 - s0 > 32) load_keys(1);
+            end_keys(kt, 1, 3);
+            landed(k);
+            landed(v);
+        }
+        return;
+    }
+
+    // Any other: the first row tile that sees a key of tile kt; the keys' part, kt by
+    // kt and tile by tile, has its next tile on the way while it works on one, and
+    // its first from here on
+    auto first_tile = [&](int kt) {
+        const int key0 = kt * 32 + s0 - p.k0;
+        return kt * 32 < s1 - s0 && key0 < p.lk ? max(key0 - shift, 0) * a.G / 32 : tiles;
+    };
+    int next = first_tile(mine);
+    int pair = 2;                            // the LDS tiles that the keys' part reads next
+    if (next < tiles) copy_q(next, pair), copy_do(next, pair + 1);
+
+    for (int tile = mine * 4; tile < mine * 4 + 4 && tile < tiles; tile++) {
+        const int end = seen_by(tile);
+        if (end > 0) copy_keys(0, end, 0, 1);
+        begin_rows(tile, true);
+        float16v s, dp;
+        for (int k0 = 0; k0 < end; k0 += 32) {
+            if (k0) copy_keys(k0, end, 0, 1);
+            wait_copies<0>();
+            products(k0, 0, 1, s, dp);
+#pragma unroll
+            for (int i = 0; i < 16; i++) delta += dp[i];
+        }
+        delta = add_halves(delta);
+        if (end > 0 && end <= 32) {
+            add(0, s, dp);
+        } else {                             // once more, with delta
+            for (int k0 = 0; k0 < end; k0 += 32) {
+                copy_keys(k0, end, 0, 1);
+                wait_copies<0>();
+                products(k0, 0, 1, s, dp);
+                add(0, s, dp);
+            }
+        }
+        end_rows(tile, 0);
     }
 
     for (int kt = mine; kt * 32 < s1 - s0; kt += shares) {
-        const int kr = s0 + kt * 32 + (lane & 31);               // this lane's key row
-        const int key0 = kt * 32 + s0 - p.k0, key = key0 + (lane & 31);
-        const bool live = kr < s1 && key >= 0 && key < p.lk;
-        float16v dk[DP / 32] = {}, dv[DP / 32] = {};
-        if (key0 < p.lk) {
-            uint4v k[C], v[C];
-            load_row<DP>(k, kp, key * a.k_row, a.d, live);
-            load_row<DP>(v, vp, key * a.v_row, a.d, live);
+        begin_keys(kt);
+        if (kt * 32 + s0 - p.k0 < p.lk) {
+            load_keys(kt);
             for (int tile = next; tile < tiles; tile++) {
                 int at = (tile & 3) * 32;
                 if (shares > 1) {
@@ -215,49 +366,11 @@ void attn_grad_short(AttnGrad a, int slots) {
                 const uint16_t *tq = lds[wave][pair], *to = lds[wave][pair + 1];
                 pair ^= 2;
                 next = tile + 1 < tiles ? tile + 1 : first_tile(kt + shares);
-                if (next < tiles) copy_rows(next, lds_at + pair * 64 * S);
-                float16v s = {}, dp = {};
-#pragma unroll
-                for (int c = 0; c < C; c++) s = T::mfma(Tile<DP>::row(tq, 0, c), k[c], s);
-#pragma unroll
-                for (int c = 0; c < C; c++) dp = T::mfma(Tile<DP>::row(to, 0, c), v[c], dp);
-                uint32_t pp[8], pd[8];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4v l4 = *(const float4v *)(lses + at + 8 * i + 4 * h);
-                    const float4v e4 = *(const float4v *)(deltas + at + 8 * i + 4 * h);
-                    const uint4v m4 = *(const uint4v *)(lims + at + 8 * i + 4 * h);
-                    float pr[4], ds[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const bool see = key <= (int)m4[j];
-                        pr[j] = see ? exp2_fast(__builtin_fmaf(s[4 * i + j], a.c, -l4[j])) : 0.0f;
-                        ds[j] = see ? pr[j] * (dp[4 * i + j] - e4[j]) : 0.0f;
-                    }
-                    pp[2 * i] = T::pack(pr[0], pr[1]);
-                    pp[2 * i + 1] = T::pack(pr[2], pr[3]);
-                    pd[2 * i] = T::pack(ds[0], ds[1]);
-                    pd[2 * i + 1] = T::pack(ds[2], ds[3]);
-                }
-#pragma unroll
-                for (int kc = 0; kc < 2; kc++) {
-                    const uint4v pb = {pp[4 * kc], pp[4 * kc + 1], pp[4 * kc + 2], pp[4 * kc + 3]};
-                    const uint4v db = {pd[4 * kc], pd[4 * kc + 1], pd[4 * kc + 2], pd[4 * kc + 3]};
-#pragma unroll
-                    for (int dt = 0; dt < DP / 32; dt++) {
-                        dv[dt] = T::mfma(Tile<DP>::transposed(to, kc * 16, dt), pb, dv[dt]);
-                        dk[dt] = T::mfma(Tile<DP>::transposed(tq, kc * 16, dt), db, dk[dt]);
-                    }
-                }
+                if (next < tiles) copy_q(next, pair), copy_do(next, pair + 1);
+                add_rows(tq, to, at);
             }
         }
-        if (!live)                           // a row that is no key's: zeros
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; dt++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) dk[dt][i] = dv[dt][i] = 0.0f;
-        store_row<T, DP>(a.g.dk, kr * a.g.dk_row + hk * a.g.dk_head, dk, a.scale, a.d, kr < s1);
-        store_row<T, DP>(a.g.dv, kr * a.g.dv_row + hk * a.g.dv_head, dv, 1.0f, a.d, kr < s1);
+        end_keys(kt, pair ^ 2, pair ^ 3);    // the next tile is on its way to the others
     }
 }
 

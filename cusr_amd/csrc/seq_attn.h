@@ -174,6 +174,7 @@ template <int N> __device__ inline void landed(uint4v (&x)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++) asm volatile("" : "+v"(x[i]));
 }
+
 // Barrier of the block that no memory access of the program moves across.
 __device__ inline void block_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
@@ -318,13 +319,11 @@ __device__ inline void load_row(uint4v *f, const void *base, int64_t off, int d,
 }
 
 // A column of a transposed accumulator (DP values of this lane's row, split
-// between the halves) scaled, packed and stored as 16-byte pieces. LOW: what the
-// packing rounds away instead.
-template <typename T, int DP, bool LOW = false>
-__device__ inline void store_row(void *base, int64_t off, const float16v *acc, float scale, int d,
-                                 bool ok) {
+// between the halves) scaled and packed to 16-byte pieces for sink(piece, value).
+// LOW: what the packing rounds away instead.
+template <typename T, int DP, bool LOW, typename F>
+__device__ inline void pack_row(const float16v *acc, float scale, F sink) {
     const int h = (threadIdx.x & 63) >> 5;
-    uint16_t *p = (uint16_t *)base + off;
 #pragma unroll
     for (int dt = 0; dt < DP / 32; dt++)
 #pragma unroll
@@ -342,9 +341,37 @@ __device__ inline void store_row(void *base, int64_t off, const float16v *acc, f
             auto s0 = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
             auto s1 = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
             uint4v v = {s0[0], s1[0], s0[1], s1[1]};
-            const int col = dt * 32 + g * 16 + h * 8;
-            if (d == DP ? ok : ok && col < d) *(uint4v *)(p + col) = v;
+            sink(dt * 4 + g * 2 + h, v);
         }
+}
+// ... stored: row `off` of this lane.
+template <typename T, int DP, bool LOW = false>
+__device__ inline void store_row(void *base, int64_t off, const float16v *acc, float scale, int d,
+                                 bool ok) {
+    uint16_t *p = (uint16_t *)base + off;
+    pack_row<T, DP, LOW>(acc, scale, [&](int piece, uint4v v) {
+        if (d == DP ? ok : ok && piece * 8 < d) *(uint4v *)(p + piece * 8) = v;
+    });
+}
+// ... stored for the wave's 32 rows, of which n exist, by way of an LDS tile: a
+// store then covers whole rows instead of 32 bytes of each. row_offset(i) is row
+// i's element offset.
+template <typename T, int DP, typename F>
+__device__ inline void store_tile(void *base, const float16v *acc, float scale, int d, int n,
+                                  uint16_t *t, F row_offset) {
+    constexpr int CHUNKS = Tile<DP>::chunks, ROWS = 64 / CHUNKS;
+    const int lane = threadIdx.x & 63;
+    pack_row<T, DP, false>(acc, scale, [&](int piece, uint4v v) {
+        *(uint4v *)(t + Tile<DP>::at(lane & 31, piece)) = v;
+    });
+    wave_sync();
+#pragma unroll
+    for (int x = 0; x < 32 / ROWS; x++) {
+        const int r = x * ROWS + lane / CHUNKS, piece = lane % CHUNKS ^ Tile<DP>::swz(r);
+        const uint4v v = *(const uint4v *)(t + (x * 64 + lane) * 8);
+        if (r < n && piece * 8 < d)
+            *(uint4v *)((uint16_t *)base + row_offset(r) + piece * 8) = v;
+    }
 }
 
 // 32 rows of a tensor to a wave's LDS tile, past the registers: row_offset(i)
