@@ -360,7 +360,8 @@ template <typename T, int DP, typename F>
 __device__ inline void store_tile(void *base, const float16v *acc, float scale, int d, int n,
                                   uint16_t *t, F row_offset) {
     constexpr int CHUNKS = Tile<DP>::chunks, ROWS = 64 / CHUNKS;
-    const int lane = threadIdx.x & 63;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));           // addresses are formed here, not held from before
     pack_row<T, DP, false>(acc, scale, [&](int piece, uint4v v) {
         *(uint4v *)(t + Tile<DP>::at(lane & 31, piece)) = v;
     });
