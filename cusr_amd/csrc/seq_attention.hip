@@ -433,7 +433,7 @@ int launch_head(const Attn &a, hipStream_t s) {
     if (plan_step(a, st)) return launch_step<T, DP>(a, st, s);
     const int64_t rows = a.n_seq ? a.tq * a.G / a.n_seq : 0;      // of a sequence, on average
     // Tiles shared by four waves from 96 rows on; below, two of the waves would idle
-    // (4 heads of 64, sequences of 32: 43 against 85 us, 64: alike, 96: 79 against 69 us).
+    // (4 heads of 64, sequences of 32: 45 against 85 us, 64: alike, 96: 74 against 69 us).
     if (rows >= 96) return launch_tiles<T, DP, 4>(a, s);
     const int slots = slot_of(a.tq, a.G, kShortRows, a.n_seq) + 1;
     const int64_t blocks = (slots * (int64_t)a.hkv + 3) / 4;

@@ -676,8 +676,8 @@ __global__ __launch_bounds__(KX * 128, KX == 4 || DP <= 64 ? 2 : 1) void attn_gr
 
 // Below these keys a sequence, on average, blocks of the long kernels mostly wait
 // for themselves; above, a wave alone takes longer (4 heads of 64: sequences of 96
-// 200 against 281 us, of 128 303 against 297 us; heads of 128, with half the waves:
-// of 64 193 against 309 us, of 100 612 against 457 us).
+// 199 against 282 us, of 128 300 against 297 us; heads of 128, with half the waves:
+// of 64 157 against 311 us, of 100 607 against 464 us).
 bool short_sequences(const Attn &a) {
     return a.tk < (padded_head(a.d) <= 64 ? 128ll : 80ll) * a.n_seq || a.n_seq == 0;
 }
