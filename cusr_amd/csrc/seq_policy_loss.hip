@@ -8,12 +8,19 @@
 
 namespace seq {
 
+// what a token brings beside its logits: read before them, so as not to wait after
+struct Token { float weight, advantage, old, ref; int64_t action; };
+__device__ inline Token token_of(const SeqPolicyLoss &p, int64_t t) {
+    return {p.weights[t], p.advantages[t], p.logp_old[t], p.logp_ref ? p.logp_ref[t] : 0.0f,
+            p.actions[t]};
+}
+
 // the token's loss term and d term / d logp
 struct Term { float loss, slope; };
-__device__ inline Term policy_term(const SeqPolicyLoss &p, int64_t t, float logp) {
+__device__ inline Term policy_term(const SeqPolicyLoss &p, const Token &k, float logp) {
     Term r;
-    const float A = p.advantages[t];
-    const float ratio = __expf(logp - p.logp_old[t]);
+    const float A = k.advantage;
+    const float ratio = __expf(logp - k.old);
     const float free_ = ratio * A;
     // comparisons rather than fminf and fmaxf, which would drop a NaN
     const float lo = 1.0f - p.clip_lo, hi = 1.0f + p.clip_hi;
@@ -21,7 +28,7 @@ __device__ inline Term policy_term(const SeqPolicyLoss &p, int64_t t, float logp
     r.loss = -(free_ <= held ? free_ : held);
     r.slope = free_ <= held ? -free_ : (held < free_ ? 0.0f : held);
     if (p.logp_ref) {
-        const float gap = p.logp_ref[t] - logp;
+        const float gap = k.ref - logp;
         const float e = expm1f(gap);
         r.loss += p.kl_coef * (gap > 80.0f ? e : e - gap);   // no inf - inf
         r.slope -= p.kl_coef * e;
@@ -107,14 +114,14 @@ __device__ inline void block_softmax(Running r, float k, float *red, float &m0, 
 // the action.
 struct RowGrad { float g, gs; };
 template <typename T>
-__device__ inline RowGrad finish_row(const SeqPolicyLoss &p, int64_t t, int64_t act, float xa,
-                                     float w, float m0, float sum, float &term, float &logp) {
+__device__ inline RowGrad finish_row(const SeqPolicyLoss &p, const Token &k, float xa, float m0,
+                                     float sum, float &term, float &logp) {
     const float inv_t = 1.0f / p.temperature;
     logp = xa == neg_inf() ? neg_inf() : (xa - m0) * inv_t - logf(sum);
-    const Term q = policy_term(p, t, logp);
-    term = w * q.loss;
+    const Term q = policy_term(p, k, logp);
+    term = k.weight * q.loss;
     RowGrad r;
-    r.g = logp == neg_inf() ? 0.0f : w * q.slope * inv_t;
+    r.g = logp == neg_inf() ? 0.0f : k.weight * q.slope * inv_t;
     if (p.dloss) r.g *= *p.dloss;
     r.gs = r.g == 0.0f ? 0.0f : -r.g / sum;
     return r;
@@ -122,7 +129,7 @@ __device__ inline RowGrad finish_row(const SeqPolicyLoss &p, int64_t t, int64_t 
 
 // A row per block, any size, stride and alignment: reads the row once for the
 // sums and, for the gradient, once more (mostly from the last cache). The loss
-// alone of 64 rows of 32,001 in fp32 takes 17 us with its sum, which is two
+// alone of 64 rows of 32,001 in fp32 takes 16 us with its sum, which is two
 // launches.
 template <typename T>
 __global__ __launch_bounds__(1024) void policy_stream(SeqPolicyLoss p, double *terms) {
@@ -130,14 +137,16 @@ __global__ __launch_bounds__(1024) void policy_stream(SeqPolicyLoss p, double *t
     const int64_t t = blockIdx.x;
     const T *x = (const T *)p.logits + t * p.row;
     T *dx = p.dlogits ? (T *)p.dlogits + t * p.drow : nullptr;
-    const float w = p.weights[t];
-    if (w == 0.0f) {
+    const Token of = token_of(p, t);
+    if (of.weight == 0.0f) {
         if (threadIdx.x == 0) { p.logp[t] = 0.0f; terms[t] = 0.0; }
         if (dx) for (int64_t j = threadIdx.x; j < p.vocab; j += 1024) dx[j] = (T)0.0f;
         return;
     }
     __shared__ float red[32];
     const float k = kLog2e / p.temperature;
+    const int64_t a = of.action;
+    const float xa = a >= 0 && a < p.vocab ? (float)x[a] : __builtin_nanf("");
     Running r;
     // whole 16-byte pieces between the row's first and last aligned address
     const int64_t head = (int64_t)((-(uintptr_t)x & 15) / sizeof(T));
@@ -156,9 +165,7 @@ __global__ __launch_bounds__(1024) void policy_stream(SeqPolicyLoss p, double *t
     }
     float m0, sum, term, logp;
     block_softmax<16>(r, k, red, m0, sum);
-    const int64_t a = p.actions[t];
-    const float xa = a >= 0 && a < p.vocab ? (float)x[a] : __builtin_nanf("");
-    const RowGrad g = finish_row<T>(p, t, a, xa, w, m0, sum, term, logp);
+    const RowGrad g = finish_row<T>(p, of, xa, m0, sum, term, logp);
     if (threadIdx.x == 0) { p.logp[t] = logp; terms[t] = term; }
     if (dx)
         for (int64_t j = threadIdx.x; j < p.vocab; j += 1024)
@@ -167,8 +174,8 @@ __global__ __launch_bounds__(1024) void policy_stream(SeqPolicyLoss p, double *t
 
 // A row per block of THREADS, kept in registers as NV pieces of 16 bytes a
 // thread: read once, written once; memory bounds it (8,192 rows of 131,071 in bf16,
-// a fifth of them without weight: 0.86 ms, 4.5 TB/s). Pieces are the aligned ones inside the row;
-// the few values before and after them go one to a thread.
+// a fifth of them without weight: 0.84 ms, 4.6 TB/s). Pieces are the aligned ones
+// inside the row; the few values before and after them go one to a thread.
 template <typename T, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS) void policy_row(SeqPolicyLoss p, double *terms) {
     constexpr int N = Vec<T>::n, WAVES = THREADS / 64;
@@ -181,8 +188,8 @@ __global__ __launch_bounds__(THREADS) void policy_row(SeqPolicyLoss p, double *t
     const int je = tid < head ? tid : pieces * N + tid;     // this thread's edge value
     const uint4v *x4 = (const uint4v *)(x + head);
     uint4v *d4 = (uint4v *)(dx + head);
-    const float w = p.weights[t];
-    if (w == 0.0f) {
+    const Token of = token_of(p, t);
+    if (of.weight == 0.0f) {
         if (tid == 0) { p.logp[t] = 0.0f; terms[t] = 0.0; }
         const uint4v z = {0, 0, 0, 0};
 #pragma unroll
@@ -202,7 +209,7 @@ __global__ __launch_bounds__(THREADS) void policy_row(SeqPolicyLoss p, double *t
         if (i * THREADS + tid < pieces) v[i] = (x4 + i * THREADS)[tid];
     }
     const float xe = tid < edge ? (float)x[je] : neg_inf();
-    const int64_t a = p.actions[t];
+    const int64_t a = of.action;
     const float xa = a >= 0 && a < V ? (float)x[a] : __builtin_nanf("");
     __shared__ float red[2 * WAVES];
     Running r;
@@ -216,7 +223,7 @@ __global__ __launch_bounds__(THREADS) void policy_row(SeqPolicyLoss p, double *t
     }
     float m0, sum, term, logp;
     block_softmax<WAVES>(r, k, red, m0, sum);
-    const RowGrad g = finish_row<T>(p, t, a, xa, w, m0, sum, term, logp);
+    const RowGrad g = finish_row<T>(p, of, xa, m0, sum, term, logp);
     if (tid == 0) { p.logp[t] = logp; terms[t] = term; }
     const int act = a >= 0 && a < V ? (int)a : -1;
 #pragma unroll
@@ -236,10 +243,13 @@ __global__ __launch_bounds__(THREADS) void policy_row(SeqPolicyLoss p, double *t
 }
 
 // Few symbols: a block takes R rows through LDS, in 16-byte pieces when they
-// lie end to end (`joined`); a thread owns a row. 1.3 M rows of 21 in bf16 take
-// 40 us, 3.5 TB/s. A thread starts its row at a column of
-// its own, so that rows of a power-of-two length spread over the banks.
-template <typename T, int R>
+// lie end to end (`joined`); a thread owns a row. TURN: a thread starts its row at a
+// column of its own, so that rows of a multiple of 16 bytes spread over the banks;
+// others do by themselves, and save half of the vector instructions, which bound
+// this beside memory: 1.3 M rows of 21 in bf16 take 34 us with their sum, 4.1 TB/s,
+// with turns 38 us. Unrolled loops take 61: the compiler joins columns to wider reads
+// off their alignment.
+template <typename T, int R, bool TURN>
 __global__ __launch_bounds__(R) void policy_symbols(SeqPolicyLoss p, bool joined, double *terms) {
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ double red[R / 64];
@@ -250,34 +260,48 @@ __global__ __launch_bounds__(R) void policy_symbols(SeqPolicyLoss p, bool joined
     const T *x = (const T *)p.logits + t0 * p.row;
     T *row = (T *)lds;
     const int n = rows * V, pieces = joined ? n / N : 0;
-    for (int i = threadIdx.x; i < pieces; i += R) ((uint4v *)lds)[i] = ((const uint4v *)x)[i];
+    const int64_t t = t0 + ((int)threadIdx.x < rows ? threadIdx.x : 0);
+    const Token of = token_of(p, t);
+    for (int i = threadIdx.x; i < pieces; i += R * 4) {
+        uint4v v[4];                         // four on their way at a time
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (i + j * R < pieces) v[j] = ((const uint4v *)x)[i + j * R];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (i + j * R < pieces) ((uint4v *)lds)[i + j * R] = v[j];
+    }
     for (int i = pieces * N + threadIdx.x; i < n; i += R) row[i] = x[(i / V) * p.row + i % V];
     __syncthreads();
-    const int64_t t = t0 + threadIdx.x;
     float term = 0.0f;
     if ((int)threadIdx.x < rows) {
         T *y = row + threadIdx.x * V;
-        const float w = p.weights[t];
-        const int j1 = (int)threadIdx.x % V;
-        if (w == 0.0f) {
+        // each column once
+        auto columns = [&](auto f) {
+            if (TURN) {
+                for (int i = 0, j = (int)threadIdx.x % V; i < V; i++, j = j + 1 == V ? 0 : j + 1) f(j);
+            } else {
+#pragma unroll 1
+                for (int j = 0; j < V; j++) f(j);
+            }
+        };
+        if (of.weight == 0.0f) {
             p.logp[t] = 0.0f;
-            for (int i = 0, j = j1; i < V; i++, j = j + 1 == V ? 0 : j + 1) y[j] = (T)0.0f;
+            columns([&](int j) { y[j] = (T)0.0f; });
         } else {
             const float k = kLog2e / p.temperature;
             float m = neg_inf(), sum = 0.0f, logp;
-            for (int i = 0, j = j1; i < V; i++, j = j + 1 == V ? 0 : j + 1)
-                m = fmaxf(m, (float)y[j]);
+            columns([&](int j) { m = fmaxf(m, (float)y[j]); });
             const float m0 = m == neg_inf() ? 0.0f : m;
-            for (int i = 0, j = j1; i < V; i++, j = j + 1 == V ? 0 : j + 1)
-                sum += exp2_fast(((float)y[j] - m0) * k);
-            const int64_t a = p.actions[t];
+            columns([&](int j) { sum += exp2_fast(((float)y[j] - m0) * k); });
+            const int64_t a = of.action;
             const float xa = a >= 0 && a < V ? (float)y[a] : __builtin_nanf("");
-            const RowGrad g = finish_row<T>(p, t, a, xa, w, m0, sum, term, logp);
+            const RowGrad g = finish_row<T>(p, of, xa, m0, sum, term, logp);
             p.logp[t] = logp;
             if (p.dlogits)
-                for (int i = 0, j = j1; i < V; i++, j = j + 1 == V ? 0 : j + 1)
-                    y[j] = (T)((j == a ? g.g : 0.0f) +
-                               g.gs * exp2_fast(((float)y[j] - m0) * k));
+                columns([&](int j) {
+                    y[j] = (T)((j == a ? g.g : 0.0f) + g.gs * exp2_fast(((float)y[j] - m0) * k));
+                });
         }
     }
     double s = term;
@@ -299,6 +323,7 @@ __global__ __launch_bounds__(R) void policy_symbols(SeqPolicyLoss p, bool joined
 __global__ __launch_bounds__(1024) void policy_sum(const double *terms, int64_t n, float *loss) {
     __shared__ double red[16];
     double s = 0.0;
+#pragma unroll 8
     for (int64_t i = threadIdx.x; i < n; i += 1024) s += terms[i];
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -327,6 +352,13 @@ int check_policy(const SeqPolicyLoss *p) {
     return CO_OK;
 }
 
+template <typename T, int R>
+void launch_symbols(const SeqPolicyLoss &p, bool turn, bool joined, dim3 grid, size_t lds,
+                    double *terms, hipStream_t s) {
+    if (turn) policy_symbols<T, R, true><<<grid, R, lds, s>>>(p, joined, terms);
+    else policy_symbols<T, R, false><<<grid, R, lds, s>>>(p, joined, terms);
+}
+
 template <typename T, int THREADS, int NV>
 void launch_row(const SeqPolicyLoss &p, double *terms, hipStream_t s) {
     policy_row<T, THREADS, NV><<<dim3((unsigned)p.tokens), THREADS, 0, s>>>(p, terms);
@@ -343,9 +375,12 @@ int64_t launch_policy(const SeqPolicyLoss &p, double *terms, hipStream_t s) {
         const bool joined = p.row == p.vocab && !((uintptr_t)p.logits & 15) &&
                             (!p.dlogits || (p.drow == p.vocab && !((uintptr_t)p.dlogits & 15)));
         const size_t lds = (size_t)rows * p.vocab * sizeof(T);
-        if (rows == 256) policy_symbols<T, 256><<<grid, 256, lds, s>>>(p, joined, terms);
-        else if (rows == 128) policy_symbols<T, 128><<<grid, 128, lds, s>>>(p, joined, terms);
-        else policy_symbols<T, 64><<<grid, 64, lds, s>>>(p, joined, terms);
+        // five waves a compute unit, for rows beyond 256 bytes, wait longer for reads one
+        // by one than the turns cost (262,144 rows of 252 in bf16: 186 against 157 us)
+        const bool turn = p.vocab * sizeof(T) % 16 == 0;
+        if (rows == 256) launch_symbols<T, 256>(p, turn, joined, grid, lds, terms, s);
+        else if (rows == 128) launch_symbols<T, 128>(p, turn, joined, grid, lds, terms, s);
+        else policy_symbols<T, 64, true><<<grid, 64, lds, s>>>(p, joined, terms);
         return blocks;
     }
     // A row stays in registers while it has at most 16 pieces for each of 1024 threads

@@ -53,8 +53,8 @@ template <typename T> struct Piece {
 
 // A thread owns one piece's place in the head (in the half layout, the piece
 // and its partner half a turn further) of one token and runs over `per` heads
-// of q and k with the same cosines and sines: 146 us, 4.6 TB/s, for the same. Needs 16-byte rows and heads and
-// pairs that fill pieces.
+// of q and k with the same cosines and sines: 146 us, 4.6 TB/s, for the same. Needs
+// 16-byte rows and heads and pairs that fill pieces.
 template <typename T, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_pieces(SeqRotary r, int items, int per) {
     constexpr int N = Piece<T>::n, P = INTERLEAVED ? N / 2 : N;    // pairs of a thread
