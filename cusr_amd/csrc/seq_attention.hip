@@ -26,7 +26,7 @@ __device__ inline void store_out(const Attn &a, int t, int head, const float16v 
 // loaded to registers while the present ones are worked on. Without it both go to
 // LDS past the registers, which leaves room for more waves.
 struct Row { int t, head; bool ok; };
-template <typename T, int DP, bool AHEAD>
+template <typename T, int DP, bool AHEAD, typename I>
 __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, int key0, int key1,
                                uint16_t *kt, uint16_t *vt, float16v *o, float &m, float &l) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -48,10 +48,10 @@ __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, 
     auto fetch = [&](int k0) {
         if (!AHEAD) {
             copy_tile<DP>(kp, a.d, lds_address(kt),
-                          [&](int i) { return min(k0 + i, end - 1) * a.k_row; });
+                          [&](int i) { return times<I>(min(k0 + i, end - 1), a.k_row); });
             if (k0 == key0) load_q();
             copy_tile<DP>(vp, a.d, lds_address(vt),
-                          [&](int i) { return min(k0 + i, end - 1) * a.v_row; });
+                          [&](int i) { return times<I>(min(k0 + i, end - 1), a.v_row); });
         } else {
             const int r = min(k0 + (lane & 31), end - 1);
             load_row<DP>(k, kp, r * a.k_row, a.d, true);
@@ -125,6 +125,27 @@ __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, 
 // 4, take 191 us (4.2 TB/s); with K to registers 207, with the output stored as 32
 // bytes of each row 205.
 constexpr int kShortRows = 128;
+template <typename T, int DP, typename I>
+__device__ inline void wave_tiles(const Attn &a, const Place &p, int hk, int first, uint16_t *kt,
+                                  uint16_t *vt) {
+    const int rows = p.lq * a.G;
+    const float inv = 1.0f / (float)a.G;
+    for (int tile = first; tile < first + kShortRows / 32 && tile * 32 < rows; tile++) {
+        float16v o[DP / 32];
+        float m, l;
+        const Row r = run_rows<T, DP, false, I>(a, p, hk, tile, 0, p.lk, kt, vt, o, m, l);
+        if (a.o_low) {
+            store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok);
+            continue;
+        }
+        uint16_t *op = (uint16_t *)a.o + p.q0 * a.o_row + hk * a.G * a.o_head;
+        store_tile<T, DP>(op, o, l == 0.0f ? 0.0f : 1.0f / l, a.d, rows - tile * 32, kt, [&](int i) {
+            const int row = min(tile * 32 + i, rows - 1), qi = quotient<I>(row, a.G, inv);
+            return times<I>(qi, a.o_row) + times<I>(row - qi * a.G, a.o_head);
+        });
+        store_lse(a, r.t, r.head, m, l, r.ok);
+    }
+}
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void attn_wave(Attn a, int slots) {
     __shared__ __align__(256) uint16_t lds[4][2][32 * Tile<DP>::stride];
@@ -138,23 +159,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void attn_wave(Attn a, int s
     const Place p = place_of(a, b, f.start, f.end);
     const int first = (slot - slot_of(p.q0, a.G, kShortRows, b)) * (kShortRows / 32);
     if (first < 0) return;
-    for (int tile = first; tile < first + kShortRows / 32 && tile * 32 < p.lq * a.G; tile++) {
-        float16v o[DP / 32];
-        float m, l;
-        const Row r = run_rows<T, DP, false>(a, p, hk, tile, 0, p.lk, kt, vt, o, m, l);
-        if (a.o_low) {
-            store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok);
-            continue;
-        }
-        const int rows = p.lq * a.G;
-        const float inv = 1.0f / (float)a.G;
-        uint16_t *op = (uint16_t *)a.o + p.q0 * a.o_row + hk * a.G * a.o_head;
-        store_tile<T, DP>(op, o, l == 0.0f ? 0.0f : 1.0f / l, a.d, rows - tile * 32, kt, [&](int i) {
-            const int row = min(tile * 32 + i, rows - 1), qi = divide(row, a.G, inv);
-            return qi * a.o_row + (row - qi * a.G) * a.o_head;
-        });
-        store_lse(a, r.t, r.head, m, l, r.ok);
-    }
+    if (a.near && p.lq * a.G <= kNear && p.lk <= kNear) wave_tiles<T, DP, uint32_t>(a, p, hk, first, kt, vt);
+    else wave_tiles<T, DP, int64_t>(a, p, hk, first, kt, vt);
 }
 
 // Long sequences: a block of WAVES waves owns WAVES * 32 rows of one key head;
@@ -310,7 +316,7 @@ __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
     for (int tile = blockIdx.y; tile * 32 < rows; tile += st.tiles) {
         float16v o[DP / 32];
         float m, l;
-        const Row r = run_rows<T, DP, true>(a, p, hk, tile, key0, key1, vt, vt, o, m, l);
+        const Row r = run_rows<T, DP, true, int64_t>(a, p, hk, tile, key0, key1, vt, vt, o, m, l);
         if (!split) {
             store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok);
             continue;

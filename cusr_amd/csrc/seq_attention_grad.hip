@@ -88,23 +88,25 @@ void attn_grad_short(AttnGrad a, int slots) {
 
     // tiles to LDS tiles, past the registers. Beyond the last row or key, the last
     // again: it is masked, by its last visible key -1
-    auto row_at = [&](int i, int64_t step, int64_t head) {
-        const int row = min(i, rows - 1), qi = divide(row, a.G, inv);
-        return qi * step + (row - qi * a.G) * head;
+    auto row_at = [&](auto as, int i, int64_t step, int64_t head) {
+        typedef decltype(as) I;
+        const int row = min(i, rows - 1), qi = quotient<I>(row, a.G, inv);
+        return times<I>(qi, step) + times<I>(row - qi * a.G, head);
     };
-    auto copy_q = [&](int tile, int to) {
+    auto copy_q = [&](auto as, int tile, int to) {
         copy_tile<DP>(qp, a.d, lds_at + to * 64 * S,
-                      [&](int i) { return row_at(tile * 32 + i, a.q_row, a.q_head); });
+                      [&](int i) { return row_at(as, tile * 32 + i, a.q_row, a.q_head); });
     };
-    auto copy_do = [&](int tile, int to) {
+    auto copy_do = [&](auto as, int tile, int to) {
         copy_tile<DP>(dop, a.d, lds_at + to * 64 * S,
-                      [&](int i) { return row_at(tile * 32 + i, a.g.do_row, a.g.do_head); });
+                      [&](int i) { return row_at(as, tile * 32 + i, a.g.do_row, a.g.do_head); });
     };
-    auto copy_keys = [&](int k0, int end, int tk, int tv) {
+    auto copy_keys = [&](auto as, int k0, int end, int tk, int tv) {
+        typedef decltype(as) I;
         copy_tile<DP>(kp, a.d, lds_at + tk * 64 * S,
-                      [&](int i) { return min(k0 + i, end - 1) * a.k_row; });
+                      [&](int i) { return times<I>(min(k0 + i, end - 1), a.k_row); });
         copy_tile<DP>(vp, a.d, lds_at + tv * 64 * S,
-                      [&](int i) { return min(k0 + i, end - 1) * a.v_row; });
+                      [&](int i) { return times<I>(min(k0 + i, end - 1), a.v_row); });
     };
     // keys that a tile of rows sees
     auto seen_by = [&](int tile) {
@@ -130,9 +132,9 @@ void attn_grad_short(AttnGrad a, int slots) {
 #pragma unroll
         for (int dt = 0; dt < DP / 32; dt++) dq[dt] = float16v{};
     };
-    auto end_rows = [&](int tile, int free) {
+    auto end_rows = [&](auto as, int tile, int free) {
         store_tile<T, DP>(dqp, dq, a.scale, a.d, rows - tile * 32, lds[wave][free], [&](int i) {
-            return row_at(tile * 32 + i, a.g.dq_row, a.g.dq_head);
+            return row_at(as, tile * 32 + i, a.g.dq_row, a.g.dq_head);
         });
         if (h == 0) {
             lses[(tile & 3) * 32 + lane] = lse2;
@@ -219,22 +221,27 @@ void attn_grad_short(AttnGrad a, int slots) {
             }
         }
     };
-    auto end_keys = [&](int kt, int free_k, int free_v) {
+    uint16_t *dkp = (uint16_t *)a.g.dk + s0 * a.g.dk_row + hk * a.g.dk_head;
+    uint16_t *dvp = (uint16_t *)a.g.dv + s0 * a.g.dv_row + hk * a.g.dv_head;
+    auto end_keys = [&](auto as, int kt, int free_k, int free_v) {
+        typedef decltype(as) I;
         const int n = s1 - s0 - kt * 32;
         if (n <= (lane & 31) || key < 0 || key >= p.lk)      // a row that is no key's: zeros
 #pragma unroll
             for (int dt = 0; dt < DP / 32; dt++) dk[dt] = dv[dt] = float16v{};
-        store_tile<T, DP>((uint16_t *)a.g.dk + hk * a.g.dk_head, dk, a.scale, a.d, n,
-                          lds[wave][free_k], [&](int i) { return (s0 + kt * 32 + i) * a.g.dk_row; });
-        store_tile<T, DP>((uint16_t *)a.g.dv + hk * a.g.dv_head, dv, 1.0f, a.d, n,
-                          lds[wave][free_v], [&](int i) { return (s0 + kt * 32 + i) * a.g.dv_row; });
+        store_tile<T, DP>(dkp, dk, a.scale, a.d, n, lds[wave][free_k],
+                          [&](int i) { return times<I>(kt * 32 + i, a.g.dk_row); });
+        store_tile<T, DP>(dvp, dv, 1.0f, a.d, n, lds[wave][free_v],
+                          [&](int i) { return times<I>(kt * 32 + i, a.g.dv_row); });
     };
 
     // Up to 64 rows and keys, the first 32 rows with up to 32 keys: each tile comes
     // from memory once or twice, and what comes next is on its way meanwhile. K
     // is in LDS tiles 0 and 1, V in 2 and 3; then the first rows in 1 and 3, the
     // second in 0 and 2.
-    if (rows > 0 && rows <= 64 && s1 - s0 <= 64 && s0 == p.k0 && seen_by(0) > 0 && seen_by(0) <= 32) {
+    if (a.near && rows > 0 && rows <= 64 && s1 - s0 <= 64 && s0 == p.k0 &&
+        seen_by(0) > 0 && seen_by(0) <= 32) {
+        const uint32_t as = 0;
         // this lane's row of an LDS tile, zero beyond d, where the tile repeats columns
         auto row_of = [&](uint4v *f, int t) {
 #pragma unroll
@@ -246,9 +253,9 @@ void attn_grad_short(AttnGrad a, int slots) {
         float16v s, dp;
         for (int tile = tiles - 1; tile >= 0; tile--) {
             const int end = seen_by(tile);
-            if (tile == tiles - 1) copy_keys(0, end, 0, 2);
-            if (tile == 1 && end > 32) copy_keys(32, end, 1, 3);
-            if (tile == 0 && tiles == 1) copy_q(0, 1), copy_do(0, 3);
+            if (tile == tiles - 1) copy_keys(as, 0, end, 0, 2);
+            if (tile == 1 && end > 32) copy_keys(as, 32, end, 1, 3);
+            if (tile == 0 && tiles == 1) copy_q(as, 0, 1), copy_do(as, 0, 3);
             begin_rows(tile, tile == 1);
             wait_copies<0>();
             if (tile == 0) {
@@ -270,14 +277,14 @@ void attn_grad_short(AttnGrad a, int slots) {
             }
             add(0, s, dp);
             if (tile == 1) {
-                end_rows(1, 3);
-                copy_q(0, 1);
-                copy_do(0, 3);
+                end_rows(as, 1, 3);
+                copy_q(as, 0, 1);
+                copy_do(as, 0, 3);
             } else {
                 row_of(k, 0);
                 row_of(v, 2);
-                end_rows(0, 2);
-                if (tiles == 2) copy_q(1, 0), copy_do(1, 2);
+                end_rows(as, 0, 2);
+                if (tiles == 2) copy_q(as, 1, 0), copy_do(as, 1, 2);
             }
         }
         wave_sync();
@@ -288,7 +295,7 @@ void attn_grad_short(AttnGrad a, int slots) {
                 add_rows(lds[wave][1 - tile], lds[wave][3 - tile], tile * 32);
             }
             if (kt == 0 && s1 - s0 > 32) load_keys(1);
-            end_keys(kt, 1, 3);
+            end_keys(as, kt, 1, 3);
             landed(k);
             landed(v);
         }
@@ -302,17 +309,18 @@ void attn_grad_short(AttnGrad a, int slots) {
         const int key0 = kt * 32 + s0 - p.k0;
         return kt * 32 < s1 - s0 && key0 < p.lk ? max(key0 - shift, 0) * a.G / 32 : tiles;
     };
+    const int64_t as = 0;
     int next = first_tile(mine);
     int pair = 2;                            // the LDS tiles that the keys' part reads next
-    if (next < tiles) copy_q(next, pair), copy_do(next, pair + 1);
+    if (next < tiles) copy_q(as, next, pair), copy_do(as, next, pair + 1);
 
     for (int tile = mine * 4; tile < mine * 4 + 4 && tile < tiles; tile++) {
         const int end = seen_by(tile);
-        if (end > 0) copy_keys(0, end, 0, 1);
+        if (end > 0) copy_keys(as, 0, end, 0, 1);
         begin_rows(tile, true);
         float16v s, dp;
         for (int k0 = 0; k0 < end; k0 += 32) {
-            if (k0) copy_keys(k0, end, 0, 1);
+            if (k0) copy_keys(as, k0, end, 0, 1);
             wait_copies<0>();
             products(k0, 0, 1, s, dp);
 #pragma unroll
@@ -323,13 +331,13 @@ void attn_grad_short(AttnGrad a, int slots) {
             add(0, s, dp);
         } else {                             // once more, with delta
             for (int k0 = 0; k0 < end; k0 += 32) {
-                copy_keys(k0, end, 0, 1);
+                copy_keys(as, k0, end, 0, 1);
                 wait_copies<0>();
                 products(k0, 0, 1, s, dp);
                 add(0, s, dp);
             }
         }
-        end_rows(tile, 0);
+        end_rows(as, tile, 0);
     }
 
     for (int kt = mine; kt * 32 < s1 - s0; kt += shares) {
@@ -366,11 +374,11 @@ void attn_grad_short(AttnGrad a, int slots) {
                 const uint16_t *tq = lds[wave][pair], *to = lds[wave][pair + 1];
                 pair ^= 2;
                 next = tile + 1 < tiles ? tile + 1 : first_tile(kt + shares);
-                if (next < tiles) copy_q(next, pair), copy_do(next, pair + 1);
+                if (next < tiles) copy_q(as, next, pair), copy_do(as, next, pair + 1);
                 add_rows(tq, to, at);
             }
         }
-        end_keys(kt, pair ^ 2, pair ^ 3);    // the next tile is on its way to the others
+        end_keys(as, kt, pair ^ 2, pair ^ 3);    // the next tile is on its way to the others
     }
 }
 
@@ -750,10 +758,10 @@ extern "C" int seq_attention_grad(const SeqAttention *sa, const SeqAttentionGrad
         return CO_ERR_DATA;
     if (sa->workspace_bytes < 8 * (sa->hq * sa->tq + 1)) return CO_ERR_DATA;
     seq::AttnGrad a;
-    static_cast<SeqAttention &>(a) = *sa;
-    a.G = a.hq / a.hkv;
-    a.c = a.scale * seq::kLog2e;
+    static_cast<seq::Attn &>(a) = seq::make_attn(sa);
     a.g = *g;
+    a.near = a.near && seq::near_strides(g->do_row, g->do_head, g->dq_row, g->dq_head) &&
+             seq::near_strides(g->dk_row, g->dk_head, g->dv_row, g->dv_head);
     a.stat = (float *)sa->workspace;
     hipStream_t s = (hipStream_t)stream;
     return a.dtype == SEQ_BF16 ? seq::launch_grad_head<seq::Bf16>(a, s)

@@ -20,7 +20,12 @@ namespace seq {
 struct Attn : SeqAttention {
     int32_t G;       // query heads per key head
     float c;         // scale * log2(e): scores in powers of two
+    int32_t near;    // every stride is below 2^16 elements
 };
+inline bool near_strides(int64_t a, int64_t b, int64_t c, int64_t d) {
+    const int64_t most = 1 << 16;
+    return a >= 0 && b >= 0 && c >= 0 && d >= 0 && a < most && b < most && c < most && d < most;
+}
 
 __device__ inline int clamp_to(int x, int lo, int64_t hi) {
     return x < lo ? lo : (x > hi ? (int)hi : x);
@@ -34,6 +39,19 @@ __device__ inline int divide(int x, int n, float inv) {
     q += (int)((float)(x - q * n) * inv);
     const int r = x - q * n;
     return q + (r >= n) - (r < 0);
+}
+
+// Offsets inside a sequence as int64_t, or as uint32_t where the strides are near and
+// rows, queries and keys at most kNear: then they, in bytes too, have 32 bits, their
+// factors 24, and the quotient of a row needs no correction.
+constexpr int kNear = 1 << 14;
+template <typename I> __device__ inline I times(int i, int64_t step) {
+    if constexpr (sizeof(I) == 4) return __umul24(i, (uint32_t)step);
+    else return i * step;
+}
+template <typename I> __device__ inline int quotient(int x, int n, float inv) {
+    if constexpr (sizeof(I) == 4) return (int)(((float)x + 0.5f) * inv);
+    else return divide(x, n, inv);
 }
 
 // Rows, query rows times heads among them, number less than 2^31 (the entry
@@ -370,13 +388,13 @@ __device__ inline void store_tile(void *base, const float16v *acc, float scale, 
     for (int x = 0; x < 32 / ROWS; x++) {
         const int r = x * ROWS + lane / CHUNKS, piece = lane % CHUNKS ^ Tile<DP>::swz(r);
         const uint4v v = *(const uint4v *)(t + (x * 64 + lane) * 8);
-        if (r < n && piece * 8 < d)
-            *(uint4v *)((uint16_t *)base + row_offset(r) + piece * 8) = v;
+        const auto at = row_offset(r) + piece * 8;
+        if (r < n && piece * 8 < d) *(uint4v *)((char *)base + 2 * at) = v;
     }
 }
 
 // 32 rows of a tensor to a wave's LDS tile, past the registers: row_offset(i)
-// is row i's element offset from `base`. Columns beyond d repeat the first.
+// is row i's element offset from `base`, which is the wave's. Columns beyond d repeat the first.
 template <int DP, typename F>
 __device__ inline void copy_tile(const void *base, int d, uint32_t to, F row_offset) {
     constexpr int STRIDE = Tile<DP>::stride * 2, ROWS = 1024 / STRIDE;
@@ -386,8 +404,9 @@ __device__ inline void copy_tile(const void *base, int d, uint32_t to, F row_off
     for (int x = 0; x < 32 / ROWS; x++) {
         const int r = x * ROWS + lane * 16 / STRIDE;
         const int ch = (lane * 16 % STRIDE / 16) ^ Tile<DP>::swz(r);
-        copy_to_lds16((const uint16_t *)base + row_offset(r) + (ch * 8 < d ? ch * 8 : 0),
-                      to + x * 1024);
+        const auto at = row_offset(r) + (ch * 8 < d ? ch * 8 : 0);
+        if constexpr (sizeof(at) == 4) copy_to_lds16(base, 2 * at, to + x * 1024);
+        else copy_to_lds16((const uint16_t *)base + at, to + x * 1024);
     }
 }
 
@@ -396,6 +415,8 @@ inline Attn make_attn(const SeqAttention *s) {
     static_cast<SeqAttention &>(a) = *s;
     a.G = a.hq / a.hkv;
     a.c = a.scale * kLog2e;
+    a.near = near_strides(a.q_row, a.q_head, a.k_row, a.k_head) &&
+             near_strides(a.v_row, a.v_head, a.o_row, a.o_head);
     return a;
 }
 

@@ -116,6 +116,20 @@ def test_attention_newest_tokens(ops, pairs, room, hq, hkv, d, dtype):
     assert not bool(dk[~rows].any()) and not bool(dv[~rows].any())
 
 
+# up to 64 rows and keys: one tile or two of each, fewer keys than queries among them
+SHORT = [
+    ([(60, 40), (64, 64), (33, 20), (20, 50), (1, 64), (64, 1), (40, 33)], 0, 2, 2, 64, BF),
+    ([(30, 20), (32, 32), (16, 16), (17, 17), (9, 31), (1, 1)], 5, 4, 2, 64, FP),
+    ([(64, 60), (31, 31), (32, 3), (50, 50)], 4, 1, 1, 128, BF),
+    ([(7, 7), (8, 2), (3, 33), (8, 40)], 1, 16, 2, 40, FP),
+]
+
+
+@pytest.mark.parametrize("pairs,room,hq,hkv,d,dtype", SHORT)
+def test_attention_short_pairs(ops, pairs, room, hq, hkv, d, dtype):
+    test_attention_newest_tokens(ops, pairs, room, hq, hkv, d, dtype)
+
+
 def test_attention_strides_and_order(ops):
     """q, k, v as slices of one projection, heads before rows, and a layout
     that the kernels do not read directly give the same bits."""
@@ -142,6 +156,29 @@ def test_attention_strides_and_order(ops):
         assert torch.equal(o, o2) and torch.equal(lse, l2), how
         g2 = ops.attention_grad(other(do, how), *a, other(o, how), lse, c)
         assert all(torch.equal(x, y) for x, y in zip(g, g2)), how
+
+
+def test_attention_far_strides(ops):
+    """Rows and heads beyond 2^16 elements apart, where offsets take 64 bits."""
+    lens, hq, hkv, d = [40, 9, 64, 25], 4, 2, 64
+    T, c = sum(lens), cu(lens)
+    q, k, v, do = (normal((T, h, d), BF, i + 40) for i, h in enumerate((hq, hkv, hkv, hq)))
+
+    def far(x):
+        y = torch.empty(x.shape[0], 70000, dtype=x.dtype, device=DEV)[:, :x.shape[1] * d]
+        return y.view(x.shape[0], x.shape[1], d).copy_(x)
+
+    def far_heads(x):
+        y = torch.empty(x.shape[1], 1100, d, dtype=x.dtype, device=DEV)[:, :x.shape[0]]
+        return y.transpose(0, 1).copy_(x)
+
+    r = ref.attention(q, k, v, c, c, do=do)
+    for how in (far, far_heads):
+        x, y, z, w = (how(t) for t in (q, k, v, do))
+        o, lse = ops.attention(x, y, z, c, return_lse=True)
+        g = ops.attention_grad(w, x, y, z, o, lse, c)
+        for n, got in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *g)):
+            check(n, got, r[n], r[n + "_tol"])
 
 
 def test_attention_same_bits_and_streams(ops):
