@@ -49,21 +49,23 @@ __device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float
 // past the registers. What bounds it is the chain of loads from the slot to the
 // rows beside vector instructions (half the time) with two waves a SIMD, hence
 // the path of its own for up to 64 rows and keys, in which few loads wait for
-// others: 8,192 sequences of 3 to 63, 8 heads of 64, take 0.60 ms (3.2 TB/s), on
-// the general path 0.73; stores of 32 bytes of each row instead of whole rows
-// took 0.02 more.
+// others and P and dS are formed once: 8,192 sequences of 3 to 63, 8 heads of 64,
+// take 0.47 ms (4.1 TB/s), with P and dS formed twice 0.58, on the general path 0.73.
 constexpr int kShortRows = 128;
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1)
 void attn_grad_short(AttnGrad a, int slots) {
     constexpr int C = DP / 16, S = Tile<DP>::stride;
-    __shared__ __align__(256) uint16_t lds[4][4][32 * S];
-    __shared__ __align__(16) float stats[4][3][kShortRows];     // lse, delta, last visible key
+    // four tiles of a wave, and a fifth for P and dS of a pair of tiles, for results on
+    // their way out, or for rows' statistics: lse, delta, last visible key
+    constexpr int FIFTH = DP < 64 ? 64 * 32 : 32 * S;
+    __shared__ __align__(256) uint16_t lds_all[4][4 * 32 * S + FIFTH];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    const uint32_t lds_at = lds_address(lds[wave][0]);
-    float *lses = stats[wave][0], *deltas = stats[wave][1];
-    int *lims = (int *)stats[wave][2];
+    uint16_t (*lds)[32 * S] = (uint16_t(*)[32 * S])lds_all[wave], *fifth = lds[4];
+    const uint32_t lds_at = lds_address(lds[0]);
+    float *lses = (float *)fifth, *deltas = lses + kShortRows;
+    int *lims = (int *)(deltas + kShortRows);
     const int item = blockIdx.x * 4 + wave;
     const int slot = item / a.hkv, hk = item - slot * a.hkv;
     if (slot >= slots) return;
@@ -132,22 +134,17 @@ void attn_grad_short(AttnGrad a, int slots) {
 #pragma unroll
         for (int dt = 0; dt < DP / 32; dt++) dq[dt] = float16v{};
     };
-    auto end_rows = [&](auto as, int tile, int free) {
-        store_tile<T, DP>(dqp, dq, a.scale, a.d, rows - tile * 32, lds[wave][free], [&](int i) {
+    auto end_rows = [&](auto as, int tile, uint16_t *free) {
+        store_tile<T, DP>(dqp, dq, a.scale, a.d, rows - tile * 32, free, [&](int i) {
             return row_at(as, tile * 32 + i, a.g.dq_row, a.g.dq_head);
         });
-        if (h == 0) {
-            lses[(tile & 3) * 32 + lane] = lse2;
-            deltas[(tile & 3) * 32 + lane] = delta;
-            lims[(tile & 3) * 32 + lane] = lim;
-        }
     };
     auto products = [&](int k0, int tk, int tv, float16v &s, float16v &dp) {
         s = dp = float16v{};
 #pragma unroll
-        for (int c = 0; c < C; c++) s = T::mfma(Tile<DP>::row(lds[wave][tk], 0, c), q[c], s);
+        for (int c = 0; c < C; c++) s = T::mfma(Tile<DP>::row(lds[tk], 0, c), q[c], s);
 #pragma unroll
-        for (int c = 0; c < C; c++) dp = T::mfma(Tile<DP>::row(lds[wave][tv], 0, c), dO[c], dp);
+        for (int c = 0; c < C; c++) dp = T::mfma(Tile<DP>::row(lds[tv], 0, c), dO[c], dp);
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const int key = k0 + 8 * (i / 4) + 4 * h + i % 4;
@@ -155,18 +152,18 @@ void attn_grad_short(AttnGrad a, int slots) {
             dp[i] = key <= lim ? s[i] * dp[i] : 0.0f;
         }
     };
-    auto add = [&](int tk, const float16v &s, const float16v &dp) {
+    // dS in the type, and dQ's sum
+    auto add = [&](int tk, const float16v &s, const float16v &dp, uint4v (&ds)[2]) {
 #pragma unroll
         for (int kc = 0; kc < 2; kc++) {
-            uint4v pb;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int i = 8 * kc + 2 * j;
-                pb[j] = T::pack(dp[i] - s[i] * delta, dp[i + 1] - s[i + 1] * delta);
+                ds[kc][j] = T::pack(dp[i] - s[i] * delta, dp[i + 1] - s[i + 1] * delta);
             }
 #pragma unroll
             for (int dt = 0; dt < DP / 32; dt++)
-                dq[dt] = T::mfma(Tile<DP>::transposed(lds[wave][tk], kc * 16, dt), pb, dq[dt]);
+                dq[dt] = T::mfma(Tile<DP>::transposed(lds[tk], kc * 16, dt), ds[kc], dq[dt]);
         }
     };
 
@@ -174,7 +171,7 @@ void attn_grad_short(AttnGrad a, int slots) {
     uint4v k[C], v[C];
     int key;
     float16v dk[DP / 32], dv[DP / 32];
-    auto begin_keys = [&](int kt) {
+    auto begin_keys = [&](int kt) {          // with zeros
         key = kt * 32 + s0 - p.k0 + (lane & 31);
 #pragma unroll
         for (int dt = 0; dt < DP / 32; dt++) dk[dt] = dv[dt] = float16v{};
@@ -223,82 +220,116 @@ void attn_grad_short(AttnGrad a, int slots) {
     };
     uint16_t *dkp = (uint16_t *)a.g.dk + s0 * a.g.dk_row + hk * a.g.dk_head;
     uint16_t *dvp = (uint16_t *)a.g.dv + s0 * a.g.dv_row + hk * a.g.dv_head;
-    auto end_keys = [&](auto as, int kt, int free_k, int free_v) {
+    auto end_keys = [&](auto as, int kt, uint16_t *free) {
         typedef decltype(as) I;
         const int n = s1 - s0 - kt * 32;
         if (n <= (lane & 31) || key < 0 || key >= p.lk)      // a row that is no key's: zeros
 #pragma unroll
             for (int dt = 0; dt < DP / 32; dt++) dk[dt] = dv[dt] = float16v{};
-        store_tile<T, DP>(dkp, dk, a.scale, a.d, n, lds[wave][free_k],
+        store_tile<T, DP>(dkp, dk, a.scale, a.d, n, free,
                           [&](int i) { return times<I>(kt * 32 + i, a.g.dk_row); });
-        store_tile<T, DP>(dvp, dv, 1.0f, a.d, n, lds[wave][free_v],
+        store_tile<T, DP>(dvp, dv, 1.0f, a.d, n, free,
                           [&](int i) { return times<I>(kt * 32 + i, a.g.dv_row); });
     };
 
-    // Up to 64 rows and keys, the first 32 rows with up to 32 keys: each tile comes
-    // from memory once or twice, and what comes next is on its way meanwhile. K
-    // is in LDS tiles 0 and 1, V in 2 and 3; then the first rows in 1 and 3, the
-    // second in 0 and 2.
-    if (a.near && rows > 0 && rows <= 64 && s1 - s0 <= 64 && s0 == p.k0 &&
-        seen_by(0) > 0 && seen_by(0) <= 32) {
+    // Up to 64 rows and keys, the first 32 rows with up to 32 keys: P and dS are formed
+    // once and turned round by way of LDS, and each tile comes from memory once or
+    // twice. K is in LDS tiles 0 and 1, V in 2 and 3; then the second rows, and at
+    // last the first, in 1 and 3.
+    if (a.near && rows > 0 && rows <= 64 && s1 - s0 <= 64 && s0 == p.k0 && seen_by(0) > 0 &&
+        seen_by(0) <= 32) {
         const uint32_t as = 0;
         // this lane's row of an LDS tile, zero beyond d, where the tile repeats columns
         auto row_of = [&](uint4v *f, int t) {
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                f[c] = Tile<DP>::row(lds[wave][t], 0, c);
+                f[c] = Tile<DP>::row(lds[t], 0, c);
                 if (a.d < DP && c * 16 + h * 8 >= a.d) f[c] = uint4v{0, 0, 0, 0};
             }
         };
+        auto pack = [&](const float16v &s, uint4v (&ps)[2]) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) ps[i / 4][i % 4] = T::pack(s[2 * i], s[2 * i + 1]);
+        };
+        // dK's and dV's sums, with the rows' tiles in 1 and 3
+        auto add_block = [&](const uint4v (&ps)[2], const uint4v (&ds)[2]) {
+            typedef Tile<32> Block;
+            uint16_t *pt = fifth, *dt_ = fifth + 32 * 32;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int at = Block::at(lane & 31, g) + 4 * h;
+                const uint2v x = {ps[g / 2][g % 2 * 2], ps[g / 2][g % 2 * 2 + 1]};
+                const uint2v y = {ds[g / 2][g % 2 * 2], ds[g / 2][g % 2 * 2 + 1]};
+                *(uint2v *)(pt + at) = x;
+                *(uint2v *)(dt_ + at) = y;
+            }
+            wave_sync();
+#pragma unroll
+            for (int kc = 0; kc < 2; kc++) {
+                const uint4v pb = Block::transposed(pt, kc * 16, 0);
+                const uint4v db = Block::transposed(dt_, kc * 16, 0);
+#pragma unroll
+                for (int dt = 0; dt < DP / 32; dt++) {
+                    dv[dt] = T::mfma(Tile<DP>::transposed(lds[3], kc * 16, dt), pb, dv[dt]);
+                    dk[dt] = T::mfma(Tile<DP>::transposed(lds[1], kc * 16, dt), db, dk[dt]);
+                }
+            }
+            wave_sync();
+        };
+        const int end = seen_by(tiles - 1);
+        const bool second = s1 - s0 > 32;    // a second tile of keys
         float16v s, dp;
-        for (int tile = tiles - 1; tile >= 0; tile--) {
-            const int end = seen_by(tile);
-            if (tile == tiles - 1) copy_keys(as, 0, end, 0, 2);
-            if (tile == 1 && end > 32) copy_keys(as, 32, end, 1, 3);
-            if (tile == 0 && tiles == 1) copy_q(as, 0, 1), copy_do(as, 0, 3);
-            begin_rows(tile, tile == 1);
+        uint4v ps[2], ds[2];
+        copy_keys(as, 0, end, 0, 2);
+        if (tiles == 2) {
+            if (end > 32) copy_keys(as, 32, end, 1, 3);
+            begin_rows(1, true);
             wait_copies<0>();
-            if (tile == 0) {
-                row_of(q, 1);
-                row_of(dO, 3);
-            }
             products(0, 0, 2, s, dp);
+            float16v s1, dp1;
+            uint4v ps1[2], ds1[2];
+            if (end > 32) products(32, 1, 3, s1, dp1);
+            else s1 = dp1 = float16v{};
 #pragma unroll
-            for (int i = 0; i < 16; i++) delta += dp[i];
-            if (end > 32) {
-                float16v s1, dp1;
-                products(32, 1, 3, s1, dp1);
+            for (int i = 0; i < 16; i++) delta += dp[i] + dp1[i];
+            delta = add_halves(delta);
+            pack(s, ps);
+            pack(s1, ps1);
+            add(0, s, dp, ds);
+            if (end > 32) add(1, s1, dp1, ds1);
+            copy_q(as, 1, 1);
+            copy_do(as, 1, 3);
+            end_rows(as, 1, fifth);
+            wait_copies<0>();
+            if (second) {
+                begin_keys(1);
+                if (end > 32) add_block(ps1, ds1);
+                end_keys(as, 1, fifth);
+            }
+            begin_keys(0);
+            add_block(ps, ds);
+        } else {
+            if (second) {
+                begin_keys(1);
+                end_keys(as, 1, fifth);
+            }
+            begin_keys(0);
+        }
+        copy_q(as, 0, 1);
+        copy_do(as, 0, 3);
+        begin_rows(0, false);
+        wait_copies<0>();
+        row_of(q, 1);
+        row_of(dO, 3);
+        products(0, 0, 2, s, dp);
 #pragma unroll
-                for (int i = 0; i < 16; i++) delta += dp1[i];
-                delta = add_halves(delta);
-                add(1, s1, dp1);
-            } else {
-                delta = add_halves(delta);
-            }
-            add(0, s, dp);
-            if (tile == 1) {
-                end_rows(as, 1, 3);
-                copy_q(as, 0, 1);
-                copy_do(as, 0, 3);
-            } else {
-                row_of(k, 0);
-                row_of(v, 2);
-                end_rows(as, 0, 2);
-                if (tiles == 2) copy_q(as, 1, 0), copy_do(as, 1, 2);
-            }
-        }
-        wave_sync();
-        for (int kt = 0; kt * 32 < s1 - s0; kt++) {
-            begin_keys(kt);
-            for (int tile = kt; tile < tiles; tile++) {
-                if (tile == 1) wait_copies<0>();
-                add_rows(lds[wave][1 - tile], lds[wave][3 - tile], tile * 32);
-            }
-            if (kt == 0 && s1 - s0 > 32) load_keys(1);
-            end_keys(as, kt, 1, 3);
-            landed(k);
-            landed(v);
-        }
+        for (int i = 0; i < 16; i++) delta += dp[i];
+        delta = add_halves(delta);
+        pack(s, ps);
+        add(0, s, dp, ds);
+        add_block(ps, ds);
+        end_rows(as, 0, fifth);
+        end_keys(as, 0, fifth);
         return;
     }
 
@@ -327,17 +358,23 @@ void attn_grad_short(AttnGrad a, int slots) {
             for (int i = 0; i < 16; i++) delta += dp[i];
         }
         delta = add_halves(delta);
+        uint4v ds[2];
         if (end > 0 && end <= 32) {
-            add(0, s, dp);
+            add(0, s, dp, ds);
         } else {                             // once more, with delta
             for (int k0 = 0; k0 < end; k0 += 32) {
                 copy_keys(as, k0, end, 0, 1);
                 wait_copies<0>();
                 products(k0, 0, 1, s, dp);
-                add(0, s, dp);
+                add(0, s, dp, ds);
             }
         }
-        end_rows(as, tile, 0);
+        end_rows(as, tile, lds[0]);
+        if (h == 0) {
+            lses[(tile & 3) * 32 + lane] = lse2;
+            deltas[(tile & 3) * 32 + lane] = delta;
+            lims[(tile & 3) * 32 + lane] = lim;
+        }
     }
 
     for (int kt = mine; kt * 32 < s1 - s0; kt += shares) {
@@ -371,14 +408,14 @@ void attn_grad_short(AttnGrad a, int slots) {
                     }
                 }
                 wait_copies<0>();
-                const uint16_t *tq = lds[wave][pair], *to = lds[wave][pair + 1];
+                const uint16_t *tq = lds[pair], *to = lds[pair + 1];
                 pair ^= 2;
                 next = tile + 1 < tiles ? tile + 1 : first_tile(kt + shares);
                 if (next < tiles) copy_q(as, next, pair), copy_do(as, next, pair + 1);
                 add_rows(tq, to, at);
             }
         }
-        end_keys(as, kt, pair ^ 2, pair ^ 3);    // the next tile is on its way to the others
+        end_keys(as, kt, lds[pair ^ 2]);     // the next tile is on its way to the others
     }
 }
 
