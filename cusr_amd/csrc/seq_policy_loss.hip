@@ -8,19 +8,48 @@
 
 namespace seq {
 
+// exp(x / temperature) for x <= 0 as a power of two. The factor has two parts, for what
+// 32 bits round away would be the same relative error in every exponent of every
+// token and so reach the loss undiminished. Both are positive: -inf stays itself. `two`:
+// the second part is a quarter of a rounding or more (at temperature 1 it is a fifth).
+// The branch on it splits the sums of a long row by pieces, which the compiler
+// otherwise runs into each other: 8,192 rows of 131,071 in bf16 take 0.75 ms with it
+// at either temperature, 0.90 with the second part always, 0.85 with none.
+struct Scale {
+    float high, low, nearest;
+    bool two;
+    double inverse;                          // 1 / temperature
+    __device__ float exp(float x) const { return exp2_fast(__builtin_fmaf(x, high, x * low)); }
+    // for a gradient, whose errors are its own
+    __device__ float exp_nearest(float x) const { return exp2_fast(x * nearest); }
+};
+struct Policy : SeqPolicyLoss { Scale scale; };
+
+Policy make_policy(const SeqPolicyLoss *p) {
+    Policy r;
+    static_cast<SeqPolicyLoss &>(r) = *p;
+    const double k = 1.4426950408889634 / (double)p->temperature;
+    r.scale.high = r.scale.nearest = (float)k;
+    if ((double)r.scale.high > k) r.scale.high = nextafterf(r.scale.high, 0.0f);
+    r.scale.two = fabs(k - (double)r.scale.nearest) > k * 0x1p-26;
+    r.scale.inverse = 1.0 / (double)p->temperature;
+    r.scale.low = fmaxf((float)(k - (double)r.scale.high), 1e-37f);
+    return r;
+}
+
 // what a token brings beside its logits: read before them, so as not to wait after
 struct Token { float weight, advantage, old, ref; int64_t action; };
-__device__ inline Token token_of(const SeqPolicyLoss &p, int64_t t) {
+__device__ inline Token token_of(const Policy &p, int64_t t) {
     return {p.weights[t], p.advantages[t], p.logp_old[t], p.logp_ref ? p.logp_ref[t] : 0.0f,
             p.actions[t]};
 }
 
 // the token's loss term and d term / d logp
 struct Term { float loss, slope; };
-__device__ inline Term policy_term(const SeqPolicyLoss &p, const Token &k, float logp) {
+__device__ inline Term policy_term(const Policy &p, const Token &k, double logp) {
     Term r;
     const float A = k.advantage;
-    const float ratio = __expf(logp - k.old);
+    const float ratio = expf((float)(logp - (double)k.old));
     const float free_ = ratio * A;
     // comparisons rather than fminf and fmaxf, which would drop a NaN
     const float lo = 1.0f - p.clip_lo, hi = 1.0f + p.clip_hi;
@@ -28,7 +57,7 @@ __device__ inline Term policy_term(const SeqPolicyLoss &p, const Token &k, float
     r.loss = -(free_ <= held ? free_ : held);
     r.slope = free_ <= held ? -free_ : (held < free_ ? 0.0f : held);
     if (p.logp_ref) {
-        const float gap = k.ref - logp;
+        const float gap = (float)((double)k.ref - logp);
         const float e = expm1f(gap);
         r.loss += p.kl_coef * (gap > 80.0f ? e : e - gap);   // no inf - inf
         r.slope -= p.kl_coef * e;
@@ -67,17 +96,21 @@ template <> struct Vec<float> {
     }
 };
 
-// Running maximum m and sum of exp2((x - m) k) of a thread.
+// Running maximum m and sum of exp((x - m) / temperature) of a thread.
 struct Running {
     float m = neg_inf(), s = 0.0f;
-    template <int N> __device__ void add(const float *x, float k) {
+    template <int N> __device__ void add(const float *x, Scale k) {
         float c = x[0];
 #pragma unroll
         for (int j = 1; j < N; j++) c = fmaxf(c, x[j]);
         const float mn = fmaxf(m, c), m0 = mn == neg_inf() ? 0.0f : mn;
-        s *= exp2_fast((m - m0) * k);
+        s *= k.exp(m - m0);
+        if (k.two)
 #pragma unroll
-        for (int j = 0; j < N; j++) s += exp2_fast((x[j] - m0) * k);
+            for (int j = 0; j < N; j++) s += k.exp(x[j] - m0);
+        else
+#pragma unroll
+            for (int j = 0; j < N; j++) s += k.exp_nearest(x[j] - m0);
         m = mn;
     }
 };
@@ -85,7 +118,7 @@ struct Running {
 // The maximum and the sum of a block's running pairs, in one order, on every
 // thread. red holds 2 * waves floats.
 template <int WAVES>
-__device__ inline void block_softmax(Running r, float k, float *red, float &m0, float &sum) {
+__device__ inline void block_softmax(Running r, Scale k, float *red, float &m0, float &sum) {
     float m = r.m;
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     const int w = threadIdx.x >> 6;
@@ -98,7 +131,7 @@ __device__ inline void block_softmax(Running r, float k, float *red, float &m0, 
     }
     m0 = m == neg_inf() ? 0.0f : m;
     // a thread without a finite value has r.m = -inf and s = 0 (or NaN)
-    float s = r.s * (r.m == neg_inf() ? 1.0f : exp2_fast((r.m - m0) * k));
+    float s = r.s * (r.m == neg_inf() ? 1.0f : k.exp(r.m - m0));
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
     if (WAVES > 1) {
         if ((threadIdx.x & 63) == 0) red[WAVES + w] = s;
@@ -110,15 +143,22 @@ __device__ inline void block_softmax(Running r, float k, float *red, float &m0, 
     sum = s;
 }
 
-// What a row's gradient needs: dlogits_j = gs * exp2((x_j - m0) k), plus g at
+// What a row's gradient needs: dlogits_j = gs exp((x_j - m0) / temperature), plus g at
 // the action.
 struct RowGrad { float g, gs; };
 template <typename T>
-__device__ inline RowGrad finish_row(const SeqPolicyLoss &p, const Token &k, float xa, float m0,
+__device__ inline RowGrad finish_row(const Policy &p, const Token &k, float xa, float m0,
                                      float sum, float &term, float &logp) {
     const float inv_t = 1.0f / p.temperature;
-    logp = xa == neg_inf() ? neg_inf() : (xa - m0) * inv_t - logf(sum);
-    const Term q = policy_term(p, k, logp);
+    // in 64 bits but for the mantissa's logarithm: differences from the other policies'
+    // follow, which are small beside the terms
+    int e;
+    const float mantissa = frexpf(sum, &e);
+    double l = ((double)xa - (double)m0) * p.scale.inverse -
+               ((double)e * 0.69314718055994531 + (double)logf(mantissa));
+    if (xa == neg_inf()) l = -__builtin_inf();
+    logp = (float)l;
+    const Term q = policy_term(p, k, l);
     term = k.weight * q.loss;
     RowGrad r;
     r.g = logp == neg_inf() ? 0.0f : k.weight * q.slope * inv_t;
@@ -132,7 +172,7 @@ __device__ inline RowGrad finish_row(const SeqPolicyLoss &p, const Token &k, flo
 // alone of 64 rows of 32,001 in fp32 takes 16 us with its sum, which is two
 // launches.
 template <typename T>
-__global__ __launch_bounds__(1024) void policy_stream(SeqPolicyLoss p, double *terms) {
+__global__ __launch_bounds__(1024) void policy_stream(Policy p, double *terms) {
     constexpr int N = Vec<T>::n;
     const int64_t t = blockIdx.x;
     const T *x = (const T *)p.logits + t * p.row;
@@ -144,7 +184,7 @@ __global__ __launch_bounds__(1024) void policy_stream(SeqPolicyLoss p, double *t
         return;
     }
     __shared__ float red[32];
-    const float k = kLog2e / p.temperature;
+    const Scale k = p.scale;
     const int64_t a = of.action;
     const float xa = a >= 0 && a < p.vocab ? (float)x[a] : __builtin_nanf("");
     Running r;
@@ -169,15 +209,15 @@ __global__ __launch_bounds__(1024) void policy_stream(SeqPolicyLoss p, double *t
     if (threadIdx.x == 0) { p.logp[t] = logp; terms[t] = term; }
     if (dx)
         for (int64_t j = threadIdx.x; j < p.vocab; j += 1024)
-            dx[j] = (T)((j == a ? g.g : 0.0f) + g.gs * exp2_fast(((float)x[j] - m0) * k));
+            dx[j] = (T)((j == a ? g.g : 0.0f) + g.gs * k.exp_nearest((float)x[j] - m0));
 }
 
 // A row per block of THREADS, kept in registers as NV pieces of 16 bytes a
 // thread: read once, written once; memory bounds it (8,192 rows of 131,071 in bf16,
-// a fifth of them without weight: 0.84 ms, 4.6 TB/s). Pieces are the aligned ones
+// a fifth of them without weight: 0.75 ms, 5.2 TB/s). Pieces are the aligned ones
 // inside the row; the few values before and after them go one to a thread.
 template <typename T, int THREADS, int NV>
-__global__ __launch_bounds__(THREADS) void policy_row(SeqPolicyLoss p, double *terms) {
+__global__ __launch_bounds__(THREADS) void policy_row(Policy p, double *terms) {
     constexpr int N = Vec<T>::n, WAVES = THREADS / 64;
     const int64_t t = blockIdx.x;
     const T *x = (const T *)p.logits + t * p.row;
@@ -198,7 +238,7 @@ __global__ __launch_bounds__(THREADS) void policy_row(SeqPolicyLoss p, double *t
         if (tid < edge) dx[je] = (T)0.0f;
         return;
     }
-    const float k = kLog2e / p.temperature;
+    const Scale k = p.scale;
     uint4v v[NV];
     const float ninf[8] = {neg_inf(), neg_inf(), neg_inf(), neg_inf(),
                            neg_inf(), neg_inf(), neg_inf(), neg_inf()};
@@ -233,24 +273,24 @@ __global__ __launch_bounds__(THREADS) void policy_row(SeqPolicyLoss p, double *t
         // the unpacked values of the first pass are not to be kept: twice the registers
         asm volatile("" : "+v"(v[i]));
 #pragma unroll
-        for (int j = 0; j < N; j++) f[j] = g.gs * exp2_fast((Vec<T>::get(v[i], j) - m0) * k);
+        for (int j = 0; j < N; j++) f[j] = g.gs * k.exp_nearest(Vec<T>::get(v[i], j) - m0);
         if (act >= j0 && act < j0 + N)
 #pragma unroll
             for (int j = 0; j < N; j++) f[j] += j0 + j == act ? g.g : 0.0f;
         if (i * THREADS + tid < pieces) (d4 + i * THREADS)[tid] = Vec<T>::pack(f);
     }
-    if (tid < edge) dx[je] = (T)((je == act ? g.g : 0.0f) + g.gs * exp2_fast((xe - m0) * k));
+    if (tid < edge) dx[je] = (T)((je == act ? g.g : 0.0f) + g.gs * k.exp_nearest(xe - m0));
 }
 
 // Few symbols: a block takes R rows through LDS, in 16-byte pieces when they
 // lie end to end (`joined`); a thread owns a row. TURN: a thread starts its row at a
 // column of its own, so that rows of a multiple of 16 bytes spread over the banks;
 // others do by themselves, and save half of the vector instructions, which bound
-// this beside memory: 1.3 M rows of 21 in bf16 take 34 us with their sum, 4.1 TB/s,
-// with turns 38 us. Unrolled loops take 61: the compiler joins columns to wider reads
+// this beside memory: 1.3 M rows of 21 in bf16 take 36 us with their sum, 3.9 TB/s,
+// with turns 40 us. Unrolled loops take 61: the compiler joins columns to wider reads
 // off their alignment.
 template <typename T, int R, bool TURN>
-__global__ __launch_bounds__(R) void policy_symbols(SeqPolicyLoss p, bool joined, double *terms) {
+__global__ __launch_bounds__(R) void policy_symbols(Policy p, bool joined, double *terms) {
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ double red[R / 64];
     constexpr int N = Vec<T>::n;
@@ -289,18 +329,18 @@ __global__ __launch_bounds__(R) void policy_symbols(SeqPolicyLoss p, bool joined
             p.logp[t] = 0.0f;
             columns([&](int j) { y[j] = (T)0.0f; });
         } else {
-            const float k = kLog2e / p.temperature;
+            const Scale k = p.scale;
             float m = neg_inf(), sum = 0.0f, logp;
             columns([&](int j) { m = fmaxf(m, (float)y[j]); });
             const float m0 = m == neg_inf() ? 0.0f : m;
-            columns([&](int j) { sum += exp2_fast(((float)y[j] - m0) * k); });
+            columns([&](int j) { sum += k.exp((float)y[j] - m0); });
             const int64_t a = of.action;
             const float xa = a >= 0 && a < V ? (float)y[a] : __builtin_nanf("");
             const RowGrad g = finish_row<T>(p, of, xa, m0, sum, term, logp);
             p.logp[t] = logp;
             if (p.dlogits)
                 columns([&](int j) {
-                    y[j] = (T)((j == a ? g.g : 0.0f) + g.gs * exp2_fast(((float)y[j] - m0) * k));
+                    y[j] = (T)((j == a ? g.g : 0.0f) + g.gs * k.exp_nearest((float)y[j] - m0));
                 });
         }
     }
@@ -353,20 +393,20 @@ int check_policy(const SeqPolicyLoss *p) {
 }
 
 template <typename T, int R>
-void launch_symbols(const SeqPolicyLoss &p, bool turn, bool joined, dim3 grid, size_t lds,
+void launch_symbols(const Policy &p, bool turn, bool joined, dim3 grid, size_t lds,
                     double *terms, hipStream_t s) {
     if (turn) policy_symbols<T, R, true><<<grid, R, lds, s>>>(p, joined, terms);
     else policy_symbols<T, R, false><<<grid, R, lds, s>>>(p, joined, terms);
 }
 
 template <typename T, int THREADS, int NV>
-void launch_row(const SeqPolicyLoss &p, double *terms, hipStream_t s) {
+void launch_row(const Policy &p, double *terms, hipStream_t s) {
     policy_row<T, THREADS, NV><<<dim3((unsigned)p.tokens), THREADS, 0, s>>>(p, terms);
 }
 
 // Launches the rows' kernel; returns the number of terms it leaves.
 template <typename T>
-int64_t launch_policy(const SeqPolicyLoss &p, double *terms, hipStream_t s) {
+int64_t launch_policy(const Policy &p, double *terms, hipStream_t s) {
     constexpr int N = Vec<T>::n;
     const int rows = symbol_rows(p);
     if (rows) {
@@ -420,14 +460,15 @@ extern "C" int seq_policy_loss(const SeqPolicyLoss *p, void *stream) {
     double *ws = (double *)p->workspace;
     int64_t terms = 0;
     if (p->tokens) {
+        const seq::Policy x = seq::make_policy(p);
         if (!p->logits || !p->actions || !p->logp_old || !p->advantages || !p->weights ||
             !p->logp || !p->workspace)
             return CO_ERR_NULLARG;
         if (p->workspace_bytes < 8 * p->tokens) return CO_ERR_DATA;
         switch (p->dtype) {
-            case SEQ_FP32: terms = seq::launch_policy<float>(*p, ws, s); break;
-            case SEQ_BF16: terms = seq::launch_policy<__bf16>(*p, ws, s); break;
-            default: terms = seq::launch_policy<_Float16>(*p, ws, s); break;
+            case SEQ_FP32: terms = seq::launch_policy<float>(x, ws, s); break;
+            case SEQ_BF16: terms = seq::launch_policy<__bf16>(x, ws, s); break;
+            default: terms = seq::launch_policy<_Float16>(x, ws, s); break;
         }
         rc = seq::launch_status();
         if (rc != CO_OK) return rc;
