@@ -572,14 +572,16 @@ __global__ __launch_bounds__(KX * 128, KX == 4 || DP <= 64 ? 2 : 1) void attn_gr
     const int wave_start = wkey0 < p.lk ? first_row(wkey0) : rows;
     const uint32_t lds0 = lds_address(lds);
     // One tile's copies: this wave's share of q and do, and two waves' statistics.
-    // When the group's heads divide 32 rows, a whole tile's rows lie at the same
+    // When the group's heads divide 32 rows, and the rows from one copy of the wave to
+    // its next (narrow blocks of wide heads: 16), a whole tile's rows lie at the same
     // lane offsets from an address of the wave.
+    constexpr int NEXT = PER > WAVES ? WAVES * (1024 / STRIDE) : RB;
     const int row_l = wave % PER * (1024 / STRIDE) + lane * 16 / STRIDE;    // in the tile
     const int ch_l = (lane * 16 % STRIDE / 16) ^ Tile<DP>::swz(row_l);
     const int col_l = ch_l * 8 < a.d ? ch_l * 8 : 0;
     const int64_t q_most = a.q_row * 64 + a.q_head * a.G, o_most = a.g.do_row * 64 + a.g.do_head * a.G;
-    const bool plain = 32 % a.G == 0 && a.q_row >= 0 && a.q_head >= 0 && a.g.do_row >= 0 &&
-                       a.g.do_head >= 0 && q_most < 1 << 30 && o_most < 1 << 30;
+    const bool plain = 32 % a.G == 0 && NEXT % a.G == 0 && a.q_row >= 0 && a.q_head >= 0 &&
+                       a.g.do_row >= 0 && a.g.do_head >= 0 && q_most < 1 << 30 && o_most < 1 << 30;
     const uint32_t q_off = 2 * (uint32_t)(row_l / a.G * a.q_row + row_l % a.G * a.q_head + col_l);
     const uint32_t o_off = 2 * (uint32_t)(row_l / a.G * a.g.do_row + row_l % a.G * a.g.do_head + col_l);
     const uint16_t *q0p = (const uint16_t *)a.q + p.q0 * a.q_row + (int64_t)hk * a.G * a.q_head;

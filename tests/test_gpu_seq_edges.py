@@ -1,0 +1,47 @@
+"""Sequence operators where layouts, launches and values meet their edges: groups
+as wide as a tile, other orders of arguments and memory, values that have no
+finite term."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import seq_reference as ref
+from test_gpu_seq import BF, F32, FP, DEV, _say, check, cu, normal
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from cusr_amd.kernel import seq_ops
+    return seq_ops
+
+
+# ------------------------------------------------------------------ attention
+
+# many query heads a key head, lengths of the long kernels: a copy's rows then begin
+# inside a query's heads
+WIDE_GROUPS = [
+    ([300, 90], 32, 1, 128, BF),
+    ([257], 32, 1, 80, FP),
+    ([200, 120], 64, 2, 96, BF),
+    ([130, 131], 32, 1, 64, BF),
+    ([140, 200], 32, 1, 24, FP),
+    ([190], 64, 1, 128, BF),
+    ([100, 85], 48, 2, 128, FP),
+    ([160], 128, 1, 96, BF),
+    ([90] * 70, 128, 4, 128, FP),          # enough blocks of 128 keys to fill the chip
+]
+
+
+@pytest.mark.parametrize("lens,hq,hkv,d,dtype", WIDE_GROUPS)
+def test_attention_wide_groups(ops, lens, hq, hkv, d, dtype):
+    T, c = sum(lens), cu(lens)
+    _say("wide groups", lens[:4], hq, hkv, d, dtype)
+    q, k, v, do = (normal((T, h, d), dtype, i + 1) for i, h in enumerate((hq, hkv, hkv, hq)))
+    o, lse = ops.attention(q, k, v, c, return_lse=True)
+    g = ops.attention_grad(do, q, k, v, o, lse, c)
+    r = ref.attention(q, k, v, c, c, do=do)
+    for n, x in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *g)):
+        check(n, x, r[n], r[n + "_tol"])
