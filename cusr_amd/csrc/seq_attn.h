@@ -167,20 +167,20 @@ __device__ inline uint32_t lds_address(const void *p) {
 // loads are on their way. Written in assembly because the compiler, which cannot
 // tell the buffers apart, would wait for the newest copy before every LDS read;
 // there is no output register, and its own waits only grow longer by the extra
-// loads.
+// loads. m0, which holds the LDS address, is written by each.
 __device__ inline void copy_to_lds16(const void *from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                 :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
+                 :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory", "m0");
 }
 __device__ inline void copy_to_lds16(const void *wave_from, uint32_t lane_offset, uint32_t to) {
     // five states between a vector instruction that wrote the address and its use
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                  :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(lane_offset), "s"(wave_from)
-                 : "memory");
+                 : "memory", "m0");
 }
 __device__ inline void copy_to_lds4(const void *from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
-                 :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
+                 :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory", "m0");
 }
 template <int N> __device__ inline void wait_copies() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
