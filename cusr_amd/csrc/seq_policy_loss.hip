@@ -56,7 +56,7 @@ __device__ inline Term policy_term(const Policy &p, const Token &k, double logp)
     const float held = (ratio < lo ? lo : (ratio > hi ? hi : ratio)) * A;
     r.loss = -(free_ <= held ? free_ : held);
     r.slope = free_ <= held ? -free_ : (held < free_ ? 0.0f : held);
-    if (p.logp_ref) {
+    if (p.logp_ref && p.kl_coef != 0.0f) {   // a coefficient of 0 is no term: no 0 * inf
         const float gap = (float)((double)k.ref - logp);
         const float e = expm1f(gap);
         r.loss += p.kl_coef * (gap > 80.0f ? e : e - gap);   // no inf - inf

@@ -610,7 +610,8 @@ def policy_loss(logits, actions, logp_old, advantages, *, logp_ref=None, weights
     With z = logits / temperature, logp = z[action] - logsumexp z and
     ratio = exp(logp - logp_old), the loss is the weighted sum over tokens of
         -min(ratio A, clip(ratio, 1 - clip[0], 1 + clip[1]) A)
-        + kl_coef (exp(logp_ref - logp) - (logp_ref - logp) - 1).
+        + kl_coef (exp(logp_ref - logp) - (logp_ref - logp) - 1),
+    without the last term when logp_ref is None or kl_coef 0.
     A token of weight 0 is not read: logp 0, gradient 0. An action whose
     logit is -inf has logp -inf and no gradient; one outside the vocabulary
     gives NaN. logp carries no gradient. Sums are held in fp32 or more."""

@@ -119,7 +119,7 @@ int seq_rotary(const SeqRotary *r, void *stream);
  *   l = -min(ratio A, clip(ratio, 1 - clip_lo, 1 + clip_hi) A)
  *       + kl_coef (exp(logp_ref - logp) - (logp_ref - logp) - 1),
  *   loss = sum over tokens of weight * l.
- * logp_ref null: no KL term. A token of weight 0 takes no part,
+ * logp_ref null or kl_coef 0: no KL term. A token of weight 0 takes no part,
  * whatever its logits: logp = 0, its gradient row is 0. A row whose action has the
  * logit -inf has logp = -inf, ratio 0 and no gradient (and with a KL term an
  * infinite loss). An action outside the vocabulary gives logp = NaN.

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import seq_reference as ref
-from test_gpu_seq import BF, F32, FP, DEV, _say, check, cu, normal
+from test_gpu_seq import BF, F32, FP, _say, check, cu, normal, policy_case
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,21 @@ def test_attention_wide_groups(ops, lens, hq, hkv, d, dtype):
     r = ref.attention(q, k, v, c, c, do=do)
     for n, x in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *g)):
         check(n, x, r[n], r[n + "_tol"])
+
+
+# ---------------------------------------------------------------- policy loss
+
+@pytest.mark.parametrize("dtype", [F32, BF, FP])
+@pytest.mark.parametrize("V", [24, 700, 9001])
+def test_policy_without_a_kl_term(ops, V, dtype):
+    """A KL coefficient of 0 is no KL term, however far the reference's
+    log-probabilities lie: the same bits as without them."""
+    c = policy_case(8, V, dtype, 3)
+    c["logp_ref"][0] += 100.0
+    c["logp_ref"][1] = float("inf")
+    c["logits"][2, c["actions"][2]] = float("-inf")
+    for fn in (ops.policy_loss, ops.policy_loss_grad):
+        got, want = fn(**c, kl_coef=0.0), fn(**dict(c, logp_ref=None))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert bool(got[0].isfinite()) and bool(got[-1][3:].isfinite().all())
+    assert bool(got[2].isfinite().all())
