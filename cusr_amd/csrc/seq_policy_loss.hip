@@ -49,7 +49,12 @@ struct Term { float loss, slope; };
 __device__ inline Term policy_term(const Policy &p, const Token &k, double logp) {
     Term r;
     const float A = k.advantage;
-    const float ratio = expf((float)(logp - (double)k.old));
+    // a forbidden action's logp is -inf: its ratio is 0 and its KL term infinite also
+    // where the other policies forbid it and the differences would be inf - inf
+    const double none = -__builtin_inf();
+    const bool old_none = logp == none && (double)k.old == none;
+    const bool ref_none = logp == none && (double)k.ref == none;
+    const float ratio = old_none ? 0.0f : expf((float)(logp - (double)k.old));
     const float free_ = ratio * A;
     // comparisons rather than fminf and fmaxf, which would drop a NaN
     const float lo = 1.0f - p.clip_lo, hi = 1.0f + p.clip_hi;
@@ -57,7 +62,7 @@ __device__ inline Term policy_term(const Policy &p, const Token &k, double logp)
     r.loss = -(free_ <= held ? free_ : held);
     r.slope = free_ <= held ? -free_ : (held < free_ ? 0.0f : held);
     if (p.logp_ref && p.kl_coef != 0.0f) {   // a coefficient of 0 is no term: no 0 * inf
-        const float gap = (float)((double)k.ref - logp);
+        const float gap = ref_none ? __builtin_inff() : (float)((double)k.ref - logp);
         const float e = expm1f(gap);
         r.loss += p.kl_coef * (gap > 80.0f ? e : e - gap);   // no inf - inf
         r.slope -= p.kl_coef * e;

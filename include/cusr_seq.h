@@ -122,7 +122,7 @@ int seq_rotary(const SeqRotary *r, void *stream);
  * logp_ref null or kl_coef 0: no KL term. A token of weight 0 takes no part,
  * whatever its logits: logp = 0, its gradient row is 0. A row whose action has the
  * logit -inf has logp = -inf, ratio 0 and no gradient (and with a KL term an
- * infinite loss). An action outside the vocabulary gives logp = NaN.
+ * infinite loss), whatever logp_old and logp_ref, -inf among them. An action outside the vocabulary gives logp = NaN.
  * dlogits (may be null: loss and logp alone) [tokens, vocab] like logits,
  * rows `drow` apart: d loss / d logits, times *dloss when dloss is given.
  * loss is one fp32. */

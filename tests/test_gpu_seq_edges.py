@@ -63,3 +63,23 @@ def test_policy_without_a_kl_term(ops, V, dtype):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert bool(got[0].isfinite()) and bool(got[-1][3:].isfinite().all())
     assert bool(got[2].isfinite().all())
+
+
+@pytest.mark.parametrize("V", [24, 700, 9001])
+def test_policy_action_that_every_policy_forbids(ops, V):
+    """An action at -inf whose old or reference log-probability is -inf too: ratio
+    0, no gradient, and a KL term that is infinite, not NaN."""
+    c = policy_case(8, V, BF, 5)
+    c["logits"][2, c["actions"][2]] = float("-inf")
+    want = ops.policy_loss_grad(**dict(c, logp_ref=None))
+    assert bool(want[0].isfinite()) and not bool(want[2][2].any())
+    old = c["logp_old"].clone()
+    old[2] = float("-inf")
+    got = ops.policy_loss_grad(**dict(c, logp_ref=None, logp_old=old))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    ref_ = c["logp_ref"].clone()
+    ref_[2] = float("-inf")
+    want = ops.policy_loss_grad(**c, kl_coef=0.1)
+    got = ops.policy_loss_grad(**dict(c, logp_ref=ref_, logp_old=old), kl_coef=0.1)
+    assert float(got[0]) == float("inf") == float(want[0])
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
