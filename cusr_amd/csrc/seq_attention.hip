@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void attn_wave(Attn a, int s
     __shared__ __align__(256) uint16_t lds[4][2][32 * Tile<DP>::stride];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint16_t *kt = lds[wave][0], *vt = lds[wave][1];
-    const int item = blockIdx.x * 4 + wave;
+    const int item = block_number() * 4 + wave;
     const int slot = item / a.hkv, hk = item - slot * a.hkv;
     if (slot >= slots) return;
     const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, kShortRows, slot);
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int slots) {
     __shared__ __align__(256) unsigned char lds[2 * Keys::BYTES];
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int slot = (int)blockIdx.x / a.hkv, hk = (int)blockIdx.x - slot * a.hkv;
+    const int item = block_number(), slot = item / a.hkv, hk = item - slot * a.hkv;
     if (slot >= slots) return;
     const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, ROWS, slot);
     const int b = f.b;
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
     __shared__ __align__(16) uint16_t lds[4][32 * Tile<DP>::stride];
     uint16_t *vt = lds[threadIdx.x >> 6];
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int item = block_number() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slot = item / a.hkv, hk = item - slot * a.hkv;
     if (slot >= st.slots) return;
     const Found f = find_sequence(a.cu_k, a.n_seq, a.tk, 1, st.chunk, slot);
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void attn_join(Attn a, Step st) {
     const int lane = threadIdx.x & 63;
-    const int item = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int item = block_number() * 4 + (int)(threadIdx.x >> 6);
     if (item >= a.tq * a.hq) return;
     const int t = item / a.hq, head = item - t * a.hq, hk = head / a.G;
     const int b = sequence_of_row(a.cu_q, a.n_seq, a.tq, t);
@@ -418,11 +418,11 @@ template <typename T, int DP>
 int launch_step(const Attn &a, Step st, hipStream_t s) {
     st.o = (float *)a.workspace;
     st.ml = st.o + step_rows(a, st) * DP;
-    const dim3 grid((unsigned)((st.slots * (int64_t)a.hkv + 3) / 4), (unsigned)st.tiles);
+    const dim3 grid = grid_of((st.slots * (int64_t)a.hkv + 3) / 4, 256, st.tiles);
     attn_step<T, DP><<<grid, 256, 0, s>>>(a, st);
     if (a.tk > st.chunk) {
         if (hipGetLastError() != hipSuccess) return CO_ERR_CUDA;
-        attn_join<T, DP><<<dim3((unsigned)((a.tq * a.hq + 3) / 4)), 256, 0, s>>>(a, st);
+        attn_join<T, DP><<<grid_of((a.tq * a.hq + 3) / 4, 256), 256, 0, s>>>(a, st);
     }
     return launch_status();
 }
@@ -430,7 +430,8 @@ int launch_step(const Attn &a, Step st, hipStream_t s) {
 template <typename T, int DP, int WAVES>
 int launch_tiles(const Attn &a, hipStream_t s) {
     const int slots = slot_of(a.tq, a.G, WAVES * 32, a.n_seq) + 1;
-    attn_tiles<T, DP, WAVES><<<dim3((unsigned)(slots * a.hkv)), WAVES * 64, 0, s>>>(a, slots);
+    const dim3 grid = grid_of((int64_t)slots * a.hkv, WAVES * 64);
+    attn_tiles<T, DP, WAVES><<<grid, WAVES * 64, 0, s>>>(a, slots);
     return launch_status();
 }
 
@@ -444,7 +445,7 @@ int launch_head(const Attn &a, hipStream_t s) {
     if (rows >= 96) return launch_tiles<T, DP, 4>(a, s);
     const int slots = slot_of(a.tq, a.G, kShortRows, a.n_seq) + 1;
     const int64_t blocks = (slots * (int64_t)a.hkv + 3) / 4;
-    attn_wave<T, DP><<<dim3((unsigned)blocks), 256, 0, s>>>(a, slots);
+    attn_wave<T, DP><<<grid_of(blocks, 256), 256, 0, s>>>(a, slots);
     return launch_status();
 }
 

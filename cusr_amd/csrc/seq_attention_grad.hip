@@ -66,7 +66,7 @@ void attn_grad_short(AttnGrad a, int slots) {
     const uint32_t lds_at = lds_address(lds[0]);
     float *lses = (float *)fifth, *deltas = lses + kShortRows;
     int *lims = (int *)(deltas + kShortRows);
-    const int item = blockIdx.x * 4 + wave;
+    const int item = block_number() * 4 + wave;
     const int slot = item / a.hkv, hk = item - slot * a.hkv;
     if (slot >= slots) return;
     const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, kShortRows, slot);
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, i
     __shared__ __align__(256) unsigned char lds[2 * Keys::BYTES];
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int slot = (int)blockIdx.x / a.hkv, hk = (int)blockIdx.x - slot * a.hkv;
+    const int item = block_number(), slot = item / a.hkv, hk = item - slot * a.hkv;
     if (slot >= slots) return;
     const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, ROWS, slot);
     const int b = f.b;
@@ -539,7 +539,7 @@ __global__ __launch_bounds__(KX * 128, KX == 4 || DP <= 64 ? 2 : 1) void attn_gr
     __shared__ __align__(256) unsigned char lds[BYTES > SUMS ? BYTES : SUMS];
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kx = wave % KX, rx = wave / KX;
-    const int slot = (int)blockIdx.x / a.hkv, hk = (int)blockIdx.x - slot * a.hkv;
+    const int item = block_number(), slot = item / a.hkv, hk = item - slot * a.hkv;
     if (slot >= slots) return;
     const Found f = find_sequence(a.cu_k, a.n_seq, a.tk, 1, KEYS, slot);
     const int b = f.b, s0 = f.start, s1 = max(f.end, s0);
@@ -735,13 +735,14 @@ template <typename T, int DP>
 int launch_grad(const AttnGrad &a, hipStream_t s) {
     if (short_sequences(a)) {
         const int slots = slot_of(a.tq, a.G, kShortRows, a.n_seq) + 1;
-        const dim3 grid((unsigned)((slots * (int64_t)a.hkv + 3) / 4));
+        const dim3 grid = grid_of((slots * (int64_t)a.hkv + 3) / 4, 256);
         attn_grad_short<T, DP><<<grid, 256, 0, s>>>(a, slots);
         return launch_status();
     }
     if (a.tq) {
         const int slots = slot_of(a.tq, a.G, 128, a.n_seq) + 1;
-        attn_grad_q_tiles<T, DP, 4><<<dim3((unsigned)(slots * a.hkv)), 256, 0, s>>>(a, slots);
+        const dim3 grid = grid_of((int64_t)slots * a.hkv, 256);
+        attn_grad_q_tiles<T, DP, 4><<<grid, 256, 0, s>>>(a, slots);
         if (hipGetLastError() != hipSuccess) return CO_ERR_CUDA;
     }
     // Blocks of 64 keys where 128 would not fill the chip once (one sequence of 2,000,
@@ -752,12 +753,14 @@ int launch_grad(const AttnGrad &a, hipStream_t s) {
     const int slots = slot_of(a.tk, 1, 128, a.n_seq) + 1;
     if constexpr (DP > 64) {
         if (slots * a.hkv > 256) {
-            attn_grad_kv_tiles<T, DP, 4><<<dim3((unsigned)(slots * a.hkv)), 512, 0, s>>>(a, slots);
+            const dim3 grid = grid_of((int64_t)slots * a.hkv, 512);
+            attn_grad_kv_tiles<T, DP, 4><<<grid, 512, 0, s>>>(a, slots);
             return launch_status();
         }
     }
     const int more = slot_of(a.tk, 1, 64, a.n_seq) + 1;
-    attn_grad_kv_tiles<T, DP, 2><<<dim3((unsigned)(more * a.hkv)), 256, 0, s>>>(a, more);
+    const dim3 grid = grid_of((int64_t)more * a.hkv, 256);
+    attn_grad_kv_tiles<T, DP, 2><<<grid, 256, 0, s>>>(a, more);
     return launch_status();
 }
 

@@ -102,6 +102,18 @@ __device__ inline uint2v read_transposed(const uint16_t *p) {
     return read_transposed((__attribute__((address_space(3))) const uint16_t *)p);
 }
 
+// Blocks of a launch. An axis has fewer than 2^32 threads (HIP starts what is left of
+// the number modulo 2^32, without an error), so more blocks continue along z, in equal
+// parts: the last numbers may be past the end, and a kernel leaves those alone.
+inline dim3 grid_of(int64_t blocks, int threads, unsigned y = 1) {
+    const int64_t most = 0xffffffffll / threads;
+    const int64_t z = (blocks + most - 1) / most;
+    return dim3((unsigned)((blocks + z - 1) / z), y, (unsigned)z);
+}
+__device__ inline int block_number() {
+    return (int)(blockIdx.x + (blockIdx.z ? blockIdx.z * gridDim.x : 0));
+}
+
 inline int launch_status() {
     return hipGetLastError() == hipSuccess ? CO_OK : CO_ERR_CUDA;
 }

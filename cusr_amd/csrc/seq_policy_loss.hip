@@ -179,7 +179,8 @@ __device__ inline RowGrad finish_row(const Policy &p, const Token &k, float xa, 
 template <typename T>
 __global__ __launch_bounds__(1024) void policy_stream(Policy p, double *terms) {
     constexpr int N = Vec<T>::n;
-    const int64_t t = blockIdx.x;
+    const int64_t t = block_number();
+    if (t >= p.tokens) return;
     const T *x = (const T *)p.logits + t * p.row;
     T *dx = p.dlogits ? (T *)p.dlogits + t * p.drow : nullptr;
     const Token of = token_of(p, t);
@@ -224,7 +225,8 @@ __global__ __launch_bounds__(1024) void policy_stream(Policy p, double *terms) {
 template <typename T, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS) void policy_row(Policy p, double *terms) {
     constexpr int N = Vec<T>::n, WAVES = THREADS / 64;
-    const int64_t t = blockIdx.x;
+    const int64_t t = block_number();
+    if (t >= p.tokens) return;
     const T *x = (const T *)p.logits + t * p.row;
     T *dx = (T *)p.dlogits + t * p.drow;
     const int V = (int)p.vocab, tid = (int)threadIdx.x;
@@ -406,7 +408,7 @@ void launch_symbols(const Policy &p, bool turn, bool joined, dim3 grid, size_t l
 
 template <typename T, int THREADS, int NV>
 void launch_row(const Policy &p, double *terms, hipStream_t s) {
-    policy_row<T, THREADS, NV><<<dim3((unsigned)p.tokens), THREADS, 0, s>>>(p, terms);
+    policy_row<T, THREADS, NV><<<grid_of(p.tokens, THREADS), THREADS, 0, s>>>(p, terms);
 }
 
 // Launches the rows' kernel; returns the number of terms it leaves.
@@ -434,7 +436,8 @@ int64_t launch_policy(const Policy &p, double *terms, hipStream_t s) {
     const int64_t n = (p.vocab + N - 1) / N;       // no row has more pieces
     const bool same = p.dlogits && !(((uintptr_t)p.logits ^ (uintptr_t)p.dlogits) & 15) &&
                       (p.row - p.drow) % N == 0;
-    if (!same || n > 1024 * 16) policy_stream<T><<<dim3((unsigned)p.tokens), 1024, 0, s>>>(p, terms);
+    if (!same || n > 1024 * 16)
+        policy_stream<T><<<grid_of(p.tokens, 1024), 1024, 0, s>>>(p, terms);
     else if (n <= 64 * 2) launch_row<T, 64, 2>(p, terms, s);
     else if (n <= 256 * 1) launch_row<T, 256, 1>(p, terms, s);
     else if (n <= 256 * 2) launch_row<T, 256, 2>(p, terms, s);

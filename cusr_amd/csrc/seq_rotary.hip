@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void rotary_pieces(SeqRotary r, int items, int
     typedef typename Piece<T>::vec vec;
     const int tokens = 256 / items;
     const int slot = (int)threadIdx.x / items, e = (int)threadIdx.x % items;
-    const int64_t t = (int64_t)blockIdx.x * tokens + slot;
+    const int64_t t = (int64_t)block_number() * tokens + slot;
     if (slot >= tokens || t >= r.tokens) return;
     const int half = r.rot / 2, turning = half / P;      // pieces that turn
     const int h0 = (int)blockIdx.y * per, h1 = min(h0 + per, r.hq + r.hkv);
@@ -143,7 +143,7 @@ int launch_rotary(const SeqRotary &r, hipStream_t s) {
         // tokens of 40 heads of 128: 1 head 236 us, 4 182 us, 8 146 us, 16 178 us, 40 164 us.
         int per = 1;
         while (per < 8 && blocks * ((heads + 2 * per - 1) / (2 * per)) >= 1024) per *= 2;
-        const dim3 grid((unsigned)blocks, (unsigned)((heads + per - 1) / per));
+        const dim3 grid = grid_of(blocks, 256, (heads + per - 1) / per);
         if (r.interleaved) rotary_pieces<T, true><<<grid, 256, 0, s>>>(r, items, per);
         else rotary_pieces<T, false><<<grid, 256, 0, s>>>(r, items, per);
         return launch_status();

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import seq_reference as ref
-from test_gpu_seq import BF, F32, FP, _say, check, cu, normal, policy_case
+from test_gpu_seq import BF, DEV, F32, FP, _say, check, cu, normal, policy_case
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,36 @@ def test_policy_action_that_every_policy_forbids(ops, V):
     got = ops.policy_loss_grad(**dict(c, logp_ref=ref_, logp_old=old), kl_coef=0.1)
     assert float(got[0]) == float("inf") == float(want[0])
     assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+
+# ------------------------------------------------------------------- launches
+
+def test_more_rows_than_one_axis_of_threads(ops):
+    """Log-probabilities of more than 2^22 rows, 1,024 threads to each: every row
+    has those of the same row of a small call."""
+    few, V, T = policy_case(1024, 300, BF, 9), 300, (1 << 22) + 5
+    at = torch.arange(T, device=DEV) % 1024
+    c = {n: x[at] for n, x in few.items()}
+    want = ops.policy_loss(**few, kl_coef=0.1)
+    loss, logp = ops.policy_loss(**c, kl_coef=0.1)
+    assert torch.equal(logp, want[1][at])
+    rest = ops.policy_loss(**{n: x[:5] for n, x in few.items()}, kl_coef=0.1)[0].double()
+    total = want[0].double() * (T // 1024) + rest
+    # each loss is rounded once to float32, from a sum in 64 bits
+    tol = ref.E32 * (want[0].double().abs() * (T // 1024) + rest.abs() + total.abs())
+    check("loss", loss, total.cpu(), tol.cpu())
+
+
+def test_more_sequences_than_one_axis_of_threads(ops):
+    """2^24 sequences, four key heads, nearly all empty: the last are worked on
+    like the first."""
+    n = (1 << 24) + 40
+    c = torch.zeros(n + 1, dtype=torch.int32, device=DEV)
+    lens = [3, 1, 2]
+    c[1:], c[-2], c[-1] = 3, 4, 6
+    q, k, v, do = (normal((6, h, 64), BF, i + 1) for i, h in enumerate((8, 4, 4, 8)))
+    o, lse = ops.attention(q, k, v, c, return_lse=True)
+    g = ops.attention_grad(do, q, k, v, o, lse, c)
+    r = ref.attention(q, k, v, cu(lens), cu(lens), do=do)
+    for name, x in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *g)):
+        check(name, x, r[name], r[name + "_tol"])
