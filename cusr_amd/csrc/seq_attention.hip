@@ -12,10 +12,10 @@ __device__ inline void store_lse(const Attn &a, int t, int head, float m, float 
 
 template <typename T, int DP>
 __device__ inline void store_out(const Attn &a, int t, int head, const float16v *o, float m,
-                                 float l, bool ok) {
+                                 float l, bool ok, bool low) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     store_row<T, DP>(a.o, t * a.o_row + head * a.o_head, o, inv, a.d, ok);
-    if (a.o_low)
+    if (low)
         store_row<T, DP, true>(a.o_low, ((int64_t)t * a.hq + head) * a.d, o, inv, a.d, ok);
     store_lse(a, t, head, m, l, ok);
 }
@@ -124,18 +124,18 @@ __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, 
 // way of LDS and whole rows stored. 16,384 sequences of 1 to 31, 8 heads of 64 over
 // 4, take 191 us (4.2 TB/s); with K to registers 207, with the output stored as 32
 // bytes of each row 205.
-constexpr int kShortRows = 128;
 template <typename T, int DP, typename I>
 __device__ inline void wave_tiles(const Attn &a, const Place &p, int hk, int first, uint16_t *kt,
                                   uint16_t *vt) {
     const int rows = p.lq * a.G;
+    const bool low = keeps_low(a, rows);
     const float inv = 1.0f / (float)a.G;
     for (int tile = first; tile < first + kShortRows / 32 && tile * 32 < rows; tile++) {
         float16v o[DP / 32];
         float m, l;
         const Row r = run_rows<T, DP, false, I>(a, p, hk, tile, 0, p.lk, kt, vt, o, m, l);
-        if (a.o_low) {
-            store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok);
+        if (low) {
+            store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok, true);
             continue;
         }
         uint16_t *op = (uint16_t *)a.o + p.q0 * a.o_row + hk * a.G * a.o_head;
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int slots) {
         work(Const<0>{}, k0);
         if (k0 + KB < keys) work(Const<1>{}, k0 + KB);
     }
-    store_out<T, DP>(a, p.q0 + qi, head, o, m, add_halves(l), ok);
+    store_out<T, DP>(a, p.q0 + qi, head, o, m, add_halves(l), ok, keeps_low(a, rows));
 }
 
 // Few rows over many keys (single tokens over a cache). A sequence's keys are
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
         float m, l;
         const Row r = run_rows<T, DP, true, int64_t>(a, p, hk, tile, key0, key1, vt, vt, o, m, l);
         if (!split) {
-            store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok);
+            store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok, keeps_low(a, rows));
             continue;
         }
         const int64_t pr = ((int64_t)slot * a.hkv + hk) * st.rows + tile * 32 + (lane & 31);
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(256) void attn_join(Attn a, Step st) {
         if (lane + 64 * e < a.d) {
             const float x = acc[e] * inv;
             out[lane + 64 * e] = (typename T::elem)x;
-            if (a.o_low) low[lane + 64 * e] = (typename T::elem)(x - (float)(typename T::elem)x);
+            if (keeps_low(a, rows)) low[lane + 64 * e] = (typename T::elem)(x - (float)(typename T::elem)x);
         }
     if (a.lse && lane == 0)
         a.lse[head * a.tq + t] = l == 0.0f ? neg_inf() : m * a.scale + logf(l);

@@ -51,7 +51,6 @@ __device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float
 // the path of its own for up to 64 rows and keys, in which few loads wait for
 // others and P and dS are formed once: 8,192 sequences of 3 to 63, 8 heads of 64,
 // take 0.47 ms (4.1 TB/s), with P and dS formed twice 0.58, on the general path 0.73.
-constexpr int kShortRows = 128;
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1)
 void attn_grad_short(AttnGrad a, int slots) {
@@ -384,8 +383,8 @@ void attn_grad_short(AttnGrad a, int slots) {
             for (int tile = next; tile < tiles; tile++) {
                 int at = (tile & 3) * 32;
                 if (shares > 1) {
-                    // the rows may be another wave's: delta from o, and what its
-                    // type rounded away if that is kept
+                    // the rows may be another wave's: delta from o and what its type
+                    // rounded away, which a sequence of so many rows keeps
                     const int row = tile * 32 + (lane & 31);
                     const bool ok = row < rows;
                     const int qi = divide(ok ? row : 0, a.G, inv), g = ok ? row - qi * a.G : 0;
@@ -721,14 +720,6 @@ __global__ __launch_bounds__(KX * 128, KX == 4 || DP <= 64 ? 2 : 1) void attn_gr
     const int64_t kr = s0 + tile * KEYS + kx * 32 + (lane & 31);
     store_row<T, DP>(a.g.dk, kr * a.g.dk_row + hk * a.g.dk_head, dk, a.scale, a.d, kr < s1);
     store_row<T, DP>(a.g.dv, kr * a.g.dv_row + hk * a.g.dv_head, dv, 1.0f, a.d, kr < s1);
-}
-
-// Below these keys a sequence, on average, blocks of the long kernels mostly wait
-// for themselves; above, a wave alone takes longer (4 heads of 64: sequences of 96
-// 199 against 282 us, of 128 300 against 297 us; heads of 128, with half the waves:
-// of 64 157 against 311 us, of 100 607 against 464 us).
-bool short_sequences(const Attn &a) {
-    return a.tk < (padded_head(a.d) <= 64 ? 128ll : 80ll) * a.n_seq || a.n_seq == 0;
 }
 
 template <typename T, int DP>

@@ -21,10 +21,32 @@ struct Attn : SeqAttention {
     int32_t G;       // query heads per key head
     float c;         // scale * log2(e): scores in powers of two
     int32_t near;    // every stride is below 2^16 elements
+    int32_t low_all; // the gradient reads o_low of every row
 };
 inline bool near_strides(int64_t a, int64_t b, int64_t c, int64_t d) {
     const int64_t most = 1 << 16;
     return a >= 0 && b >= 0 && c >= 0 && d >= 0 && a < most && b < most && c < most && d < most;
+}
+
+// Rows that a wave owns where a sequence is mostly one wave's.
+constexpr int kShortRows = 128;
+
+// Whether the gradient of a call is that of short sequences. Below these keys a
+// sequence, on average, blocks of the long kernels mostly wait for themselves; above, a
+// wave alone takes longer (4 heads of 64: sequences of 96 199 against 282 us, of 128 300
+// against 297 us; heads of 128, with half the waves: of 64 157 against 311 us, of 100
+// 607 against 464 us).
+inline int padded_head(int d) { return (d + 31) / 32 * 32; }   // 32, 64, 96 or 128
+inline bool short_sequences(const SeqAttention &a) {
+    return a.tk < (padded_head(a.d) <= 64 ? 128ll : 80ll) * a.n_seq || a.n_seq == 0;
+}
+
+// Whether a sequence's rows leave in o_low what rounding took from o. The gradient needs
+// delta = sum(o * do) of a row wherever another wave than the row's uses it: everywhere in
+// the long kernels, and in the short one for a sequence of more rows than a wave has.
+// Elsewhere delta is summed anew from P and dP.
+__device__ inline bool keeps_low(const Attn &a, int rows) {
+    return a.o_low && (a.low_all || rows > kShortRows);
 }
 
 __device__ inline int clamp_to(int x, int lo, int64_t hi) {
@@ -417,12 +439,11 @@ inline Attn make_attn(const SeqAttention *s) {
     a.c = a.scale * kLog2e;
     a.near = near_strides(a.q_row, a.q_head, a.k_row, a.k_head) &&
              near_strides(a.v_row, a.v_head, a.o_row, a.o_head);
+    a.low_all = !short_sequences(*s);
     return a;
 }
 
 int check_attention(const SeqAttention *a);
-// the head size that the kernels are built for (32, 64, 96, 128)
-inline int padded_head(int d) { return (d + 31) / 32 * 32; }
 
 }  // namespace seq
 #endif

@@ -254,11 +254,11 @@ def _attention(q, k, v, cu_q, cu_k, k_lens, scale, return_lse):
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) \
         if return_lse else None
-    low, n_seq = None, cu_q.shape[0] - 1
-    if return_lse and (k.shape[0] >= 128 * n_seq
-                       or q.shape[0] * q.shape[1] > 64 * n_seq * k.shape[1]):
-        # The gradient of sequences this long takes sum(o * do) from o: it gets the
-        # part of o that o's type rounds away. Shorter ones form the sum anew.
+    low = None
+    if return_lse:
+        # Where the gradient takes sum(o * do) from o it gets the part of o that o's
+        # type rounds away. The kernels know the rows: those that form the sum anew
+        # leave theirs unwritten.
         low = lse.o_low = torch.empty_like(o)
     if q.shape[0]:
         lib, dev = load_library(), q.get_device()

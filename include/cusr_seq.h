@@ -53,7 +53,8 @@ extern "C" {
  *
  * lse (may be null for the forward) [hq, tq] fp32: log of the sum of
  * exp(scale q.k) over the visible keys. o_low (may be null): what rounding o to
- * its type took away, itself rounded to it. A gradient needs sum(o * d_o) of each
+ * its type took away, itself rounded to it, in the rows whose gradient reads it (the
+ * others are not written). A gradient needs sum(o * d_o) of each
  * row; from o alone its error is that of o's rounding and goes into every key of
  * the row alike. */
 typedef struct SeqAttention {

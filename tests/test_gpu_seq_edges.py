@@ -116,3 +116,53 @@ def test_more_sequences_than_one_axis_of_threads(ops):
     r = ref.attention(q, k, v, cu(lens), cu(lens), do=do)
     for name, x in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *g)):
         check(name, x, r[name], r[name + "_tol"])
+
+
+# ------------------------------------------------------------- gradient's sums
+
+# (queries, keys) of one sequence, and of how many short ones beside it
+SKEWED = [
+    ((700, 700), (10, 10), 40, 4, 4, 64),
+    ((150, 150), (5, 5), 100, 4, 2, 128),
+    ((45, 45), (5, 5), 100, 8, 2, 64),
+    ((40, 60), (2, 3), 30, 32, 4, 64),
+    ((40, 100), (40, 100), 5, 4, 4, 128),
+    ((129, 129), (1, 1), 300, 1, 1, 32),
+]
+
+
+def skewed(long, short, n, hq, hkv, d):
+    """Sharp attention, whose outputs are as large as single values: what rounding
+    them takes away is then large beside the gradients of scores."""
+    lq, lk = [short[0]] * n, [short[1]] * n
+    lq.insert(n // 2, long[0])
+    lk.insert(n // 2, long[1])
+    cq = cu(lq)
+    ck = cq if lq == lk else cu(lk)
+    q, do = normal((sum(lq), hq, d), BF, 1, 4.0), normal((sum(lq), hq, d), BF, 2)
+    k, v = (normal((sum(lk), hkv, d), BF, i) for i in (3, 4))
+    rows = slice(sum(lq[:n // 2]), sum(lq[:n // 2]) + long[0])
+    keys = slice(sum(lk[:n // 2]), sum(lk[:n // 2]) + long[1])
+    return (q, k, v), do, cq, ck, rows, keys
+
+
+def off_by(got, want):
+    """Root mean square error over that of rounding the exact values alone."""
+    def rms(x):
+        return float(x.square().mean().sqrt())
+    return rms(got.cpu().double() - want) / rms(want.to(got.dtype).double() - want)
+
+
+@pytest.mark.parametrize("long,short,n,hq,hkv,d", SKEWED)
+def test_gradient_of_a_long_sequence_among_short_ones(ops, long, short, n, hq, hkv, d):
+    """Each sequence's gradient is as good as its type, whatever the others': the
+    roundings of P, dS and the result are sqrt(2) of one, and 1.75 leaves a fifth."""
+    x, do, cq, ck, rows, keys = skewed(long, short, n, hq, hkv, d)
+    o, lse = ops.attention(*x, cq, ck, return_lse=True)
+    got = ops.attention_grad(do, *x, o, lse, cq, ck)
+    r = ref.attention(*x, cq, ck, do=do)
+    for name, g, at in zip(("dq", "dk", "dv"), got, (rows, keys, keys)):
+        f = off_by(g[at], r[name][at])
+        _say(f"  {long} among {n} of {short} {name}: {f:.3f} of a rounding")
+        assert f <= 1.75, name
+        check(name, g, r[name], r[name + "_tol"])
