@@ -275,9 +275,9 @@ def _attention(q, k, v, cu_q, cu_k, k_lens, scale, return_lse):
 def attention_grad(do, q, k, v, o, lse, cu_q, cu_k=None, *, k_lens=None, scale=None):
     """(dq, dk, dv) of attention for the gradient `do` of its output; o and
     lse are what attention(..., return_lse=True) gave. The same call gives the
-    same bits. lse comes with an attribute o_low where it helps: what o's type
-    rounded away of it. A copy of lse without it gives gradients of long
-    sequences that are off by up to half as much again."""
+    same bits. lse comes with an attribute o_low, as large as o: what o's type
+    rounded away of it, which the gradient of long sequences needs. For a copy
+    of lse without it the forward pass runs again."""
     _check_attention(q, k, v, cu_q, cu_k, k_lens, scale)
     _need(do, "do", (q.dtype,), 3, q.device)
     _need(o, "o", (q.dtype,), 3, q.device)
@@ -293,6 +293,8 @@ def attention_grad(do, q, k, v, o, lse, cu_q, cu_k=None, *, k_lens=None, scale=N
     cu_q, lse = cu_q.contiguous(), lse.contiguous()
     cu_k = cu_q if cu_k is None else cu_k.contiguous()
     k_lens = None if k_lens is None else k_lens.contiguous()
+    if low is None and q.shape[0] and k.shape[0]:
+        low = _attention(q, k, v, cu_q, cu_k, k_lens, scale, True)[1].o_low
     dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
     if q.shape[0] == 0 or k.shape[0] == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()

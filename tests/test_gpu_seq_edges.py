@@ -166,3 +166,16 @@ def test_gradient_of_a_long_sequence_among_short_ones(ops, long, short, n, hq, h
         _say(f"  {long} among {n} of {short} {name}: {f:.3f} of a rounding")
         assert f <= 1.75, name
         check(name, g, r[name], r[name + "_tol"])
+
+
+def test_gradient_from_a_copy_of_lse(ops):
+    """lse may be copied, moved or saved: the gradient has the same bits, and
+    loses nothing of its precision."""
+    x, do, cq, ck, rows, keys = skewed((300, 300), (12, 12), 9, 4, 2, 64)
+    for c, a in ((cq, x), (cu([300]), [t[rows] for t in x])):
+        d = do if c is cq else do[rows]
+        o, lse = ops.attention(*a, c, return_lse=True)
+        want = ops.attention_grad(d, *a, o, lse, c)
+        for copy in (lse.clone(), lse.detach(), lse.cpu().to(DEV)):
+            got = ops.attention_grad(d, *a, o, copy, c)
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
