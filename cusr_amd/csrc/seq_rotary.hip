@@ -9,6 +9,9 @@
 namespace seq {
 
 template <typename T> __device__ inline float load1(const T *p) { return (float)*p; }
+__device__ inline int64_t position(const SeqRotary &r, int64_t t) {
+    return r.positions_64 ? ((const int64_t *)r.positions)[t] : ((const int32_t *)r.positions)[t];
+}
 
 // Any size, stride and alignment: a thread per pair or copied element. 32,768
 // tokens of 40 heads of 128 in bf16 would take 331 us, 2.0 TB/s.
@@ -32,7 +35,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(SeqRotary r) {
             continue;
         }
         const int ia = r.interleaved ? 2 * e : e, ib = r.interleaved ? 2 * e + 1 : e + half;
-        const int64_t p = r.positions[t];
+        const int64_t p = position(r, t);
         float c = __builtin_nanf(""), s = c;
         if (p >= 0 && p < r.table_len) {
             c = r.table[(p * half + e) * 2];
@@ -68,9 +71,9 @@ __global__ __launch_bounds__(256) void rotary_pieces(SeqRotary r, int items, int
     const bool turn = e < turning;
     float c[P], s[P];
     if (turn) {
-        const int64_t pos = r.positions[t];
+        const int64_t pos = position(r, t);
         const bool in = pos >= 0 && pos < r.table_len;
-        const float4v *cs = (const float4v *)(r.table + (pos * half + e * P) * 2);
+        const float4v *cs = (const float4v *)(r.table + ((in ? pos : 0) * half + e * P) * 2);
 #pragma unroll
         for (int j = 0; j < P; j += 2) {
             const float nan = __builtin_nanf("");

@@ -66,7 +66,7 @@ class SeqRotary(ctypes.Structure):
                 ("table_len", _I64), ("q_row", _I64), ("q_head", _I64), ("k_row", _I64),
                 ("k_head", _I64), ("qo_row", _I64), ("qo_head", _I64), ("ko_row", _I64),
                 ("ko_head", _I64), ("q", _P), ("k", _P), ("q_out", _P), ("k_out", _P),
-                ("positions", _P), ("table", _P)]
+                ("positions", _P), ("table", _P), ("positions_64", _I32), ("reserved", _I32)]
 
 
 class SeqPolicyLoss(ctypes.Structure):
@@ -417,15 +417,14 @@ def _rotary(q, k, positions, table, interleaved, inverse, q_out=None, k_out=None
         if k_out is None:
             k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         kos = k_out.stride()
-    if positions.dtype is not torch.int32:
-        positions = positions.to(torch.int32)
     positions, table = positions.contiguous(), table.contiguous()
     if tokens:
         qos = q_out.stride()
         r = _pack_rotary(_SIZE_ROTARY, _DTYPES[q.dtype], hq, hkv, d, 2 * table.shape[1],
                          bool(interleaved), bool(inverse), tokens, table.shape[0], qs[0], qs[1],
                          ks[0], ks[1], qos[0], qos[1], kos[0], kos[1], q.data_ptr(), _ptr(k),
-                         q_out.data_ptr(), _ptr(k_out), positions.data_ptr(), table.data_ptr())
+                         q_out.data_ptr(), _ptr(k_out), positions.data_ptr(), table.data_ptr(),
+                         positions.dtype is torch.int64, 0)
         _run(load_library().seq_rotary, "seq_rotary", q.get_device(), r)
     return q_out, k_out
 

@@ -108,8 +108,9 @@ typedef struct SeqRotary {
     int64_t q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head;
     const void *q, *k;
     void *q_out, *k_out;
-    const int32_t *positions;
+    const void *positions;    /* [tokens], int32_t, or int64_t when positions_64 */
     const float *table;
+    int32_t positions_64, reserved;
 } SeqRotary;
 
 int seq_rotary(const SeqRotary *r, void *stream);

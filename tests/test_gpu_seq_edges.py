@@ -179,3 +179,24 @@ def test_gradient_from_a_copy_of_lse(ops):
         for copy in (lse.clone(), lse.detach(), lse.cpu().to(DEV)):
             got = ops.attention_grad(d, *a, o, copy, c)
             assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+# --------------------------------------------------------------------- rotary
+
+@pytest.mark.parametrize("d,rot", [(48, 32), (20, 6)])
+def test_rotary_positions_beyond_32_bits(ops, d, rot):
+    """A 64-bit position outside the table gives NaN also where its low 32 bits lie
+    inside it; one inside turns like the same in 32 bits."""
+    table = ops.rotary_table(rot, 64)
+    far = [2 ** 32, 2 ** 32 + 5, -2 ** 32, -2 ** 32 + 1, 2 ** 40 + 63, -2 ** 63, 2 ** 63 - 1]
+    q, k = normal((len(far) + 3, 2, d), BF, 1), normal((len(far) + 3, 1, d), BF, 2)
+    near = [0, 63, 5]
+    pos = torch.tensor(near + far, device=DEV)
+    a, b = ops.rotary(q, k, pos, table)
+    assert bool(a[3:, :, :rot].isnan().all()) and bool(b[3:, :, :rot].isnan().all())
+    assert torch.equal(a[..., rot:], q[..., rot:]) and torch.equal(b[..., rot:], k[..., rot:])
+    few = ops.rotary(q[:3], k[:3], pos[:3].to(torch.int32), table)
+    assert torch.equal(a[:3], few[0]) and torch.equal(b[:3], few[1])
+    step = torch.tensor(near + [9], device=DEV).repeat(2)[::2]      # every other of them
+    want = ops.rotary(q[:4], None, step.to(torch.int32), table)
+    assert torch.equal(ops.rotary(q[:4], None, step, table), want)
