@@ -453,8 +453,8 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, inplace=
     from rotary_table. The first rot = 2 * table.shape[1] elements of each head
     turn in pairs (i, i + rot/2), or (2i, 2i + 1) when interleaved; the rest is
     copied. inverse turns back, which is the gradient. inplace writes into q
-    and k. A position outside the table gives NaN in its token's turned
-    elements. Returns (q', k'), or q' alone when k is None."""
+    and k, and autograd sees it. A position outside the table gives NaN in its
+    token's turned elements. Returns (q', k'), or q' alone when k is None."""
     if not _plain_rotary(q, k, positions, table):
         _check_rotary(q, k, positions, table)
     grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
@@ -464,6 +464,9 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, inplace=
         if q.stride(2) != 1 or (k is not None and k.stride(2) != 1):
             raise ValueError("inplace needs heads that are contiguous")
         out = _rotary(q, k, positions, table, interleaved, inverse, q, k)
+        # autograd has to see that they changed: an earlier graph may have saved them
+        torch.autograd.graph.increment_version(
+            [x for x in (q, k) if x is not None and not x.is_inference()])
     elif grad:
         return _RotaryFn.apply(q, k, positions, table, bool(interleaved), bool(inverse))
     else:

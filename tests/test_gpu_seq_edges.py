@@ -200,3 +200,23 @@ def test_rotary_positions_beyond_32_bits(ops, d, rot):
     step = torch.tensor(near + [9], device=DEV).repeat(2)[::2]      # every other of them
     want = ops.rotary(q[:4], None, step.to(torch.int32), table)
     assert torch.equal(ops.rotary(q[:4], None, step, table), want)
+
+
+def test_rotary_in_place_is_seen_by_autograd(ops):
+    """What an earlier graph saved and rotary overwrites makes its backward raise,
+    as torch's own operations in place do."""
+    table, pos = ops.rotary_table(32, 64), torch.arange(4, device=DEV)
+    for which in "qk":
+        q, k = normal((4, 2, 32), F32, 1), normal((4, 1, 32), F32, 2)
+        x = q if which == "q" else k
+        w = torch.ones_like(x, requires_grad=True)
+        y = (w * x).sum()
+        before = x._version
+        ops.rotary(q, k, pos, table, inplace=True)
+        assert x._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.backward()
+    with torch.inference_mode():
+        q = normal((4, 2, 32), F32, 1).clone()
+        want = ops.rotary(q, None, pos, table)
+        assert torch.equal(ops.rotary(q, None, pos, table, inplace=True), want)
