@@ -12,7 +12,8 @@ are that model's operators on the GPU; the reference has no counterpart.
 
 Tensors are torch CUDA tensors; the work is queued on the current stream of
 their device and the call returns at once. attention, rotary and policy_loss
-take part in autograd when an input requires a gradient. Arguments are checked
+take part in autograd when an input requires a gradient; there are no
+forward-mode derivatives, and dual tensors are refused. Arguments are checked
 before anything is launched (TypeError, ValueError); a refusal of the library
 raises COError. Import torch before the library is loaded, as for
 co_data_upload_device. There is no CPU path.
@@ -26,6 +27,7 @@ import threading
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from cusr_amd.kernel.co_inproc import CO_OK, COError, _HERE
@@ -164,6 +166,16 @@ def _need(x, name, dtypes, dim, device=None):
     return x
 
 
+def _no_tangents(*tensors):
+    """Forward-mode derivatives are not formed: a dual tensor would lose its
+    tangent without a word. One comparison outside a dual level."""
+    if forward_ad._current_level < 0:
+        return
+    for x in tensors:
+        if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+            raise ValueError("the sequence operators have no forward-mode derivatives")
+
+
 def _ptr(x):
     return 0 if x is None else x.data_ptr()
 
@@ -207,6 +219,7 @@ _HALF = (torch.bfloat16, torch.float16)
 
 
 def _check_attention(q, k, v, cu_q, cu_k, k_lens, scale):
+    _no_tangents(q, k, v)
     if _plain_attention(q, k, v, cu_q, cu_k, k_lens) and (scale is None or 0.0 < scale <= 1e30):
         return
     _need(q, "q", _HALF, 3)
@@ -279,6 +292,7 @@ def attention_grad(do, q, k, v, o, lse, cu_q, cu_k=None, *, k_lens=None, scale=N
     rounded away of it, which the gradient of long sequences needs. For a copy
     of lse without it the forward pass runs again."""
     _check_attention(q, k, v, cu_q, cu_k, k_lens, scale)
+    _no_tangents(do)
     _need(do, "do", (q.dtype,), 3, q.device)
     _need(o, "o", (q.dtype,), 3, q.device)
     _need(lse, "lse", (torch.float32,), 2, q.device)
@@ -455,6 +469,7 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, inplace=
     copied. inverse turns back, which is the gradient. inplace writes into q
     and k, and autograd sees it. A position outside the table gives NaN in its
     token's turned elements. Returns (q', k'), or q' alone when k is None."""
+    _no_tangents(q, k, table)
     if not _plain_rotary(q, k, positions, table):
         _check_rotary(q, k, positions, table)
     grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
@@ -531,6 +546,7 @@ def _plain_policy(logits, actions, given, maybe):
 
 def _check_policy(logits, actions, logp_old, advantages, logp_ref, weights, clip, kl_coef,
                   temperature):
+    _no_tangents(logits, logp_old, advantages, logp_ref, weights)
     lo, hi = (float(c) for c in clip)
     if (_plain_policy(logits, actions, (logp_old, advantages), (logp_ref, weights))
             and lo >= 0 and hi >= 0 and 0 < temperature < math.inf and math.isfinite(kl_coef)):
