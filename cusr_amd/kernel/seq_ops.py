@@ -176,6 +176,14 @@ def _no_tangents(*tensors):
             raise ValueError("the sequence operators have no forward-mode derivatives")
 
 
+def _no_gradient(**tensors):
+    """Refuses tensors that would get no gradient although they ask for one."""
+    if torch.is_grad_enabled():
+        for name, x in tensors.items():
+            if x is not None and x.requires_grad:
+                raise ValueError(f"{name} gets no gradient: pass {name}.detach()")
+
+
 def _ptr(x):
     return 0 if x is None else x.data_ptr()
 
@@ -358,10 +366,11 @@ def attention(q, k, v, cu_q, cu_k=None, *, k_lens=None, scale=None, return_lse=F
     A query that sees no key gives 0. scale defaults to D ** -0.5.
 
     Returns o like q, or (o, lse) with return_lse: lse fp32 [Hq, Tq], -inf
-    where no key is seen. A key or value that is not finite, in a place that a
-    query does not see, is kept from it beyond its sequence's length, but reaches
-    queries up to 94 places before its own within it. Probabilities are rounded to the tensors' type for
-    the product with v; sums and statistics are held in fp32."""
+    where no key is seen; it carries no gradient. A key or value that is not
+    finite, in a place that a query does not see, is kept from it beyond its
+    sequence's length, but reaches queries up to 94 places before its own within
+    it. Probabilities are rounded to the tensors' type for the product with v;
+    sums and statistics are held in fp32."""
     _check_attention(q, k, v, cu_q, cu_k, k_lens, scale)
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -468,10 +477,12 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, inplace=
     turn in pairs (i, i + rot/2), or (2i, 2i + 1) when interleaved; the rest is
     copied. inverse turns back, which is the gradient. inplace writes into q
     and k, and autograd sees it. A position outside the table gives NaN in its
-    token's turned elements. Returns (q', k'), or q' alone when k is None."""
+    token's turned elements. Gradients go to q and k, not to the table. Returns
+    (q', k'), or q' alone when k is None."""
     _no_tangents(q, k, table)
     if not _plain_rotary(q, k, positions, table):
         _check_rotary(q, k, positions, table)
+    _no_gradient(table=table)
     grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
     if inplace:
         if grad:
@@ -634,9 +645,11 @@ def policy_loss(logits, actions, logp_old, advantages, *, logp_ref=None, weights
     without the last term when logp_ref is None or kl_coef 0.
     A token of weight 0 is not read: logp 0, gradient 0. An action whose
     logit is -inf has logp -inf and no gradient; one outside the vocabulary
-    gives NaN. logp carries no gradient. Sums are held in fp32 or more."""
+    gives NaN. The gradient goes to the logits alone: logp carries none, and
+    other inputs that require one are refused. Sums are held in fp32 or more."""
     lo_hi = _check_policy(logits, actions, logp_old, advantages, logp_ref, weights, clip,
                           kl_coef, temperature)
+    _no_gradient(logp_old=logp_old, advantages=advantages, logp_ref=logp_ref, weights=weights)
     args = (logits, actions, logp_old, advantages, logp_ref, weights, lo_hi, kl_coef, temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _PolicyFn.apply(*args)
@@ -646,7 +659,7 @@ def policy_loss(logits, actions, logp_old, advantages, *, logp_ref=None, weights
 def policy_loss_grad(logits, actions, logp_old, advantages, *, logp_ref=None, weights=None,
                      clip=(0.2, 0.2), kl_coef=0.0, temperature=1.0):
     """policy_loss and its gradient in one pass: (loss, logp, dlogits), dlogits
-    like logits."""
+    like logits. The results are no part of a graph."""
     lo_hi = _check_policy(logits, actions, logp_old, advantages, logp_ref, weights, clip,
                           kl_coef, temperature)
     return _policy(logits, actions, logp_old, advantages, logp_ref, weights, lo_hi, kl_coef,

@@ -69,3 +69,13 @@ def test_dual_tensors_are_refused():
                 dual = forward_ad.make_dual(x, torch.ones_like(x))
                 with pytest.raises(ValueError, match="forward-mode"):
                     fn(**{**real, **other, name: dual})
+
+
+def test_inputs_without_a_gradient_are_refused():
+    for fn, real, other in calls():
+        names = {ops.rotary: ["table"],
+                 ops.policy_loss: ["logp_old", "advantages", "logp_ref", "weights"]}.get(fn, [])
+        for name in names:
+            x = real[name].clone().requires_grad_()
+            with pytest.raises(ValueError, match=f"{name} gets no gradient"):
+                fn(**{**real, **other, name: x})
