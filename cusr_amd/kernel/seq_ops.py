@@ -452,6 +452,40 @@ def _rotary(q, k, positions, table, interleaved, inverse, q_out=None, k_out=None
     return q_out, k_out
 
 
+def _own_memory(x):
+    """Elements that x [T, H, D] spans, heads contiguous, or None when two of its
+    places share memory (a broadcast or sliding view)."""
+    (T, H, d), (s0, s1, _) = x.shape, x.stride()
+    if not x.numel():
+        return 0
+    row, head = ((T - 1) * s0, (H - 1) * s1)
+    if (H == 1 or s1 >= d) and (T == 1 or s0 >= head + d):            # rows outside
+        return row + head + d
+    if (T == 1 or s0 >= d) and (H == 1 or s1 >= row + d):             # heads outside
+        return row + head + d
+    return None
+
+
+def _share_memory(q, k):
+    """Whether an element of k is one of q; each is its own memory."""
+    (T, hq, d), (q0, q1, _) = q.shape, q.stride()
+    (_, hk, _), (k0, k1, _) = k.shape, k.stride()
+    gap = (k.data_ptr() - q.data_ptr()) // q.element_size()
+    if not (-_own_memory(k) < gap < _own_memory(q)):
+        return False
+    if T == 1:
+        q0 = k0 = max(q0, k0, 1)
+    q_row, k_row = (hq - 1) * q1 + d, (hk - 1) * k1 + d
+    if q0 == k0 and ((gap >= q_row and gap + k_row <= q0) or (-gap >= k_row and q_row - gap <= q0)):
+        return False                                # other columns of the same rows
+    if q0 != k0:
+        return True                                 # rows of two lengths in one range
+    # places of a head of k in one of q, a number of rows apart
+    d0 = gap + np.arange(hk)[:, None] * k1 - np.arange(hq)[None] * q1
+    rows = np.clip(np.rint(d0 / q0), 1 - T, T - 1).astype(np.int64)
+    return bool((np.abs(d0 - rows * q0) < d).any())
+
+
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, table, interleaved, inverse):
@@ -489,6 +523,9 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, inplace=
             raise ValueError("inplace takes no part in autograd")
         if q.stride(2) != 1 or (k is not None and k.stride(2) != 1):
             raise ValueError("inplace needs heads that are contiguous")
+        if _own_memory(q) is None or (k is not None and (_own_memory(k) is None
+                                                         or _share_memory(q, k))):
+            raise ValueError("inplace needs memory of its own for every element of q and k")
         out = _rotary(q, k, positions, table, interleaved, inverse, q, k)
         # autograd has to see that they changed: an earlier graph may have saved them
         torch.autograd.graph.increment_version(

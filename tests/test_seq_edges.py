@@ -79,3 +79,56 @@ def test_inputs_without_a_gradient_are_refused():
             x = real[name].clone().requires_grad_()
             with pytest.raises(ValueError, match=f"{name} gets no gradient"):
                 fn(**{**real, **other, name: x})
+
+
+def test_rotary_in_place_needs_memory_of_its_own():
+    """Broadcast views and tensors that share elements would be turned twice, or by
+    several threads at once."""
+    pos, table = gpu(6, dtype=torch.int64), gpu(9, 8, 2, dtype=F32)
+    wide = gpu(6, 8, 16)
+    flat = gpu(6 * 8 * 16 + 16)
+    rows = flat[:6 * 64].view(6, 4, 16)
+    for q, k in ((gpu(1, 4, 16).expand(6, 4, 16), None), (gpu(6, 1, 16).expand(6, 4, 16), None),
+                 (wide, gpu(1, 2, 16).expand(6, 2, 16)), (wide, wide), (wide[:, :4], wide[:, 3:5]),
+                 (wide[:, 3:5], wide[:, :4]), (wide[:, :4], wide[:, 2:3]),
+                 (flat.as_strided((6, 4, 16), (64, 8, 1)), None),
+                 (flat.as_strided((6, 4, 16), (40, 16, 1)), None),
+                 (rows, flat.as_strided((6, 1, 16), (64, 16, 1), 6)),
+                 (rows, flat.as_strided((6, 1, 16), (80, 16, 1), 64))):
+        with pytest.raises(ValueError, match="memory of its own"):
+            ops.rotary(q, k, pos, table, inplace=True)
+
+
+def test_memory_that_is_not_shared():
+    """Layouts that models have: slices of a projection, heads before rows, one
+    allocation after the other, one token."""
+    wide, first = gpu(6, 8, 16), gpu(8, 6, 16).transpose(0, 1)
+    one = gpu(1, 8, 16)
+    flat = gpu(2 * 6 * 32)
+    for q, k in ((wide[:, :4], wide[:, 4:6]), (wide[:, 6:], wide[:, :6]),
+                 (first[:, :4], first[:, 4:]), (one[:, :4], one[:, 4:]),
+                 (flat[:192].view(6, 2, 16), flat[192:].view(6, 2, 16)),
+                 (wide[:, 0::2], wide[:, 1::2]), (wide[:, :, :8], wide[:, :, 8:])):
+        assert ops._own_memory(q) and ops._own_memory(k)
+        assert not ops._share_memory(q, k) and not ops._share_memory(k, q)
+    assert ops._own_memory(gpu(0, 8, 16)) == 0
+    # against sets of elements
+    g = torch.Generator().manual_seed(0)
+    pick = lambda n: int(torch.randint(n, (1,), generator=g))  # noqa: E731
+    base, seen = gpu(4000), [0, 0]
+    for _ in range(4000):
+        T, hq, hk, d = 1 + pick(4), 1 + pick(3), 1 + pick(3), 1 + pick(6)
+        both = [base.as_strided((T, h, d), (pick(40), pick(40), 1), pick(60)) for h in (hq, hk)]
+        own = [ops._own_memory(x) for x in both]
+        at = []
+        for x, n in zip(both, own):
+            i = [x.storage_offset() + t * x.stride(0) + h * x.stride(1) + e
+                 for t in range(T) for h in range(x.shape[1]) for e in range(d)]
+            assert n is None or (len(set(i)) == len(i) and max(i) - min(i) < n)
+            at.append(set(i))
+        if None not in own:
+            shared = bool(at[0] & at[1])
+            seen[shared] += 1
+            if shared or both[0].stride(0) == both[1].stride(0) or T == 1:
+                assert ops._share_memory(*both) == shared, (both[0].stride(), both[1].stride())
+    assert min(seen) > 100
