@@ -472,8 +472,8 @@ int check_attention(const SeqAttention *a) {
         // the most waves that a launch has: a slot for 32 rows of either kind
         (a->tq / 32 * (a->hq / a->hkv) + a->tk / 32 + a->n_seq + 2) * a->hkv > SEQ_MAX_ROWS)
         return CO_ERR_BOUNDS;
-    if ((a->dtype != SEQ_BF16 && a->dtype != SEQ_FP16) || !(a->scale > 0.0f) ||
-        a->scale > 1e30f)
+    if ((a->dtype != SEQ_BF16 && a->dtype != SEQ_FP16) || !(a->scale >= SEQ_LEAST) ||
+        a->scale > SEQ_MOST)
         return CO_ERR_DATA;
     return CO_OK;
 }

@@ -463,7 +463,9 @@ extern "C" int seq_policy_loss(const SeqPolicyLoss *p, void *stream) {
     int rc = seq::check_policy(p);
     if (rc != CO_OK) return rc;
     if (!p->loss) return CO_ERR_NULLARG;
-    if (!(p->temperature > 0.0f)) return CO_ERR_DATA;
+    if (!(p->temperature >= SEQ_LEAST && p->temperature <= SEQ_MOST) || !(p->clip_lo >= 0.0f) ||
+        !(p->clip_hi >= 0.0f) || !(fabsf(p->kl_coef) <= 3.4028235e38f))
+        return CO_ERR_DATA;
     hipStream_t s = (hipStream_t)stream;
     double *ws = (double *)p->workspace;
     int64_t terms = 0;

@@ -33,6 +33,8 @@ from torch.autograd.function import once_differentiable
 from cusr_amd.kernel.co_inproc import CO_OK, COError, _HERE
 
 SEQ_MAX_HEAD = 128
+_LEAST, _MOST = 1e-30, 1e30          # scale and temperature
+_FLOAT32 = float(np.finfo(np.float32).max)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
@@ -228,7 +230,8 @@ _HALF = (torch.bfloat16, torch.float16)
 
 def _check_attention(q, k, v, cu_q, cu_k, k_lens, scale):
     _no_tangents(q, k, v)
-    if _plain_attention(q, k, v, cu_q, cu_k, k_lens) and (scale is None or 0.0 < scale <= 1e30):
+    if _plain_attention(q, k, v, cu_q, cu_k, k_lens) and (scale is None
+                                                             or _LEAST <= scale <= _MOST):
         return
     _need(q, "q", _HALF, 3)
     dev = q.device
@@ -254,8 +257,8 @@ def _check_attention(q, k, v, cu_q, cu_k, k_lens, scale):
         _need(k_lens, "k_lens", (torch.int32,), 1, dev)
         if k_lens.numel() != cu_q.numel() - 1:
             raise ValueError("k_lens must have one entry per sequence")
-    if scale is not None and not 0.0 < scale <= 1e30:
-        raise ValueError(f"scale must be positive, not {scale}")
+    if scale is not None and not _LEAST <= scale <= _MOST:
+        raise ValueError(f"scale must be from {_LEAST} to {_MOST}, not {scale}")
 
 
 def _attention_args(q, k, v, o, lse, low, cu_q, cu_k, k_lens, scale):
@@ -597,7 +600,8 @@ def _check_policy(logits, actions, logp_old, advantages, logp_ref, weights, clip
     _no_tangents(logits, logp_old, advantages, logp_ref, weights)
     lo, hi = (float(c) for c in clip)
     if (_plain_policy(logits, actions, (logp_old, advantages), (logp_ref, weights))
-            and lo >= 0 and hi >= 0 and 0 < temperature < math.inf and math.isfinite(kl_coef)):
+            and 0 <= lo <= _FLOAT32 and 0 <= hi <= _FLOAT32 and _LEAST <= temperature <= _MOST
+            and abs(kl_coef) <= _FLOAT32):
         return lo, hi
     _need(logits, "logits", tuple(_DTYPES), 2)
     T, V = logits.shape
@@ -614,11 +618,12 @@ def _check_policy(logits, actions, logp_old, advantages, logp_ref, weights, clip
             raise ValueError(f"{name} must have {T} entries, not {x.numel()}")
     if not (lo >= 0 and hi >= 0):
         raise ValueError(f"clip must be two widths of at least 0; got {clip}")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError("temperature must be positive")
-    if not math.isfinite(kl_coef):
-        raise ValueError("kl_coef must be finite")
-    return lo, hi
+    if not _LEAST <= temperature <= _MOST:
+        raise ValueError(f"temperature must be from {_LEAST} to {_MOST}, not {temperature}")
+    if not abs(kl_coef) <= _FLOAT32:
+        raise ValueError("kl_coef must be a finite float32")
+    # a width that float32 does not hold is none
+    return tuple(x if x <= _FLOAT32 else math.inf for x in (lo, hi))
 
 
 def _policy(logits, actions, logp_old, advantages, logp_ref, weights, clip, kl_coef, temperature,

@@ -15,8 +15,9 @@
  *
  * Return codes are cusr_co.h's: CO_OK, CO_ERR_NULLARG (null pointer, negative
  * size, struct of another size), CO_ERR_BOUNDS (a size beyond the bounds
- * below), CO_ERR_DATA (alignment, stride or workspace that does not fit),
- * CO_ERR_CUDA (a HIP error at launch). */
+ * below), CO_ERR_DATA (alignment, stride or workspace that does not fit; a
+ * scale, temperature, clip width or coefficient out of range), CO_ERR_CUDA (a
+ * HIP error at launch). */
 #ifndef CUSR_SEQ_H
 #define CUSR_SEQ_H
 
@@ -35,6 +36,8 @@ extern "C" {
 
 #define SEQ_MAX_HEAD 128          /* head size of attention, a multiple of 8 */
 #define SEQ_MAX_ROWS 2147000000LL /* query rows times heads, key rows, tokens */
+#define SEQ_LEAST 1e-30f          /* least and largest scale and temperature */
+#define SEQ_MOST 1e30f
 
 /* Causal attention over packed sequences, bf16 or fp16.
  *
@@ -47,7 +50,7 @@ extern "C" {
  * cu_q[0] is 0. Queries are the last ones of the keys: query i of lq sees
  * keys 0 .. i + lk - lq. A query that sees no key, and a query row in no
  * sequence, give o = 0 and lse = -inf. Offsets out of order or out of range
- * are clamped into the tensors. scale is positive. Within a sequence's keys a
+ * are clamped into the tensors. Within a sequence's keys a
  * value that is not finite also reaches queries that do not see it, up to 94
  * places before it (a masked probability is a 0 in a matrix product).
  *

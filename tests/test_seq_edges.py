@@ -2,6 +2,7 @@
 refusals at the edges of arguments and layouts."""
 from __future__ import annotations
 
+import ctypes
 import re
 from pathlib import Path
 
@@ -10,6 +11,7 @@ import torch
 from torch.autograd import forward_ad
 
 from cusr_amd.kernel import seq_ops as ops
+from cusr_amd.kernel.co_inproc import CO_ERR_DATA
 
 CSRC = Path(__file__).resolve().parents[1] / "cusr_amd" / "csrc"
 
@@ -132,3 +134,45 @@ def test_memory_that_is_not_shared():
             if shared or both[0].stride(0) == both[1].stride(0) or T == 1:
                 assert ops._share_memory(*both) == shared, (both[0].stride(), both[1].stride())
     assert min(seen) > 100
+
+
+@pytest.mark.parametrize("kw", [dict(temperature=1e-50), dict(temperature=1e-40),
+                                dict(temperature=1e39), dict(temperature=-1.0),
+                                dict(temperature=float("nan")), dict(kl_coef=1e39),
+                                dict(kl_coef=-1e300), dict(kl_coef=float("inf"))])
+def test_policy_numbers_beyond_float32_are_refused(kw):
+    for fn, real, other in calls():
+        if fn in (ops.policy_loss, ops.policy_loss_grad):
+            with pytest.raises(ValueError):
+                fn(**real, **other, **kw)
+
+
+def test_scales_beyond_float32_are_refused():
+    for fn, real, other in calls()[:2]:
+        for scale in (0.0, -1.0, 1e-50, 1e-39, 1e31, float("nan")):
+            with pytest.raises(ValueError, match="scale"):
+                fn(**real, **other, scale=scale)
+
+
+def test_clip_widths_beyond_float32_do_not_clip():
+    _, real, other = calls()[3]
+    x = {n: t for n, t in {**real, **other}.items()}
+    got = ops._check_policy(x["logits"], x["actions"], x["logp_old"], x["advantages"], None, None,
+                            (1e39, float("inf")), 0.0, 1.0)
+    assert got == (float("inf"), float("inf"))
+
+
+def test_library_refuses_numbers_out_of_range():
+    lib, ref = ops.load_library(), ctypes.addressof
+    for kw in (dict(temperature=float("inf")), dict(temperature=1e-35), dict(clip_lo=-0.1),
+               dict(clip_hi=float("nan")), dict(kl_coef=float("nan")),
+               dict(kl_coef=float("inf"))):
+        p = ops.SeqPolicyLoss(ctypes.sizeof(ops.SeqPolicyLoss), 1, 4, 10, 10, 10, 0.2, 0.2, 0.0,
+                              1.0)
+        for n in ("logits", "actions", "logp_old", "advantages", "weights", "loss", "logp",
+                  "workspace"):
+            setattr(p, n, 4096)
+        p.workspace_bytes = 1 << 20
+        for n, x in kw.items():
+            setattr(p, n, x)
+        assert lib.seq_policy_loss(ref(p), None) == CO_ERR_DATA, kw
