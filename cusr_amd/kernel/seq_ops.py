@@ -199,7 +199,7 @@ def _heads16(x):
     if x.numel():
         return x.contiguous() if x.shape[2] % 8 == 0 and not x.is_contiguous() else x.clone(
             memory_format=torch.contiguous_format)
-    return x
+    return x.new_empty(x.shape)          # nothing to copy, and strides that fit
 
 
 def _plain_attention(q, k, v, cu_q, cu_k, k_lens):

@@ -220,3 +220,23 @@ def test_rotary_in_place_is_seen_by_autograd(ops):
         q = normal((4, 2, 32), F32, 1).clone()
         want = ops.rotary(q, None, pos, table)
         assert torch.equal(ops.rotary(q, None, pos, table, inplace=True), want)
+
+
+# --------------------------------------------------------------- empty layouts
+
+def test_attention_empty_tensors_of_any_layout(ops):
+    """No rows or no keys, as slices whose strides the kernels would not read."""
+    def odd(n, h):
+        return torch.empty(n, h, 67, dtype=BF, device=DEV)[..., 3:]
+
+    q, k = normal((7, 4, 64), BF, 1), odd(0, 2)
+    o, lse = ops.attention(q, k, odd(0, 2), cu([7]), cu([0]), return_lse=True)
+    assert not bool(o.any()) and bool((lse == float("-inf")).all())
+    g = ops.attention_grad(q, q, k, k, o, lse, cu([7]), cu([0]))
+    assert [x.shape for x in g] == [q.shape, k.shape, k.shape] and not bool(g[0].any())
+    q, k = odd(0, 4), normal((5, 2, 64), BF, 2)
+    o, lse = ops.attention(q, k, k, cu([0]), cu([5]), return_lse=True)
+    assert o.shape == (0, 4, 64) and lse.shape == (4, 0)
+    g = ops.attention_grad(odd(0, 4), q, k, k, odd(0, 4), lse, cu([0]), cu([5]))
+    assert [x.shape for x in g] == [q.shape, k.shape, k.shape]
+    assert not any(bool(x.any()) for x in g)
