@@ -242,8 +242,8 @@ def rewards_of(losses, y):
 def search(X, y, *, rounds=10, population=1024, max_iter=10, seed=0, proposer=None, trainer=None,
            backend=None, log=print):
     """Rounds of sampling, fitting and training. Returns (best, history): the
-    best program as (loss, (nt, nv, ci), constants) and each round's mean and
-    best reward."""
+    best program as (loss, (nt, nv, ci), constants), (inf, None, None) when none
+    was fitted, and each round's mean and best reward."""
     X, y = np.asarray(X, np.float64), np.asarray(y, np.float64)
     p = proposer or Proposer(X.shape[1], seed=seed)
     tr = trainer or Trainer(p, top=0.1, kl_coef=0.05)
@@ -279,6 +279,9 @@ def main(argv=None):
     X = rng.uniform(-2, 2, size=(512, 2))
     y = 1.5 * np.sin(0.8 * X[:, 0]) * X[:, 1] + 0.5
     best, _ = search(X, y, rounds=a.rounds, population=a.population, seed=a.seed)
+    if best[1] is None:
+        print("no program was fitted")
+        return
     nt, nv, _ = best[1]
     print(f"best loss {best[0]:.3g}: nodes {nt.tolist()}, values {nv.tolist()}, constants "
           f"{np.round(best[2], 4).tolist()}")

@@ -3,6 +3,7 @@ refusals at the edges of arguments and layouts."""
 from __future__ import annotations
 
 import ctypes
+import math
 import re
 from pathlib import Path
 
@@ -176,3 +177,12 @@ def test_library_refuses_numbers_out_of_range():
         for n, x in kw.items():
             setattr(p, n, x)
         assert lib.seq_policy_loss(ref(p), None) == CO_ERR_DATA, kw
+
+
+# ------------------------------------------------------------------- proposer
+
+def test_a_search_that_fits_nothing_says_so(monkeypatch, capsys):
+    from cusr_amd.demonstrator import proposer
+    monkeypatch.setattr(proposer, "search", lambda *a, **k: ((math.inf, None, None), []))
+    proposer.main(["--rounds", "0"])
+    assert capsys.readouterr().out == "no program was fitted\n"
