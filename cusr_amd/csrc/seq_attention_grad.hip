@@ -419,9 +419,10 @@ void attn_grad_short(AttnGrad a, int slots) {
 }
 
 // Long sequences, rows: a block of four waves owns 128 rows of one key head; keys
-// and values pass through LDS 64 at a time, as in the forward. The matrix cores bound
-// it, busy 54 % beside the vector instructions: five sequences of 700 to 4,801, 32
-// heads of 128 over 8, 0.49 ms (the keys' part 0.74, 49 %).
+// and values pass through LDS 64 at a time, as in the forward. No unit is full: the
+// matrix cores are busy 51 % of the time, the vector instructions 31 %, and the waves
+// wait 47 % of theirs, for tiles and for each other: five sequences of 700 to 4,801, 32
+// heads of 128 over 8, 0.50 ms.
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, int slots) {
     typedef KeyTiles<DP, 64, WAVES> Keys;
@@ -524,9 +525,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, i
 // longest run over the rows would last twice as long, and the longest run is what
 // few sequences wait for. Rows pass through LDS 64 at a time, copied there past
 // the registers one tile ahead of their use. Rows beyond the last repeat it with
-// lse +inf, which makes their P and dS 0. Bound by the matrix cores, 48 % busy,
-// and the waits of eight waves at one barrier: 32 heads of 128 over 8, five
-// sequences of 700 to 4,801 in about 0.6 ms, 1 PFLOP/s.
+// lse +inf, which makes their P and dS 0. No unit is full: the matrix cores are busy
+// 49 % of the time, the vector instructions 28 %, and eight waves wait at one barrier
+// for a third of theirs; with heads of 128 twelve registers are spilled. 32 heads of 128
+// over 8, five sequences of 700 to 4,801 in 0.74 ms, 0.84 PFLOP/s.
 template <typename T, int DP, int KX>
 __global__ __launch_bounds__(KX * 128, KX == 4 || DP <= 64 ? 2 : 1) void attn_grad_kv_tiles(AttnGrad a, int slots) {
     constexpr int RB = 64, KEYS = KX * 32, WAVES = KX * 2;

@@ -512,7 +512,8 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, inplace=
     launch; float32, bfloat16 or float16. positions int32 or int64 [T]; table
     from rotary_table. The first rot = 2 * table.shape[1] elements of each head
     turn in pairs (i, i + rot/2), or (2i, 2i + 1) when interleaved; the rest is
-    copied. inverse turns back, which is the gradient. inplace writes into q
+    copied. inverse turns by the opposite angles, which is the gradient, and the
+    way back unless the table has a magnitude ("parts"). inplace writes into q
     and k, and autograd sees it. A position outside the table gives NaN in its
     token's turned elements. Gradients go to q and k, not to the table. Returns
     (q', k'), or q' alone when k is None."""

@@ -52,7 +52,9 @@ extern "C" {
  * sequence, give o = 0 and lse = -inf. Offsets out of order or out of range
  * are clamped into the tensors. Within a sequence's keys a
  * value that is not finite also reaches queries that do not see it, up to 94
- * places before it (a masked probability is a 0 in a matrix product).
+ * places before it (a masked probability is a 0 in a matrix product); in the
+ * gradient a key's, a value's, a query's or an output gradient's alike, queries'
+ * up to 62 places after them.
  *
  * lse (may be null for the forward) [hq, tq] fp32: log of the sum of
  * exp(scale q.k) over the visible keys. o_low (may be null): what rounding o to
@@ -99,9 +101,11 @@ int seq_attention_grad(const SeqAttention *a, const SeqAttentionGrad *g, void *s
 /* Rotary positions of q [tokens, hq, d] and k [tokens, hkv, d] (hkv 0: q
  * alone) in one launch. table [table_len, rot/2, 2] fp32 holds (cos, sin);
  * the first rot elements of each head turn, the rest is copied. Pairs are
- * (i, i + rot/2), or (2i, 2i + 1) when interleaved. inverse turns back: the
- * gradient. In place (q_out == q with equal strides) is allowed. A position
- * outside the table gives NaN in the turned elements of its token. */
+ * (i, i + rot/2), or (2i, 2i + 1) when interleaved. inverse turns by the opposite
+ * angles: the gradient (and the way back where cos^2 + sin^2 is 1 in the table).
+ * In place (q_out == q with equal strides, every element of q and k in memory of
+ * its own) is allowed. A position outside the table gives NaN in the turned
+ * elements of its token. */
 typedef struct SeqRotary {
     int32_t struct_size;
     int32_t dtype;            /* SEQ_FP32, SEQ_BF16 or SEQ_FP16 */
