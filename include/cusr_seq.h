@@ -52,9 +52,9 @@ extern "C" {
  * sequence, give o = 0 and lse = -inf. Offsets out of order or out of range
  * are clamped into the tensors. Within a sequence's keys a
  * value that is not finite also reaches queries that do not see it, up to 94
- * places before it (a masked probability is a 0 in a matrix product); in the
- * gradient a key's, a value's, a query's or an output gradient's alike, queries'
- * up to 62 places after them.
+ * places before it (a masked probability is a 0 in a matrix product). In the
+ * gradient so does a key, and a query or output gradient reaches keys that it does
+ * not see, up to 62 places after it.
  *
  * lse (may be null for the forward) [hq, tq] fp32: log of the sum of
  * exp(scale q.k) over the visible keys. o_low (may be null): what rounding o to
@@ -131,7 +131,8 @@ int seq_rotary(const SeqRotary *r, void *stream);
  * logp_ref null or kl_coef 0: no KL term. A token of weight 0 takes no part,
  * whatever its logits: logp = 0, its gradient row is 0. A row whose action has the
  * logit -inf has logp = -inf, ratio 0 and no gradient (and with a KL term an
- * infinite loss), whatever logp_old and logp_ref, -inf among them. An action outside the vocabulary gives logp = NaN.
+ * infinite loss), whatever logp_old and logp_ref, -inf among them. An action
+ * outside the vocabulary gives logp = NaN.
  * dlogits (may be null: loss and logp alone) [tokens, vocab] like logits,
  * rows `drow` apart: d loss / d logits, times *dloss when dloss is given.
  * loss is one fp32. */
