@@ -1,6 +1,6 @@
 // seq_attention.hip -- causal attention over packed sequences
 // (include/cusr_seq.h, seq_attention).
-#include "seq_attn.h"
+#include "seq_hidden.h"
 
 namespace seq {
 
@@ -18,6 +18,65 @@ __device__ inline void store_out(const Attn &a, int t, int head, const float16v 
     if (low)
         store_row<T, DP, true>(a.o_low, ((int64_t)t * a.hq + head) * a.d, o, inv, a.d, ok);
     store_lse(a, t, head, m, l, ok);
+}
+
+// Outputs of rows first + r of a sequence, for the r of `bad`, where hidden keys among
+// key0 .. key1-1 reached them; of a chunk of keys, its unscaled sums, to sums + row *
+// width, for the maximum and sum at stat + 2 row.
+template <typename T>
+__device__ __attribute__((noinline)) void mend_out(Arguments<Attn> args, Place place, int hk,
+                                                   int first, uint32_t bad, int key0, int key1,
+                                                   float *sums, const float *stat, int width) {
+    const Attn &a = *(const Attn *)uniform(args);
+    const Place p = uniform(place);
+    hk = uniform(hk), first = uniform(first), bad = uniform((int)bad);
+    key0 = uniform(key0), key1 = uniform(key1), width = uniform(width);
+    sums = uniform(sums), stat = uniform(stat);
+    const int lane = threadIdx.x & 63, rows = p.lq * a.G;
+    auto k = [&](int j) {
+        return (const uint16_t *)a.k + (p.k0 + j) * a.k_row + hk * a.k_head;
+    };
+    auto v = [&](int j) {
+        return (const uint16_t *)a.v + (p.k0 + j) * a.v_row + hk * a.v_head;
+    };
+    wait_copies<0>();                // stores on their way come first
+    for (; bad && first + __builtin_ctz(bad) < rows; bad &= bad - 1) {
+        const int row = first + __builtin_ctz(bad);
+        const int qi = row / a.G, head = hk * a.G + row % a.G;
+        const int end = min(qi + p.lk - p.lq + 1, key1);         // beyond its last key
+        if (!hidden_cause<T>(v, a.d, max(end, key0), min(end + kReach, key1),
+                             end > key0 ? end - 1 : -1))
+            continue;
+        const int64_t t = p.q0 + qi;
+        const uint16_t *q = (const uint16_t *)a.q + t * a.q_row + head * a.q_head;
+        auto score = [&](int j) { return dot<T>(q, k(j), a.d); };
+        float m = neg_inf(), l = 0.0f;
+        if (stat) {
+            m = stat[2 * row];
+            l = stat[2 * row + 1];
+        } else {
+            for (int j = key0 + lane; j < end; j += 64) m = fmaxf(m, score(j));
+            for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+            for (int j = key0 + lane; j < end; j += 64) l += exp2_fast((score(j) - m) * a.c);
+            for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+        }
+        if (!__all(finite(l))) continue;         // not finite by what it sees
+        float sum[2] = {0.0f, 0.0f};
+        add_seen<T>(v, a.d, key0, end, [&](int j) {
+            return rounded<T>(exp2_fast((score(j) - m) * a.c));
+        }, sum);
+        typedef typename T::elem E;
+        each_column(a.d, [&](int e, int col) {
+            if (sums) {
+                sums[(int64_t)row * width + col] = sum[e];
+                return;
+            }
+            const float x = l == 0.0f ? 0.0f : sum[e] / l;
+            ((E *)a.o)[t * a.o_row + head * a.o_head + col] = (E)x;
+            if (keeps_low(a, rows))
+                ((E *)a.o_low)[(t * a.hq + head) * a.d + col] = (E)(x - (float)(E)x);
+        });
+    }
 }
 
 // A wave's tile of 32 rows over the keys key0 .. key1-1, 32 at a time with a
@@ -124,16 +183,19 @@ __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, 
 // way of LDS and whole rows stored. 16,384 sequences of 1 to 31, 8 heads of 64 over
 // 4, take 191 us (4.2 TB/s); with K to registers 207, with the output stored as 32
 // bytes of each row 205.
+// Returns a bit for each tile with a sum that is not finite.
 template <typename T, int DP, typename I>
-__device__ inline void wave_tiles(const Attn &a, const Place &p, int hk, int first, uint16_t *kt,
+__device__ inline uint32_t wave_tiles(const Attn &a, const Place &p, int hk, int first, uint16_t *kt,
                                   uint16_t *vt) {
     const int rows = p.lq * a.G;
     const bool low = keeps_low(a, rows);
     const float inv = 1.0f / (float)a.G;
+    uint32_t bad = 0;
     for (int tile = first; tile < first + kShortRows / 32 && tile * 32 < rows; tile++) {
         float16v o[DP / 32];
         float m, l;
         const Row r = run_rows<T, DP, false, I>(a, p, hk, tile, 0, p.lk, kt, vt, o, m, l);
+        if (not_finite<DP>(o) & row_bits(finite(l))) bad |= 1 << (tile - first);
         if (low) {
             store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok, true);
             continue;
@@ -145,6 +207,7 @@ __device__ inline void wave_tiles(const Attn &a, const Place &p, int hk, int fir
         });
         store_lse(a, r.t, r.head, m, l, r.ok);
     }
+    return bad;
 }
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void attn_wave(Attn a, int slots) {
@@ -159,8 +222,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void attn_wave(Attn a, int s
     const Place p = place_of(a, b, f.start, f.end);
     const int first = (slot - slot_of(p.q0, a.G, kShortRows, b)) * (kShortRows / 32);
     if (first < 0) return;
-    if (a.near && p.lq * a.G <= kNear && p.lk <= kNear) wave_tiles<T, DP, uint32_t>(a, p, hk, first, kt, vt);
-    else wave_tiles<T, DP, int64_t>(a, p, hk, first, kt, vt);
+    uint32_t bad;
+    if (a.near && p.lq * a.G <= kNear && p.lk <= kNear)
+        bad = wave_tiles<T, DP, uint32_t>(a, p, hk, first, kt, vt);
+    else
+        bad = wave_tiles<T, DP, int64_t>(a, p, hk, first, kt, vt);
+    for (; __builtin_expect(bad, 0); bad &= bad - 1)
+        mend_out<T>(arguments<Attn>(), p, hk, (first + __builtin_ctz(bad)) * 32, ~0u, 0, p.lk,
+                    nullptr, nullptr, 0);
 }
 
 // Long sequences: a block of WAVES waves owns WAVES * 32 rows of one key head;
@@ -276,7 +345,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int slots) {
         work(Const<0>{}, k0);
         if (k0 + KB < keys) work(Const<1>{}, k0 + KB);
     }
-    store_out<T, DP>(a, p.q0 + qi, head, o, m, add_halves(l), ok, keeps_low(a, rows));
+    l = add_halves(l);
+    const uint32_t bad = not_finite<DP>(o) & row_bits(finite(l));
+    store_out<T, DP>(a, p.q0 + qi, head, o, m, l, ok, keeps_low(a, rows));
+    if (__builtin_expect(bad, 0))
+        mend_out<T>(arguments<Attn>(), p, hk, w0, bad, 0, p.lk, nullptr, nullptr, 0);
 }
 
 // Few rows over many keys (single tokens over a cache). A sequence's keys are
@@ -314,16 +387,19 @@ __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
     if (chunk >= (split ? chunks : 1)) return;
     const int key0 = split ? chunk * st.chunk : 0;
     const int key1 = split && key0 + st.chunk < p.lk ? key0 + st.chunk : p.lk;
+    const int64_t first = ((int64_t)slot * a.hkv + hk) * st.rows;
+    bool bad = false;
     // a sequence with more rows than the partials have room for is not split
     for (int tile = blockIdx.y; tile * 32 < rows; tile += st.tiles) {
         float16v o[DP / 32];
         float m, l;
         const Row r = run_rows<T, DP, true, int64_t>(a, p, hk, tile, key0, key1, vt, vt, o, m, l);
+        bad |= (not_finite<DP>(o) & row_bits(finite(l))) != 0;
         if (!split) {
             store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok, keeps_low(a, rows));
             continue;
         }
-        const int64_t pr = ((int64_t)slot * a.hkv + hk) * st.rows + tile * 32 + (lane & 31);
+        const int64_t pr = first + tile * 32 + (lane & 31);
         if (!r.ok) continue;
 #pragma unroll
         for (int dt = 0; dt < DP / 32; dt++)
@@ -338,6 +414,10 @@ __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
             st.ml[2 * pr + 1] = l;
         }
     }
+    if (__builtin_expect(bad, 0))
+        for (int tile = blockIdx.y; tile * 32 < rows; tile += st.tiles)
+            mend_out<T>(arguments<Attn>(), p, hk, tile * 32, ~0u, key0, key1,
+                        split ? st.o + first * DP : nullptr, split ? st.ml + 2 * first : nullptr, DP);
 }
 
 // Joins the chunks of a split sequence: a wave to a row of the output, which

@@ -6,7 +6,7 @@
 // dK = scale dS^T Q,  dV = P^T do. One kernel owns rows and sums over keys
 // (dQ, delta), one owns keys and sums over rows (dK, dV, all heads of the
 // group): every sum has one owner and one order, so no atomics.
-#include "seq_attn.h"
+#include "seq_hidden.h"
 
 namespace seq {
 
@@ -40,6 +40,131 @@ __device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float
     }
 }
 
+// A key head's rows and keys, for what seq_hidden.h does with them.
+template <typename T> struct HeadRows {
+    const AttnGrad &a;
+    const Place &p;
+    int hk;
+    __device__ int64_t t(int row) const { return p.q0 + row / a.G; }
+    __device__ int head(int row) const { return hk * a.G + row % a.G; }
+    __device__ const uint16_t *q(int row) const {
+        return (const uint16_t *)a.q + t(row) * a.q_row + head(row) * a.q_head;
+    }
+    __device__ const uint16_t *d_o(int row) const {
+        return (const uint16_t *)a.g.d_o + t(row) * a.g.do_row + head(row) * a.g.do_head;
+    }
+    __device__ const uint16_t *k(int key) const {
+        return (const uint16_t *)a.k + (p.k0 + key) * a.k_row + hk * a.k_head;
+    }
+    __device__ const uint16_t *v(int key) const {
+        return (const uint16_t *)a.v + (p.k0 + key) * a.v_row + hk * a.v_head;
+    }
+    __device__ float lse2(int row) const { return a.lse[head(row) * a.tq + t(row)] * kLog2e; }
+    __device__ float delta(int row) const {
+        const uint16_t *y = d_o(row);
+        float s = dot<T>((const uint16_t *)a.o + t(row) * a.o_row + head(row) * a.o_head, y, a.d);
+        if (keeps_low(a, p.lq * a.G))
+            s += dot<T>((const uint16_t *)a.o_low + (t(row) * a.hq + head(row)) * a.d, y, a.d);
+        return s;
+    }
+    __device__ float probability(int row, int key, float lse2) const {
+        return exp2_fast(__builtin_fmaf(dot<T>(q(row), k(key), a.d), a.c, -lse2));
+    }
+    __device__ float dp(int row, int key) const { return dot<T>(d_o(row), v(key), a.d); }
+};
+
+// dq of rows first + r, for the r of `bad`, where a hidden key reached them.
+template <typename T>
+__device__ inline void mend_rows(const AttnGrad &a, const Place &p, int hk, int first,
+                                 uint32_t bad) {
+    const HeadRows<T> of{a, p, hk};
+    auto k = [&](int key) { return of.k(key); };
+    const int rows = p.lq * a.G;
+    wait_copies<0>();                // stores on their way come first
+    for (; bad && first + __builtin_ctz(bad) < rows; bad &= bad - 1) {
+        const int row = first + __builtin_ctz(bad);
+        const int end = row / a.G + p.lk - p.lq + 1;             // beyond its last key
+        float sum[2] = {0.0f, 0.0f}, lse2 = 0.0f, delta = 0.0f;
+        if (end > 0) {
+            lse2 = of.lse2(row);
+            delta = of.delta(row);
+            if (!__all(finite(lse2) && finite(delta))) continue;     // not finite by what it sees
+        }
+        if (!hidden_cause<T>(k, a.d, max(end, 0), min(end + kReach, p.lk), end > 0 ? end - 1 : -1))
+            continue;
+        add_seen<T>(k, a.d, 0, end, [&](int key) {
+            return rounded<T>(of.probability(row, key, lse2) * (of.dp(row, key) - delta));
+        }, sum);
+        typename T::elem *to = (typename T::elem *)a.g.dq + of.t(row) * a.g.dq_row +
+                               of.head(row) * a.g.dq_head;
+        each_column(a.d, [&](int e, int col) { to[col] = (typename T::elem)(sum[e] * a.scale); });
+    }
+}
+
+// dk and dv of keys first + r, where a row that does not see them reached them. Tiles of
+// rows begin less than a tile of keys and a tile of rows before the first that does.
+template <typename T>
+__device__ inline void mend_keys(const AttnGrad &a, const Place &p, int hk, int first,
+                                 uint32_t bad) {
+    const HeadRows<T> of{a, p, hk};
+    auto q = [&](int row) { return of.q(row); };
+    auto d_o = [&](int row) { return of.d_o(row); };
+    const int rows = p.lq * a.G;
+    if (rows == 0 || !__all(finite(of.lse2(rows - 1)))) return;  // the last sees every key
+    wait_copies<0>();
+    for (; bad && first + __builtin_ctz(bad) < p.lk; bad &= bad - 1) {
+        const int key = first + __builtin_ctz(bad);
+        if (key < 0) continue;
+        const int start = max(key - p.lk + p.lq, 0) * a.G;       // the first row that sees it
+        const int before = max(start - 31 * a.G - 31, 0);
+        if (!hidden_cause<T>(q, a.d, before, start, -1) &&
+            !hidden_cause<T>(d_o, a.d, before, start, rows - 1))
+            continue;
+        float dk[2] = {0.0f, 0.0f}, dv[2] = {0.0f, 0.0f};
+        add_seen<T>(d_o, a.d, start, rows, [&](int row) {
+            return rounded<T>(of.probability(row, key, of.lse2(row)));
+        }, dv);
+        add_seen<T>(q, a.d, start, rows, [&](int row) {
+            return rounded<T>(of.probability(row, key, of.lse2(row)) *
+                              (of.dp(row, key) - of.delta(row)));
+        }, dk);
+        typedef typename T::elem E;
+        E *to_k = (E *)a.g.dk + (p.k0 + key) * a.g.dk_row + hk * a.g.dk_head;
+        E *to_v = (E *)a.g.dv + (p.k0 + key) * a.g.dv_row + hk * a.g.dv_head;
+        each_column(a.d, [&](int e, int col) {
+            to_k[col] = (E)(dk[e] * a.scale);
+            to_v[col] = (E)dv[e];
+        });
+    }
+}
+
+// Called by the long kernels: of rows, or of keys.
+template <typename T, bool KEYS>
+__device__ __attribute__((noinline)) void mend_long(Arguments<AttnGrad> args, Place place, int hk,
+                                                    int first, uint32_t bad) {
+    const AttnGrad &a = *(const AttnGrad *)uniform(args);
+    const Place p = uniform(place);
+    if (KEYS) mend_keys<T>(a, p, uniform(hk), uniform(first), uniform((int)bad));
+    else mend_rows<T>(a, p, uniform(hk), uniform(first), uniform((int)bad));
+}
+// Called by the short kernel: all of a wave's rows and keys, the wave's number `item`.
+template <typename T>
+__device__ __attribute__((noinline)) void mend_short(Arguments<AttnGrad> args, int item) {
+    const AttnGrad &a = *(const AttnGrad *)uniform(args);
+    item = uniform(item);
+    const int slot = item / a.hkv, hk = item - slot * a.hkv;
+    const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, kShortRows, slot);
+    const Place p = place_of(a, f.b, f.start, f.end);
+    const int mine = slot - slot_of(f.start, a.G, kShortRows, f.b);
+    const int shares = max((p.lq * a.G + kShortRows - 1) / kShortRows, 1);
+    const int s0 = a.cu_k == a.cu_q && a.tk == a.tq ? f.start : offset_at(a.cu_k, f.b, a.tk);
+#pragma unroll 1
+    for (int tile = mine * 4; tile < mine * 4 + 4; tile++) mend_rows<T>(a, p, hk, tile * 32, ~0u);
+#pragma unroll 1
+    for (int first = mine * 32 + s0 - p.k0; first < p.lk; first += shares * 32)
+        mend_keys<T>(a, p, hk, first, ~0u);
+}
+
 // Short sequences: a wave owns up to 128 rows of a sequence and key head, and
 // every so many tiles of 32 of its keys; most have a sequence to themselves and
 // need no statistics from another kernel. First the rows: delta = sum of P dP,
@@ -51,29 +176,30 @@ __device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float
 // the path of its own for up to 64 rows and keys, in which few loads wait for
 // others and P and dS are formed once: 8,192 sequences of 3 to 63, 8 heads of 64,
 // take 0.47 ms (4.1 TB/s), with P and dS formed twice 0.58, on the general path 0.73.
+// Its part of a wave, in LDS: four tiles, and a fifth for P and dS of a pair of tiles,
+// for results on their way out, or for rows' statistics: lse, delta, last visible key.
+// Returns whether all sums are finite.
+template <int DP> constexpr int kShortLds = 4 * 32 * Tile<DP>::stride +
+                                            (DP < 64 ? 64 * 32 : 32 * Tile<DP>::stride);
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1)
-void attn_grad_short(AttnGrad a, int slots) {
+__device__ inline bool grad_short(const AttnGrad &a, int slots, uint16_t *lds_wave) {
     constexpr int C = DP / 16, S = Tile<DP>::stride;
-    // four tiles of a wave, and a fifth for P and dS of a pair of tiles, for results on
-    // their way out, or for rows' statistics: lse, delta, last visible key
-    constexpr int FIFTH = DP < 64 ? 64 * 32 : 32 * S;
-    __shared__ __align__(256) uint16_t lds_all[4][4 * 32 * S + FIFTH];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    uint16_t (*lds)[32 * S] = (uint16_t(*)[32 * S])lds_all[wave], *fifth = lds[4];
+    uint16_t (*lds)[32 * S] = (uint16_t(*)[32 * S])lds_wave, *fifth = lds[4];
+    float odd = 0.0f;
     const uint32_t lds_at = lds_address(lds[0]);
     float *lses = (float *)fifth, *deltas = lses + kShortRows;
     int *lims = (int *)(deltas + kShortRows);
     const int item = block_number() * 4 + wave;
     const int slot = item / a.hkv, hk = item - slot * a.hkv;
-    if (slot >= slots) return;
+    if (slot >= slots) return true;
     const Found f = find_sequence(a.cu_q, a.n_seq, a.tq, a.G, kShortRows, slot);
     const Place p = place_of(a, f.b, f.start, f.end);
     const int rows = p.lq * a.G, tiles = (rows + 31) / 32;
     const int mine = slot - slot_of(f.start, a.G, kShortRows, f.b);
     const int shares = max((rows + kShortRows - 1) / kShortRows, 1);
-    if (mine < 0 || mine >= shares) return;
+    if (mine < 0 || mine >= shares) return true;
     // the key rows of the segment, of which p.lk are keys
     const bool same = a.cu_k == a.cu_q && a.tk == a.tq;
     const int s0 = same ? f.start : offset_at(a.cu_k, f.b, a.tk);
@@ -134,6 +260,7 @@ void attn_grad_short(AttnGrad a, int slots) {
         for (int dt = 0; dt < DP / 32; dt++) dq[dt] = float16v{};
     };
     auto end_rows = [&](auto as, int tile, uint16_t *free) {
+        watch<DP>(odd, dq);
         store_tile<T, DP>(dqp, dq, a.scale, a.d, rows - tile * 32, free, [&](int i) {
             return row_at(as, tile * 32 + i, a.g.dq_row, a.g.dq_head);
         });
@@ -225,6 +352,12 @@ void attn_grad_short(AttnGrad a, int slots) {
         if (n <= (lane & 31) || key < 0 || key >= p.lk)      // a row that is no key's: zeros
 #pragma unroll
             for (int dt = 0; dt < DP / 32; dt++) dk[dt] = dv[dt] = float16v{};
+        // a row with a value that is not finite has such a dq itself, if it sees a key
+        // and is this wave's
+        if (shares > 1 || shift < 0) {
+            watch<DP>(odd, dk);
+            watch<DP>(odd, dv);
+        }
         store_tile<T, DP>(dkp, dk, a.scale, a.d, n, free,
                           [&](int i) { return times<I>(kt * 32 + i, a.g.dk_row); });
         store_tile<T, DP>(dvp, dv, 1.0f, a.d, n, free,
@@ -329,7 +462,7 @@ void attn_grad_short(AttnGrad a, int slots) {
         add_block(ps, ds);
         end_rows(as, 0, fifth);
         end_keys(as, 0, fifth);
-        return;
+        return finite(odd);
     }
 
     // Any other: the first row tile that sees a key of tile kt; the keys' part, kt by
@@ -416,6 +549,16 @@ void attn_grad_short(AttnGrad a, int slots) {
         }
         end_keys(as, kt, lds[pair ^ 2]);     // the next tile is on its way to the others
     }
+    return finite(odd);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1)
+void attn_grad_short(AttnGrad a, int slots) {
+    __shared__ __align__(256) uint16_t lds[4][kShortLds<DP>];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool plain = grad_short<T, DP>(a, slots, lds[wave]);
+    if (__builtin_expect(__any(!plain), 0)) mend_short<T>(arguments<AttnGrad>(), block_number() * 4 + wave);
 }
 
 // Long sequences, rows: a block of four waves owns 128 rows of one key head; keys
@@ -514,7 +657,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, i
         work(Const<0>{}, k0);
         if (k0 + KB < keys) work(Const<1>{}, k0 + KB);
     }
+    const uint32_t bad = not_finite<DP>(dq);
     store_row<T, DP>(a.g.dq, t * a.g.dq_row + head * a.g.dq_head, dq, a.scale, a.d, ok);
+    if (__builtin_expect(bad, 0)) mend_long<T, false>(arguments<AttnGrad>(), p, hk, w0, bad);
 }
 
 // Long sequences, keys: a block owns KX * 32 keys of one key head, a wave 32 of
@@ -527,8 +672,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_grad_q_tiles(AttnGrad a, i
 // the registers one tile ahead of their use. Rows beyond the last repeat it with
 // lse +inf, which makes their P and dS 0. No unit is full: the matrix cores are busy
 // 49 % of the time, the vector instructions 28 %, and eight waves wait at one barrier
-// for a third of theirs; with heads of 128 twelve registers are spilled. 32 heads of 128
-// over 8, five sequences of 700 to 4,801 in 0.74 ms, 0.84 PFLOP/s.
+// for a third of theirs. 32 heads of 128 over 8, five sequences of 700 to 4,801 in 0.74 ms, 0.84 PFLOP/s.
 template <typename T, int DP, int KX>
 __global__ __launch_bounds__(KX * 128, KX == 4 || DP <= 64 ? 2 : 1) void attn_grad_kv_tiles(AttnGrad a, int slots) {
     constexpr int RB = 64, KEYS = KX * 32, WAVES = KX * 2;
@@ -720,8 +864,10 @@ __global__ __launch_bounds__(KX * 128, KX == 4 || DP <= 64 ? 2 : 1) void attn_gr
             }
         }
     const int64_t kr = s0 + tile * KEYS + kx * 32 + (lane & 31);
+    const uint32_t bad = not_finite<DP>(dk) | not_finite<DP>(dv);
     store_row<T, DP>(a.g.dk, kr * a.g.dk_row + hk * a.g.dk_head, dk, a.scale, a.d, kr < s1);
     store_row<T, DP>(a.g.dv, kr * a.g.dv_row + hk * a.g.dv_head, dv, 1.0f, a.d, kr < s1);
+    if (__builtin_expect(bad, 0)) mend_long<T, true>(arguments<AttnGrad>(), p, hk, wkey0, bad);
 }
 
 template <typename T, int DP>

@@ -370,9 +370,7 @@ def attention(q, k, v, cu_q, cu_k=None, *, k_lens=None, scale=None, return_lse=F
 
     Returns o like q, or (o, lse) with return_lse: lse fp32 [Hq, Tq], -inf
     where no key is seen; it carries no gradient. A key or value that is not
-    finite, in a place that a query does not see, is kept from it beyond its
-    sequence's length, but reaches queries up to 94 places before its own within
-    it. Probabilities are rounded to the tensors' type for the product with v;
+    finite reaches only queries that see it. Probabilities are rounded to the tensors' type for the product with v;
     sums and statistics are held in fp32."""
     _check_attention(q, k, v, cu_q, cu_k, k_lens, scale)
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)

@@ -50,11 +50,9 @@ extern "C" {
  * cu_q[0] is 0. Queries are the last ones of the keys: query i of lq sees
  * keys 0 .. i + lk - lq. A query that sees no key, and a query row in no
  * sequence, give o = 0 and lse = -inf. Offsets out of order or out of range
- * are clamped into the tensors. Within a sequence's keys a
- * value that is not finite also reaches queries that do not see it, up to 94
- * places before it (a masked probability is a 0 in a matrix product). In the
- * gradient so does a key, and a query or output gradient reaches keys that it does
- * not see, up to 62 places after it.
+ * are clamped into the tensors. A key or value that is not finite reaches only
+ * queries that see it, and in the gradient a query or output gradient only keys
+ * that it sees; near one a call takes longer.
  *
  * lse (may be null for the forward) [hq, tq] fp32: log of the sum of
  * exp(scale q.k) over the visible keys. o_low (may be null): what rounding o to

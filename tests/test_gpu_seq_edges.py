@@ -240,3 +240,105 @@ def test_attention_empty_tensors_of_any_layout(ops):
     g = ops.attention_grad(odd(0, 4), q, k, k, odd(0, 4), lse, cu([0]), cu([5]))
     assert [x.shape for x in g] == [q.shape, k.shape, k.shape]
     assert not any(bool(x.any()) for x in g)
+
+
+# ------------------------------------------------------------- hidden values
+
+# (queries, keys) of sequences, heads, head size, type: every kernel and split, with
+# queries that see no key among them
+HIDDEN = [
+    ([(40, 40), (9, 9), (64, 64), (33, 33)], 2, 2, 64, BF),        # short, formed once
+    ([(31, 31), (20, 20), (64, 64), (7, 7)], 8, 2, 64, FP),        # short, up to 256 rows
+    ([(60, 40), (10, 64), (30, 50), (5, 3)], 4, 2, 40, BF),
+    ([(100, 100), (3, 3), (2, 2), (5, 5)], 16, 1, 32, BF),         # rows of many waves
+    ([(25, 25), (64, 64), (50, 50)], 3, 1, 128, FP),
+    ([(300, 300), (140, 140), (97, 97)], 4, 2, 64, BF),            # long
+    ([(260, 260), (200, 200)], 8, 1, 128, FP),
+    ([(90, 200), (150, 100), (130, 130)], 4, 1, 96, BF),
+    ([(129, 129)] * 40, 16, 8, 128, BF),                           # blocks of 128 keys
+    ([(5, 1500), (2, 900), (40, 700)], 8, 2, 64, BF),              # few rows, split
+    ([(3, 1111), (7, 600)], 4, 1, 128, FP),
+    ([(6, 300), (2, 260)], 32, 8, 96, BF),
+]
+
+
+def planted(x, rows, value, seed):
+    """x with `value` in one column of each of its `rows`, in some of its heads."""
+    y = x.clone()
+    g = torch.Generator().manual_seed(seed)
+    for r in rows:
+        h = int(torch.randint(x.shape[1], (1,), generator=g))
+        y[r, h, int(torch.randint(x.shape[2], (1,), generator=g))] = value
+    return y
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("pairs,hq,hkv,d,dtype", HIDDEN)
+def test_hidden_values_do_not_reach(ops, pairs, hq, hkv, d, dtype, value):
+    """A key or value that is not finite leaves the outputs and gradients of queries
+    before it as they are without it, and a query or output gradient those of keys
+    after it: all of them, to the bounds of finite inputs."""
+    _say("hidden", pairs[:4], hq, hkv, d, dtype, value)
+    lq, lk = [a for a, _ in pairs], [b for _, b in pairs]
+    cq = cu(lq)
+    ck = cq if lq == lk else cu(lk)
+    q, do = (normal((sum(lq), hq, d), dtype, i) for i in (1, 2))
+    k, v = (normal((sum(lk), hkv, d), dtype, i) for i in (3, 4))
+    r = ref.attention(q, k, v, cq, ck, do=do)
+    q_at = torch.repeat_interleave(torch.arange(len(lq)), torch.tensor(lq))
+    k_at = torch.repeat_interleave(torch.arange(len(lk)), torch.tensor(lk))
+    # what query row i sees: keys of its sequence up to number lim (within it)
+    lim = torch.cat([torch.arange(a) + b - a for a, b in pairs])
+    number = torch.cat([torch.arange(b) for _, b in pairs])
+    sees = (q_at[:, None] == k_at[None]) & (number[None] <= lim[:, None])
+    G = hq // hkv
+
+    def run(q, k, v, do):
+        o, lse = ops.attention(q, k, v, cq, ck, return_lse=True)
+        assert torch.equal(o.isnan(), ops.attention(q, k, v, cq, ck).isnan())
+        return (o, lse) + ops.attention_grad(do, q, k, v, o, lse, cq, ck)
+
+    def hold(got, name, clean):
+        """Checks the elements that nothing visible makes other than finite."""
+        x = got.detach().cpu().double()
+        assert bool(x[clean].isfinite().all()), name
+        check(name, torch.where(clean, x, r[name]), r[name], r[name + "_tol"])
+
+    # the last keys of each sequence, and one that half of the queries see
+    keys, rows = [], []
+    for b, n in enumerate(lk):
+        keys += sorted({sum(lk[:b]) + n - 1, sum(lk[:b]) + max(n - 1 - min(lq[b], n) // 2, 0)})
+    for b, n in enumerate(lq):
+        rows += sorted({sum(lq[:b]), sum(lq[:b]) + n // 3, sum(lq[:b]) + n // 2})
+    for name, x, at in (("k", k, keys), ("v", v, keys), ("q", q, rows), ("do", do, rows)):
+        a = dict(q=q, k=k, v=v, do=do)
+        a[name] = planted(x, at, value, len(at))
+        odd = ~a[name].cpu().float().isfinite()
+        o, lse, dq, dk, dv = run(**a)
+        if name in "kv":
+            # [row, key head]: sees such a place; with a value only its columns of o
+            hit = (sees.double() @ odd.any(2).double()) > 0
+            col = (sees.double() @ odd.double().flatten(1)).view(len(q_at), hkv, d) > 0
+            row_hit = hit.repeat_interleave(G, 1)[..., None].expand(-1, -1, d)
+            o_hit = col.repeat_interleave(G, 1) if name == "v" else row_hit
+            hold(o, "o", ~o_hit)
+            hold(dq, "dq", ~row_hit)
+            if name == "v":
+                assert not bool(o.cpu()[o_hit].isfinite().any())
+                hold(dv, "dv", torch.ones_like(r["dv"], dtype=torch.bool))
+                check("lse", lse, r["lse"], r["lse_tol"])
+            # a key is clean when no row that sees it is hit
+            key_hit = (sees.double().T @ hit.double()) > 0
+            hold(dk, "dk", ~key_hit[..., None].expand(-1, -1, d))
+            if name == "k":
+                hold(dv, "dv", ~key_hit[..., None].expand(-1, -1, d))
+        else:
+            hit = odd.any(2)                                     # [row, head]
+            by_head = hit.view(len(q_at), hkv, G).any(2)
+            key_hit = (sees.double().T @ by_head.double()) > 0
+            row_hit = hit[..., None].expand(-1, -1, d)
+            hold(o, "o", ~row_hit if name == "q" else torch.ones_like(row_hit))
+            hold(dq, "dq", ~row_hit)
+            clean = ~key_hit[..., None].expand(-1, -1, d)
+            hold(dk, "dk", clean)
+            hold(dv, "dv", clean)

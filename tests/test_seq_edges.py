@@ -31,6 +31,23 @@ def test_assembly_names_what_it_overwrites():
     assert found >= 3
 
 
+def test_arguments_are_found_by_kernels_alone():
+    """A called function has no pointer of its own to the kernel's arguments: where
+    one is formed, the function is a kernel (or is inlined without fail)."""
+    found = 0
+    for path in sorted(CSRC.glob("seq_*")):
+        function = ""
+        for line in path.read_text().splitlines():
+            if re.match(r"(template <[^>]*> )?(__global__|__device__)", line):
+                function = line
+            if "__builtin_amdgcn_kernarg_segment_ptr" in line:
+                assert "always_inline" in function, (path.name, function)
+            elif re.search(r"\barguments<\w+>\(\)", line) and line != function:
+                assert function.startswith("__global__"), (path.name, function)
+                found += 1
+    assert found >= 6
+
+
 # ------------------------------------------------------------------- refusals
 
 class _Gpu(torch.Tensor):
