@@ -183,19 +183,19 @@ __device__ inline Row run_rows(const Attn &a, const Place &p, int hk, int tile, 
 // way of LDS and whole rows stored. 16,384 sequences of 1 to 31, 8 heads of 64 over
 // 4, take 191 us (4.2 TB/s); with K to registers 207, with the output stored as 32
 // bytes of each row 205.
-// Returns a bit for each tile with a sum that is not finite.
+// Returns whether all sums are finite.
 template <typename T, int DP, typename I>
-__device__ inline uint32_t wave_tiles(const Attn &a, const Place &p, int hk, int first, uint16_t *kt,
+__device__ inline bool wave_tiles(const Attn &a, const Place &p, int hk, int first, uint16_t *kt,
                                   uint16_t *vt) {
     const int rows = p.lq * a.G;
     const bool low = keeps_low(a, rows);
     const float inv = 1.0f / (float)a.G;
-    uint32_t bad = 0;
+    float odd = 0.0f;
     for (int tile = first; tile < first + kShortRows / 32 && tile * 32 < rows; tile++) {
         float16v o[DP / 32];
         float m, l;
         const Row r = run_rows<T, DP, false, I>(a, p, hk, tile, 0, p.lk, kt, vt, o, m, l);
-        if (not_finite<DP>(o) & row_bits(finite(l))) bad |= 1 << (tile - first);
+        watch<DP>(odd, o);
         if (low) {
             store_out<T, DP>(a, r.t, r.head, o, m, l, r.ok, true);
             continue;
@@ -207,7 +207,7 @@ __device__ inline uint32_t wave_tiles(const Attn &a, const Place &p, int hk, int
         });
         store_lse(a, r.t, r.head, m, l, r.ok);
     }
-    return bad;
+    return finite(odd);
 }
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void attn_wave(Attn a, int slots) {
@@ -222,14 +222,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void attn_wave(Attn a, int s
     const Place p = place_of(a, b, f.start, f.end);
     const int first = (slot - slot_of(p.q0, a.G, kShortRows, b)) * (kShortRows / 32);
     if (first < 0) return;
-    uint32_t bad;
+    bool plain;
     if (a.near && p.lq * a.G <= kNear && p.lk <= kNear)
-        bad = wave_tiles<T, DP, uint32_t>(a, p, hk, first, kt, vt);
+        plain = wave_tiles<T, DP, uint32_t>(a, p, hk, first, kt, vt);
     else
-        bad = wave_tiles<T, DP, int64_t>(a, p, hk, first, kt, vt);
-    for (; __builtin_expect(bad, 0); bad &= bad - 1)
-        mend_out<T>(arguments<Attn>(), p, hk, (first + __builtin_ctz(bad)) * 32, ~0u, 0, p.lk,
-                    nullptr, nullptr, 0);
+        plain = wave_tiles<T, DP, int64_t>(a, p, hk, first, kt, vt);
+    if (__builtin_expect(__any(!plain), 0))
+        for (int tile = first; tile < first + kShortRows / 32; tile++)
+            mend_out<T>(arguments<Attn>(), p, hk, tile * 32, ~0u, 0, p.lk, nullptr, nullptr, 0);
 }
 
 // Long sequences: a block of WAVES waves owns WAVES * 32 rows of one key head;

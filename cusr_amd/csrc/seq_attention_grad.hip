@@ -40,6 +40,12 @@ __device__ inline void put_stat(const AttnGrad &a, int64_t at, float lse2, float
     }
 }
 
+__device__ inline uint32_t pinned(int64_t x) {
+    uint32_t y = (uint32_t)x;
+    asm("" : "+s"(y));
+    return y;
+}
+
 // A key head's rows and keys, for what seq_hidden.h does with them.
 template <typename T> struct HeadRows {
     const AttnGrad &a;
@@ -60,6 +66,8 @@ template <typename T> struct HeadRows {
         return (const uint16_t *)a.v + (p.k0 + key) * a.v_row + hk * a.v_head;
     }
     __device__ float lse2(int row) const { return a.lse[head(row) * a.tq + t(row)] * kLog2e; }
+    // from o and what rounding took from it; short sequences keep only o: within the
+    // bounds that follow from its rounding
     __device__ float delta(int row) const {
         const uint16_t *y = d_o(row);
         float s = dot<T>((const uint16_t *)a.o + t(row) * a.o_row + head(row) * a.o_head, y, a.d);
@@ -213,6 +221,17 @@ __device__ inline bool grad_short(const AttnGrad &a, int slots, uint16_t *lds_wa
     uint16_t *dqp = (uint16_t *)a.g.dq + p.q0 * a.g.dq_row + hk * a.G * a.g.dq_head;
     const uint16_t *dop = (const uint16_t *)a.g.d_o + p.q0 * a.g.do_row + hk * a.G * a.g.do_head;
 
+    // Strides in 32 bits, each in a register of its own: as parts of the arguments they
+    // would be laid by and fetched 16 at a time.
+    const uint32_t n_q_row = pinned(a.q_row), n_q_head = pinned(a.q_head), n_k_row = pinned(a.k_row),
+                   n_v_row = pinned(a.v_row), n_do_row = pinned(a.g.do_row),
+                   n_do_head = pinned(a.g.do_head), n_dq_row = pinned(a.g.dq_row),
+                   n_dq_head = pinned(a.g.dq_head), n_dk_row = pinned(a.g.dk_row),
+                   n_dv_row = pinned(a.g.dv_row);
+    auto step = [](auto as, int64_t wide, uint32_t near) {
+        if constexpr (sizeof(as) == 4) return (int64_t)near;
+        else return wide;
+    };
     // tiles to LDS tiles, past the registers. Beyond the last row or key, the last
     // again: it is masked, by its last visible key -1
     auto row_at = [&](auto as, int i, int64_t step, int64_t head) {
@@ -221,19 +240,22 @@ __device__ inline bool grad_short(const AttnGrad &a, int slots, uint16_t *lds_wa
         return times<I>(qi, step) + times<I>(row - qi * a.G, head);
     };
     auto copy_q = [&](auto as, int tile, int to) {
-        copy_tile<DP>(qp, a.d, lds_at + to * 64 * S,
-                      [&](int i) { return row_at(as, tile * 32 + i, a.q_row, a.q_head); });
+        copy_tile<DP>(qp, a.d, lds_at + to * 64 * S, [&](int i) {
+            return row_at(as, tile * 32 + i, step(as, a.q_row, n_q_row), step(as, a.q_head, n_q_head));
+        });
     };
     auto copy_do = [&](auto as, int tile, int to) {
-        copy_tile<DP>(dop, a.d, lds_at + to * 64 * S,
-                      [&](int i) { return row_at(as, tile * 32 + i, a.g.do_row, a.g.do_head); });
+        copy_tile<DP>(dop, a.d, lds_at + to * 64 * S, [&](int i) {
+            return row_at(as, tile * 32 + i, step(as, a.g.do_row, n_do_row),
+                          step(as, a.g.do_head, n_do_head));
+        });
     };
     auto copy_keys = [&](auto as, int k0, int end, int tk, int tv) {
         typedef decltype(as) I;
         copy_tile<DP>(kp, a.d, lds_at + tk * 64 * S,
-                      [&](int i) { return times<I>(min(k0 + i, end - 1), a.k_row); });
+                      [&](int i) { return times<I>(min(k0 + i, end - 1), step(as, a.k_row, n_k_row)); });
         copy_tile<DP>(vp, a.d, lds_at + tv * 64 * S,
-                      [&](int i) { return times<I>(min(k0 + i, end - 1), a.v_row); });
+                      [&](int i) { return times<I>(min(k0 + i, end - 1), step(as, a.v_row, n_v_row)); });
     };
     // keys that a tile of rows sees
     auto seen_by = [&](int tile) {
@@ -262,7 +284,8 @@ __device__ inline bool grad_short(const AttnGrad &a, int slots, uint16_t *lds_wa
     auto end_rows = [&](auto as, int tile, uint16_t *free) {
         watch<DP>(odd, dq);
         store_tile<T, DP>(dqp, dq, a.scale, a.d, rows - tile * 32, free, [&](int i) {
-            return row_at(as, tile * 32 + i, a.g.dq_row, a.g.dq_head);
+            return row_at(as, tile * 32 + i, step(as, a.g.dq_row, n_dq_row),
+                          step(as, a.g.dq_head, n_dq_head));
         });
     };
     auto products = [&](int k0, int tk, int tv, float16v &s, float16v &dp) {
@@ -359,9 +382,9 @@ __device__ inline bool grad_short(const AttnGrad &a, int slots, uint16_t *lds_wa
             watch<DP>(odd, dv);
         }
         store_tile<T, DP>(dkp, dk, a.scale, a.d, n, free,
-                          [&](int i) { return times<I>(kt * 32 + i, a.g.dk_row); });
+                          [&](int i) { return times<I>(kt * 32 + i, step(as, a.g.dk_row, n_dk_row)); });
         store_tile<T, DP>(dvp, dv, 1.0f, a.d, n, free,
-                          [&](int i) { return times<I>(kt * 32 + i, a.g.dv_row); });
+                          [&](int i) { return times<I>(kt * 32 + i, step(as, a.g.dv_row, n_dv_row)); });
     };
 
     // Up to 64 rows and keys, the first 32 rows with up to 32 keys: P and dS are formed
