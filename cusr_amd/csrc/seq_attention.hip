@@ -20,19 +20,22 @@ __device__ inline void store_out(const Attn &a, int t, int head, const float16v 
     store_lse(a, t, head, m, l, ok);
 }
 
-// Outputs of rows first + r of a sequence, for the r of `bad`, where hidden keys among
-// key0 .. key1-1 reached them; of a chunk of keys, its unscaled sums, to sums + row *
-// width, for the maximum and sum at stat + 2 row.
+// Outputs of rows first + r of a sequence, for the r of `bad`, and so on every `step` rows
+// before `last`, where hidden keys among key0 .. key1-1 reached them; of a chunk of keys,
+// its unscaled sums, to sums + row * width, for the maximum and sum at stat + 2 row.
 template <typename T>
 __device__ __attribute__((noinline)) void mend_out(Arguments<Attn> args, Place place, int hk,
-                                                   int first, uint32_t bad, int key0, int key1,
-                                                   float *sums, const float *stat, int width) {
+                                                   int first, int last, int step, uint32_t bad,
+                                                   int key0, int key1, float *sums,
+                                                   const float *stat, int width) {
     const Attn &a = *(const Attn *)uniform(args);
     const Place p = uniform(place);
-    hk = uniform(hk), first = uniform(first), bad = uniform((int)bad);
+    hk = uniform(hk), first = uniform(first), last = uniform(last), step = uniform(step);
+    bad = uniform((int)bad);
     key0 = uniform(key0), key1 = uniform(key1), width = uniform(width);
     sums = uniform(sums), stat = uniform(stat);
     const int lane = threadIdx.x & 63, rows = p.lq * a.G;
+    last = min(last, rows);
     auto k = [&](int j) {
         return (const uint16_t *)a.k + (p.k0 + j) * a.k_row + hk * a.k_head;
     };
@@ -40,8 +43,12 @@ __device__ __attribute__((noinline)) void mend_out(Arguments<Attn> args, Place p
         return (const uint16_t *)a.v + (p.k0 + j) * a.v_row + hk * a.v_head;
     };
     wait_copies<0>();                // stores on their way come first
-    for (; bad && first + __builtin_ctz(bad) < rows; bad &= bad - 1) {
-        const int row = first + __builtin_ctz(bad);
+    uint32_t left = bad;
+    for (;; left &= left - 1) {
+        while (first < last && !left) first += step, left = bad;
+        if (first >= last) return;
+        const int row = first + __builtin_ctz(left);
+        if (row >= last) return;
         const int qi = row / a.G, head = hk * a.G + row % a.G;
         const int end = min(qi + p.lk - p.lq + 1, key1);         // beyond its last key
         if (!hidden_cause<T>(v, a.d, max(end, key0), min(end + kReach, key1),
@@ -228,8 +235,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void attn_wave(Attn a, int s
     else
         plain = wave_tiles<T, DP, int64_t>(a, p, hk, first, kt, vt);
     if (__builtin_expect(__any(!plain), 0))
-        for (int tile = first; tile < first + kShortRows / 32; tile++)
-            mend_out<T>(arguments<Attn>(), p, hk, tile * 32, ~0u, 0, p.lk, nullptr, nullptr, 0);
+        mend_out<T>(arguments<Attn>(), p, hk, first * 32, first * 32 + kShortRows, 32, ~0u, 0, p.lk,
+                    nullptr, nullptr, 0);
 }
 
 // Long sequences: a block of WAVES waves owns WAVES * 32 rows of one key head;
@@ -349,7 +356,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_tiles(Attn a, int slots) {
     const uint32_t bad = not_finite<DP>(o) & row_bits(finite(l));
     store_out<T, DP>(a, p.q0 + qi, head, o, m, l, ok, keeps_low(a, rows));
     if (__builtin_expect(bad, 0))
-        mend_out<T>(arguments<Attn>(), p, hk, w0, bad, 0, p.lk, nullptr, nullptr, 0);
+        mend_out<T>(arguments<Attn>(), p, hk, w0, w0 + 32, 32, bad, 0, p.lk, nullptr, nullptr, 0);
 }
 
 // Few rows over many keys (single tokens over a cache). A sequence's keys are
@@ -415,9 +422,8 @@ __global__ __launch_bounds__(256, 2) void attn_step(Attn a, Step st) {
         }
     }
     if (__builtin_expect(bad, 0))
-        for (int tile = blockIdx.y; tile * 32 < rows; tile += st.tiles)
-            mend_out<T>(arguments<Attn>(), p, hk, tile * 32, ~0u, key0, key1,
-                        split ? st.o + first * DP : nullptr, split ? st.ml + 2 * first : nullptr, DP);
+        mend_out<T>(arguments<Attn>(), p, hk, blockIdx.y * 32, rows, st.tiles * 32, ~0u, key0, key1,
+                    split ? st.o + first * DP : nullptr, split ? st.ml + 2 * first : nullptr, DP);
 }
 
 // Joins the chunks of a split sequence: a wave to a row of the output, which
