@@ -59,7 +59,8 @@ DEVICE_FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-ffp-co
 # are fused.
 SEQ_FLAGS = [f for f in DEVICE_FLAGS if f != "-ffp-contract=off"
              and "structurizecfg" not in f and f != "-mllvm"]
-SEQ_SOURCES = ("seq_rotary", "seq_policy_loss", "seq_attention", "seq_attention_grad")
+SEQ_SOURCES = ("seq_rotary", "seq_policy_loss", "seq_attention", "seq_attention_grad", "seq_norm",
+               "seq_embedding", "seq_int8", "seq_logprobs")
 
 FIT_VARIANTS = [("double", 0, "f64_fwd"), ("double", 1, "f64_rev"),
                 ("float", 0, "f32_fwd"), ("float", 1, "f32_rev")]

@@ -1,0 +1,470 @@
+// seq_embedding.hip -- rows of a table by token, and the table's gradient
+// (include/cusr_seq.h, seq_embedding, seq_embedding_grad).
+//
+// The bound is memory. The lookup reads a row and writes it. The gradient adds the rows
+// of each token: tokens are sorted first (stably, by counting digits), so that a row of
+// the table is one run of places, added in the order of the tokens, with nothing
+// left to atomics. Runs are cut into chunks of equal length, however many tokens a row
+// has: what a run leaves in a chunk that it only passes through goes to a slot, and
+// slots are joined in order at the end.
+#include "seq_rows.h"
+
+namespace seq {
+
+template <typename T, int W> struct Cells;       // W values side by side
+template <typename T> struct Cells<T, 8> : Eight<T> {};
+template <typename T> struct Cells<T, 1> {
+    T a;
+    __device__ void load(const T *p) { a = *p; }
+    __device__ void zero() { a = (T)0.0f; }
+    __device__ void get(float *f) const { f[0] = (float)a; }
+    static __device__ void put(T *p, const float *f) { *p = (T)f[0]; }
+};
+template <int W> __device__ inline void put_cells(void *p, int dtype, int64_t at, const float *f) {
+    if constexpr (W == 8) put8(p, dtype, at, f);
+    else put1(p, dtype, at, f[0]);
+}
+
+// log2 of the threads of a row of `parts` parts
+inline int group_log(int64_t parts) {
+    int g = 0;
+    while (g < 8 && (1 << g) < parts) g++;
+    return g;
+}
+
+// 2^g threads a token, a part of its row each at a time
+template <typename T, int W>
+__global__ __launch_bounds__(256) void embed_rows(SeqEmbedding p, int g) {
+    const int64_t t = (int64_t)block_number() * (256 >> g) + (threadIdx.x >> g);
+    if (t >= p.tokens) return;
+    const int parts = (int)(p.width / W), lane = threadIdx.x & ((1 << g) - 1);
+    const int64_t id = get_id(p.ids, p.ids_64, t);
+    const bool in = id >= 0 && id < p.rows;
+    const T *row = (const T *)p.table + (in ? id : 0) * p.table_row;
+    const float scale = in ? p.scale : __builtin_nanf("");
+#pragma unroll 4
+    for (int at = lane; at < parts; at += 1 << g) {
+        Cells<T, W> v;
+        v.zero();
+        if (in) v.load(row + at * W);            // a table may have no row at all
+        float f[W];
+        v.get(f);
+#pragma unroll
+        for (int j = 0; j < W; j++) f[j] *= scale;
+        put_cells<W>(p.out, p.out_dtype, t * p.out_row + at * W, f);
+    }
+}
+
+// ----------------------------------------------------------------------- sort
+
+// Tokens are sorted by digits of at most 9 bits, the lowest first, each time in two
+// launches: the digits of each tile are counted; then every tile's block adds up the
+// counts of the tiles before it and of the lower digits, and moves its keys to their
+// places. Tokens outside the table become the key `rows`, behind all others.
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
+constexpr int kSortSub = kSortThreads * 4;       // keys of a block at a time
+constexpr int kSortTiles = 256, kDigits = 512;
+
+struct Sort {
+    const void *ids;                             // first time round; then keys and places
+    const uint32_t *keys, *places;
+    uint32_t *keys_to, *places_to, *counts;
+    uint32_t rows, tile;                         // tile: keys of a block
+    uint32_t tokens;
+    int ids_64, shift, bits, tiles;
+    __device__ uint32_t key(uint32_t t) const {
+        if (!ids) return keys[t];
+        const int64_t id = get_id(ids, ids_64, t);
+        return id >= 0 && id < (int64_t)rows ? (uint32_t)id : rows;
+    }
+    __device__ int digit(uint32_t key) const { return (key >> shift) & ((1u << bits) - 1); }
+};
+
+__global__ __launch_bounds__(kSortThreads) void sort_count(Sort s) {
+    __shared__ uint32_t n[kDigits];
+    n[threadIdx.x] = 0;
+    __syncthreads();
+    const uint64_t a = (uint64_t)blockIdx.x * s.tile;
+    const uint64_t b = a + s.tile < s.tokens ? a + s.tile : s.tokens;
+    for (uint64_t t = a + threadIdx.x; t < b; t += kSortThreads)
+        atomicAdd(&n[s.digit(s.key((uint32_t)t))], 1u);     // a count: any order
+    __syncthreads();
+    if ((int)threadIdx.x < 1 << s.bits) s.counts[(blockIdx.x << s.bits) + threadIdx.x] = n[threadIdx.x];
+}
+
+__global__ __launch_bounds__(kSortThreads) void sort_move(Sort s) {
+    __shared__ uint32_t wave_n[kSortWaves][kDigits];
+    __shared__ uint32_t base[kDigits], total[kSortThreads], before[kSortThreads];
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    const int digits = 1 << s.bits, d = tid & (digits - 1);
+    // counts of digit d in all tiles and in those before this one, by several threads
+    uint32_t all = 0, prior = 0;
+#pragma unroll 8
+    for (int t = tid >> s.bits; t < s.tiles; t += kSortThreads >> s.bits) {
+        const uint32_t c = s.counts[(t << s.bits) + d];
+        all += c;
+        prior += t < (int)blockIdx.x ? c : 0;
+    }
+    total[tid] = all;
+    before[tid] = prior;
+    __syncthreads();
+    if (tid < digits)
+        for (int t = tid + digits; t < kSortThreads; t += digits) {
+            all += total[t];
+            prior += before[t];
+        }
+    __syncthreads();
+    total[tid] = tid < digits ? all : 0;
+    __syncthreads();
+    uint32_t sum = total[tid];                   // counts of lower digits: a running sum
+    for (int o = 1; o < digits; o *= 2) {
+        const uint32_t add = tid >= o ? total[tid - o] : 0;
+        __syncthreads();
+        sum += add;
+        total[tid] = sum;
+        __syncthreads();
+    }
+    if (tid < digits) base[tid] = sum - all + prior;
+    const uint64_t first = (uint64_t)blockIdx.x * s.tile;
+    const uint64_t end = first + s.tile < s.tokens ? first + s.tile : s.tokens;
+    for (uint64_t at = first; at < end; at += kSortSub) {
+        for (int i = tid; i < kSortWaves * kDigits; i += kSortThreads) (&wave_n[0][0])[i] = 0;
+        __syncthreads();
+        uint32_t key[4], rank[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {            // a wave's 256 keys in order, 64 at a time
+            const uint64_t t = at + wave * 256 + r * 64 + lane;
+            const bool is = t < end;
+            key[r] = is ? s.key((uint32_t)t) : 0;
+            const int x = s.digit(key[r]);
+            uint64_t same = __ballot(is);
+            for (int b = 0; b < s.bits; b++) {
+                const uint64_t set = __ballot((x >> b) & 1);
+                same &= (x >> b) & 1 ? set : ~set;
+            }
+            const uint32_t lower = __popcll(same & ((1ull << lane) - 1));
+            const uint32_t have = wave_n[wave][x];
+            wave_sync();
+            if (is && lower == 0) wave_n[wave][x] = have + __popcll(same);
+            wave_sync();
+            rank[r] = have + lower;
+        }
+        __syncthreads();
+        if (tid < digits) {
+            uint32_t run = base[tid];
+#pragma unroll
+            for (int w = 0; w < kSortWaves; w++) {
+                const uint32_t n = wave_n[w][tid];
+                wave_n[w][tid] = run;
+                run += n;
+            }
+            base[tid] = run;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const uint64_t t = at + wave * 256 + r * 64 + lane;
+            if (t >= end) continue;
+            const uint32_t to = wave_n[wave][s.digit(key[r])] + rank[r];
+            s.keys_to[to] = key[r];
+            s.places_to[to] = s.ids ? (uint32_t)t : s.places[t];
+        }
+        __syncthreads();
+    }
+}
+
+// ----------------------------------------------------------------------- sums
+
+struct Runs {
+    const uint32_t *keys, *places;               // sorted
+    float *slots;                                // two rows of `pitch` a chunk
+    int64_t chunks, pitch, sum_blocks;
+    int chunk, g, slabs, zero_rows;
+};
+
+// Whether row v has a token: the first key not below v
+__device__ inline bool has_token(const uint32_t *keys, uint32_t n, uint32_t v) {
+    uint32_t lo = 0, hi = n;
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (keys[mid] < v) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo < n && keys[lo] == v;
+}
+
+// The first blocks: 2^g threads add a chunk's rows, a slab of columns at a time. The
+// others write zeros where a row of the table has no token.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void embed_sum(SeqEmbeddingGrad p, Runs r) {
+    constexpr int AHEAD = 8;                     // rows on their way
+    __shared__ bool present[256];
+    const uint32_t n = (uint32_t)p.tokens, V = (uint32_t)p.rows;
+    const int64_t block = block_number();
+    if (block >= r.sum_blocks) {
+        const int64_t v0 = (block - r.sum_blocks) * r.zero_rows;
+        if (v0 >= p.rows) return;                // the launch's last numbers
+        const int rows = (int)(p.rows - v0 < r.zero_rows ? p.rows - v0 : r.zero_rows);
+        if ((int)threadIdx.x < rows)
+            present[threadIdx.x] = has_token(r.keys, n, (uint32_t)(v0 + threadIdx.x));
+        __syncthreads();
+        const float zero[W] = {};
+        const int parts = (int)(p.width / W);
+        for (int i = threadIdx.x; i < rows * parts; i += 256) {
+            const int row = i / parts;
+            if (!present[row])
+                put_cells<W>(p.dtable, p.out_dtype,
+                             (v0 + row) * p.dtable_row + (int64_t)(i - row * parts) * W, zero);
+        }
+        return;
+    }
+    const int groups = 256 >> r.g, lane = threadIdx.x & ((1 << r.g) - 1);
+    const int slab = (int)(block % r.slabs);
+    const int64_t c = block / r.slabs * groups + (threadIdx.x >> r.g);
+    const int64_t col = ((int64_t)slab * (1 << r.g) + lane) * W;
+    if (c >= r.chunks || col >= p.width) return;
+    const uint32_t a = (uint32_t)(c * r.chunk);
+    const uint32_t b = n - a < (uint32_t)r.chunk ? n : a + r.chunk;
+    const uint32_t last = a ? r.keys[a - 1] : 0xffffffffu, next = b < n ? r.keys[b] : 0xffffffffu;
+    const T *x = (const T *)p.d_out + col;
+    float sum[W] = {};
+    uint32_t run = r.keys[a];
+    bool from_before = run == last;
+    auto flush = [&](bool goes_on) {
+        if (run >= V) return;
+        if (from_before || goes_on) {
+            Cells<float, W>::put(r.slots + (2 * c + !from_before) * r.pitch + col, sum);
+        } else {
+            float f[W];
+#pragma unroll
+            for (int j = 0; j < W; j++) f[j] = sum[j] * p.scale;
+            put_cells<W>(p.dtable, p.out_dtype, run * p.dtable_row + col, f);
+        }
+    };
+    for (uint32_t at = a; at < b; at += AHEAD) {
+        uint32_t key[AHEAD];
+        Cells<T, W> v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            key[i] = at + i < b ? r.keys[at + i] : V;
+            v[i].zero();
+            if (key[i] < V) v[i].load(x + r.places[at + i] * p.dout_row);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            if (at + i >= b) break;
+            if (key[i] != run) {
+                flush(false);
+                run = key[i];
+                from_before = false;
+#pragma unroll
+                for (int j = 0; j < W; j++) sum[j] = 0.0f;
+            }
+            float f[W];
+            v[i].get(f);
+#pragma unroll
+            for (int j = 0; j < W; j++) sum[j] += f[j];
+        }
+    }
+    flush(run == next);
+}
+
+// Joins the slots of a run that begins in a chunk and goes on: 32 columns at a time, each
+// by 8 threads.
+__global__ __launch_bounds__(256) void embed_join(SeqEmbeddingGrad p, Runs r) {
+    __shared__ float part[8][33];
+    const int64_t c = block_number();
+    if (c >= r.chunks - 1) return;
+    const uint32_t a = (uint32_t)(c * r.chunk), b = a + r.chunk;      // not the last chunk
+    const uint32_t run = r.keys[b - 1];
+    if (run >= (uint32_t)p.rows || r.keys[b] != run) return;
+    if (a && r.keys[a] == run && r.keys[a - 1] == run) return;        // began before
+    // the first chunk that does not begin with the run, past c
+    int64_t lo = c + 1, hi = r.chunks;
+    while (lo < hi) {
+        const int64_t mid = lo + (hi - lo) / 2;
+        if (r.keys[mid * r.chunk] == run) lo = mid + 1;
+        else hi = mid;
+    }
+    const int x = threadIdx.x % 32, g = threadIdx.x / 32;
+    for (int64_t col0 = blockIdx.y * 32ll; col0 < p.width; col0 += gridDim.y * 32ll) {
+        const int64_t col = col0 + x;
+        float s = 0.0f;
+        if (col < p.width) {
+            if (g == 0) s = r.slots[(2 * c + 1) * r.pitch + col];
+#pragma unroll 8
+            for (int64_t k = c + 1 + g; k < lo; k += 8) s += r.slots[2 * k * r.pitch + col];
+        }
+        part[g][x] = s;
+        __syncthreads();
+        if (g == 0 && col < p.width) {
+            s = part[0][x];
+#pragma unroll
+            for (int i = 1; i < 8; i++) s += part[i][x];
+            put1(p.dtable, p.out_dtype, (int64_t)run * p.dtable_row + col, s * p.scale);
+        }
+        __syncthreads();
+    }
+}
+
+__global__ __launch_bounds__(256) void embed_zero(SeqEmbeddingGrad p) {
+    const int64_t v = block_number();
+    if (v >= p.rows) return;
+    for (int64_t j = threadIdx.x; j < p.width; j += 256)
+        put1(p.dtable, p.out_dtype, v * p.dtable_row + j, 0.0f);
+}
+
+// ------------------------------------------------------------------- launches
+
+int check_embedding(const SeqEmbedding *p) {
+    if (!p || p->struct_size != (int32_t)sizeof(SeqEmbedding)) return CO_ERR_NULLARG;
+    if (p->tokens < 0 || p->rows < 0 || p->width < 1) return CO_ERR_NULLARG;
+    if (p->tokens > SEQ_MAX_ROWS || p->rows > SEQ_MAX_ROWS || p->width > SEQ_MAX_WIDTH)
+        return CO_ERR_BOUNDS;
+    if (!float_type(p->dtype) || !float_type(p->out_dtype) || !(fabsf(p->scale) <= 3.4028235e38f))
+        return CO_ERR_DATA;
+    return CO_OK;
+}
+int check_embedding_grad(const SeqEmbeddingGrad *p) {
+    if (!p || p->struct_size != (int32_t)sizeof(SeqEmbeddingGrad)) return CO_ERR_NULLARG;
+    if (p->tokens < 0 || p->rows < 0 || p->width < 1) return CO_ERR_NULLARG;
+    if (p->tokens > SEQ_MAX_ROWS || p->rows > SEQ_MAX_ROWS || p->width > SEQ_MAX_WIDTH)
+        return CO_ERR_BOUNDS;
+    if (!float_type(p->dtype) || !float_type(p->out_dtype) || !(fabsf(p->scale) <= 3.4028235e38f))
+        return CO_ERR_DATA;
+    return CO_OK;
+}
+
+int64_t chunk_of(int64_t tokens) { return tokens <= 1 << 16 ? 32 : (tokens <= 1 << 22 ? 64 : 256); }
+int64_t aligned256(int64_t n) { return (n + 255) / 256 * 256; }
+
+struct GradPlan {
+    int passes, bits;
+    int64_t tile, tiles, chunk, chunks, pitch;
+    int64_t keys, counts, slots, total;          // bytes of one list, of the rest; offsets
+};
+GradPlan grad_plan(const SeqEmbeddingGrad &p) {
+    GradPlan r;
+    int bits = 1;
+    while (bits < 31 && (1ll << bits) <= p.rows) bits++;              // holds `rows` itself
+    r.passes = (bits + 8) / 9;
+    r.bits = (bits + r.passes - 1) / r.passes;
+    const int64_t subs = (p.tokens + kSortSub - 1) / kSortSub;
+    r.tile = (subs + kSortTiles - 1) / kSortTiles * kSortSub;
+    r.tiles = (p.tokens + r.tile - 1) / r.tile;
+    r.chunk = chunk_of(p.tokens);
+    r.chunks = (p.tokens + r.chunk - 1) / r.chunk;
+    r.pitch = (p.width + 7) / 8 * 8;
+    r.keys = aligned256(4 * p.tokens);
+    r.counts = 4 * r.keys;                       // two lists of keys and two of places
+    r.slots = r.counts + 4ll * kSortTiles * kDigits;
+    r.total = r.slots + 8 * r.chunks * r.pitch;
+    return r;
+}
+
+template <typename T, int W> void launch_sum(const SeqEmbeddingGrad &p, Runs r, hipStream_t s) {
+    const int64_t parts = p.width / W;
+    r.g = group_log(parts);
+    r.slabs = (int)((parts + (1 << r.g) - 1) >> r.g);
+    const int groups = 256 >> r.g;
+    r.sum_blocks = (r.chunks + groups - 1) / groups * r.slabs;
+    const int64_t zero = 65536 / p.width;        // rows that make a block's worth of zeros
+    r.zero_rows = (int)(zero < 4 ? 4 : (zero > 256 ? 256 : zero));
+    const int64_t blocks = r.sum_blocks + (p.rows + r.zero_rows - 1) / r.zero_rows;
+    embed_sum<T, W><<<grid_of(blocks, 256), 256, 0, s>>>(p, r);
+}
+template <typename T> void launch_sum(const SeqEmbeddingGrad &p, const Runs &r, hipStream_t s) {
+    const bool eights = p.width % 8 == 0 && in_eights(p.d_out, p.dout_row) &&
+                        in_eights(p.dtable, p.dtable_row);
+    if (eights) launch_sum<T, 8>(p, r, s);
+    else launch_sum<T, 1>(p, r, s);
+}
+
+template <typename T> void launch_embed(const SeqEmbedding &p, hipStream_t s) {
+    const bool eights = p.width % 8 == 0 && in_eights(p.table, p.table_row) &&
+                        in_eights(p.out, p.out_row);
+    const int g = group_log(p.width / (eights ? 8 : 1));
+    const int rows = 256 >> g;
+    const dim3 grid = grid_of((p.tokens + rows - 1) / rows, 256);
+    if (eights) embed_rows<T, 8><<<grid, 256, 0, s>>>(p, g);
+    else embed_rows<T, 1><<<grid, 256, 0, s>>>(p, g);
+}
+
+}  // namespace seq
+
+extern "C" int seq_embedding(const SeqEmbedding *p, void *stream) {
+    const int rc = seq::check_embedding(p);
+    if (rc != CO_OK) return rc;
+    if (p->tokens == 0) return CO_OK;
+    if (!p->ids || (!p->table && p->rows) || !p->out) return CO_ERR_NULLARG;
+    hipStream_t s = (hipStream_t)stream;
+    switch (p->dtype) {
+        case SEQ_FP32: seq::launch_embed<float>(*p, s); break;
+        case SEQ_BF16: seq::launch_embed<__bf16>(*p, s); break;
+        default: seq::launch_embed<_Float16>(*p, s); break;
+    }
+    return seq::launch_status();
+}
+
+extern "C" int64_t seq_embedding_grad_workspace(const SeqEmbeddingGrad *p) {
+    const int rc = seq::check_embedding_grad(p);
+    if (rc != CO_OK) return rc > 0 ? -rc : rc;
+    return p->tokens && p->rows ? seq::grad_plan(*p).total : 0;
+}
+
+extern "C" int seq_embedding_grad(const SeqEmbeddingGrad *p, void *stream) {
+    const int rc = seq::check_embedding_grad(p);
+    if (rc != CO_OK) return rc;
+    if (p->rows == 0) return CO_OK;
+    if (!p->dtable) return CO_ERR_NULLARG;
+    hipStream_t s = (hipStream_t)stream;
+    if (p->tokens == 0) {
+        seq::embed_zero<<<seq::grid_of(p->rows, 256), 256, 0, s>>>(*p);
+        return seq::launch_status();
+    }
+    if (!p->ids || !p->d_out || !p->workspace) return CO_ERR_NULLARG;
+    const seq::GradPlan plan = seq::grad_plan(*p);
+    if (p->workspace_bytes < plan.total || ((uintptr_t)p->workspace & 255)) return CO_ERR_DATA;
+    char *ws = (char *)p->workspace;
+    uint32_t *keys[2] = {(uint32_t *)ws, (uint32_t *)(ws + plan.keys)};
+    uint32_t *places[2] = {(uint32_t *)(ws + 2 * plan.keys), (uint32_t *)(ws + 3 * plan.keys)};
+    seq::Sort sort = {};
+    sort.counts = (uint32_t *)(ws + plan.counts);
+    sort.rows = (uint32_t)p->rows;
+    sort.tokens = (uint32_t)p->tokens;
+    sort.tile = (uint32_t)plan.tile;
+    sort.tiles = (int)plan.tiles;
+    sort.ids_64 = p->ids_64;
+    sort.bits = plan.bits;
+    int at = 0;
+    for (int i = 0; i < plan.passes; i++, at ^= 1) {
+        sort.ids = i ? nullptr : p->ids;
+        sort.keys = keys[at ^ 1];
+        sort.places = places[at ^ 1];
+        sort.keys_to = keys[at];
+        sort.places_to = places[at];
+        sort.shift = i * plan.bits;
+        seq::sort_count<<<sort.tiles, seq::kSortThreads, 0, s>>>(sort);
+        seq::sort_move<<<sort.tiles, seq::kSortThreads, 0, s>>>(sort);
+    }
+    seq::Runs r = {};
+    r.keys = keys[at ^ 1];
+    r.places = places[at ^ 1];
+    r.slots = (float *)(ws + plan.slots);
+    r.chunks = plan.chunks;
+    r.chunk = (int)plan.chunk;
+    r.pitch = plan.pitch;
+    switch (p->dtype) {
+        case SEQ_FP32: seq::launch_sum<float>(*p, r, s); break;
+        case SEQ_BF16: seq::launch_sum<__bf16>(*p, r, s); break;
+        default: seq::launch_sum<_Float16>(*p, r, s); break;
+    }
+    if (r.chunks > 1) {
+        // columns of a run go to several blocks while chunks are too few to fill the chip
+        const int64_t slabs = (p->width + 31) / 32;
+        int64_t y = 4096 / r.chunks + 1;
+        if (y > slabs) y = slabs;
+        seq::embed_join<<<seq::grid_of(r.chunks - 1, 256, (unsigned)y), 256, 0, s>>>(*p, r);
+    }
+    return seq::launch_status();
+}

@@ -1,0 +1,96 @@
+// seq_rows.h -- pieces of the row kernels (embedding, norm, log-probabilities).
+#ifndef CUSR_SEQ_ROWS_H
+#define CUSR_SEQ_ROWS_H
+
+#include "seq_common.h"
+
+namespace seq {
+
+// 8 values of a row side by side, as loaded: one piece of 16 bytes in a 16-bit type,
+// two in fp32. Loading and unpacking are apart, so that several are on their way.
+template <typename T> struct Eight {
+    uint4v a;
+    __device__ void load(const T *p) { a = *(const uint4v *)p; }
+    __device__ void zero() { a = uint4v{0, 0, 0, 0}; }
+    __device__ void get(float *f) const {
+        typedef T vec __attribute__((ext_vector_type(8)));
+        const vec v = __builtin_bit_cast(vec, a);
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] = (float)v[j];
+    }
+    static __device__ void put(T *p, const float *f) {
+        typedef T vec __attribute__((ext_vector_type(8)));
+        vec v;
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = (T)f[j];
+        *(vec *)p = v;
+    }
+};
+template <> struct Eight<float> {
+    float4v a, b;
+    __device__ void load(const float *p) { a = *(const float4v *)p; b = *(const float4v *)(p + 4); }
+    __device__ void zero() { a = b = float4v{0, 0, 0, 0}; }
+    __device__ void get(float *f) const {
+#pragma unroll
+        for (int j = 0; j < 4; j++) { f[j] = a[j]; f[j + 4] = b[j]; }
+    }
+    static __device__ void put(float *p, const float *f) {
+        *(float4v *)p = float4v{f[0], f[1], f[2], f[3]};
+        *(float4v *)(p + 4) = float4v{f[4], f[5], f[6], f[7]};
+    }
+};
+
+// the same where the type is known to the call only: the branch is the wave's
+__device__ inline void get8(const void *p, int dtype, int64_t at, float *f) {
+    if (dtype == SEQ_FP32) { Eight<float> v; v.load((const float *)p + at); v.get(f); }
+    else if (dtype == SEQ_BF16) { Eight<__bf16> v; v.load((const __bf16 *)p + at); v.get(f); }
+    else { Eight<_Float16> v; v.load((const _Float16 *)p + at); v.get(f); }
+}
+__device__ inline void put8(void *p, int dtype, int64_t at, const float *f) {
+    if (dtype == SEQ_FP32) Eight<float>::put((float *)p + at, f);
+    else if (dtype == SEQ_BF16) Eight<__bf16>::put((__bf16 *)p + at, f);
+    else Eight<_Float16>::put((_Float16 *)p + at, f);
+}
+__device__ inline float get1(const void *p, int dtype, int64_t at) {
+    if (dtype == SEQ_FP32) return ((const float *)p)[at];
+    if (dtype == SEQ_BF16) return (float)((const __bf16 *)p)[at];
+    return (float)((const _Float16 *)p)[at];
+}
+__device__ inline void put1(void *p, int dtype, int64_t at, float f) {
+    if (dtype == SEQ_FP32) ((float *)p)[at] = f;
+    else if (dtype == SEQ_BF16) ((__bf16 *)p)[at] = (__bf16)f;
+    else ((_Float16 *)p)[at] = (_Float16)f;
+}
+__device__ inline int64_t get_id(const void *p, int ids_64, int64_t at) {
+    return ids_64 ? ((const int64_t *)p)[at] : ((const int32_t *)p)[at];
+}
+
+inline bool float_type(int t) { return t >= SEQ_FP32 && t <= SEQ_FP16; }
+inline int type_bytes(int t) { return t == SEQ_FP32 ? 4 : (t == SEQ_INT8 ? 1 : 2); }
+// whether rows hold whole pieces of 8 values, each on a boundary of 16 bytes (8 of int8)
+inline bool in_eights(const void *p, int64_t row) {
+    return !p || (!((uintptr_t)p & 15) && row % 8 == 0);
+}
+
+// Sum and largest value over a group of G threads (a power of two up to the block's
+// 1,024): in a wave by exchanges, beyond through LDS, `red` with a float for each wave.
+// Every thread gets the result, formed in one order.
+struct Add { static __device__ float of(float a, float b) { return a + b; } };
+// keeps a NaN, as fmaxf would not
+struct Most { static __device__ float of(float a, float b) { return a > b || a != a ? a : b; } };
+template <typename Op, int G> __device__ inline float over_group(float x, float *red) {
+#pragma unroll
+    for (int o = (G < 64 ? G : 64) / 2; o; o >>= 1) x = Op::of(x, __shfl_xor(x, o));
+    if constexpr (G > 64) {
+        __syncthreads();                     // red may still be read from a call before
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = red[0];
+#pragma unroll
+        for (int i = 1; i < G / 64; i++) x = Op::of(x, red[i]);
+    }
+    return x;
+}
+
+}  // namespace seq
+#endif

@@ -41,7 +41,10 @@ _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_f
 # every extern "C" symbol of include/cusr_seq.h
 EXPORTED = ("seq_attention", "seq_attention_workspace", "seq_attention_grad",
             "seq_attention_grad_workspace", "seq_rotary", "seq_policy_loss",
-            "seq_policy_loss_workspace")
+            "seq_policy_loss_workspace", "seq_embedding", "seq_embedding_grad",
+            "seq_embedding_grad_workspace", "seq_norm", "seq_norm_grad",
+            "seq_norm_grad_workspace", "seq_int8_product", "seq_int8_product_workspace",
+            "seq_logprobs", "seq_logprobs_workspace", "seq_logprobs_grad")
 
 
 class SeqAttention(ctypes.Structure):
@@ -120,11 +123,8 @@ def load_library() -> ctypes.CDLL:
             for name in EXPORTED:
                 fn = getattr(lib, name)
                 fn.restype = ctypes.c_int64 if name.endswith("workspace") else ctypes.c_int
-            for name in ("seq_attention", "seq_rotary", "seq_policy_loss"):
-                getattr(lib, name).argtypes = [_P, _P]
+                fn.argtypes = [_P] if name.endswith("workspace") else [_P, _P]
             lib.seq_attention_grad.argtypes = [_P, _P, _P]
-            for name in ("seq_attention", "seq_attention_grad", "seq_policy_loss"):
-                getattr(lib, name + "_workspace").argtypes = [_P]
             _lib = lib
     return _lib
 

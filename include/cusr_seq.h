@@ -33,9 +33,13 @@ extern "C" {
 #define SEQ_FP32 0
 #define SEQ_BF16 1
 #define SEQ_FP16 2
+#define SEQ_INT8 3
 
 #define SEQ_MAX_HEAD 128          /* head size of attention, a multiple of 8 */
 #define SEQ_MAX_ROWS 2147000000LL /* query rows times heads, key rows, tokens */
+#define SEQ_MAX_WIDTH 65536       /* elements of a row of embedding and norm */
+#define SEQ_MAX_INNER 131071      /* inner size of int8_product: 128 * 128 of them fit 31 bits */
+#define SEQ_MAX_TOP 64            /* alternatives of a token */
 #define SEQ_LEAST 1e-30f          /* least and largest scale and temperature */
 #define SEQ_MOST 1e30f
 
@@ -151,6 +155,152 @@ typedef struct SeqPolicyLoss {
 
 int64_t seq_policy_loss_workspace(const SeqPolicyLoss *p);
 int seq_policy_loss(const SeqPolicyLoss *p, void *stream);
+
+/* ---- the layers around attention. Types are SEQ_FP32, SEQ_BF16 or SEQ_FP16 where
+ * nothing else is said; rows are `..._row` elements apart, their elements side by
+ * side; no output may overlap an input. Sums are held in fp32 or more, and the same
+ * call gives the same bits. */
+
+/* Rows of a table [rows, width] by token, times scale:
+ * out[t] = scale table[ids[t]], rounded once to out_dtype. A token outside the table
+ * gives a row of NaN. */
+typedef struct SeqEmbedding {
+    int32_t struct_size;
+    int32_t dtype, out_dtype; /* of the table, of out */
+    int32_t ids_64;           /* ids are int64_t rather than int32_t */
+    int64_t tokens, rows, width, table_row, out_row;
+    float scale;              /* finite */
+    int32_t reserved;
+    const void *ids, *table;
+    void *out;
+} SeqEmbedding;
+
+int seq_embedding(const SeqEmbedding *e, void *stream);
+
+/* Gradient of the table: dtable[v] = scale * the sum of d_out[t] over the tokens t
+ * with ids[t] = v, 0 where there is none. Tokens are sorted, and a row's terms are
+ * added in their order. Tokens outside the table take no part. */
+typedef struct SeqEmbeddingGrad {
+    int32_t struct_size;
+    int32_t dtype, out_dtype; /* of d_out, of dtable */
+    int32_t ids_64;
+    int64_t tokens, rows, width, dout_row, dtable_row;
+    float scale;
+    int32_t reserved;
+    const void *ids, *d_out;
+    void *dtable;
+    void *workspace;          /* seq_embedding_grad_workspace bytes, 256-aligned */
+    int64_t workspace_bytes;
+} SeqEmbeddingGrad;
+
+int64_t seq_embedding_grad_workspace(const SeqEmbeddingGrad *e);
+int seq_embedding_grad(const SeqEmbeddingGrad *e, void *stream);
+
+/* Root-mean-square norm of rows, after the addition of a residual stream, its output
+ * rounded to a type or to 8-bit integers with a scale for each row:
+ *   h = x + residual, rounded to the stream's type (h = x without a residual);
+ *   y = gain h / sqrt(mean h^2 + eps)       (gain null: 1; identity: y = h)
+ *   y_dtype SEQ_INT8: y_scale = max |y| / 127, y = round(y / y_scale), halves to even;
+ *   a row of zeros has the scale 0, one with a value that is not finite the scale NaN
+ *   and the integers 0.
+ * The stream's type is fp32 or x's. The quotients are taken from y in fp32. */
+typedef struct SeqNorm {
+    int32_t struct_size;
+    int32_t x_dtype, h_dtype, y_dtype, gain_dtype;
+    int32_t identity;         /* no norm, no gain, no residual: rows to 8 bits */
+    int64_t tokens, width, x_row, residual_row, h_row, y_row;
+    float eps;                /* finite, not negative */
+    int32_t reserved;
+    const void *x, *residual, *gain;
+    void *h;                  /* with a residual only */
+    void *y;
+    float *y_scale;           /* [tokens], with SEQ_INT8 only */
+} SeqNorm;
+
+int seq_norm(const SeqNorm *n, void *stream);
+
+/* Gradient of seq_norm (not of 8-bit outputs): with u = gain dy and n = h / sqrt(mean
+ * h^2 + eps), d = (u - n mean(u n)) / sqrt(mean h^2 + eps) + dh, in h's type and, where
+ * dx is given, in x_dtype too; dgain = the sum of dy n over the rows (null: not formed). */
+typedef struct SeqNormGrad {
+    int32_t struct_size;
+    int32_t dy_dtype, h_dtype, x_dtype, gain_dtype;
+    int32_t reserved;
+    int64_t tokens, width, dy_row, h_row, dh_row, d_row, dx_row;
+    float eps;
+    int32_t reserved2;
+    const void *dy, *h, *gain, *dh; /* dh null: 0 */
+    void *d, *dx;
+    float *dgain;             /* [width] */
+    void *workspace;          /* seq_norm_grad_workspace bytes, 256-aligned */
+    int64_t workspace_bytes;
+} SeqNormGrad;
+
+int64_t seq_norm_grad_workspace(const SeqNormGrad *n);
+int seq_norm_grad(const SeqNormGrad *n, void *stream);
+
+/* Product of 8-bit integers: o[i, j] = a_scale[i] w_scale[j] * sum over l of
+ * a[i, l] w[j, l], the sum exact, the rest in fp32, rounded once to out_dtype.
+ * a [m, inner], w [n, inner] (a row holds what one output takes). */
+typedef struct SeqInt8Product {
+    int32_t struct_size;
+    int32_t out_dtype;
+    int64_t m, n, inner, a_row, w_row, o_row;
+    const int8_t *a, *w;
+    const float *a_scale, *w_scale;
+    void *o;
+    void *workspace;          /* seq_int8_product_workspace bytes, 256-aligned */
+    int64_t workspace_bytes;
+} SeqInt8Product;
+
+int64_t seq_int8_product_workspace(const SeqInt8Product *p);
+int seq_int8_product(const SeqInt8Product *p, void *stream);
+
+/* Log-probabilities of given tokens under logits [tokens, vocab], with z = logits /
+ * temperature: logp = z[id] - logsumexp z, entropy = -sum p log p (0 log 0 = 0), and
+ * the `top` largest log-probabilities of each row with their columns, the lower column
+ * first among equals. A row whose logits are all -inf has logp -inf, entropy 0 and
+ * the alternatives 0, 1, .. at -inf; one with NaN or +inf gives NaN (its columns are
+ * some of the row's); a token outside the vocabulary gives logp NaN.
+ * stats [tokens, 2], for the gradient: the row's largest logit and the sum of
+ * exp(z - largest z) over the others (both 0 where all are -inf): what rounding
+ * would take from logsumexp, or from the sum with its 1, is in every p. */
+typedef struct SeqLogprobs {
+    int32_t struct_size;
+    int32_t dtype;
+    int32_t ids_64, top;
+    int64_t tokens, vocab, row;
+    float temperature;
+    int32_t reserved;
+    const void *logits, *ids;
+    float *logp, *entropy, *stats;  /* stats may be null */
+    float *top_logp;                /* [tokens, top] */
+    int64_t *top_ids;
+    void *workspace;                /* seq_logprobs_workspace bytes, 256-aligned */
+    int64_t workspace_bytes;
+} SeqLogprobs;
+
+int64_t seq_logprobs_workspace(const SeqLogprobs *p);
+int seq_logprobs(const SeqLogprobs *p, void *stream);
+
+/* Gradient of the logits from those of logp and entropy (null: 0):
+ *   dlogits_j = (dlogp (1[j = id] - p_j) - dentropy p_j (log p_j + entropy)) / temperature.
+ * A logit of -inf has the gradient 0, and a logp of -inf gives none. A row whose dlogp
+ * and dentropy are 0 is not read and gets 0. Another gives NaN when it has NaN or
+ * +inf, or a token outside the vocabulary and dlogp not 0. */
+typedef struct SeqLogprobsGrad {
+    int32_t struct_size;
+    int32_t dtype;
+    int32_t ids_64, reserved;
+    int64_t tokens, vocab, row, drow;
+    float temperature;
+    int32_t reserved2;
+    const void *logits, *ids;
+    const float *stats, *entropy, *dlogp, *dentropy;
+    void *dlogits;
+} SeqLogprobsGrad;
+
+int seq_logprobs_grad(const SeqLogprobsGrad *p, void *stream);
 
 #ifdef __cplusplus
 }
