@@ -102,6 +102,38 @@ __device__ inline uint2v read_transposed(const uint16_t *p) {
     return read_transposed((__attribute__((address_space(3))) const uint16_t *)p);
 }
 
+typedef __attribute__((address_space(3))) const uint16_t *lds_ptr;
+typedef __attribute__((address_space(3))) const uint4v *lds_ptr4;
+__device__ inline uint32_t lds_address(const void *p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+
+// Copies from memory to LDS past the registers: 16 (or 4) bytes a lane, to
+// `to` + 16 (4) lane; `to` is the same for the wave. The second form adds a
+// lane's offset to an address of the wave, which costs no vector instruction.
+// Copies count as loads: wait_copies<N> waits until at most the wave's last N
+// loads are on their way. Written in assembly because the compiler, which cannot
+// tell the buffers apart, would wait for the newest copy before every LDS read;
+// there is no output register, and its own waits only grow longer by the extra
+// loads. m0, which holds the LDS address, is written by each.
+__device__ inline void copy_to_lds16(const void *from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory", "m0");
+}
+__device__ inline void copy_to_lds16(const void *wave_from, uint32_t lane_offset, uint32_t to) {
+    // five states between a vector instruction that wrote the address and its use
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(lane_offset), "s"(wave_from)
+                 : "memory", "m0");
+}
+__device__ inline void copy_to_lds4(const void *from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory", "m0");
+}
+template <int N> __device__ inline void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
+}
+
 // Blocks of a launch. An axis has fewer than 2^32 threads (HIP starts what is left of
 // the number modulo 2^32, without an error), so more blocks continue along z, in equal
 // parts: the last numbers may be past the end, and a kernel leaves those alone.

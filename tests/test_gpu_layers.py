@@ -298,7 +298,9 @@ PRODUCT = [
     (1, 1, 1), (1, 64, 16), (3, 17, 5), (16, 128, 256), (24, 4096, 384), (33, 100, 130),
     (128, 64, 128), (129, 65, 127), (200, 1000, 72), (257, 256, 300), (7, 16, 1000),
     (300, 131, 33), (64, 2064, 260), (1000, 512, 520), (32, 131071, 17), (5, 0, 7), (0, 8, 4),
-    (4, 8, 0), (17, 1280, 640), (2, 5008, 2050), (260, 4100, 258),
+    (4, 8, 0), (17, 1280, 640), (2, 5008, 2050), (260, 4100, 258), (65, 48, 100), (64, 528, 31),
+    # enough tiles of 128 and of 256 to be taken, whole and cut ones
+    (1500, 128, 1450), (1536, 16, 1408), (4000, 80, 4100), (4096, 208, 4104),
 ]
 
 
