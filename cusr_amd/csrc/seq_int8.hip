@@ -28,54 +28,61 @@ __device__ inline uint4v row_piece(const int8_t *row, int64_t l, int64_t inner) 
     return v;
 }
 
-// Outputs j .. j + 7 of row i from their sums; `whole`: all of them are inside and lie on
-// a boundary of 16 bytes.
-__device__ inline void put_sums(const SeqInt8Product &p, int64_t i, int64_t j, const int4v &lo,
-                                const int4v &hi, const float *sw, bool whole) {
-    const float sa = p.a_scale[i];
-    float f[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = (float)(e < 4 ? lo[e] : hi[e - 4]) * sa * sw[e];
-    if (whole) {
-        put8(p.o, p.out_dtype, i * p.o_row + j, f);
-    } else {
-        for (int e = 0; e < 8; e++)
-            if (j + e < p.n) put1(p.o, p.out_dtype, i * p.o_row + j + e, f[e]);
-    }
-}
-
-// A wave's TW columns of 32 rows from its accumulators to memory: turned round through the
-// wave's own LDS, so that a lane has 8 columns of a row.
-template <int TW>
-__device__ inline void put_slab(const SeqInt8Product &p, int64_t i0, int64_t j0,
-                                const int16v *acc, int *lds, const float *sw, bool wide) {
-    constexpr int PITCH = TW + 8;      // halves of a wave, 4 rows apart, in other banks
+// A wave's F x F products of 32 channels by 32 tokens to memory; scales: the wave's, in
+// LDS. A lane of a product has one token's channels 8 g + 4 h .. + 3, h its half of the
+// wave; two groups g change halves, and it has 8 channels side by side. 32 tokens' go
+// through LDS to leave as whole rows: stores of 32 bytes a row took 156 us for 8,192 x
+// 16,384 outputs of 128 terms. WIDE: every 8 channels lie on a boundary of 16 bytes
+// and are all inside or all outside.
+template <typename O, int F> constexpr int slab_pitch() { return F * 32 + 16 / (int)sizeof(O); }
+template <typename O, bool WIDE, int F>
+__device__ inline void put_sums(const SeqInt8Product &p, int64_t i0, int64_t j0,
+                                const int16v (&acc)[F][F], const float *a_scale,
+                                const float *w_scale, O *slab) {
+    constexpr int N = F * 32, PITCH = slab_pitch<O, F>();
     const int lane = threadIdx.x & 63;
-    wave_sync();
 #pragma unroll
-    for (int y = 0; y < TW / 32; y++)
+    for (int x = 0; x < F; x++) {
+        const float sa = a_scale[x * 32 + lane % 32];
+        wave_sync();
 #pragma unroll
-        for (int r = 0; r < 16; r++)
-            lds[(8 * (r / 4) + 4 * (lane / 32) + r % 4) * PITCH + y * 32 + lane % 32] = acc[y][r];
-    wave_sync();
-    constexpr int LANES = TW / 8, ROWS = 64 / LANES;       // of a row; at a time
-    const int col = lane % LANES * 8;
-    const int64_t j = j0 + col;
-    if (j >= p.n) return;
-    const bool whole = wide && j + 8 <= p.n;
+        for (int y = 0; y < F; y++)
 #pragma unroll
-    for (int r = 0; r < 32; r += ROWS) {
-        const int row = r + lane / LANES;
-        const int4v lo = *(const int4v *)(lds + row * PITCH + col);
-        const int4v hi = *(const int4v *)(lds + row * PITCH + col + 4);
-        if (i0 + row < p.m) put_sums(p, i0 + row, j, lo, hi, sw, whole);
+            for (int g = 0; g < 2; g++) {
+                __builtin_amdgcn_sched_barrier(0);           // few sums in registers at a time
+                const int col = y * 32 + g * 16 + lane / 32 * 8;
+                const float4v lo = *(const float4v *)(w_scale + col);
+                const float4v hi = *(const float4v *)(w_scale + col + 4);
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const auto s = __builtin_amdgcn_permlane32_swap(
+                        (uint32_t)acc[x][y][g * 8 + e], (uint32_t)acc[x][y][g * 8 + 4 + e], false, false);
+                    f[e] = (float)(int)s[0] * sa * lo[e];
+                    f[4 + e] = (float)(int)s[1] * sa * hi[e];
+                }
+                Eight<O>::put(slab + lane % 32 * PITCH + col, f);
+            }
+        wave_sync();
+        const int64_t i = i0 + x * 32;
+        if constexpr (WIDE) {
+            constexpr int PER = 16 / sizeof(O), LANES = N / PER, ROWS = LANES < 64 ? 64 / LANES : 1;
+            const int col = lane % LANES * PER;
+            O *to = (O *)p.o + (i + lane / LANES) * p.o_row + j0 + col;
+            const bool in = j0 + col < p.n;
+#pragma unroll
+            for (int r = lane / LANES; r < 32; r += ROWS) {
+                const uint4v v = *(const uint4v *)(slab + r * PITCH + col);
+                if (in && i + r < p.m) *(uint4v *)to = v;
+                to += ROWS * p.o_row;
+            }
+        } else {
+            for (int r = 0; r < 32 && i + r < p.m; r++)
+#pragma unroll
+                for (int c = lane; c < N; c += 64)
+                    if (j0 + c < p.n) ((O *)p.o)[(i + r) * p.o_row + j0 + c] = slab[r * PITCH + c];
+        }
     }
-}
-template <int TW>
-__device__ inline void column_scales(const SeqInt8Product &p, int64_t j0, float *sw) {
-    const int64_t j = j0 + (int)(threadIdx.x & 63) % (TW / 8) * 8;
-#pragma unroll
-    for (int e = 0; e < 8; e++) sw[e] = j + e < p.n ? p.w_scale[j + e] : 0.0f;
 }
 
 // A block's tile. Blocks go to the eight dies in turn, so each die takes a run of tiles of
@@ -93,48 +100,58 @@ __device__ inline bool tile_of(int64_t block, int64_t rows, int64_t columns, int
 }
 
 // T x T outputs a block of four waves, T / 2 x T / 2 a wave, 64 terms a step. Operands come
-// to LDS past the registers, three steps ahead in four buffers; a step's second half and
-// the next one's first are read from LDS while the half before is multiplied. Row r of a
-// buffer holds its four pieces of 16 bytes turned by r / 4, so that 16 lanes' reads meet
-// every bank once.
-constexpr int kStep = 64, kStages = 4;
+// to LDS past the registers into five buffers, so that a copy has two and a half steps to
+// arrive: a step of 256 x 256 is a microsecond's half, an operand's way from beyond the
+// die's cache more than one. A step's second half is read from LDS while its first is
+// multiplied, and the next one's first with its second. Row r of a buffer holds its four
+// pieces of 16 bytes turned by r / 4, so that 16 lanes' reads meet every bank once.
+constexpr int kStep = 64, kStages = 5;
 template <int T> constexpr int tile_bytes() { return 2 * T * kStep; }
 
-template <int T>
-__global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Product p, bool wide) {
+template <typename O, bool WIDE, int T>
+__global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Product p) {
     constexpr int W = T / 2, F = W / 32;         // a wave's side, in products
     constexpr int COPIES = tile_bytes<T>() / 4096;           // a wave's copies of a step
+    constexpr uint32_t BYTES = tile_bytes<T>(), ALL = kStages * BYTES;
     extern __shared__ __align__(16) unsigned char lds[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int64_t ti, tj;
     if (!tile_of(block_number(), (p.m + T - 1) / T, (p.n + T - 1) / T, ti, tj)) return;
     const int64_t i0 = ti * T, j0 = tj * T;
+    float a_scale = 0.0f, w_scale = 0.0f;        // of row and column tid
+    if (tid < T && i0 + tid < p.m) a_scale = p.a_scale[i0 + tid];
+    if (tid < T && j0 + tid < p.n) w_scale = p.w_scale[j0 + tid];
     const uint32_t base = lds_address(lds);
-    // copy x of the wave fills 16 rows: this lane row lane / 4, place lane % 4
-    const int8_t *from[COPIES];
+    // Waves 0 and 1 bring a, waves 2 and 3 w. Copy x fills 16 rows, this lane row lane / 4,
+    // place lane % 4; rows past the last are the last.
+    const bool is_a = wave < 2;
+    const int64_t row_bytes = is_a ? p.a_row : p.w_row, first = is_a ? i0 : j0;
+    const int64_t left = (is_a ? p.m : p.n) - 1 - first;
+    const int8_t *from = (is_a ? p.a : p.w) + first * row_bytes;
+    uint32_t offset[COPIES];                     // below 2^32: the launch sees to it
     int piece[COPIES];
 #pragma unroll
     for (int x = 0; x < COPIES; x++) {
-        const int row = (wave * COPIES + x) * 16 + lane / 4;           // of a, then of w
-        const bool is_a = row < T;
-        const int64_t r = is_a ? i0 + row : j0 + row - T, most = (is_a ? p.m : p.n) - 1;
+        const int row = (wave % 2 * COPIES + x) * 16 + lane / 4;
         piece[x] = (lane % 4 - row / 4 % 4 + 4) % 4 * 16;
-        from[x] = (is_a ? p.a : p.w) + (r < most ? r : most) * (is_a ? p.a_row : p.w_row) + piece[x];
+        offset[x] = (uint32_t)((row < left ? row : (int)left) * row_bytes) + piece[x];
     }
-    auto fetch = [&](int64_t step) {
-        const uint32_t to = base + (uint32_t)(step % kStages) * tile_bytes<T>() +
-                            wave * COPIES * 1024;
-#pragma unroll
-        for (int x = 0; x < COPIES; x++) {
-            const int64_t l = step * kStep;
-            const void *at = l + piece[x] < p.inner ? (const void *)(from[x] + l) : kZeros;
-            copy_to_lds16(at, to + x * 1024);
+    // Copy x of the step at l to the buffer at `to`. CUT: of a step that passes the rows' end,
+    // whose pieces there are zeros; steps past the last are, so that every step counts alike.
+    auto copy = [&](int l, uint32_t to, int x, auto cut) {
+        to += base + wave * COPIES * 1024 + x * 1024;
+        if constexpr (cut.value) {
+            uint32_t o = offset[x];
+            asm volatile("" : "+v"(o));          // no addresses kept over steps
+            copy_to_lds16(piece[x] < (int)p.inner - l ? (const void *)(from + l + o) : kZeros, to);
+        } else {
+            copy_to_lds16(from + l, offset[x], to);
         }
     };
     const int row = lane % 32;
-    auto read = [&](int64_t step, int half, int4v *a, int4v *w) {
-        const uint32_t at = base + (uint32_t)(step % kStages) * tile_bytes<T>() +
-                            (half * 2 + lane / 32 + row / 4) % 4 * 16 + row * kStep;
+    auto read = [&](uint32_t at, int half, int4v *a, int4v *w) {
+        at += base + (half * 2 + lane / 32 + row / 4) % 4 * 16 + row * kStep;
 #pragma unroll
         for (int x = 0; x < F; x++) {
             a[x] = __builtin_bit_cast(int4v, *(lds_ptr4)(uintptr_t)(at + (wave / 2 * W + x * 32) * kStep));
@@ -148,54 +165,87 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Produ
         for (int y = 0; y < F; y++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[x][y][r] = 0;
-    auto multiply = [&](const int4v *a, const int4v *w) {
+    int4v a0[F], w0[F], a1[F], w1[F];
+    // until at most the newest N steps' copies are on their way, everyone's
+    auto wait = [&](auto steps) {
+        wait_copies<steps.value * COPIES>();
+        asm volatile("s_barrier" ::: "memory");
+    };
+    uint32_t here = 0, ahead = (kStages - 1) * BYTES;        // buffers of this step and of the copies
+    int l = 0;
+    // Copies go between products: issued together they would leave the matrix unit idle.
+    constexpr int EVERY = F * F / COPIES ? F * F / COPIES : 1;
+    auto step = [&](auto cut) {
+        read(here, 1, a1, w1);
+#pragma unroll
+        for (int x = 0; x < F; x++)
+#pragma unroll
+            for (int y = 0; y < F; y++) {
+                const int at = x * F + y;
+                if (at % EVERY == 0)             // to where the step before was: all have read it
+#pragma unroll
+                    for (int c = at / EVERY; c < COPIES; c += F * F)
+                        copy(l + (kStages - 1) * kStep, ahead, c, cut);
+                __builtin_amdgcn_sched_barrier(0);
+                acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w0[y], a0[x], acc[x][y], 0, 0, 0);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        wait(Const<kStages - 2>());              // the next step is here
+        ahead = here;
+        here = here + BYTES == ALL ? 0 : here + BYTES;
+        // a1 and w1 are too, which the compiler is told: it would wait for the newer reads
+#pragma unroll
+        for (int x = 0; x < F; x++) asm volatile("" : "+v"(a1[x]), "+v"(w1[x]));
+        read(here, 0, a0, w0);
 #pragma unroll
         for (int x = 0; x < F; x++)
 #pragma unroll
             for (int y = 0; y < F; y++)
-                acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[x], w[y], acc[x][y], 0, 0, 0);
+                acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w1[y], a1[x], acc[x][y], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        l += kStep;
     };
-    auto all_here = [] { asm volatile("s_barrier" ::: "memory"); };
-    int4v a0[F], w0[F], a1[F], w1[F];
-    fetch(0);
-    fetch(1);
-    fetch(2);
-    wait_copies<COPIES>();
-    all_here();
-    read(0, 0, a0, w0);
-    const int64_t steps = (p.inner + kStep - 1) / kStep;
-    for (int64_t s = 0; s < steps; s++) {
-        fetch(s + 3);                            // where step s - 1 was: all have read it
-        read(s, 1, a1, w1);
-        multiply(a0, w0);
-        read(s + 1, 0, a0, w0);
-        multiply(a1, w1);
-        wait_copies<COPIES>();                   // step s + 2 is here
-        all_here();
-    }
-    wait_copies<0>();
-    all_here();
-    float sw[8];
-    const int64_t j = j0 + wave % 2 * W;
-    column_scales<W>(p, j, sw);
 #pragma unroll
-    for (int x = 0; x < F; x++)
-        put_slab<W>(p, i0 + wave / 2 * W + x * 32, j, acc[x], (int *)lds + wave * 32 * (W + 8), sw,
-                    wide);
+    for (int x = 0; x < (kStages - 1) * COPIES; x++)
+        copy(x / COPIES * kStep, x / COPIES * BYTES, x % COPIES, Const<1>());
+    wait(Const<kStages - 2>());
+    read(here, 0, a0, w0);
+    const int inner = (int)p.inner, whole = inner - kStages * kStep;
+    while (l <= whole) step(Const<0>());
+    while (l < inner) step(Const<1>());
+    wait(Const<0>());                            // the last step's reads are done
+    float *scales = (float *)lds;
+    static_assert(8 * T + 4 * 32 * slab_pitch<O, F>() * sizeof(O) <= ALL, "");
+    if (tid < T) {
+        scales[tid] = a_scale;
+        scales[T + tid] = w_scale;
+    }
+    __syncthreads();
+    put_sums<O, WIDE, F>(p, i0 + wave / 2 * W, j0 + wave % 2 * W, acc, scales + wave / 2 * W,
+                         scales + T + wave % 2 * W,
+                         (O *)(scales + 2 * T) + wave * 32 * slab_pitch<O, F>());
 }
 
 // The same for operands off 16-byte boundaries or rows that no whole number of pieces
 // fills: 128 x 128 outputs, operands by way of registers.
 constexpr int kPitch = kStep + 16;
-__global__ __launch_bounds__(256) void int8_any(SeqInt8Product p, bool wide) {
+template <typename O, bool WIDE> __global__ __launch_bounds__(256) void int8_any(SeqInt8Product p) {
     constexpr int T = 128, W = 64;
-    __shared__ __align__(16) int8_t lds[4 * 32 * (W + 8) * 4];         // 2 T kPitch, or the sums
+    // operands, then the waves' slabs of outputs
+    __shared__ __align__(16) int8_t lds[4 * 32 * slab_pitch<float, 2>() * 4];
+    __shared__ __align__(16) float scales[2][T];
     int8_t *as = lds, *ws = lds + T * kPitch;
+    static_assert(2 * T * kPitch <= sizeof(lds), "");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int64_t ti, tj;
     if (!tile_of(block_number(), (p.m + T - 1) / T, (p.n + T - 1) / T, ti, tj)) return;
     const int64_t i0 = ti * T, j0 = tj * T;
     const int wi = wave / 2 * W, wj = wave % 2 * W;
+    if (tid < T) {
+        scales[0][tid] = i0 + tid < p.m ? p.a_scale[i0 + tid] : 0.0f;
+        scales[1][tid] = j0 + tid < p.n ? p.w_scale[j0 + tid] : 0.0f;
+    }
+    __syncthreads();
     int16v acc[2][2];
 #pragma unroll
     for (int x = 0; x < 2; x++)
@@ -233,15 +283,12 @@ __global__ __launch_bounds__(256) void int8_any(SeqInt8Product p, bool wide) {
             for (int x = 0; x < 2; x++)
 #pragma unroll
                 for (int y = 0; y < 2; y++)
-                    acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[x], w[y], acc[x][y], 0, 0, 0);
+                    acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[y], a[x], acc[x][y], 0, 0, 0);
         }
     }
     __syncthreads();
-    float sw[8];
-    column_scales<W>(p, j0 + wj, sw);
-#pragma unroll
-    for (int x = 0; x < 2; x++)
-        put_slab<W>(p, i0 + wi + x * 32, j0 + wj, acc[x], (int *)lds + wave * 32 * (W + 8), sw, wide);
+    put_sums<O, WIDE, 2>(p, i0 + wi, j0 + wj, acc, scales[0] + wi, scales[1] + wj,
+                         (O *)lds + wave * 32 * slab_pitch<O, 2>());
 }
 
 // Few tokens: 16 channels a block and up to 16 M tokens, the terms cut among eight waves,
@@ -314,9 +361,26 @@ int check_int8(const SeqInt8Product *p) {
 template <int M> void launch_few(const SeqInt8Product &p, hipStream_t s) {
     int8_few<M><<<grid_of((p.n + 15) / 16, 512), 512, 0, s>>>(p);
 }
-template <int T> void launch_tiles(const SeqInt8Product &p, bool wide, hipStream_t s) {
+template <typename O, bool WIDE, int T> void launch_tiles(const SeqInt8Product &p, hipStream_t s) {
     const int64_t blocks = (tiles_of(p, T) + 7) / 8 * 8;
-    int8_tiles<T><<<grid_of(blocks, 256), 256, kStages * tile_bytes<T>(), s>>>(p, wide);
+    int8_tiles<O, WIDE, T><<<grid_of(blocks, 256), 256, kStages * tile_bytes<T>(), s>>>(p);
+}
+template <typename O, bool WIDE>
+void launch_tiles(const SeqInt8Product &p, bool pieces, hipStream_t s) {
+    if (!pieces) {
+        const int64_t blocks = (tiles_of(p, 128) + 7) / 8 * 8;
+        int8_any<O, WIDE><<<grid_of(blocks, 256), 256, 0, s>>>(p);
+    } else if (tiles_of(p, 256) >= 256) {
+        launch_tiles<O, WIDE, 256>(p, s);
+    } else if (tiles_of(p, 128) >= 128) {
+        launch_tiles<O, WIDE, 128>(p, s);
+    } else {
+        launch_tiles<O, WIDE, 64>(p, s);
+    }
+}
+template <typename O> void launch_tiles(const SeqInt8Product &p, bool pieces, hipStream_t s) {
+    if (in_eights(p.o, p.o_row) && p.n % 8 == 0) launch_tiles<O, true>(p, pieces, s);
+    else launch_tiles<O, false>(p, pieces, s);
 }
 
 }  // namespace seq
@@ -333,24 +397,21 @@ extern "C" int seq_int8_product(const SeqInt8Product *p, void *stream) {
     if (!p->a_scale || !p->w_scale || !p->o || (p->inner && (!p->a || !p->w)))
         return CO_ERR_NULLARG;
     hipStream_t s = (hipStream_t)stream;
-    const bool wide = seq::in_eights(p->o, p->o_row);
+    // 256 rows and a step within 2^32 bytes, and whole pieces
+    const int64_t far = 1ll << 23;
     const bool pieces = !(((uintptr_t)p->a | (uintptr_t)p->w) & 15) && p->a_row % 16 == 0 &&
-                        p->w_row % 16 == 0 && p->inner % 16 == 0;
-    if (!pieces) {
-        const int64_t blocks = (seq::tiles_of(*p, 128) + 7) / 8 * 8;
-        seq::int8_any<<<seq::grid_of(blocks, 256), 256, 0, s>>>(*p, wide);
-    } else if (p->m <= 16) {
-        seq::launch_few<1>(*p, s);
-    } else if (p->m <= 32) {
-        seq::launch_few<2>(*p, s);
-    } else if (p->m <= 64) {
-        seq::launch_few<4>(*p, s);
-    } else if (seq::tiles_of(*p, 256) >= 256) {
-        seq::launch_tiles<256>(*p, wide, s);
-    } else if (seq::tiles_of(*p, 128) >= 128) {
-        seq::launch_tiles<128>(*p, wide, s);
-    } else {
-        seq::launch_tiles<64>(*p, wide, s);
+                        p->w_row % 16 == 0 && p->inner % 16 == 0 && p->a_row >= 0 &&
+                        p->w_row >= 0 && p->a_row < far && p->w_row < far;
+    if (pieces && p->m <= 64) {
+        if (p->m <= 16) seq::launch_few<1>(*p, s);
+        else if (p->m <= 32) seq::launch_few<2>(*p, s);
+        else seq::launch_few<4>(*p, s);
+        return seq::launch_status();
+    }
+    switch (p->out_dtype) {
+        case SEQ_FP32: seq::launch_tiles<float>(*p, pieces, s); break;
+        case SEQ_BF16: seq::launch_tiles<__bf16>(*p, pieces, s); break;
+        default: seq::launch_tiles<_Float16>(*p, pieces, s); break;
     }
     return seq::launch_status();
 }
