@@ -55,6 +55,140 @@ __global__ __launch_bounds__(256) void embed_rows(SeqEmbedding p, int g) {
     }
 }
 
+// ------------------------------------------------------------- few rows: symbols
+
+// A table of few rows: a wave keeps the sums of its tokens, 128 columns of every row, in
+// LDS and reads its tokens' gradients one after the other, so no order of tokens is
+// needed. A lane adds to columns of its own, in the tokens' order, four tokens at a
+// time: where two of them have one row the later takes the earlier's sum. (LDS adds
+// floats by itself, but hardly a lane at a time: 839 us for 1.3 M tokens of 128 in fp32
+// and 22 rows.)
+constexpr int kSymbolRows = 128, kSymbolCols = 128;
+
+template <typename T, bool PAIR>
+__global__ __launch_bounds__(256) void embed_symbols(SeqEmbeddingGrad p, int slabs, int64_t chunk,
+                                                     float *partial) {
+    constexpr int AHEAD = 8;                     // rows on their way
+    extern __shared__ __align__(16) float sums[];            // of each wave: rows + 1 by 128
+    const int V = (int)p.rows, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int slab = (int)(blockIdx.x % slabs);
+    const int64_t c = blockIdx.x / slabs;
+    for (int i = threadIdx.x; i < waves * (V + 1) * kSymbolCols; i += blockDim.x) sums[i] = 0.0f;
+    __syncthreads();
+    // PAIR: columns 2 lane and 2 lane + 1, else lane and lane + 64
+    const int64_t col0 = (int64_t)slab * kSymbolCols + (PAIR ? 2 * lane : lane);
+    const int64_t col1 = PAIR ? col0 + 1 : col0 + 64;
+    const bool in0 = col0 < p.width, in1 = col1 < p.width;
+    // the lane's two places of a row; tokens outside the table have one behind the rows
+    float *mine = sums + wave * (V + 1) * kSymbolCols + (PAIR ? 2 * lane : lane);
+    auto at = [&](int id) -> float2v {
+        const float *q = mine + id * kSymbolCols;
+        if constexpr (PAIR) return *(const float2v *)q;
+        else return float2v{q[0], q[64]};
+    };
+    auto put = [&](int id, float2v v) {
+        float *q = mine + id * kSymbolCols;
+        if constexpr (PAIR) {
+            *(float2v *)q = v;
+        } else {
+            q[0] = v[0];
+            q[64] = v[1];
+        }
+    };
+    // the wave's tokens
+    const int64_t first = c * chunk, end = first + chunk < p.tokens ? first + chunk : p.tokens;
+    const int64_t each = (chunk + waves - 1) / waves;
+    const int64_t a = first + wave * each, b = a + each < end ? a + each : end;
+    typedef T pair __attribute__((ext_vector_type(2)));
+    // the rows of 64 tokens from t on, a lane each; V: none
+    auto rows_of = [&](int64_t t) {
+        const int64_t id = t + lane < b ? get_id(p.ids, p.ids_64, t + lane) : -1;
+        return id >= 0 && id < V ? (int)id : V;
+    };
+    struct Batch { int id[AHEAD]; T x0[AHEAD], x1[AHEAD]; };
+    auto load = [&](Batch &r, int ids, int k, int64_t t0) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            r.id[u] = __builtin_amdgcn_readlane(ids, k + u);
+            r.x0[u] = r.x1[u] = (T)0.0f;
+            if (r.id[u] == V) continue;          // behind the last token too
+            const T *row = (const T *)p.d_out + (t0 + k + u) * p.dout_row;
+            if constexpr (PAIR) {
+                if (in0) {
+                    const pair v = *(const pair *)(row + col0);
+                    r.x0[u] = v[0];
+                    r.x1[u] = v[1];
+                }
+            } else {
+                if (in0) r.x0[u] = row[col0];
+                if (in1) r.x1[u] = row[col1];
+            }
+        }
+    };
+    auto add = [&](const Batch &r) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; u += 4) {
+            float2v sum[4];
+#pragma unroll
+            for (int v = 0; v < 4; v++) sum[v] = at(r.id[u + v]);
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+#pragma unroll
+                for (int o = 0; o < v; o++)
+                    if (r.id[u + o] == r.id[u + v]) sum[v] = sum[o];
+                sum[v][0] += (float)r.x0[u + v];
+                sum[v][1] += (float)r.x1[u + v];
+            }
+#pragma unroll
+            for (int v = 0; v < 4; v++) put(r.id[u + v], sum[v]);
+        }
+    };
+    // a batch is added while the next one is on its way
+    int ids = rows_of(a);
+    Batch even, odd;
+    load(even, ids, 0, a);
+    for (int64_t t0 = a; t0 < b; t0 += 64) {
+        const int next = rows_of(t0 + 64);
+        for (int k = 0; k < 64; k += 2 * AHEAD) {
+            load(odd, ids, k + AHEAD, t0);
+            add(even);
+            if (k + 2 * AHEAD < 64) load(even, ids, k + 2 * AHEAD, t0);
+            else load(even, next, 0, t0 + 64);
+            add(odd);
+        }
+        ids = next;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < V * kSymbolCols; i += blockDim.x) {
+        const int64_t col = (int64_t)slab * kSymbolCols + i % kSymbolCols;
+        if (col >= p.width) continue;
+        float s = sums[i];
+        for (int w = 1; w < waves; w++) s += sums[w * (V + 1) * kSymbolCols + i];
+        partial[(c * V + i / kSymbolCols) * p.width + col] = s;
+    }
+}
+
+// The chunks' sums in their order: 32 places of the table a block, each by 32 threads.
+__global__ __launch_bounds__(1024) void embed_chunks(SeqEmbeddingGrad p, int64_t chunks,
+                                                     const float *partial) {
+    __shared__ float part[32][33];
+    const int x = threadIdx.x % 32, g = threadIdx.x / 32;
+    const int64_t all = p.rows * p.width, at = blockIdx.x * 32ll + x;
+    float s = 0.0f;
+    if (at < all)
+#pragma unroll 8
+        for (int64_t c = g; c < chunks; c += 32) s += partial[c * all + at];
+    part[g][x] = s;
+    __syncthreads();
+    if (g == 0 && at < all) {
+        s = part[0][x];
+#pragma unroll
+        for (int i = 1; i < 32; i++) s += part[i][x];
+        put1(p.dtable, p.out_dtype, at / p.width * p.dtable_row + at % p.width, s * p.scale);
+    }
+}
+
 // ----------------------------------------------------------------------- sort
 
 // Tokens are sorted by digits of at most 9 bits, the lowest first, each time in two
@@ -97,7 +231,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_move(Sort s) {
     __shared__ uint32_t base[kDigits], total[kSortThreads], before[kSortThreads];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
     const int digits = 1 << s.bits, d = tid & (digits - 1);
-    // counts of digit d in all tiles and in those before this one, by several threads
+    // counts of digit d in all tiles and in those before this one
     uint32_t all = 0, prior = 0;
 #pragma unroll 8
     for (int t = tid >> s.bits; t < s.tiles; t += kSortThreads >> s.bits) {
@@ -113,17 +247,19 @@ __global__ __launch_bounds__(kSortThreads) void sort_move(Sort s) {
             all += total[t];
             prior += before[t];
         }
-    __syncthreads();
-    total[tid] = tid < digits ? all : 0;
-    __syncthreads();
-    uint32_t sum = total[tid];                   // counts of lower digits: a running sum
-    for (int o = 1; o < digits; o *= 2) {
-        const uint32_t add = tid >= o ? total[tid - o] : 0;
-        __syncthreads();
-        sum += add;
-        total[tid] = sum;
-        __syncthreads();
+    // counts of lower digits: running sums in waves, then over them
+    if (tid >= digits) all = 0;
+    uint32_t sum = all;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const uint32_t add = __shfl_up(sum, o);
+        sum += lane >= o ? add : 0;
     }
+    if (lane == 63) base[wave] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSortWaves - 1; w++) sum += w < wave ? base[w] : 0;
+    __syncthreads();
     if (tid < digits) base[tid] = sum - all + prior;
     const uint64_t first = (uint64_t)blockIdx.x * s.tile;
     const uint64_t end = first + s.tile < s.tokens ? first + s.tile : s.tokens;
@@ -208,13 +344,16 @@ __global__ __launch_bounds__(256) void embed_sum(SeqEmbeddingGrad p, Runs r) {
         if ((int)threadIdx.x < rows)
             present[threadIdx.x] = has_token(r.keys, n, (uint32_t)(v0 + threadIdx.x));
         __syncthreads();
-        const float zero[W] = {};
-        const int parts = (int)(p.width / W);
-        for (int i = threadIdx.x; i < rows * parts; i += 256) {
-            const int row = i / parts;
-            if (!present[row])
-                put_cells<W>(p.dtable, p.out_dtype,
-                             (v0 + row) * p.dtable_row + (int64_t)(i - row * parts) * W, zero);
+        for (int row = 0; row < rows; row++) {
+            if (present[row]) continue;
+            if constexpr (W == 8) {              // 16 bytes a thread
+                const int e = p.out_dtype == SEQ_FP32 ? 4 : 2;
+                uint4v *to = (uint4v *)((char *)p.dtable + (v0 + row) * p.dtable_row * e);
+                for (int i = threadIdx.x; i < p.width * e / 16; i += 256) to[i] = uint4v{0, 0, 0, 0};
+            } else {
+                for (int i = threadIdx.x; i < p.width; i += 256)
+                    put1(p.dtable, p.out_dtype, (v0 + row) * p.dtable_row + i, 0.0f);
+            }
         }
         return;
     }
@@ -269,41 +408,77 @@ __global__ __launch_bounds__(256) void embed_sum(SeqEmbeddingGrad p, Runs r) {
     flush(run == next);
 }
 
-// Joins the slots of a run that begins in a chunk and goes on: 32 columns at a time, each
-// by 8 threads.
+// Joins the slots of a run that begins in a chunk and goes on, 128 columns at a time, 4 to a
+// thread. A block looks at eight chunks, 32 threads each, and those join a run of up to
+// eight more chunks by themselves; a longer one is the whole block's, in eight parts.
 __global__ __launch_bounds__(256) void embed_join(SeqEmbeddingGrad p, Runs r) {
-    __shared__ float part[8][33];
-    const int64_t c = block_number();
-    if (c >= r.chunks - 1) return;
-    const uint32_t a = (uint32_t)(c * r.chunk), b = a + r.chunk;      // not the last chunk
-    const uint32_t run = r.keys[b - 1];
-    if (run >= (uint32_t)p.rows || r.keys[b] != run) return;
-    if (a && r.keys[a] == run && r.keys[a - 1] == run) return;        // began before
-    // the first chunk that does not begin with the run, past c
-    int64_t lo = c + 1, hi = r.chunks;
-    while (lo < hi) {
-        const int64_t mid = lo + (hi - lo) / 2;
-        if (r.keys[mid * r.chunk] == run) lo = mid + 1;
-        else hi = mid;
-    }
+    __shared__ float4v part[8][33];
+    __shared__ bool longer[8];
+    constexpr int FEW = 8;
     const int x = threadIdx.x % 32, g = threadIdx.x / 32;
-    for (int64_t col0 = blockIdx.y * 32ll; col0 < p.width; col0 += gridDim.y * 32ll) {
-        const int64_t col = col0 + x;
-        float s = 0.0f;
-        if (col < p.width) {
-            if (g == 0) s = r.slots[(2 * c + 1) * r.pitch + col];
-#pragma unroll 8
-            for (int64_t k = c + 1 + g; k < lo; k += 8) s += r.slots[2 * k * r.pitch + col];
-        }
-        part[g][x] = s;
-        __syncthreads();
-        if (g == 0 && col < p.width) {
-            s = part[0][x];
+    const int64_t c0 = block_number() * 8ll, c = c0 + g;
+    uint32_t run = 0;
+    bool begins = false;
+    if (c < r.chunks - 1) {
+        const uint32_t a = (uint32_t)(c * r.chunk), b = a + r.chunk;
+        run = r.keys[b - 1];
+        begins = run < (uint32_t)p.rows && r.keys[b] == run &&
+                 !(a && r.keys[a] == run && r.keys[a - 1] == run);    // began before
+    }
+    // how many of the next 32 chunks begin with it
+    const int64_t k = c + 1 + x;
+    const uint64_t with = __ballot(begins && k < r.chunks && r.keys[k * r.chunk] == run);
+    const int more = __popc((uint32_t)(with >> (threadIdx.x & 32)));
+    if (x == 0) longer[g] = more > FEW;
+    __syncthreads();
+    auto put = [&](uint32_t row, int64_t col, const float4v &s) {
 #pragma unroll
-            for (int i = 1; i < 8; i++) s += part[i][x];
-            put1(p.dtable, p.out_dtype, (int64_t)run * p.dtable_row + col, s * p.scale);
+        for (int e = 0; e < 4; e++)
+            if (col + e < p.width)
+                put1(p.dtable, p.out_dtype, (int64_t)row * p.dtable_row + col + e, s[e] * p.scale);
+    };
+    auto slot = [&](int64_t at, int64_t col) {               // slots are whole eights of columns
+        return *(const float4v *)(r.slots + at * r.pitch + col);
+    };
+    if (begins && more <= FEW)
+        for (int64_t col = blockIdx.y * 128ll + x * 4; col < p.width; col += gridDim.y * 128ll) {
+            float4v s = slot(2 * c + 1, col), v[FEW];
+#pragma unroll
+            for (int o = 0; o < FEW; o++)
+                if (o < more) v[o] = slot(2 * (c + 1 + o), col);
+#pragma unroll
+            for (int o = 0; o < FEW; o++)
+                if (o < more) s += v[o];
+            put(run, col, s);
         }
-        __syncthreads();
+    for (int i = 0; i < 8; i++) {
+        if (!longer[i]) continue;                // the block's branch
+        const int64_t from = c0 + i;
+        const uint32_t row = r.keys[(from + 1) * r.chunk - 1];
+        // the first chunk that does not begin with it, 256 looked at at a time
+        int64_t end = from + 1;
+        for (int n = 256; n == 256; end += n) {
+            const int64_t at = end + threadIdx.x;
+            n = __syncthreads_count(at < r.chunks && r.keys[at * r.chunk] == row);
+        }
+        for (int64_t col0 = blockIdx.y * 128ll; col0 < p.width; col0 += gridDim.y * 128ll) {
+            const int64_t col = col0 + x * 4;
+            float4v s = {0, 0, 0, 0};
+            if (col < p.width) {
+                if (g == 0) s = slot(2 * from + 1, col);
+#pragma unroll 8
+                for (int64_t at = from + 1 + g; at < end; at += 8) s += slot(2 * at, col);
+            }
+            __syncthreads();
+            part[g][x] = s;
+            __syncthreads();
+            if (g == 0 && col < p.width) {
+                s = part[0][x];
+#pragma unroll
+                for (int o = 1; o < 8; o++) s += part[o][x];
+                put(row, col, s);
+            }
+        }
     }
 }
 
@@ -338,13 +513,45 @@ int check_embedding_grad(const SeqEmbeddingGrad *p) {
 int64_t chunk_of(int64_t tokens) { return tokens <= 1 << 16 ? 32 : (tokens <= 1 << 22 ? 64 : 256); }
 int64_t aligned256(int64_t n) { return (n + 255) / 256 * 256; }
 
+// Rows, slabs of columns and chunks of tokens of the symbols' kernel; chunks fill the chip
+// and have 16 tokens a wave at least.
+struct SymbolPlan { int waves, slabs; int64_t chunk, chunks; };
+bool few_symbols(const SeqEmbeddingGrad &p) { return p.rows <= kSymbolRows; }
+SymbolPlan symbol_plan(const SeqEmbeddingGrad &p) {
+    SymbolPlan r;
+    r.waves = p.rows <= 40 ? 4 : 2;              // 80 KB of LDS at most
+    if (p.rows > 80) r.waves = 1;
+    r.slabs = (int)((p.width + kSymbolCols - 1) / kSymbolCols);
+    const int64_t lds = r.waves * (p.rows + 1) * kSymbolCols * 4, fit = (160 << 10) / lds;
+    int64_t chunks = 256 * (fit < 8 ? fit : 8) / r.slabs;
+    const int64_t most = (p.tokens + 16 * r.waves - 1) / (16 * r.waves);
+    if (chunks < 1) chunks = 1;
+    if (chunks > most) chunks = most;
+    r.chunk = (p.tokens + chunks - 1) / chunks;
+    r.chunks = (p.tokens + r.chunk - 1) / r.chunk;
+    return r;
+}
+template <typename T> void launch_symbols(const SeqEmbeddingGrad &p, float *partial, hipStream_t s) {
+    const SymbolPlan r = symbol_plan(p);
+    const unsigned grid = (unsigned)(r.chunks * r.slabs);
+    const size_t lds = (size_t)r.waves * (p.rows + 1) * kSymbolCols * 4;
+    const bool pairs = !((uintptr_t)p.d_out % (2 * sizeof(T))) && p.dout_row % 2 == 0 && p.width % 2 == 0;
+    if (pairs) embed_symbols<T, true><<<grid, r.waves * 64, lds, s>>>(p, r.slabs, r.chunk, partial);
+    else embed_symbols<T, false><<<grid, r.waves * 64, lds, s>>>(p, r.slabs, r.chunk, partial);
+    embed_chunks<<<(unsigned)((p.rows * p.width + 31) / 32), 1024, 0, s>>>(p, r.chunks, partial);
+}
+
 struct GradPlan {
     int passes, bits;
     int64_t tile, tiles, chunk, chunks, pitch;
     int64_t keys, counts, slots, total;          // bytes of one list, of the rest; offsets
 };
 GradPlan grad_plan(const SeqEmbeddingGrad &p) {
-    GradPlan r;
+    GradPlan r = {};
+    if (few_symbols(p)) {
+        r.total = 4 * symbol_plan(p).chunks * p.rows * p.width;
+        return r;
+    }
     int bits = 1;
     while (bits < 31 && (1ll << bits) <= p.rows) bits++;              // holds `rows` itself
     r.passes = (bits + 8) / 9;
@@ -426,6 +633,14 @@ extern "C" int seq_embedding_grad(const SeqEmbeddingGrad *p, void *stream) {
     const seq::GradPlan plan = seq::grad_plan(*p);
     if (p->workspace_bytes < plan.total || ((uintptr_t)p->workspace & 255)) return CO_ERR_DATA;
     char *ws = (char *)p->workspace;
+    if (seq::few_symbols(*p)) {
+        switch (p->dtype) {
+            case SEQ_FP32: seq::launch_symbols<float>(*p, (float *)ws, s); break;
+            case SEQ_BF16: seq::launch_symbols<__bf16>(*p, (float *)ws, s); break;
+            default: seq::launch_symbols<_Float16>(*p, (float *)ws, s); break;
+        }
+        return seq::launch_status();
+    }
     uint32_t *keys[2] = {(uint32_t *)ws, (uint32_t *)(ws + plan.keys)};
     uint32_t *places[2] = {(uint32_t *)(ws + 2 * plan.keys), (uint32_t *)(ws + 3 * plan.keys)};
     seq::Sort sort = {};
@@ -461,10 +676,10 @@ extern "C" int seq_embedding_grad(const SeqEmbeddingGrad *p, void *stream) {
     }
     if (r.chunks > 1) {
         // columns of a run go to several blocks while chunks are too few to fill the chip
-        const int64_t slabs = (p->width + 31) / 32;
-        int64_t y = 4096 / r.chunks + 1;
+        const int64_t slabs = (p->width + 127) / 128, blocks = (r.chunks + 6) / 8;
+        int64_t y = 4096 / blocks + 1;
         if (y > slabs) y = slabs;
-        seq::embed_join<<<seq::grid_of(r.chunks - 1, 256, (unsigned)y), 256, 0, s>>>(*p, r);
+        seq::embed_join<<<seq::grid_of(blocks, 256, (unsigned)y), 256, 0, s>>>(*p, r);
     }
     return seq::launch_status();
 }

@@ -196,8 +196,9 @@ def embedding(tokens, table, *, scale=1.0, dtype=None):
 
 def embedding_grad(dout, tokens, rows, *, scale=1.0, dtype=torch.float32):
     """Gradient [rows, D] of embedding's table for the gradient `dout` [T, D] of its
-    output: each row the sum of its tokens' rows, in their order and in float32, times
-    scale; 0 where there is none. The result is no part of a graph."""
+    output: each row the sum of its tokens' rows, in float32 and in an order that depends
+    on the tokens alone, times scale; 0 where there is none. The result is no part of a
+    graph."""
     _no_tangents(dout)
     _matrix(dout, "dout", _FLOATS)
     T, D = dout.shape

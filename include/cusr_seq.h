@@ -178,8 +178,8 @@ typedef struct SeqEmbedding {
 int seq_embedding(const SeqEmbedding *e, void *stream);
 
 /* Gradient of the table: dtable[v] = scale * the sum of d_out[t] over the tokens t
- * with ids[t] = v, 0 where there is none. Tokens are sorted, and a row's terms are
- * added in their order. Tokens outside the table take no part. */
+ * with ids[t] = v, 0 where there is none; a row's terms are added in one order, which
+ * depends on the tokens alone. Tokens outside the table take no part. */
 typedef struct SeqEmbeddingGrad {
     int32_t struct_size;
     int32_t dtype, out_dtype; /* of d_out, of dtable */
