@@ -69,26 +69,34 @@ struct Sums {
 
 // A block's sums: every thread gets the largest value and both sums, formed in one order.
 template <int WAVES> __device__ inline Sums over_block(Sums a, const Warmth &w, float *red) {
-    auto most = [](float x, float y) { return fmaxf(x, y); };
-    auto across = [&](float x, float *at, auto op) {
-#pragma unroll
-        for (int o = 32; o; o >>= 1) x = op(x, __shfl_xor(x, o));
-        if constexpr (WAVES > 1) {
-            if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = x;
-            __syncthreads();
-            x = at[0];
-#pragma unroll
-            for (int i = 1; i < WAVES; i++) x = op(x, at[i]);
-        }
-        return x;
-    };
     Sums r;
-    r.m = across(a.m, red, most);
+    r.m = over_lanes<Larger, 64>(a.m);
+    const int wave = threadIdx.x >> 6;
+    const bool first = (threadIdx.x & 63) == 0;
+    if constexpr (WAVES > 1) {
+        if (first) red[wave] = r.m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) r.m = fmaxf(r.m, red[i]);
+    }
     const float m0 = r.m == neg_inf() ? 0.0f : r.m;
     if (a.m != neg_inf()) a.lower(m0, w);        // else s = u = 0, or NaN
-    auto add = [](float x, float y) { return x + y; };
-    r.s = across(a.s, red + WAVES, add);
-    r.u = across(a.u, red + 2 * WAVES, add);
+    r.s = over_lanes<Add, 64>(a.s);
+    r.u = over_lanes<Add, 64>(a.u);
+    if constexpr (WAVES > 1) {
+        if (first) {
+            red[WAVES + wave] = r.s;
+            red[2 * WAVES + wave] = r.u;
+        }
+        __syncthreads();
+        r.s = red[WAVES];
+        r.u = red[2 * WAVES];
+#pragma unroll
+        for (int i = 1; i < WAVES; i++) {
+            r.s += red[WAVES + i];
+            r.u += red[2 * WAVES + i];
+        }
+    }
     return r;
 }
 
@@ -135,10 +143,11 @@ __device__ inline float value_of(Key k) {
     return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o);
 }
 __device__ inline Key larger(Key a, Key b) { return a > b ? a : b; }
+// over the wave's lanes, all of them: the value first, then the place among its equals
 __device__ inline Key wave_largest(Key k) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) k = larger(k, __shfl_xor(k, o));
-    return k;
+    const uint32_t high = over_lanes<Larger, 64>((uint32_t)(k >> 32));
+    const uint32_t low = (uint32_t)(k >> 32) == high ? (uint32_t)k : 0;
+    return ((Key)high << 32) | over_lanes<Larger, 64>(low);
 }
 __device__ inline void put_top(const SeqLogprobs &p, const Warmth &w, int64_t t, int i, Key k,
                                const Row &r, bool none) {
@@ -274,6 +283,141 @@ __global__ __launch_bounds__(THREADS) void logprob_rows(SeqLogprobs p, Warmth w)
     }
 }
 
+// Few long rows: a row is cut into parts of PART pieces, a block of 256 each, which keeps its
+// values in registers and leaves its sums and its largest alternatives in the workspace;
+// a wave a row joins them. 64 rows of 32,001 in fp32 with five alternatives: ... us, with a
+// block a row 20 us.
+constexpr int kPartPieces = 1024, kMostParts = 64;
+struct Part { float m, rest, u; int32_t bad; };  // sums over a part; bad: a value was NaN or inf
+
+template <typename T>
+__global__ __launch_bounds__(256) void logprob_parts(SeqLogprobs p, Warmth w, int parts, Part *sums,
+                                                     Key *keys) {
+    constexpr int N = Sixteen<T>::n, NV = kPartPieces / 256;
+    typedef typename Sixteen<T>::vec vec;
+    __shared__ float red[12];
+    __shared__ Key best[4];
+    const int64_t block = block_number(), t = block / parts;
+    if (t >= p.tokens) return;
+    const int part = (int)(block % parts), tid = threadIdx.x, lane = tid & 63;
+    const T *x = (const T *)p.logits + t * p.row;
+    int64_t head = (int64_t)((-(uintptr_t)x & 15) / sizeof(T));
+    if (head > p.vocab) head = p.vocab;
+    const int64_t pieces = (p.vocab - head) / N, edge = p.vocab - pieces * N;
+    const vec *x4 = (const vec *)(x + head);
+    // the row's first part takes the values outside the pieces, one to a thread
+    const bool has_edge = part == 0 && tid < edge;
+    const int64_t at_edge = tid < head ? tid : pieces * N + tid;
+    const int64_t piece0 = (int64_t)part * kPartPieces + tid;
+    vec v[NV];
+    const float on_edge = has_edge ? (float)x[at_edge] : neg_inf();
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+#pragma unroll
+        for (int j = 0; j < N; j++) v[i][j] = (T)neg_inf();
+        if (piece0 + i * 256 < pieces) v[i] = x4[piece0 + i * 256];
+    }
+    float m = on_edge;
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < N; j++) m = fmaxf(m, (float)v[i][j]);
+    m = over_group<Larger, 256>(m, red);
+    const float m0 = m == neg_inf() ? 0.0f : m;
+    float rest = 0.0f, u = 0.0f, tops = 0.0f;    // values at the largest: all but one count
+    auto add = [&](float f) {
+        const float d = f - m0, e = w.exp(d);
+        if (d == 0.0f) tops += 1.0f;
+        else rest += e;
+        u += times_or_0(e, d);
+    };
+    add(on_edge);
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < N; j++) add((float)v[i][j]);
+    rest = over_group<Add, 256>(rest, red);
+    u = over_group<Add, 256>(u, red);
+    tops = over_group<Add, 256>(tops, red);
+    if (tid == 0) {
+        // a part of -inf alone adds nothing; a NaN stays one
+        Part r = {m, m == neg_inf() ? rest : rest + (tops - 1.0f), u, 0};
+        r.bad = r.rest != r.rest || m == __builtin_inff();
+        sums[t * parts + part] = r;
+    }
+    if (p.top == 0) return;
+    Key last = ~0ull;
+    auto next = [&] {                            // the thread's largest below `last`
+        Key k = 0;
+        if (has_edge) {
+            const Key e = key_of(on_edge, (uint32_t)at_edge);
+            if (e < last) k = e;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            if (piece0 + i * 256 < pieces)
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    const Key e = key_of((float)v[i][j], (uint32_t)(head + (piece0 + i * 256) * N + j));
+                    if (e < last) k = larger(k, e);
+                }
+        return k;
+    };
+    Key mine = next(), wave_best = wave_largest(mine);
+    Key *out = keys + (t * parts + part) * p.top;
+    for (int i = 0; i < p.top; i++) {
+        if (lane == 0) best[tid >> 6] = wave_best;
+        __syncthreads();
+        last = larger(larger(best[0], best[1]), larger(best[2], best[3]));
+        __syncthreads();
+        if (tid == 0) out[i] = last;             // 0: the part has no more
+        if (last == 0) continue;
+        if (__ballot(mine == last)) {            // this wave's branch
+            if (mine == last) mine = next();
+            wave_best = wave_largest(mine);
+        }
+    }
+}
+
+__global__ __launch_bounds__(64) void logprob_join(SeqLogprobs p, Warmth w, int parts,
+                                                   const Part *sums, const Key *keys) {
+    extern __shared__ __align__(8) Key lists[];  // parts x top
+    const int64_t t = block_number();
+    if (t >= p.tokens) return;
+    const int lane = threadIdx.x;
+    const int64_t id = get_id(p.ids, p.ids_64, t);
+    const float xa = id >= 0 && id < p.vocab
+                         ? get1(p.logits, p.dtype, t * p.row + id) : 0.0f;
+    Part a = {neg_inf(), 0.0f, 0.0f, 0};
+    if (lane < parts) a = sums[t * parts + lane];
+    for (int i = lane; i < parts * p.top; i += 64) lists[i] = keys[t * parts * p.top + i];
+    __syncthreads();
+    const float m = over_lanes<Larger, 64>(a.m);
+    const float m0 = m == neg_inf() ? 0.0f : m;
+    const bool bad = __ballot(a.bad) != 0;
+    // the first part with the largest value gives the one that the others are beside
+    const uint64_t with = __ballot(a.m == m);
+    const bool owner = with && lane == __ffsll((unsigned long long)with) - 1;
+    float rest = 0.0f, u = 0.0f;
+    if (a.m != neg_inf()) {
+        const float d = a.m - m0, f = w.exp(d), s = 1.0f + a.rest;
+        rest = owner ? a.rest : times_or_0(f, s);
+        u = times_or_0(f, a.u + times_or_0(s, d));
+    }
+    rest = over_group<Add, 64>(rest, nullptr);
+    u = over_group<Add, 64>(u, nullptr);
+    const bool none = m == neg_inf() && !bad;
+    Row r = none ? empty_row() : row_of(m0, bad ? __builtin_nanf("") : rest, u, w);
+    if (lane == 0) put_row(p, w, t, r, none, id, xa);
+    int at = 0;                                  // in the part's list
+    Key mine = lane < parts && p.top ? lists[lane * p.top] : 0;
+    for (int i = 0; i < p.top; i++) {
+        const Key k = wave_largest(mine);
+        if (lane == 0) put_top(p, w, t, i, k, r, none);
+        if (mine == k) mine = ++at < p.top ? lists[lane * p.top + at] : 0;
+    }
+}
+
 // Few symbols: a block takes R rows through LDS, in 16-byte pieces when they lie end to
 // end (`joined`); a thread owns a row and goes through its columns. A thread starts at a
 // column of its own where rows of a multiple of 16 bytes would meet in the banks.
@@ -388,11 +532,14 @@ __device__ inline RowGrad grad_of(const SeqLogprobsGrad &p, const Warmth &w, int
     return r;
 }
 
+// A row is cut among `cuts` blocks, in turns of 256 pieces.
 template <typename T>
-__global__ __launch_bounds__(256) void logprob_grad_rows(SeqLogprobsGrad p, Warmth w, bool same) {
+__global__ __launch_bounds__(256) void logprob_grad_rows(SeqLogprobsGrad p, Warmth w, bool same,
+                                                         int cuts) {
     constexpr int N = Sixteen<T>::n;
     typedef typename Sixteen<T>::vec vec;
-    const int64_t t = block_number();
+    const int64_t t = cuts == 1 ? block_number() : block_number() / cuts;
+    const int cut = cuts == 1 ? 0 : block_number() % cuts;
     if (t >= p.tokens) return;
     const T *x = (const T *)p.logits + t * p.row;
     T *dx = (T *)p.dlogits + t * p.drow;
@@ -409,7 +556,7 @@ __global__ __launch_bounds__(256) void logprob_grad_rows(SeqLogprobsGrad p, Warm
         return (T)(j == id ? r.own : r.of(f, w));
     };
 #pragma unroll 4
-    for (int64_t i = threadIdx.x; i < pieces; i += 256) {
+    for (int64_t i = cut * 256 + threadIdx.x; i < pieces; i += cuts * 256) {
         vec v = {};
         if (!r.skip) {
             v = x4[i];
@@ -418,7 +565,7 @@ __global__ __launch_bounds__(256) void logprob_grad_rows(SeqLogprobsGrad p, Warm
         }
         d4[i] = v;
     }
-    for (int64_t i = threadIdx.x; i < edge; i += 256) {
+    for (int64_t i = cut * 256 + threadIdx.x; i < edge; i += cuts * 256) {
         const int64_t j = i < head ? i : pieces * N + i;
         dx[j] = r.skip ? (T)0.0f : value((float)x[j], j);
     }
@@ -481,8 +628,22 @@ void launch_rows(const SeqLogprobs &p, const Warmth &w, hipStream_t s) {
     if (p.top) logprob_rows<T, THREADS, true><<<grid, THREADS, 0, s>>>(p, w);
     else logprob_rows<T, THREADS, false><<<grid, THREADS, 0, s>>>(p, w);
 }
+// Parts of a row where rows are few and long; 0: a block a row
+int parts_of(const SeqLogprobs &p) {
+    const int n = 16 / type_bytes(p.dtype);
+    const int64_t parts = (p.vocab / n + kPartPieces - 1) / kPartPieces;
+    return p.tokens < 512 && parts > 1 && parts <= kMostParts ? (int)parts : 0;
+}
 template <typename T> void launch_logprobs(const SeqLogprobs &p, hipStream_t s) {
     const Warmth w = make_warmth(p.temperature);
+    const int parts = parts_of(p);
+    if (parts) {
+        Part *sums = (Part *)p.workspace;
+        Key *keys = (Key *)(sums + p.tokens * parts);
+        logprob_parts<T><<<(unsigned)(p.tokens * parts), 256, 0, s>>>(p, w, parts, sums, keys);
+        logprob_join<<<(unsigned)p.tokens, 64, (size_t)parts * p.top * sizeof(Key), s>>>(p, w, parts, sums, keys);
+        return;
+    }
     const int rows = symbol_rows_of(p.vocab, p.dtype);
     if (rows) {
         const dim3 grid((unsigned)((p.tokens + rows - 1) / rows));
@@ -517,14 +678,20 @@ template <typename T> void launch_grad(const SeqLogprobsGrad &p, hipStream_t s) 
     }
     const bool same = !(((uintptr_t)p.logits ^ (uintptr_t)p.dlogits) & 15) &&
                       (p.row - p.drow) % Sixteen<T>::n == 0;
-    logprob_grad_rows<T><<<grid_of(p.tokens, 256), 256, 0, s>>>(p, w, same);
+    // blocks to fill the chip, with a turn of pieces each at least
+    const int64_t turns = (p.vocab / Sixteen<T>::n + 255) / 256;
+    int64_t cuts = p.tokens < 2048 ? 2048 / p.tokens : 1;
+    if (cuts > turns) cuts = turns;
+    if (cuts < 1) cuts = 1;
+    logprob_grad_rows<T><<<grid_of(p.tokens * cuts, 256), 256, 0, s>>>(p, w, same, (int)cuts);
 }
 
 }  // namespace seq
 
 extern "C" int64_t seq_logprobs_workspace(const SeqLogprobs *p) {
     const int rc = seq::check_logprobs(p);
-    return rc == CO_OK ? 0 : (rc > 0 ? -rc : rc);
+    if (rc != CO_OK) return rc > 0 ? -rc : rc;
+    return p->tokens * seq::parts_of(*p) * (int64_t)(sizeof(seq::Part) + p->top * sizeof(seq::Key));
 }
 
 extern "C" int seq_logprobs(const SeqLogprobs *p, void *stream) {
@@ -533,6 +700,9 @@ extern "C" int seq_logprobs(const SeqLogprobs *p, void *stream) {
     if (p->tokens == 0) return CO_OK;
     if (!p->logits || !p->ids || !p->logp || !p->entropy || (p->top && (!p->top_logp || !p->top_ids)))
         return CO_ERR_NULLARG;
+    const int64_t bytes = seq_logprobs_workspace(p);
+    if (bytes && !p->workspace) return CO_ERR_NULLARG;
+    if (p->workspace_bytes < bytes || ((uintptr_t)p->workspace & 15)) return CO_ERR_DATA;
     hipStream_t s = (hipStream_t)stream;
     switch (p->dtype) {
         case SEQ_FP32: seq::launch_logprobs<float>(*p, s); break;

@@ -72,15 +72,43 @@ inline bool in_eights(const void *p, int64_t row) {
     return !p || (!((uintptr_t)p & 15) && row % 8 == 0);
 }
 
-// Sum and largest value over a group of G threads (a power of two up to the block's
-// 1,024): in a wave by exchanges, beyond through LDS, `red` with a float for each wave.
-// Every thread gets the result, formed in one order.
+// Reductions over lanes by exchanges that stay in vector registers (a wave's sum by way of
+// the LDS crossbar waits for it six times): lanes 1 and 2 apart, mirrored eights and
+// sixteens, whose halves are alike by then, and swapped sixteens and halves.
 struct Add { static __device__ float of(float a, float b) { return a + b; } };
 // keeps a NaN, as fmaxf would not
 struct Most { static __device__ float of(float a, float b) { return a > b || a != a ? a : b; } };
+// drops a NaN
+struct Larger {
+    static __device__ float of(float a, float b) { return fmaxf(a, b); }
+    static __device__ uint32_t of(uint32_t a, uint32_t b) { return a > b ? a : b; }
+};
+template <int CTRL, typename T> __device__ inline T moved(T x) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL,
+                                                             0xf, 0xf, false));
+}
+// over G lanes side by side, a power of two up to 64; every lane gets the result
+template <typename Op, int G, typename T> __device__ inline T over_lanes(T x) {
+    if constexpr (G >= 2) x = Op::of(x, moved<0xb1>(x));
+    if constexpr (G >= 4) x = Op::of(x, moved<0x4e>(x));
+    if constexpr (G >= 8) x = Op::of(x, moved<0x141>(x));
+    if constexpr (G >= 16) x = Op::of(x, moved<0x140>(x));
+    if constexpr (G >= 32) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        x = Op::of(__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1]));
+    }
+    if constexpr (G >= 64) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        x = Op::of(__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1]));
+    }
+    return x;
+}
+// over G threads, up to the block's 1,024: beyond a wave through LDS, `red` with a float
+// for each wave. Every thread gets the result, formed in one order.
 template <typename Op, int G> __device__ inline float over_group(float x, float *red) {
-#pragma unroll
-    for (int o = (G < 64 ? G : 64) / 2; o; o >>= 1) x = Op::of(x, __shfl_xor(x, o));
+    x = over_lanes<Op, (G < 64 ? G : 64)>(x);
     if constexpr (G > 64) {
         __syncthreads();                     // red may still be read from a call before
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;

@@ -384,6 +384,9 @@ LOGPROBS = [
     (33, 1000, FP, 10, 0.3, 1.0), (7, 4099, BF, 64, 0.0, 1.0), (5, 8193, F32, 3, 0.0, 0.8),
     (4, 32001, F32, 5, 0.0, 0.8), (3, 32001, BF, 20, 0.9, 1.0), (1030, 5003, BF, 2, 0.0, 1.0),
     (2, 131071, BF, 64, 0.0, 1.0), (2, 200000, F32, 2, 0.0, 0.1), (0, 50, BF, 2, 0.0, 1.0),
+    # enough rows for a block each
+    (520, 9001, F32, 7, 0.1, 1.0), (600, 33000, FP, 64, 0.0, 0.9), (512, 4104, F32, 1, 0.9, 1.0),
+    (1, 600000, F32, 64, 0.0, 1.0), (511, 8200, BF, 3, 0.0, 1.0),
 ]
 
 
@@ -437,12 +440,11 @@ def test_token_logprobs_grad(ops, T, V, dt, top, share, temperature):
                                             temperature=temperature).any())
 
 
-@pytest.mark.parametrize("V", [21, 256, 3001, 40000])
+@pytest.mark.parametrize("V,T", [(21, 12), (256, 12), (3001, 12), (40000, 12), (6001, 520)])
 @pytest.mark.parametrize("dt", [F32, BF])
-def test_logprobs_of_sure_rows(ops, V, dt):
+def test_logprobs_of_sure_rows(ops, V, T, dt):
     """Rows of nearly all weight on one symbol keep the relative precision of the rest, in
     the log-probability, in the entropy and in the gradient."""
-    T = 12
     x, _ = logits_case(T, V, dt, 0.0, spread=1.0)
     tokens = (torch.arange(T, device=DEV) * 7) % V
     gap = torch.linspace(4.0, 40.0, T, device=DEV) + math.log(V)
@@ -468,9 +470,10 @@ def test_logprobs_of_sure_rows(ops, V, dt):
     assert r["p"].shape == (T, V)
 
 
-@pytest.mark.parametrize("V", [7, 256, 700, 5000, 33000])
+@pytest.mark.parametrize("V,reps", [(7, 1), (256, 1), (700, 1), (5000, 1), (5000, 60), (33000, 1),
+                                    (33000, 60), (300001, 1)])
 @pytest.mark.parametrize("dt", [F32, BF, FP])
-def test_logprobs_of_odd_rows(ops, V, dt):
+def test_logprobs_of_odd_rows(ops, V, reps, dt):
     """All -inf, all the same, all but one -inf, NaN, +inf, the type's lowest value, tokens
     outside the vocabulary, and a token that is not allowed."""
     low = torch.finfo(dt).min
@@ -486,7 +489,11 @@ def test_logprobs_of_odd_rows(ops, V, dt):
     x[9, 2] = float("-inf")
     tokens = torch.tensor([0, V - 1, V // 2, 0, 1, 2, 0, -1, V, 2], device=DEV)
     top = min(V, 9)
-    logp, entropy, tl, ti, stats = ops.token_logprobs(x, tokens, top=top, return_stats=True)
+    x, tokens = x.repeat(reps, 1), tokens.repeat(reps)
+    out = ops.token_logprobs(x, tokens, top=top, return_stats=True)
+    assert all(torch.equal(o[:10].nan_to_num(7.0), o[-10:].nan_to_num(7.0)) for o in out)
+    x, tokens = x[-10:], tokens[-10:]
+    logp, entropy, tl, ti, stats = (o[-10:] for o in out)
     ninf = float("-inf")
     assert logp[0] == ninf and entropy[0] == 0 and ti[0].tolist() == list(range(top))
     assert bool((tl[0] == ninf).all())
@@ -519,25 +526,25 @@ def test_logprobs_of_odd_rows(ops, V, dt):
 
 def test_logprobs_ties(ops):
     """Equal values by column, -0 and +0 among them, over pieces, threads and edges."""
-    for V in (40, 300, 5001, 70000):
+    for T, V in ((6, 40), (6, 300), (6, 5001), (6, 70000), (515, 9000)):
         g = torch.Generator().manual_seed(V)
-        x = torch.randint(-1, 2, (6, V), generator=g).to(BF)
+        x = torch.randint(-1, 2, (T, V), generator=g).to(BF)
         x[x == 0] *= -1.0
         x[:, ::3] = x[:, ::3].abs()
         x = x.to(DEV)
         for xx in layouts(x):
-            ti = ops.token_logprobs(xx, ids(6, V, 1), top=40)[3]
+            ti = ops.token_logprobs(xx, ids(T, V, 1), top=40)[3]
             want = (x.double() + 0.0).cpu().sort(dim=1, descending=True, stable=True).indices
             assert torch.equal(ti.cpu(), want[:, :40])
 
 
 def test_logprobs_alternatives_side_by_side(ops):
     """The largest values in one thread's pieces, in falling and rising order."""
-    for V in (600, 9000, 131071):
-        x = torch.linspace(5, -5, V, device=DEV)[None].repeat(2, 1)
+    for T, V in ((2, 600), (2, 9000), (512, 9000), (2, 131071)):
+        x = torch.linspace(5, -5, V, device=DEV)[None].repeat(T, 1)
         x[1] = x[1].flip(0)
         x[:, 2048:2048 + 64] += 20.0
-        out = ops.token_logprobs(x, ids(2, V, 1), top=64)
+        out = ops.token_logprobs(x, ids(T, V, 1), top=64)
         assert torch.equal(out[3].cpu(), x.cpu().sort(dim=1, descending=True, stable=True)
                            .indices[:, :64])
 
