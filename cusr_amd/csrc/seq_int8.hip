@@ -385,11 +385,6 @@ template <typename O> void launch_tiles(const SeqInt8Product &p, bool pieces, hi
 
 }  // namespace seq
 
-extern "C" int64_t seq_int8_product_workspace(const SeqInt8Product *p) {
-    const int rc = seq::check_int8(p);
-    return rc == CO_OK ? 0 : (rc > 0 ? -rc : rc);
-}
-
 extern "C" int seq_int8_product(const SeqInt8Product *p, void *stream) {
     const int rc = seq::check_int8(p);
     if (rc != CO_OK) return rc;

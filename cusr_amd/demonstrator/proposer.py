@@ -1,6 +1,6 @@
 """A learned proposer of expressions: search by sampling, fitting, reinforcing.
 
-    python -m cusr_amd.demonstrator.proposer [--rounds 10] [--population 1024]
+    python -m cusr_amd.demonstrator.proposer [--rounds 10] [--population 1024] [--fused] [--int8]
 
 A small causal model emits prefix programs symbol by symbol; KernelLM fits
 their constants to the data on the device; the fits' losses become rewards,
@@ -16,6 +16,11 @@ demonstrator, cusr/demonstrator/pipeline.py); this shows the sequence operators
              positions, packed attention, the policy loss's log-probabilities
   training   the same under autograd, the policy loss's gradient through them
 
+The layers around attention (cusr_amd.kernel.seq_layers) come in by choice: `fused`
+makes each lookup, and each norm with the residual's addition before it, one kernel
+in every pass; `int8` samples with 8-bit products; a trainer's entropy_coef holds up the
+policy's entropy; alternatives() says what a policy would have written instead.
+
 Symbols are pop.bin's: constants, variables, unary and binary operators. A
 symbol that cannot complete a program of the allowed length or number of
 constants has the logit -inf, in sampling and in training.
@@ -30,7 +35,7 @@ import torch
 
 from cusr_amd.benchmark import popio
 from cusr_amd.demonstrator.co_backend import KernelLM
-from cusr_amd.kernel import seq_ops
+from cusr_amd.kernel import seq_layers, seq_ops
 
 BINARY = (1, 2, 3, 32)                  # + - * protected /
 UNARY = (14, 15, 33, 34)                # sin cos clamped exp, square
@@ -77,10 +82,11 @@ class Population:
 
 class Proposer:
     """Causal model: layers of attention (grouped heads, rotary positions) and
-    a gated map, parameters in float32, products in bfloat16."""
+    a gated map, parameters in float32, products in bfloat16. fused: lookups and norms
+    as one kernel each (the same model, other roundings)."""
 
     def __init__(self, n_vars, *, width=128, layers=2, heads=4, kv_heads=2, longest=31,
-                 most_constants=8, seed=0, device="cuda:0"):
+                 most_constants=8, seed=0, device="cuda:0", fused=False):
         if width % heads or heads % kv_heads or (width // heads) % 8:
             raise ValueError("width must be heads times a multiple of 8, heads a multiple of "
                              "kv_heads")
@@ -88,7 +94,7 @@ class Proposer:
             raise ValueError("longest must be positive and most_constants not negative")
         self.symbols = Symbols(n_vars)
         self.heads, self.kv_heads, self.d = heads, kv_heads, width // heads
-        self.longest, self.most_constants = longest, most_constants
+        self.longest, self.most_constants, self.fused = longest, most_constants, fused
         self.device = torch.device(device)
         g = torch.Generator().manual_seed(seed)
         V, kv = self.symbols.size, kv_heads * self.d
@@ -115,6 +121,8 @@ class Proposer:
 
     def _logits(self, inputs, positions, attend):
         """Logits [T, V] of input symbols; attend(layer, q, k, v) -> o."""
+        if self.fused:
+            return self._fused(inputs, positions, attend, None)
         p, bf = self.parameters, torch.bfloat16
         x = p["embed"][inputs]
         kv = self.kv_heads * self.d
@@ -128,6 +136,46 @@ class Proposer:
             x = x + ((a * torch.sigmoid(a) * b) @ p[f"down{i}"].to(bf)).float()
         return (self._norm(x).to(bf) @ p["out"].to(bf)).float()
 
+    @torch.no_grad()
+    def int8_weights(self):
+        """The products' weights as 8-bit integers with a scale for each channel."""
+        return {k: seq_layers.quantize_rows(v.t()) for k, v in self.parameters.items()
+                if k != "embed"}
+
+    def _fused(self, inputs, positions, attend, weights):
+        """_logits with a kernel for each lookup, and for each norm and the addition before
+        it. weights: None, or int8_weights, for 8-bit products of the norms' and the
+        gated maps' outputs and attention's."""
+        p, bf = self.parameters, torch.bfloat16
+
+        def product(name, x):
+            if weights is None:
+                return x @ p[name].to(bf)
+            return seq_layers.int8_product(*x, *weights[name])
+
+        def normed(x, residual=None):
+            if weights is not None:
+                q, scale, *h = seq_layers.rms_norm_int8(x, residual=residual)
+                return (q, scale), (h[0] if h else x)
+            if residual is None:
+                return seq_layers.rms_norm(x, dtype=bf), x
+            return seq_layers.rms_norm(x, residual=residual, dtype=bf)
+
+        n, x = normed(seq_layers.embedding(inputs, p["embed"]))
+        kv = self.kv_heads * self.d
+        for i in range(self.layers):
+            qkv = product(f"qkv{i}", n)
+            q, k, v = (t.unflatten(1, (-1, self.d)) for t in qkv.split([self.width, kv, kv], 1))
+            q, k = seq_ops.rotary(q, k, positions, self.table)
+            o = attend(i, q, k, v).flatten(1)
+            n, x = normed(product(f"o{i}", o if weights is None else seq_layers.quantize_rows(o)),
+                          x)
+            a, b = product(f"up{i}", n).chunk(2, 1)
+            m = a * torch.sigmoid(a) * b
+            n, x = normed(product(f"down{i}", m if weights is None else seq_layers.quantize_rows(m)),
+                          x)
+        return product("out", n).float()
+
     def logits(self, pop):
         """Logits [T, V] of a population's symbols, forbidden ones -inf."""
         def attend(_, q, k, v):
@@ -137,8 +185,10 @@ class Proposer:
                                                                            float("-inf"))
 
     @torch.no_grad()
-    def sample(self, M, generator=None):
-        """M programs, one symbol a step for all of them."""
+    def sample(self, M, generator=None, int8=False):
+        """M programs, one symbol a step for all of them. int8: with 8-bit products, whose
+        weights are made from the present parameters at the start."""
+        weights = self.int8_weights() if int8 else None
         dev, V, cap = self.device, self.symbols.size, self.longest
         shape = (self.layers, M, cap, self.kv_heads, self.d)
         keys, values = (torch.empty(shape, dtype=torch.bfloat16, device=dev) for _ in "kv")
@@ -154,7 +204,8 @@ class Proposer:
                 return seq_ops.attention(q, keys[i].flatten(0, 1), values[i].flatten(0, 1), cu_q,
                                          cu_k, k_lens=here + 1)
 
-            z = self._logits(last, here, attend)
+            z = self._logits(last, here, attend) if weights is None else \
+                self._fused(last, here, attend, weights)
             # what is left to write has to fit, with a leaf for every open subtree
             ok = open_[:, None] - 1 + self.arity[None] <= cap - t - 1
             ok[:, 0] = False
@@ -180,6 +231,14 @@ class Proposer:
         return [self.symbols.program(flat[a:b]) for a, b in zip(cu[:-1], cu[1:])]
 
     @torch.no_grad()
+    def alternatives(self, pop, top=3, temperature=1.0):
+        """What the present policy makes of each of the population's symbols: (log-probability
+        [T], entropy [T], the `top` likeliest symbols' log-probabilities [T, top], those
+        symbols [T, top]). A symbol that is not allowed there comes last, at -inf."""
+        return seq_layers.token_logprobs(self.logits(pop), pop.symbols, temperature=temperature,
+                                         top=min(top, self.symbols.size))
+
+    @torch.no_grad()
     def log_probabilities(self, pop):
         """[T] of the population's symbols under the present parameters."""
         z, zero = self.logits(pop), torch.zeros(len(pop.symbols), device=self.device)
@@ -192,11 +251,17 @@ class Trainer:
     top: the share of a population, by reward, that is learnt from. A search
     wants the best program rather than a good mean, so it learns from the best
     few, by how far they pass the last of them; 1 learns from all, by how far
-    they pass the mean."""
+    they pass the mean.
+    entropy_coef: weight of the policy's mean entropy over the symbols that are learnt
+    from, which is added to what is reinforced."""
 
-    def __init__(self, proposer, *, rate=3e-3, clip=0.2, kl_coef=0.01, epochs=4, top=1.0):
+    def __init__(self, proposer, *, rate=3e-3, clip=0.2, kl_coef=0.01, epochs=4, top=1.0,
+                 entropy_coef=0.0):
         if not 0.0 < top <= 1.0:
             raise ValueError("top must be a share of the population")
+        if not math.isfinite(entropy_coef):
+            raise ValueError("entropy_coef must be finite")
+        self.entropy_coef = entropy_coef
         self.p, self.clip, self.kl_coef, self.epochs = proposer, clip, kl_coef, epochs
         self.top = top
         self.start = {k: v.detach().clone() for k, v in proposer.parameters.items()}
@@ -222,9 +287,13 @@ class Trainer:
         weights = (used / pop.lengths.float() / used.sum())[pop.sequence]
         losses = []
         for _ in range(self.epochs):
-            loss, _ = seq_ops.policy_loss(self.p.logits(pop), pop.symbols, old, advantage,
+            z = self.p.logits(pop)
+            loss, _ = seq_ops.policy_loss(z, pop.symbols, old, advantage,
                                           logp_ref=ref, weights=weights,
                                           clip=(self.clip, self.clip), kl_coef=self.kl_coef)
+            if self.entropy_coef:
+                entropy = seq_layers.token_logprobs(z, pop.symbols)[1]
+                loss = loss - self.entropy_coef * (weights * entropy).sum()
             self.opt.zero_grad(set_to_none=True)
             loss.backward()
             self.opt.step()
@@ -240,8 +309,9 @@ def rewards_of(losses, y):
 
 
 def search(X, y, *, rounds=10, population=1024, max_iter=10, seed=0, proposer=None, trainer=None,
-           backend=None, log=print):
-    """Rounds of sampling, fitting and training. Returns (best, history): the
+           backend=None, log=print, int8=False):
+    """Rounds of sampling (int8: with 8-bit products), fitting and training. Returns (best,
+    history): the
     best program as (loss, (nt, nv, ci), constants), (inf, None, None) when none
     was fitted, and each round's mean and best reward."""
     X, y = np.asarray(X, np.float64), np.asarray(y, np.float64)
@@ -252,7 +322,7 @@ def search(X, y, *, rounds=10, population=1024, max_iter=10, seed=0, proposer=No
     rng = np.random.default_rng(seed)
     best, history = (math.inf, None, None), []
     for i in range(rounds):
-        pop = p.sample(population, generator=g)
+        pop = p.sample(population, generator=g, int8=int8)
         native = p.programs(pop)
         inits = [rng.normal(size=int(np.sum(n[0] == popio.NODE_CONST))) for n in native]
         fits = lm.fit_batch(None, inits, X, y, native=native)
@@ -274,11 +344,15 @@ def main(argv=None):
     ap.add_argument("--rounds", type=int, default=10)
     ap.add_argument("--population", type=int, default=1024)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--fused", action="store_true", help="lookups and norms as one kernel each")
+    ap.add_argument("--int8", action="store_true", help="sample with 8-bit products")
     a = ap.parse_args(argv)
     rng = np.random.default_rng(a.seed)
     X = rng.uniform(-2, 2, size=(512, 2))
     y = 1.5 * np.sin(0.8 * X[:, 0]) * X[:, 1] + 0.5
-    best, _ = search(X, y, rounds=a.rounds, population=a.population, seed=a.seed)
+    p = Proposer(X.shape[1], seed=a.seed, fused=a.fused)
+    best, _ = search(X, y, rounds=a.rounds, population=a.population, seed=a.seed, proposer=p,
+                     int8=a.int8)
     if best[1] is None:
         print("no program was fitted")
         return

@@ -79,8 +79,7 @@ class SeqInt8Product(ctypes.Structure):
     """cusr_seq.h SeqInt8Product."""
     _fields_ = [("struct_size", _I32), ("out_dtype", _I32), ("m", _I64), ("n", _I64),
                 ("inner", _I64), ("a_row", _I64), ("w_row", _I64), ("o_row", _I64), ("a", _P),
-                ("w", _P), ("a_scale", _P), ("w_scale", _P), ("o", _P), ("workspace", _P),
-                ("workspace_bytes", _I64)]
+                ("w", _P), ("a_scale", _P), ("w_scale", _P), ("o", _P)]
 
 
 class SeqLogprobs(ctypes.Structure):
@@ -125,6 +124,26 @@ def _matrix(x, name, dtypes, device=None, width=None, rows=None, most=SEQ_MAX_WI
     if not 1 <= x.shape[1] <= most:
         raise ValueError(f"{name} must have 1 to {most} columns, not {x.shape[1]}")
     return x
+
+
+def _plain(x):
+    """Whether x is a matrix of floats as the row operators take it: the common case, in a
+    few comparisons. _matrix says what is wrong with another. A tensor that answers
+    oddly is left to it too."""
+    try:
+        return (x.is_cuda and x.get_device() >= 0 and x.dtype in _DTYPES and x.dim() == 2
+                and 0 < x.shape[1] <= SEQ_MAX_WIDTH)
+    except AttributeError:
+        return False
+
+
+def _beside(x, dtypes, to, n=None):
+    """The same of a vector (of n entries) on the device of `to`."""
+    try:
+        return (x.is_cuda and x.dtype in dtypes and x.dim() == 1
+                and x.get_device() == to.get_device() and (n is None or x.shape[0] == n))
+    except AttributeError:
+        return False
 
 
 def _vector(x, name, dtypes, n, device):
@@ -186,8 +205,9 @@ def embedding(tokens, table, *, scale=1.0, dtype=None):
     default). A token outside the table gives a row of NaN. The gradient goes to the
     table; tokens outside it take no part."""
     _no_tangents(table)
-    _matrix(table, "table", _FLOATS)
-    _need(tokens, "tokens", _INTS, 1, table.device)
+    if not (_plain(table) and _beside(tokens, _INTS, table)):
+        _matrix(table, "table", _FLOATS)
+        _need(tokens, "tokens", _INTS, 1, table.device)
     scale, dtype = _number(scale, "scale"), _type(dtype, table.dtype)
     if table.requires_grad and torch.is_grad_enabled():
         return _EmbeddingFn.apply(tokens, table, scale, dtype)
@@ -226,6 +246,11 @@ def embedding_grad(dout, tokens, rows, *, scale=1.0, dtype=torch.float32):
 
 def _check_norm(x, gain, residual, eps):
     _no_tangents(x, gain, residual)
+    if (_plain(x) and (gain is None or _beside(gain, _DTYPES, x, x.shape[1]))
+            and (residual is None or (_plain(residual) and residual.shape == x.shape
+                                      and residual.get_device() == x.get_device()
+                                      and residual.dtype in (x.dtype, torch.float32)))):
+        return _number(eps, "eps", 0.0)
     _matrix(x, "x", _FLOATS)
     if residual is not None:
         types = (x.dtype,) if x.dtype is torch.float32 else (x.dtype, torch.float32)
@@ -239,11 +264,11 @@ def _norm(x, gain, residual, eps, dtype, identity=False):
     """(y, scale, h): y of dtype, or 8-bit integers with scales where dtype is int8; h the
     stream, or None without a residual."""
     (T, D), dev = x.shape, x.device
-    y = torch.empty((T, D), dtype=dtype, device=dev)
+    y = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
     scale = torch.empty(T, dtype=torch.float32, device=dev) if dtype is torch.int8 else None
     h = None
     if residual is not None:
-        h = torch.empty((T, D), dtype=residual.dtype, device=dev)
+        h = torch.empty_like(residual, memory_format=torch.contiguous_format)
         residual = _rows(residual)
     if T:
         x = _rows(x)
@@ -288,8 +313,9 @@ def rms_norm(x, gain=None, *, residual=None, eps=1e-6, dtype=None):
     float32, to `dtype` (x's by default). Returns y, or (y, h) with a residual. Gradients
     go to x, residual and gain."""
     eps, dtype = _check_norm(x, gain, residual, eps), _type(dtype, x.dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, gain, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad
+                                    or (gain is not None and gain.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         return _NormFn.apply(x, gain, residual, eps, dtype)
     y, _, h = _norm(x, gain, residual, eps, dtype)
     return y if h is None else (y, h)
@@ -298,8 +324,10 @@ def rms_norm(x, gain=None, *, residual=None, eps=1e-6, dtype=None):
 def rms_norm_int8(x, gain=None, *, residual=None, eps=1e-6):
     """rms_norm with its output as 8-bit integers: (q, scale) or, with a residual,
     (q, scale, h). q int8 [T, D] and scale float32 [T]: scale is the largest magnitude
-    of a row of y over 127, q the nearest integers to y / scale, halves to even. A row of
-    zeros has the scale 0; one with a value that is not finite the scale NaN and q 0."""
+    of a row of y over 127, q the nearest integers to y / scale, halves to even, both
+    quotients in float32. A row of zeros has the scale 0; one with a value that is not
+    finite the scale NaN and q 0. (Rows below some 1e-36 lose precision with their
+    scale.)"""
     eps = _check_norm(x, gain, residual, eps)
     _no_gradient(x=x, gain=gain, residual=residual)
     y, scale, h = _norm(x, gain, residual, eps, torch.int8)
@@ -356,6 +384,19 @@ def rms_norm_grad(dy, h, gain=None, *, dh=None, eps=1e-6, x_dtype=None):
 
 # --------------------------------------------------------------- 8-bit product
 
+_FP32 = (torch.float32,)
+
+
+def _plain_int8(a, w):
+    """Whether both are 8-bit matrices of one inner size on one GPU."""
+    try:
+        return (a.is_cuda and a.dtype is torch.int8 and w.dtype is torch.int8 and a.dim() == 2
+                and w.dim() == 2 and a.shape[1] == w.shape[1] <= SEQ_MAX_INNER
+                and w.get_device() == a.get_device() >= 0)
+    except AttributeError:
+        return False
+
+
 def int8_product(a, a_scale, w, w_scale, *, dtype=torch.bfloat16):
     """Product of 8-bit integers with scales: out[t, n] = a_scale[t] * w_scale[n] *
     sum over k of a[t, k] w[n, k], [T, N] of `dtype`.
@@ -364,16 +405,19 @@ def int8_product(a, a_scale, w, w_scale, *, dtype=torch.bfloat16):
     with w_scale float32 [N] (quantize_rows of weights [N, K], once), K up to 131,071.
     The sum is exact; the rest is formed in float32 and rounded once."""
     _no_tangents(a_scale, w_scale)
-    _need(a, "a", (torch.int8,), 2)
-    dev = a.device
-    _need(w, "w", (torch.int8,), 2, dev)
-    (T, K), N = a.shape, w.shape[0]
-    if w.shape[1] != K or K > SEQ_MAX_INNER:
-        raise ValueError(f"a and w must have the same number of columns, up to {SEQ_MAX_INNER}; "
-                         f"got {tuple(a.shape)} and {tuple(w.shape)}")
-    a_scale = _vector(a_scale, "a_scale", (torch.float32,), T, dev)
-    w_scale = _vector(w_scale, "w_scale", (torch.float32,), N, dev)
-    _no_gradient(a_scale=a_scale, w_scale=w_scale)
+    if not (_plain_int8(a, w) and _beside(a_scale, _FP32, a, a.shape[0])
+            and _beside(w_scale, _FP32, a, w.shape[0])):
+        _need(a, "a", (torch.int8,), 2)
+        _need(w, "w", (torch.int8,), 2, a.device)
+        if w.shape[1] != a.shape[1] or a.shape[1] > SEQ_MAX_INNER:
+            raise ValueError(f"a and w must have the same number of columns, up to "
+                             f"{SEQ_MAX_INNER}; got {tuple(a.shape)} and {tuple(w.shape)}")
+        _vector(a_scale, "a_scale", _FP32, a.shape[0], a.device)
+        _vector(w_scale, "w_scale", _FP32, w.shape[0], a.device)
+    if a_scale.requires_grad or w_scale.requires_grad:
+        _no_gradient(a_scale=a_scale, w_scale=w_scale)
+    dev, (T, K), N = a.device, a.shape, w.shape[0]
+    a_scale, w_scale = a_scale.contiguous(), w_scale.contiguous()
     dtype = _type(dtype, torch.bfloat16)
     out = torch.empty((T, N), dtype=dtype, device=dev)
     if not T or not N:
@@ -381,20 +425,17 @@ def int8_product(a, a_scale, w, w_scale, *, dtype=torch.bfloat16):
     if K:
         a, w = _rows(a), _rows(w)
     lib = load_library()
-    args = (_SIZE_INT8, _DTYPES[dtype], T, N, K, a.stride(0), w.stride(0), N, a.data_ptr(),
-            w.data_ptr(), a_scale.data_ptr(), w_scale.data_ptr(), out.data_ptr())
-    packed = _pack_int8(*args, 0, 0)
-    ptr, n, ws = _workspace(lib.seq_int8_product_workspace, "seq_int8_product", packed, dev)
-    if n:
-        packed = _pack_int8(*args, ptr, n)
-    _run(lib.seq_int8_product, "seq_int8_product", a.get_device(), packed)
-    del ws
+    _run(lib.seq_int8_product, "seq_int8_product", a.get_device(), _pack_int8(
+        _SIZE_INT8, _DTYPES[dtype], T, N, K, a.stride(0), w.stride(0), N, a.data_ptr(),
+        w.data_ptr(), a_scale.data_ptr(), w_scale.data_ptr(), out.data_ptr()))
     return out
 
 
 # ----------------------------------------------------------- log-probabilities
 
 def _check_logits(logits, tokens, temperature):
+    if _plain(logits) and _beside(tokens, _INTS, logits, logits.shape[0]):
+        return tokens.contiguous(), _number(temperature, "temperature", _LEAST, _MOST)
     _matrix(logits, "logits", _FLOATS, most=SEQ_MAX_ROWS)
     return (_vector(tokens, "tokens", _INTS, logits.shape[0], logits.device),
             _number(temperature, "temperature", _LEAST, _MOST))
@@ -403,13 +444,13 @@ def _check_logits(logits, tokens, temperature):
 def _logprobs(logits, tokens, temperature, top, need_stats):
     (T, V), dev = logits.shape, logits.device
 
-    def floats(*shape):
-        return torch.empty(shape, dtype=torch.float32, device=dev)
-
-    logp, entropy = floats(T), floats(T)
-    stats = floats(T, 2) if need_stats else None
-    top_logp, top_ids = (floats(T, top), torch.empty((T, top), dtype=torch.int64, device=dev)) \
-        if top else (None, None)
+    logp = torch.empty(T, dtype=torch.float32, device=dev)
+    entropy, stats, top_logp, top_ids = torch.empty_like(logp), None, None, None
+    if need_stats:
+        stats = torch.empty((T, 2), dtype=torch.float32, device=dev)
+    if top:
+        top_logp = torch.empty((T, top), dtype=torch.float32, device=dev)
+        top_ids = torch.empty_like(top_logp, dtype=torch.int64)
     if T:
         logits, lib = _rows(logits), load_library()
         args = (_SIZE_LOGPROBS, _DTYPES[logits.dtype], tokens.dtype is torch.int64, top, T, V,

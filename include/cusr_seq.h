@@ -200,10 +200,10 @@ int seq_embedding_grad(const SeqEmbeddingGrad *e, void *stream);
  * rounded to a type or to 8-bit integers with a scale for each row:
  *   h = x + residual, rounded to the stream's type (h = x without a residual);
  *   y = gain h / sqrt(mean h^2 + eps)       (gain null: 1; identity: y = h)
- *   y_dtype SEQ_INT8: y_scale = max |y| / 127, y = round(y / y_scale), halves to even;
- *   a row of zeros has the scale 0, one with a value that is not finite the scale NaN
- *   and the integers 0.
- * The stream's type is fp32 or x's. The quotients are taken from y in fp32. */
+ *   y_dtype SEQ_INT8: y_scale = max |y| / 127, y = round(y / y_scale), halves to even,
+ *   both quotients rounded to fp32; a row of zeros (or so small that its scale is 0) has
+ *   the integers 0, one with a value that is not finite those and the scale NaN.
+ * The stream's type is fp32 or x's. */
 typedef struct SeqNorm {
     int32_t struct_size;
     int32_t x_dtype, h_dtype, y_dtype, gain_dtype;
@@ -249,11 +249,8 @@ typedef struct SeqInt8Product {
     const int8_t *a, *w;
     const float *a_scale, *w_scale;
     void *o;
-    void *workspace;          /* seq_int8_product_workspace bytes, 256-aligned */
-    int64_t workspace_bytes;
 } SeqInt8Product;
 
-int64_t seq_int8_product_workspace(const SeqInt8Product *p);
 int seq_int8_product(const SeqInt8Product *p, void *stream);
 
 /* Log-probabilities of given tokens under logits [tokens, vocab], with z = logits /
