@@ -57,24 +57,27 @@ __global__ __launch_bounds__(256) void embed_rows(SeqEmbedding p, int g) {
 
 // ------------------------------------------------------------- few rows: symbols
 
-// A table of few rows: a wave keeps the sums of its tokens, 128 columns of every row, in
+// A table of up to kSymbolRows rows: a wave keeps the sums of its tokens, 128 columns of every row, in
 // LDS and reads its tokens' gradients one after the other, so no order of tokens is
 // needed. A lane adds to columns of its own, in the tokens' order, four tokens at a
 // time: where two of them have one row the later takes the earlier's sum. (LDS adds
 // floats by itself, but hardly a lane at a time: 839 us for 1.3 M tokens of 128 in fp32
-// and 22 rows.)
-constexpr int kSymbolRows = 128, kSymbolCols = 128;
+// and 22 rows.) Against sorting, that takes 126 against 229 us, with 30 rows 128 against
+// 227, with 40 rows of 1,024 columns 1,320 against 1,183 and with 80 rows 321 against 229:
+// fewer blocks find room in LDS.
+constexpr int kSymbolRows = 32, kSymbolCols = 128, kSymbolWaves = 4;
 
 template <typename T, bool PAIR>
 __global__ __launch_bounds__(256) void embed_symbols(SeqEmbeddingGrad p, int slabs, int64_t chunk,
                                                      float *partial) {
     constexpr int AHEAD = 8;                     // rows on their way
     extern __shared__ __align__(16) float sums[];            // of each wave: rows + 1 by 128
-    const int V = (int)p.rows, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    constexpr int waves = kSymbolWaves;
+    const int V = (int)p.rows, lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slab = (int)(blockIdx.x % slabs);
     const int64_t c = blockIdx.x / slabs;
-    for (int i = threadIdx.x; i < waves * (V + 1) * kSymbolCols; i += blockDim.x) sums[i] = 0.0f;
+    for (int i = threadIdx.x; i < waves * (V + 1) * kSymbolCols; i += 256) sums[i] = 0.0f;
     __syncthreads();
     // PAIR: columns 2 lane and 2 lane + 1, else lane and lane + 64
     const int64_t col0 = (int64_t)slab * kSymbolCols + (PAIR ? 2 * lane : lane);
@@ -160,7 +163,7 @@ __global__ __launch_bounds__(256) void embed_symbols(SeqEmbeddingGrad p, int sla
         ids = next;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < V * kSymbolCols; i += blockDim.x) {
+    for (int i = threadIdx.x; i < V * kSymbolCols; i += 256) {
         const int64_t col = (int64_t)slab * kSymbolCols + i % kSymbolCols;
         if (col >= p.width) continue;
         float s = sums[i];
@@ -510,21 +513,25 @@ int check_embedding_grad(const SeqEmbeddingGrad *p) {
     return CO_OK;
 }
 
-int64_t chunk_of(int64_t tokens) { return tokens <= 1 << 16 ? 32 : (tokens <= 1 << 22 ? 64 : 256); }
+// Places of a chunk: few tokens fill the chip with short ones (4,096 words of 4,096 in bf16:
+// 137 us with 16, 143 with 32; 16,384: 187, 185, with 64 214; 60,000 of 1,024: 101, 88, 98;
+// 500,000 of 128 with 64 99, with 128 131)
+int64_t chunk_of(int64_t tokens) {
+    return tokens <= 1 << 13 ? 16 : (tokens <= 1 << 16 ? 32 : (tokens <= 1 << 22 ? 64 : 256));
+}
 int64_t aligned256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Rows, slabs of columns and chunks of tokens of the symbols' kernel; chunks fill the chip
-// and have 16 tokens a wave at least.
-struct SymbolPlan { int waves, slabs; int64_t chunk, chunks; };
+// Slabs of columns and chunks of tokens of the symbols' kernel; chunks fill the chip and
+// have 16 tokens a wave at least.
+struct SymbolPlan { int slabs; int64_t chunk, chunks; };
 bool few_symbols(const SeqEmbeddingGrad &p) { return p.rows <= kSymbolRows; }
+int64_t symbol_lds(const SeqEmbeddingGrad &p) { return kSymbolWaves * (p.rows + 1) * kSymbolCols * 4; }
 SymbolPlan symbol_plan(const SeqEmbeddingGrad &p) {
     SymbolPlan r;
-    r.waves = p.rows <= 40 ? 4 : 2;              // 80 KB of LDS at most
-    if (p.rows > 80) r.waves = 1;
     r.slabs = (int)((p.width + kSymbolCols - 1) / kSymbolCols);
-    const int64_t lds = r.waves * (p.rows + 1) * kSymbolCols * 4, fit = (160 << 10) / lds;
+    const int64_t fit = (160 << 10) / symbol_lds(p), least = 16 * kSymbolWaves;
     int64_t chunks = 256 * (fit < 8 ? fit : 8) / r.slabs;
-    const int64_t most = (p.tokens + 16 * r.waves - 1) / (16 * r.waves);
+    const int64_t most = (p.tokens + least - 1) / least;
     if (chunks < 1) chunks = 1;
     if (chunks > most) chunks = most;
     r.chunk = (p.tokens + chunks - 1) / chunks;
@@ -534,10 +541,10 @@ SymbolPlan symbol_plan(const SeqEmbeddingGrad &p) {
 template <typename T> void launch_symbols(const SeqEmbeddingGrad &p, float *partial, hipStream_t s) {
     const SymbolPlan r = symbol_plan(p);
     const unsigned grid = (unsigned)(r.chunks * r.slabs);
-    const size_t lds = (size_t)r.waves * (p.rows + 1) * kSymbolCols * 4;
+    const size_t lds = (size_t)symbol_lds(p);
     const bool pairs = !((uintptr_t)p.d_out % (2 * sizeof(T))) && p.dout_row % 2 == 0 && p.width % 2 == 0;
-    if (pairs) embed_symbols<T, true><<<grid, r.waves * 64, lds, s>>>(p, r.slabs, r.chunk, partial);
-    else embed_symbols<T, false><<<grid, r.waves * 64, lds, s>>>(p, r.slabs, r.chunk, partial);
+    if (pairs) embed_symbols<T, true><<<grid, 256, lds, s>>>(p, r.slabs, r.chunk, partial);
+    else embed_symbols<T, false><<<grid, 256, lds, s>>>(p, r.slabs, r.chunk, partial);
     embed_chunks<<<(unsigned)((p.rows * p.width + 31) / 32), 1024, 0, s>>>(p, r.chunks, partial);
 }
 

@@ -226,69 +226,17 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Produ
                          (O *)(scales + 2 * T) + wave * 32 * slab_pitch<O, F>());
 }
 
-// The same for operands off 16-byte boundaries or rows that no whole number of pieces
-// fills: 128 x 128 outputs, operands by way of registers.
-constexpr int kPitch = kStep + 16;
-template <typename O, bool WIDE> __global__ __launch_bounds__(256) void int8_any(SeqInt8Product p) {
-    constexpr int T = 128, W = 64;
-    // operands, then the waves' slabs of outputs
-    __shared__ __align__(16) int8_t lds[4 * 32 * slab_pitch<float, 2>() * 4];
-    __shared__ __align__(16) float scales[2][T];
-    int8_t *as = lds, *ws = lds + T * kPitch;
-    static_assert(2 * T * kPitch <= sizeof(lds), "");
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int64_t ti, tj;
-    if (!tile_of(block_number(), (p.m + T - 1) / T, (p.n + T - 1) / T, ti, tj)) return;
-    const int64_t i0 = ti * T, j0 = tj * T;
-    const int wi = wave / 2 * W, wj = wave % 2 * W;
-    if (tid < T) {
-        scales[0][tid] = i0 + tid < p.m ? p.a_scale[i0 + tid] : 0.0f;
-        scales[1][tid] = j0 + tid < p.n ? p.w_scale[j0 + tid] : 0.0f;
-    }
-    __syncthreads();
-    int16v acc[2][2];
-#pragma unroll
-    for (int x = 0; x < 2; x++)
-#pragma unroll
-        for (int y = 0; y < 2; y++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) acc[x][y][r] = 0;
-    for (int64_t l = 0; l < p.inner; l += kStep) {
-        uint4v va[2], vw[2];
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const int at = x * 256 + tid, row = at / 4, col = at % 4 * 16;
-            va[x] = vw[x] = uint4v{0, 0, 0, 0};
-            if (i0 + row < p.m) va[x] = row_piece(p.a + (i0 + row) * p.a_row, l + col, p.inner);
-            if (j0 + row < p.n) vw[x] = row_piece(p.w + (j0 + row) * p.w_row, l + col, p.inner);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const int at = x * 256 + tid, row = at / 4, col = at % 4 * 16;
-            *(uint4v *)(as + row * kPitch + col) = va[x];
-            *(uint4v *)(ws + row * kPitch + col) = vw[x];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kStep; k += 32) {
-            int4v a[2], w[2];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const int col = k + lane / 32 * 16;
-                a[x] = *(const int4v *)(as + (wi + x * 32 + lane % 32) * kPitch + col);
-                w[x] = *(const int4v *)(ws + (wj + x * 32 + lane % 32) * kPitch + col);
-            }
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int y = 0; y < 2; y++)
-                    acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[y], a[x], acc[x][y], 0, 0, 0);
-        }
-    }
-    __syncthreads();
-    put_sums<O, WIDE, 2>(p, i0 + wi, j0 + wj, acc, scales[0] + wi, scales[1] + wj,
-                         (O *)lds + wave * 32 * slab_pitch<O, 2>());
+// Rows off 16-byte boundaries, or that no whole number of pieces fills, are laid out anew
+// first, padded with zeros: 2^g threads a row, a piece each at a time. Products that read
+// such rows as they lie took 280 us rather than 158 for 8,192 x 4,095 x 4,096, and 48 rather
+// than 29 for 24 x 4,095 x 6,144.
+__global__ __launch_bounds__(256) void int8_pack(const int8_t *from, int64_t row, int64_t rows,
+                                                 int64_t inner, int g, int8_t *to, int64_t to_row) {
+    const int64_t r = (int64_t)block_number() * (256 >> g) + (threadIdx.x >> g);
+    if (r >= rows) return;
+#pragma unroll 4
+    for (int64_t l = (threadIdx.x & ((1 << g) - 1)) * 16; l < to_row; l += 16 << g)
+        *(uint4v *)(to + r * to_row + l) = row_piece(from + r * row, l, inner);
 }
 
 // Few tokens: 16 channels a block and up to 16 M tokens, the terms cut among eight waves,
@@ -358,6 +306,34 @@ int check_int8(const SeqInt8Product *p) {
     return tiles_of(*p, 64) > SEQ_MAX_ROWS ? CO_ERR_BOUNDS : CO_OK;
 }
 
+// Whether rows are laid out anew: whole pieces on their boundaries, and 256 rows and a step
+// within 2^32 bytes
+bool needs_pack(const SeqInt8Product &p, const int8_t *x, int64_t row) {
+    return p.inner % 16 || ((uintptr_t)x & 15) || row % 16 || row < 0 || row >= 1 << 23;
+}
+int64_t packed_row(const SeqInt8Product &p) { return (p.inner + 15) / 16 * 16; }
+int64_t packed_bytes(int64_t rows, const SeqInt8Product &p) {
+    return (rows * packed_row(p) + 255) / 256 * 256;
+}
+int64_t int8_bytes(const SeqInt8Product &p) {
+    if (p.m == 0 || p.n == 0 || p.inner == 0) return 0;
+    return (needs_pack(p, p.a, p.a_row) ? packed_bytes(p.m, p) : 0) +
+           (needs_pack(p, p.w, p.w_row) ? packed_bytes(p.n, p) : 0);
+}
+void pack(const int8_t *&x, int64_t &row, int64_t rows, const SeqInt8Product &p, char *&ws,
+          hipStream_t s) {
+    if (!needs_pack(p, x, row)) return;
+    const int64_t to_row = packed_row(p);
+    int g = 0;
+    while (g < 8 && (16 << g) < to_row) g++;
+    const int64_t each = 256 >> g;
+    int8_pack<<<grid_of((rows + each - 1) / each, 256), 256, 0, s>>>(x, row, rows, p.inner, g,
+                                                                     (int8_t *)ws, to_row);
+    x = (const int8_t *)ws;
+    row = to_row;
+    ws += packed_bytes(rows, p);
+}
+
 template <int M> void launch_few(const SeqInt8Product &p, hipStream_t s) {
     int8_few<M><<<grid_of((p.n + 15) / 16, 512), 512, 0, s>>>(p);
 }
@@ -365,25 +341,28 @@ template <typename O, bool WIDE, int T> void launch_tiles(const SeqInt8Product &
     const int64_t blocks = (tiles_of(p, T) + 7) / 8 * 8;
     int8_tiles<O, WIDE, T><<<grid_of(blocks, 256), 256, kStages * tile_bytes<T>(), s>>>(p);
 }
-template <typename O, bool WIDE>
-void launch_tiles(const SeqInt8Product &p, bool pieces, hipStream_t s) {
-    if (!pieces) {
-        const int64_t blocks = (tiles_of(p, 128) + 7) / 8 * 8;
-        int8_any<O, WIDE><<<grid_of(blocks, 256), 256, 0, s>>>(p);
-    } else if (tiles_of(p, 256) >= 256) {
-        launch_tiles<O, WIDE, 256>(p, s);
-    } else if (tiles_of(p, 128) >= 128) {
-        launch_tiles<O, WIDE, 128>(p, s);
-    } else {
-        launch_tiles<O, WIDE, 64>(p, s);
-    }
+// The tiles that take the least time: 256 of them, one to a compute unit, take 9, 21 and 46
+// us for 4,096 terms (sides of 64, 128 and 256), and more take as many times as long
+// (512 x 4,096 x 4,096: 19, 19, 48 us; 1,024: 36, 24, 52; 3,000: 97, 61, 58; 4,096: 122, 80, 66).
+template <typename O, bool WIDE> void launch_tiles(const SeqInt8Product &p, hipStream_t s) {
+    auto time = [&](int64_t t, int64_t each) { return (tiles_of(p, t) + 255) / 256 * each; };
+    const int64_t t64 = time(64, 9), t128 = time(128, 21), t256 = time(256, 46);
+    if (t64 <= t128 && t64 <= t256) launch_tiles<O, WIDE, 64>(p, s);
+    else if (t128 <= t256) launch_tiles<O, WIDE, 128>(p, s);
+    else launch_tiles<O, WIDE, 256>(p, s);
 }
-template <typename O> void launch_tiles(const SeqInt8Product &p, bool pieces, hipStream_t s) {
-    if (in_eights(p.o, p.o_row) && p.n % 8 == 0) launch_tiles<O, true>(p, pieces, s);
-    else launch_tiles<O, false>(p, pieces, s);
+template <typename O> void launch_tiles(const SeqInt8Product &p, hipStream_t s) {
+    if (in_eights(p.o, p.o_row) && p.n % 8 == 0) launch_tiles<O, true>(p, s);
+    else launch_tiles<O, false>(p, s);
 }
 
 }  // namespace seq
+
+extern "C" int64_t seq_int8_product_workspace(const SeqInt8Product *p) {
+    const int rc = seq::check_int8(p);
+    if (rc != CO_OK) return rc > 0 ? -rc : rc;
+    return seq::int8_bytes(*p);
+}
 
 extern "C" int seq_int8_product(const SeqInt8Product *p, void *stream) {
     const int rc = seq::check_int8(p);
@@ -391,22 +370,33 @@ extern "C" int seq_int8_product(const SeqInt8Product *p, void *stream) {
     if (p->m == 0 || p->n == 0) return CO_OK;
     if (!p->a_scale || !p->w_scale || !p->o || (p->inner && (!p->a || !p->w)))
         return CO_ERR_NULLARG;
+    const int64_t bytes = seq::int8_bytes(*p);
+    if (bytes && !p->workspace) return CO_ERR_NULLARG;
+    if (p->workspace_bytes < bytes || (bytes && ((uintptr_t)p->workspace & 255))) return CO_ERR_DATA;
     hipStream_t s = (hipStream_t)stream;
-    // 256 rows and a step within 2^32 bytes, and whole pieces
-    const int64_t far = 1ll << 23;
-    const bool pieces = !(((uintptr_t)p->a | (uintptr_t)p->w) & 15) && p->a_row % 16 == 0 &&
-                        p->w_row % 16 == 0 && p->inner % 16 == 0 && p->a_row >= 0 &&
-                        p->w_row >= 0 && p->a_row < far && p->w_row < far;
-    if (pieces && p->m <= 64) {
-        if (p->m <= 16) seq::launch_few<1>(*p, s);
-        else if (p->m <= 32) seq::launch_few<2>(*p, s);
-        else seq::launch_few<4>(*p, s);
-        return seq::launch_status();
+    SeqInt8Product q = *p;
+    if (q.inner) {
+        char *ws = (char *)q.workspace;
+        seq::pack(q.a, q.a_row, q.m, *p, ws, s);
+        seq::pack(q.w, q.w_row, q.n, *p, ws, s);
+        q.inner = seq::packed_row(*p);           // zeros beyond it, or nothing
+    } else {
+        q.a_row = q.w_row = 0;                   // no row is read
     }
-    switch (p->out_dtype) {
-        case SEQ_FP32: seq::launch_tiles<float>(*p, pieces, s); break;
-        case SEQ_BF16: seq::launch_tiles<__bf16>(*p, pieces, s); break;
-        default: seq::launch_tiles<_Float16>(*p, pieces, s); break;
+    // Few tokens and so few channels that tiles would not fill the chip: the terms are cut
+    // (24 x 16,384 x 1,024: 21 against 31 us, 16 x 16,384 x 4,096: 20 against 32; but 16 x
+    // 4,096 x 16,384: 18 against 12, and 32 x 4,096 x 6,144: 14 against 10).
+    const int64_t sixteens = (q.m + 15) / 16, channels = (q.n + 15) / 16;
+    if (sixteens == 1 && channels <= 512) {
+        seq::launch_few<1>(q, s);
+    } else if (sixteens == 2 && channels <= 128) {
+        seq::launch_few<2>(q, s);
+    } else {
+        switch (q.out_dtype) {
+            case SEQ_FP32: seq::launch_tiles<float>(q, s); break;
+            case SEQ_BF16: seq::launch_tiles<__bf16>(q, s); break;
+            default: seq::launch_tiles<_Float16>(q, s); break;
+        }
     }
     return seq::launch_status();
 }

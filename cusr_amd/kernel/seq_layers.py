@@ -79,7 +79,8 @@ class SeqInt8Product(ctypes.Structure):
     """cusr_seq.h SeqInt8Product."""
     _fields_ = [("struct_size", _I32), ("out_dtype", _I32), ("m", _I64), ("n", _I64),
                 ("inner", _I64), ("a_row", _I64), ("w_row", _I64), ("o_row", _I64), ("a", _P),
-                ("w", _P), ("a_scale", _P), ("w_scale", _P), ("o", _P)]
+                ("w", _P), ("a_scale", _P), ("w_scale", _P), ("o", _P), ("workspace", _P),
+                ("workspace_bytes", _I64)]
 
 
 class SeqLogprobs(ctypes.Structure):
@@ -403,7 +404,8 @@ def int8_product(a, a_scale, w, w_scale, *, dtype=torch.bfloat16):
 
     a int8 [T, K] with a_scale float32 [T] (rms_norm_int8, quantize_rows), w int8 [N, K]
     with w_scale float32 [N] (quantize_rows of weights [N, K], once), K up to 131,071.
-    The sum is exact; the rest is formed in float32 and rounded once."""
+    The sum is exact; the rest is formed in float32 and rounded once. K and rows of a
+    multiple of 16 spare a copy of the operands."""
     _no_tangents(a_scale, w_scale)
     if not (_plain_int8(a, w) and _beside(a_scale, _FP32, a, a.shape[0])
             and _beside(w_scale, _FP32, a, w.shape[0])):
@@ -425,9 +427,14 @@ def int8_product(a, a_scale, w, w_scale, *, dtype=torch.bfloat16):
     if K:
         a, w = _rows(a), _rows(w)
     lib = load_library()
-    _run(lib.seq_int8_product, "seq_int8_product", a.get_device(), _pack_int8(
-        _SIZE_INT8, _DTYPES[dtype], T, N, K, a.stride(0), w.stride(0), N, a.data_ptr(),
-        w.data_ptr(), a_scale.data_ptr(), w_scale.data_ptr(), out.data_ptr()))
+    args = (_SIZE_INT8, _DTYPES[dtype], T, N, K, a.stride(0), w.stride(0), N, a.data_ptr(),
+            w.data_ptr(), a_scale.data_ptr(), w_scale.data_ptr(), out.data_ptr())
+    packed = _pack_int8(*args, 0, 0)
+    ptr, n, ws = _workspace(lib.seq_int8_product_workspace, "seq_int8_product", packed, dev)
+    if n:
+        packed = _pack_int8(*args, ptr, n)
+    _run(lib.seq_int8_product, "seq_int8_product", a.get_device(), packed)
+    del ws
     return out
 
 

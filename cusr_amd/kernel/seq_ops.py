@@ -43,8 +43,8 @@ EXPORTED = ("seq_attention", "seq_attention_workspace", "seq_attention_grad",
             "seq_attention_grad_workspace", "seq_rotary", "seq_policy_loss",
             "seq_policy_loss_workspace", "seq_embedding", "seq_embedding_grad",
             "seq_embedding_grad_workspace", "seq_norm", "seq_norm_grad",
-            "seq_norm_grad_workspace", "seq_int8_product", "seq_logprobs", "seq_logprobs_workspace",
-            "seq_logprobs_grad")
+            "seq_norm_grad_workspace", "seq_int8_product", "seq_int8_product_workspace",
+            "seq_logprobs", "seq_logprobs_workspace", "seq_logprobs_grad")
 
 
 class SeqAttention(ctypes.Structure):

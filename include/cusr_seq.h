@@ -241,7 +241,8 @@ int seq_norm_grad(const SeqNormGrad *n, void *stream);
 
 /* Product of 8-bit integers: o[i, j] = a_scale[i] w_scale[j] * sum over l of
  * a[i, l] w[j, l], the sum exact, the rest in fp32, rounded once to out_dtype.
- * a [m, inner], w [n, inner] (a row holds what one output takes). */
+ * a [m, inner], w [n, inner] (a row holds what one output takes). Operands whose address,
+ * rows or inner size are no multiples of 16 are copied into the workspace first. */
 typedef struct SeqInt8Product {
     int32_t struct_size;
     int32_t out_dtype;
@@ -249,8 +250,11 @@ typedef struct SeqInt8Product {
     const int8_t *a, *w;
     const float *a_scale, *w_scale;
     void *o;
+    void *workspace;          /* seq_int8_product_workspace bytes, 256-aligned */
+    int64_t workspace_bytes;
 } SeqInt8Product;
 
+int64_t seq_int8_product_workspace(const SeqInt8Product *p);
 int seq_int8_product(const SeqInt8Product *p, void *stream);
 
 /* Log-probabilities of given tokens under logits [tokens, vocab], with z = logits /

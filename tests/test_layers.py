@@ -217,7 +217,10 @@ def test_library_refusals():
          (dict(w=None), CO_ERR_NULLARG), (dict(a_scale=None), CO_ERR_NULLARG),
          (dict(w_scale=None), CO_ERR_NULLARG), (dict(o=None), CO_ERR_NULLARG),
          (dict(inner=131072), CO_ERR_BOUNDS), (dict(m=far), CO_ERR_BOUNDS),
-         (dict(m=1 << 30, n=1 << 30), CO_ERR_BOUNDS), (dict(out_dtype=3), CO_ERR_DATA)], dict(m=0), False)
+         (dict(m=1 << 30, n=1 << 30), CO_ERR_BOUNDS), (dict(out_dtype=3), CO_ERR_DATA),
+         (dict(inner=15), CO_ERR_NULLARG),                          # needs a workspace
+         (dict(a=4097, workspace=4096, workspace_bytes=8), CO_ERR_DATA),
+         (dict(w_row=17, workspace=4100, workspace_bytes=1 << 20), CO_ERR_DATA)], dict(m=0))
     rows = ("logits", "ids", "logp", "entropy", "stats", "top_logp", "top_ids")
     library_refuses(
         "seq_logprobs", ops.SeqLogprobs, rows,
@@ -226,9 +229,9 @@ def test_library_refusals():
          (dict(top=-1), CO_ERR_NULLARG), (dict(tokens=far), CO_ERR_BOUNDS),
          (dict(top=11), CO_ERR_BOUNDS), (dict(vocab=100, top=65), CO_ERR_BOUNDS),
          (dict(dtype=3), CO_ERR_DATA), (dict(temperature=0.0), CO_ERR_DATA),
-         (dict(vocab=40000, row=40000), CO_ERR_NULLARG),            # needs a workspace
-         (dict(vocab=40000, row=40000, workspace=4096, workspace_bytes=8), CO_ERR_DATA),
-         (dict(vocab=40000, row=40000, workspace=4100, workspace_bytes=1 << 20), CO_ERR_DATA)]
+         (dict(vocab=90000, row=90000), CO_ERR_NULLARG),            # needs a workspace
+         (dict(vocab=90000, row=90000, workspace=4096, workspace_bytes=8), CO_ERR_DATA),
+         (dict(vocab=90000, row=90000, workspace=4100, workspace_bytes=1 << 20), CO_ERR_DATA)]
         + [({n: None}, CO_ERR_NULLARG) for n in rows if n != "stats"], dict(tokens=0))
     library_refuses(
         "seq_logprobs_grad", ops.SeqLogprobsGrad, ("logits", "ids", "stats", "entropy", "dlogits"),
