@@ -36,6 +36,9 @@ Warmth make_warmth(float temperature) {
 // x y, but 0 where x is 0, whatever y
 __device__ inline float times_or_0(float x, float y) { return x == 0.0f ? 0.0f : x * y; }
 
+// t, or the lowest number for -inf, whose e is 0: no 0 * inf. A NaN shows in the sum of e.
+__device__ inline float finite(float t) { return max2(t, -3.4028235e38f); }
+
 // 16 bytes of a row
 template <typename T> struct Sixteen {
     static constexpr int n = 16 / sizeof(T);
@@ -56,7 +59,7 @@ struct Sums {
         for (int j = 0; j < N; j++) {
             const float t = x[j] - m0, e = w.exp(t);
             s += e;
-            u += times_or_0(e, t);
+            u = __builtin_fmaf(e, finite(t), u);
         }
     }
     // the sums for a larger value m0: t falls by its distance
@@ -328,7 +331,7 @@ __global__ __launch_bounds__(256) void logprob_parts(SeqLogprobs p, Warmth w, in
         const float d = f - m0, e = w.exp(d);
         if (d == 0.0f) tops += 1.0f;
         else rest += e;
-        u += times_or_0(e, d);
+        u = __builtin_fmaf(e, finite(d), u);
     };
     add(on_edge);
 #pragma unroll
@@ -465,7 +468,7 @@ __global__ __launch_bounds__(R) void logprob_symbols(SeqLogprobs p, Warmth w, bo
     columns([&](int j) {
         const float d = (float)y[j] - m0, e = w.exp(d);
         s += e;
-        u += times_or_0(e, d);
+        u = __builtin_fmaf(e, finite(d), u);
     });
     const bool none = m == neg_inf() && s == 0.0f;
     Row r = empty_row();
@@ -506,8 +509,9 @@ struct RowGrad {
     bool skip;                                   // both gradients are 0: nothing is read
     __device__ float of(float x, const Warmth &w) const {
         const float t = x - m0, prob = w.exp(t) * inverse;
-        const float lp = w.times(t) - log_sum;
-        return -times_or_0(prob, g + times_or_0(h, lp + entropy));
+        // below -256 prob is 0, and lp may be -inf
+        const float lp = max2(w.times(t) - log_sum, -256.0f);
+        return -prob * __builtin_fmaf(h, lp + entropy, g);
     }
 };
 __device__ inline RowGrad grad_of(const SeqLogprobsGrad &p, const Warmth &w, int64_t t, int64_t id,
@@ -523,7 +527,7 @@ __device__ inline RowGrad grad_of(const SeqLogprobsGrad &p, const Warmth &w, int
     r.g = w.times(dl);
     r.h = w.times(dh);
     if (!in && dl != 0.0f) r.g = __builtin_nanf("");
-    if (in && xa == neg_inf()) r.g = 0.0f;       // logp is -inf
+    if (in && w.times(xa - r.m0) - r.log_sum == neg_inf()) r.g = 0.0f;       // logp is
     r.own = r.of(xa, w) + r.g;
     // at the largest logit 1 - p is what the rest has: formed as such, for p rounds it away
     if (in && xa == r.m0)

@@ -39,11 +39,11 @@ __device__ inline float rms_factor(float sum, int64_t width, float eps) {
 // 8-bit integers of a row whose largest magnitude is `most`. The quotient by the scale is
 // rounded as a division is. A product with the scale's reciprocal is off by 2^-16 at most;
 // where that leaves the integer open, next to a half, the division is made: 8,192 rows of
-// 4,096 in bf16 take 21 us rather than 28 with a division for each value.
+// 4,096 in bf16 take 23 us at best rather than 28 with a division for each value.
 struct Bits8 {
     float scale, inverse;
     __device__ explicit Bits8(float most) {
-        scale = most < __builtin_inff() ? most / 127.0f : __builtin_nanf("");
+        scale = most < __builtin_inff() ? most * (1.0f / 127.0f) : __builtin_nanf("");
         // no number, which leaves every integer open, where the scale has not all its bits
         inverse = scale >= 0x1p-126f ? 1.0f / scale : __builtin_nanf("");
     }

@@ -172,13 +172,13 @@ def _number(x, name, least=-_FLOAT32, most=_FLOAT32):
 # ------------------------------------------------------------------ embedding
 
 def _embedding(tokens, table, scale, dtype):
-    T, D = tokens.shape[0], table.shape[1]
-    out = torch.empty((T, D), dtype=dtype, device=table.device)
+    T, (V, D) = tokens.shape[0], table.shape
+    out = table.new_empty((T, D)) if dtype is table.dtype else table.new_empty((T, D), dtype=dtype)
     if T:
-        table, tokens = _rows(table), tokens.contiguous()
+        table = _rows(table)
         _run(load_library().seq_embedding, "seq_embedding", table.get_device(), _pack_embedding(
             _SIZE_EMBEDDING, _DTYPES[table.dtype], _DTYPES[dtype], tokens.dtype is torch.int64, T,
-            table.shape[0], D, table.stride(0), D, scale, 0, tokens.data_ptr(), table.data_ptr(),
+            V, D, table.stride(0), D, scale, 0, tokens.contiguous().data_ptr(), table.data_ptr(),
             out.data_ptr()))
     return out
 
@@ -325,8 +325,8 @@ def rms_norm(x, gain=None, *, residual=None, eps=1e-6, dtype=None):
 def rms_norm_int8(x, gain=None, *, residual=None, eps=1e-6):
     """rms_norm with its output as 8-bit integers: (q, scale) or, with a residual,
     (q, scale, h). q int8 [T, D] and scale float32 [T]: scale is the largest magnitude
-    of a row of y over 127, q the nearest integers to y / scale, halves to even, both
-    quotients in float32. A row of zeros has the scale 0; one with a value that is not
+    of a row of y times 1 / 127, q the nearest integers to y / scale, halves to even,
+    each step in float32. A row of zeros has the scale 0; one with a value that is not
     finite the scale NaN and q 0. (Rows below some 1e-36 lose precision with their
     scale.)"""
     eps = _check_norm(x, gain, residual, eps)

@@ -132,7 +132,7 @@ def load_library() -> ctypes.CDLL:
 def _run(fn, where, device, *structs):
     """Call an entry point with packed structures on the device's current
     stream (torch.cuda.current_stream without its wrapper object)."""
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():
         rc = fn(*structs, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):

@@ -200,8 +200,8 @@ int seq_embedding_grad(const SeqEmbeddingGrad *e, void *stream);
  * rounded to a type or to 8-bit integers with a scale for each row:
  *   h = x + residual, rounded to the stream's type (h = x without a residual);
  *   y = gain h / sqrt(mean h^2 + eps)       (gain null: 1; identity: y = h)
- *   y_dtype SEQ_INT8: y_scale = max |y| / 127, y = round(y / y_scale), halves to even,
- *   both quotients rounded to fp32; a row of zeros (or so small that its scale is 0) has
+ *   y_dtype SEQ_INT8: y_scale = max |y| * (1 / 127), y = round(y / y_scale), halves to
+ *   even, each step rounded to fp32; a row of zeros (or so small that its scale is 0) has
  *   the integers 0, one with a value that is not finite those and the scale NaN.
  * The stream's type is fp32 or x's. */
 typedef struct SeqNorm {

@@ -177,7 +177,7 @@ def test_library_refusals():
          (dict(out_dtype=-1), CO_ERR_DATA), (dict(scale=nan), CO_ERR_DATA)], dict(tokens=0), False)
     library_refuses(
         "seq_embedding_grad", ops.SeqEmbeddingGrad, ("ids", "d_out", "dtable", "workspace"),
-        dict(tokens=4, rows=9, width=8, dout_row=8, dtable_row=8, scale=1.0,
+        dict(tokens=400, rows=9, width=8, dout_row=8, dtable_row=8, scale=1.0,
              workspace_bytes=1 << 30),
         [(dict(tokens=-1), CO_ERR_NULLARG), (dict(width=0), CO_ERR_NULLARG),
          (dict(ids=None), CO_ERR_NULLARG), (dict(d_out=None), CO_ERR_NULLARG),
