@@ -32,8 +32,9 @@ __device__ inline uint4v row_piece(const int8_t *row, int64_t l, int64_t inner) 
 // LDS. A lane of a product has one token's channels 8 g + 4 h .. + 3, h its half of the
 // wave; two groups g change halves, and it has 8 channels side by side. 32 tokens' go
 // through LDS to leave as whole rows: stores of 32 bytes a row took 156 us for 8,192 x
-// 16,384 outputs of 128 terms. WIDE: every 8 channels lie on a boundary of 16 bytes
-// and are all inside or all outside.
+// 16,384 outputs of 128 terms. Those of large tiles pass the caches by, which hold operands
+// that are read again: 8,192 x 4,096 x 16,384 in 513 us rather than 565. WIDE: every 8
+// channels lie on a boundary of 16 bytes and are all inside or all outside.
 template <typename O, int F> constexpr int slab_pitch() { return F * 32 + 16 / (int)sizeof(O); }
 template <typename O, bool WIDE, int F>
 __device__ inline void put_sums(const SeqInt8Product &p, int64_t i0, int64_t j0,
@@ -73,7 +74,10 @@ __device__ inline void put_sums(const SeqInt8Product &p, int64_t i0, int64_t j0,
 #pragma unroll
             for (int r = lane / LANES; r < 32; r += ROWS) {
                 const uint4v v = *(const uint4v *)(slab + r * PITCH + col);
-                if (in && i + r < p.m) *(uint4v *)to = v;
+                if (in && i + r < p.m) {
+                    if constexpr (F == 4) __builtin_nontemporal_store(v, (uint4v *)to);
+                    else *(uint4v *)to = v;
+                }
                 to += ROWS * p.o_row;
             }
         } else {
@@ -104,7 +108,10 @@ __device__ inline bool tile_of(int64_t block, int64_t rows, int64_t columns, int
 // arrive: a step of 256 x 256 is a microsecond's half, an operand's way from beyond the
 // die's cache more than one. A step's second half is read from LDS while its first is
 // multiplied, and the next one's first with its second. Row r of a buffer holds its four
-// pieces of 16 bytes turned by r / 4, so that 16 lanes' reads meet every bank once.
+// pieces of 16 bytes turned by r / 4, so that 16 lanes' reads meet every bank once. At 8,192
+// x 8,192 x 16,384 the products alone take 578 us (3.8 POP/s at the clock that the card
+// falls to), with the reads from LDS 718, with the copies into it 718, with both 941: LDS
+// bounds it.
 constexpr int kStep = 64, kStages = 5;
 template <int T> constexpr int tile_bytes() { return 2 * T * kStep; }
 
