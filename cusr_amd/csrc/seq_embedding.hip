@@ -344,8 +344,10 @@ __device__ inline void zero_absent(const SeqEmbeddingGrad &p, int64_t v0, int ro
     for (int row = threadIdx.x >> g; row < rows; row += 256 >> g) {
         if (present[row]) continue;
         for (int i = threadIdx.x & ((1 << g) - 1); i < parts; i += 1 << g) {
-            if constexpr (W == 8)
-                ((uint4v *)((char *)p.dtable + (v0 + row) * p.dtable_row * e))[i] = uint4v{0, 0, 0, 0};
+            if constexpr (W == 8)                // past the caches, which hold what is added
+                __builtin_nontemporal_store(
+                    uint4v{0, 0, 0, 0},
+                    (uint4v *)((char *)p.dtable + (v0 + row) * p.dtable_row * e) + i);
             else
                 put1(p.dtable, p.out_dtype, (v0 + row) * p.dtable_row + i, 0.0f);
         }
