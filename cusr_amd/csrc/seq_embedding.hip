@@ -11,20 +11,6 @@
 
 namespace seq {
 
-template <typename T, int W> struct Cells;       // W values side by side
-template <typename T> struct Cells<T, 8> : Eight<T> {};
-template <typename T> struct Cells<T, 1> {
-    T a;
-    __device__ void load(const T *p) { a = *p; }
-    __device__ void zero() { a = (T)0.0f; }
-    __device__ void get(float *f) const { f[0] = (float)a; }
-    static __device__ void put(T *p, const float *f) { *p = (T)f[0]; }
-};
-template <int W> __device__ inline void put_cells(void *p, int dtype, int64_t at, const float *f) {
-    if constexpr (W == 8) put8(p, dtype, at, f);
-    else put1(p, dtype, at, f[0]);
-}
-
 // log2 of the threads of a row of `parts` parts
 inline int group_log(int64_t parts) {
     int g = 0;
@@ -57,9 +43,9 @@ __global__ __launch_bounds__(256) void embed_rows(SeqEmbedding p, int g) {
 
 // ------------------------------------------------------------- few rows: symbols
 
-// A table of up to kSymbolRows rows: a wave keeps the sums of its tokens, 128 columns of every row, in
-// LDS and reads its tokens' gradients one after the other, so no order of tokens is
-// needed. A lane adds to columns of its own, in the tokens' order, four tokens at a
+// A table of up to kSymbolRows rows: a wave keeps the sums of its tokens, 128 columns of
+// every row, in LDS and reads its tokens' gradients one after the other, so no order of
+// tokens is needed. A lane adds to columns of its own, in the tokens' order, four tokens at a
 // time: where two of them have one row the later takes the earlier's sum. (LDS adds
 // floats by itself, but hardly a lane at a time: 839 us for 1.3 M tokens of 128 in fp32
 // and 22 rows.) Against sorting, that takes 126 against 229 us, with 30 rows 128 against

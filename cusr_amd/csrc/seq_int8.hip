@@ -161,8 +161,10 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Produ
         at += base + (half * 2 + lane / 32 + row / 4) % 4 * 16 + row * kStep;
 #pragma unroll
         for (int x = 0; x < F; x++) {
-            a[x] = __builtin_bit_cast(int4v, *(lds_ptr4)(uintptr_t)(at + (wave / 2 * W + x * 32) * kStep));
-            w[x] = __builtin_bit_cast(int4v, *(lds_ptr4)(uintptr_t)(at + (T + wave % 2 * W + x * 32) * kStep));
+            const uint32_t ra = at + (wave / 2 * W + x * 32) * kStep;
+            const uint32_t rw = at + (T + wave % 2 * W + x * 32) * kStep;
+            a[x] = __builtin_bit_cast(int4v, *(lds_ptr4)(uintptr_t)ra);
+            w[x] = __builtin_bit_cast(int4v, *(lds_ptr4)(uintptr_t)rw);
         }
     };
     int16v acc[F][F];

@@ -286,14 +286,14 @@ __global__ __launch_bounds__(THREADS) void logprob_rows(SeqLogprobs p, Warmth w)
     }
 }
 
-// Few long rows: a row is cut into parts of PART pieces, a block of 256 each, which keeps its
+// Few long rows: a row is cut into parts of kPartPieces, a block of 256 each, which keeps its
 // values in registers and leaves its sums and its largest alternatives in the workspace;
 // a wave a row joins them.
 constexpr int kPartPieces = 1024, kMostParts = 64;
-struct Part { float m, rest, u; int32_t bad; };  // sums over a part; bad: a value was NaN or inf
+struct RowPart { float m, rest, u; int32_t bad; };  // sums over a part; bad: a value was NaN or inf
 
 template <typename T>
-__global__ __launch_bounds__(256) void logprob_parts(SeqLogprobs p, Warmth w, int parts, Part *sums,
+__global__ __launch_bounds__(256) void logprob_parts(SeqLogprobs p, Warmth w, int parts, RowPart *sums,
                                                      Key *keys) {
     constexpr int N = Sixteen<T>::n, NV = kPartPieces / 256;
     typedef typename Sixteen<T>::vec vec;
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256) void logprob_parts(SeqLogprobs p, Warmth w, in
     tops = over_group<Add, 256>(tops, red);
     if (tid == 0) {
         // a part of -inf alone adds nothing; a NaN stays one
-        Part r = {m, m == neg_inf() ? rest : rest + (tops - 1.0f), u, 0};
+        RowPart r = {m, m == neg_inf() ? rest : rest + (tops - 1.0f), u, 0};
         r.bad = r.rest != r.rest || m == __builtin_inff();
         sums[t * parts + part] = r;
     }
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(256) void logprob_parts(SeqLogprobs p, Warmth w, in
 }
 
 __global__ __launch_bounds__(64) void logprob_join(SeqLogprobs p, Warmth w, int parts,
-                                                   const Part *sums, const Key *keys) {
+                                                   const RowPart *sums, const Key *keys) {
     extern __shared__ __align__(8) Key lists[];  // parts x top
     const int64_t t = block_number();
     if (t >= p.tokens) return;
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(64) void logprob_join(SeqLogprobs p, Warmth w, int 
     const int64_t id = get_id(p.ids, p.ids_64, t);
     const float xa = id >= 0 && id < p.vocab
                          ? get1(p.logits, p.dtype, t * p.row + id) : 0.0f;
-    Part a = {neg_inf(), 0.0f, 0.0f, 0};
+    RowPart a = {neg_inf(), 0.0f, 0.0f, 0};
     if (lane < parts) a = sums[t * parts + lane];
     for (int i = lane; i < parts * p.top; i += 64) lists[i] = keys[t * parts * p.top + i];
     __syncthreads();
@@ -494,7 +494,7 @@ __global__ __launch_bounds__(R) void logprob_symbols(SeqLogprobs p, Warmth w, bo
 
 // A row's gradient: d_j = g [j = id] - p_j (g + h (log p_j + entropy)), with g and h the
 // gradients of logp and entropy over the temperature.
-struct RowGrad {
+struct LogprobGrad {
     float m0, inverse, log_sum, entropy, g, h;
     float own;                                   // the token's own
     bool skip;                                   // both gradients are 0: nothing is read
@@ -505,9 +505,9 @@ struct RowGrad {
         return -prob * __builtin_fmaf(h, lp + entropy, g);
     }
 };
-__device__ inline RowGrad grad_of(const SeqLogprobsGrad &p, const Warmth &w, int64_t t, int64_t id,
+__device__ inline LogprobGrad grad_of(const SeqLogprobsGrad &p, const Warmth &w, int64_t t, int64_t id,
                                   bool in, float xa) {
-    RowGrad r;
+    LogprobGrad r;
     const float dl = p.dlogp ? p.dlogp[t] : 0.0f, dh = p.dentropy ? p.dentropy[t] : 0.0f;
     const float rest = p.stats[2 * t + 1];
     r.skip = dl == 0.0f && dh == 0.0f;
@@ -539,7 +539,7 @@ __global__ __launch_bounds__(256) void logprob_grad_rows(SeqLogprobsGrad p, Warm
     T *dx = (T *)p.dlogits + t * p.drow;
     const int64_t id = get_id(p.ids, p.ids_64, t);
     const bool in = id >= 0 && id < p.vocab;
-    const RowGrad r = grad_of(p, w, t, id, in, in ? (float)x[id] : 0.0f);
+    const LogprobGrad r = grad_of(p, w, t, id, in, in ? (float)x[id] : 0.0f);
     // Pieces where both rows have them at the same places, from a boundary of 128 bytes of the
     // gradient's row on, so that waves write whole lines; past the caches, which keep the
     // logits: 8,192 rows of 131,071 in bf16 take 840 us (from the first boundary of 16 bytes
@@ -583,7 +583,7 @@ __global__ __launch_bounds__(R) void logprob_grad_symbols(SeqLogprobsGrad p, War
     __syncthreads();
     if ((int)threadIdx.x < rows) {
         T *y = (T *)lds + threadIdx.x * V;
-        const RowGrad r = grad_of(p, w, t, id, in, in ? (float)y[id] : 0.0f);
+        const LogprobGrad r = grad_of(p, w, t, id, in, in ? (float)y[id] : 0.0f);
         Rows<T, R>::columns(V, turn, [&](int j) {
             const float d = j == id ? r.own : r.of((float)y[j], w);
             y[j] = (T)(r.skip ? 0.0f : d);
@@ -637,10 +637,11 @@ template <typename T> void launch_logprobs(const SeqLogprobs &p, hipStream_t s) 
     const Warmth w = make_warmth(p.temperature);
     const int parts = parts_of(p);
     if (parts) {
-        Part *sums = (Part *)p.workspace;
+        RowPart *sums = (RowPart *)p.workspace;
         Key *keys = (Key *)(sums + p.tokens * parts);
         logprob_parts<T><<<(unsigned)(p.tokens * parts), 256, 0, s>>>(p, w, parts, sums, keys);
-        logprob_join<<<(unsigned)p.tokens, 64, (size_t)parts * p.top * sizeof(Key), s>>>(p, w, parts, sums, keys);
+        const size_t lds = (size_t)parts * p.top * sizeof(Key);
+        logprob_join<<<(unsigned)p.tokens, 64, lds, s>>>(p, w, parts, sums, keys);
         return;
     }
     const int rows = symbol_rows_of(p.vocab, p.dtype);
@@ -691,7 +692,7 @@ template <typename T> void launch_grad(const SeqLogprobsGrad &p, hipStream_t s) 
 extern "C" int64_t seq_logprobs_workspace(const SeqLogprobs *p) {
     const int rc = seq::check_logprobs(p);
     if (rc != CO_OK) return rc > 0 ? -rc : rc;
-    return p->tokens * seq::parts_of(*p) * (int64_t)(sizeof(seq::Part) + p->top * sizeof(seq::Key));
+    return p->tokens * seq::parts_of(*p) * (int64_t)(sizeof(seq::RowPart) + p->top * sizeof(seq::Key));
 }
 
 extern "C" int seq_logprobs(const SeqLogprobs *p, void *stream) {

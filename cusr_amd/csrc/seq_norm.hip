@@ -13,25 +13,6 @@ template <typename H> __device__ inline float stream_sum(float x, float r) {
     return (float)(H)(x + r);
 }
 
-// W values of a row side by side: 8 in pieces, or 1 of any place
-template <typename T, int W> struct Part;
-template <typename T> struct Part<T, 8> : Eight<T> {};
-template <typename T> struct Part<T, 1> {
-    T a;
-    __device__ void load(const T *p) { a = *p; }
-    __device__ void zero() { a = (T)0.0f; }
-    __device__ void get(float *f) const { f[0] = (float)a; }
-    static __device__ void put(T *p, const float *f) { *p = (T)f[0]; }
-};
-template <int W> __device__ inline void get_part(const void *p, int dtype, int64_t at, float *f) {
-    if constexpr (W == 8) get8(p, dtype, at, f);
-    else f[0] = get1(p, dtype, at);
-}
-template <int W> __device__ inline void put_part(void *p, int dtype, int64_t at, const float *f) {
-    if constexpr (W == 8) put8(p, dtype, at, f);
-    else put1(p, dtype, at, f[0]);
-}
-
 __device__ inline float rms_factor(float sum, int64_t width, float eps) {
     return 1.0f / sqrtf(sum / (float)width + eps);
 }
@@ -66,8 +47,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
     const int lane = threadIdx.x % G;
     const int parts = (int)(p.width / W);
     const X *x = (const X *)p.x + t * p.x_row;
-    Part<X, W> xs[NV];
-    Part<H, W> rs[RES ? NV : 1];
+    Cells<X, W> xs[NV];
+    Cells<H, W> rs[RES ? NV : 1];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int at = i * G + lane;
@@ -93,7 +74,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
 #pragma unroll
             for (int j = 0; j < W; j++) f[i][j] = stream_sum<H>(f[i][j], r[j]);
             const int at = i * G + lane;
-            if (at < parts) Part<H, W>::put((H *)p.h + t * p.h_row + at * W, f[i]);
+            if (at < parts) Cells<H, W>::put((H *)p.h + t * p.h_row + at * W, f[i]);
         }
 #pragma unroll
         for (int j = 0; j < W; j++) sum += f[i][j] * f[i][j];
@@ -104,7 +85,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const int at = i * G + lane;
-                if (at < parts) get_part<W>(p.gain, p.gain_dtype, at * W, g[i]);
+                if (at < parts) get_cells<W>(p.gain, p.gain_dtype, at * W, g[i]);
             }
         }
         const float rho = rms_factor(over_group<Add, G>(sum, red), p.width, p.eps);
@@ -123,7 +104,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int at = i * G + lane;
-            if (at < parts) put_part<W>(p.y, p.y_dtype, t * p.y_row + at * W, f[i]);
+            if (at < parts) put_cells<W>(p.y, p.y_dtype, t * p.y_row + at * W, f[i]);
         }
         return;
     }
@@ -211,8 +192,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_grad_rows(SeqNormGrad 
         for (int j = 0; j < W; j++) dgain[i][j] = 0.0f;
     const int64_t step = (int64_t)gridDim.x * gridDim.z * ROWS;
     for (int64_t t = (int64_t)block_number() * ROWS + group; t < p.tokens; t += step) {
-        Part<Y, W> ys[NV];
-        Part<H, W> hs[NV], es[NV];
+        Cells<Y, W> ys[NV];
+        Cells<H, W> hs[NV], es[NV];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int at = i * G + lane;
@@ -240,7 +221,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_grad_rows(SeqNormGrad 
                 float g[W];
 #pragma unroll
                 for (int j = 0; j < W; j++) g[j] = 0.0f;
-                if (i * G + lane < parts) get_part<W>(p.gain, p.gain_dtype, (i * G + lane) * W, g);
+                if (i * G + lane < parts) get_cells<W>(p.gain, p.gain_dtype, (i * G + lane) * W, g);
 #pragma unroll
                 for (int j = 0; j < W; j++) u[j] *= g[j];
             }
@@ -262,7 +243,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_grad_rows(SeqNormGrad 
             if (at >= parts) continue;
             if (p.gain) {
                 float g[W];
-                get_part<W>(p.gain, p.gain_dtype, at * W, g);
+                get_cells<W>(p.gain, p.gain_dtype, at * W, g);
 #pragma unroll
                 for (int j = 0; j < W; j++) u[j] *= g[j];
             }
@@ -274,8 +255,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_grad_rows(SeqNormGrad 
 #pragma unroll
                 for (int j = 0; j < W; j++) d[j] += e[j];
             }
-            Part<H, W>::put((H *)p.d + t * p.d_row + at * W, d);
-            if (p.dx) put_part<W>(p.dx, p.x_dtype, t * p.dx_row + at * W, d);
+            Cells<H, W>::put((H *)p.d + t * p.d_row + at * W, d);
+            if (p.dx) put_cells<W>(p.dx, p.x_dtype, t * p.dx_row + at * W, d);
         }
     }
     if (!partial) return;
@@ -283,7 +264,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_grad_rows(SeqNormGrad 
     if constexpr (ROWS == 1) {
 #pragma unroll
         for (int i = 0; i < NV; i++)
-            if (i * G + lane < parts) Part<float, W>::put(out + (i * G + lane) * W, dgain[i]);
+            if (i * G + lane < parts) Cells<float, W>::put(out + (i * G + lane) * W, dgain[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < NV; i++)

@@ -65,6 +65,25 @@ __device__ inline int64_t get_id(const void *p, int ids_64, int64_t at) {
     return ids_64 ? ((const int64_t *)p)[at] : ((const int32_t *)p)[at];
 }
 
+// W values of a row side by side: 8 in pieces of 16 bytes, or 1 of any place
+template <typename T, int W> struct Cells;
+template <typename T> struct Cells<T, 8> : Eight<T> {};
+template <typename T> struct Cells<T, 1> {
+    T a;
+    __device__ void load(const T *p) { a = *p; }
+    __device__ void zero() { a = (T)0.0f; }
+    __device__ void get(float *f) const { f[0] = (float)a; }
+    static __device__ void put(T *p, const float *f) { *p = (T)f[0]; }
+};
+template <int W> __device__ inline void get_cells(const void *p, int dtype, int64_t at, float *f) {
+    if constexpr (W == 8) get8(p, dtype, at, f);
+    else f[0] = get1(p, dtype, at);
+}
+template <int W> __device__ inline void put_cells(void *p, int dtype, int64_t at, const float *f) {
+    if constexpr (W == 8) put8(p, dtype, at, f);
+    else put1(p, dtype, at, f[0]);
+}
+
 inline bool float_type(int t) { return t >= SEQ_FP32 && t <= SEQ_FP16; }
 inline int type_bytes(int t) { return t == SEQ_FP32 ? 4 : (t == SEQ_INT8 ? 1 : 2); }
 // whether rows hold whole pieces of 8 values, each on a boundary of 16 bytes (8 of int8)

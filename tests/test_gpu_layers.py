@@ -84,7 +84,9 @@ EMBED_GRAD = [
     (700, 40, 2056, BF, F32), (640, 3, 333, FP, F32), (66000, 22, 40, BF, F32),
     (70001, 9, 8, F32, F32), (600000, 1000, 1, F32, F32), (530000, 2, 16, BF, F32),
     (3, 4, 65536, BF, F32), (0, 5, 16, BF, F32), (40000, 128, 130, BF, F32), (9001, 129, 130, F32, F32),
-    (33000, 32, 257, FP, F32), (33000, 33, 257, FP, F32), (5000, 20, 1024, BF, BF), (200, 129, 65536, BF, F32),
+    (33000, 32, 257, FP, F32), (33000, 33, 257, FP, F32), (5000, 20, 1024, BF, BF),
+    (200, 129, 65536, BF, F32), (256, 700, 33, BF, BF), (257, 700, 40, FP, F32),
+    (255, 100000, 8, F32, F32), (256, 1, 2056, BF, F32), (64, 5, 300, FP, FP),
     (33000, 5000, 264, F32, F32), (32768, 513, 9, BF, F32), (80000, 200, 136, BF, F32),
 ]
 
@@ -287,9 +289,11 @@ def test_norm_autograd(ops, st):
     loss.backward()
     r = ref.rms_grad(wy, x if h is None else h, gain, None if h is None else wh.to(st), eps)
     check("dx", x.grad, r["d"], ref.rounded(r["d"], BF, r["d_err"]))
-    check("dgain", gain.grad, r["dgain"], ref.rounded(r["dgain"], BF, r["dgain_err"] + E32 * r["dgain"].abs()))
+    check("dgain", gain.grad, r["dgain"],
+          ref.rounded(r["dgain"], BF, r["dgain_err"] + E32 * r["dgain"].abs()))
     if res is not None:
         check("dresidual", res.grad, r["d"], ref.rounded(r["d"], st, r["d_err"]))
+        assert res.grad.data_ptr() != x.grad.data_ptr()
         # the stream alone, the norm alone, and neither
         for pick in ("y", "h"):
             for t in (x, gain, res):
@@ -672,6 +676,45 @@ def test_captured_and_replayed(ops):
             graphs[i].replay()
             torch.cuda.synchronize()
             assert same(outs[i], want), (turn, i)
+
+
+def test_a_large_product_captured(ops):
+    """The largest tiles, and rows that are laid out anew, in a graph that is replayed with other
+    operands."""
+    for M, K, N in ((4096, 272, 4104), (700, 401, 300)):
+        a, sa, w, sw, _ = product_case(M, K, N)
+        stream, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream):
+            ops.int8_product(a, sa, w, sw)
+        stream.synchronize()
+        with torch.cuda.graph(g, stream=stream):
+            out = ops.int8_product(a, sa, w, sw)
+        for seed in range(3):
+            a.copy_(int8s((M, K), 10 + seed))
+            want = ops.int8_product(a, sa, w, sw)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+
+
+def test_refuses_nothing_silently(ops):
+    """Gradients that are asked for are formed or refused, under a graph of a graph too."""
+    x = normal((4, 64), BF, 1).requires_grad_()
+    for fn in (lambda: ops.quantize_rows(x), lambda: ops.rms_norm_int8(x),
+               lambda: ops.rms_norm_int8(x.detach(), x[0])):
+        with pytest.raises(ValueError):
+            fn()
+    with torch.no_grad():
+        ops.quantize_rows(x)
+    y = ops.rms_norm(x, dtype=F32)
+    g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()
+    z = x.float().detach().requires_grad_()
+    logp, entropy = ops.token_logprobs(z, ids(4, 64, 1))
+    entropy.add_(1.0)                                # what the backward pass reads has changed
+    with pytest.raises(RuntimeError):
+        logp.sum().backward()
 
 
 def test_far_offsets(ops):
