@@ -309,13 +309,13 @@ def rewards_of(losses, y):
 
 
 def search(X, y, *, rounds=10, population=1024, max_iter=10, seed=0, proposer=None, trainer=None,
-           backend=None, log=print, int8=False):
-    """Rounds of sampling (int8: with 8-bit products), fitting and training. Returns (best,
-    history): the
+           backend=None, log=print, fused=False, int8=False):
+    """Rounds of sampling (int8: with 8-bit products), fitting and training; fused: of the
+    proposer that is made here when none is given. Returns (best, history): the
     best program as (loss, (nt, nv, ci), constants), (inf, None, None) when none
     was fitted, and each round's mean and best reward."""
     X, y = np.asarray(X, np.float64), np.asarray(y, np.float64)
-    p = proposer or Proposer(X.shape[1], seed=seed)
+    p = proposer or Proposer(X.shape[1], seed=seed, fused=fused)
     tr = trainer or Trainer(p, top=0.1, kl_coef=0.05)
     lm = backend or KernelLM(max_iter=max_iter)
     g = torch.Generator(device=p.device).manual_seed(seed)
@@ -350,8 +350,7 @@ def main(argv=None):
     rng = np.random.default_rng(a.seed)
     X = rng.uniform(-2, 2, size=(512, 2))
     y = 1.5 * np.sin(0.8 * X[:, 0]) * X[:, 1] + 0.5
-    p = Proposer(X.shape[1], seed=a.seed, fused=a.fused)
-    best, _ = search(X, y, rounds=a.rounds, population=a.population, seed=a.seed, proposer=p,
+    best, _ = search(X, y, rounds=a.rounds, population=a.population, seed=a.seed, fused=a.fused,
                      int8=a.int8)
     if best[1] is None:
         print("no program was fitted")

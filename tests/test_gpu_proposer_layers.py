@@ -83,3 +83,10 @@ def test_training_with_an_entropy_term():
     assert entropy > 0 and losses[1] < losses[0]
     with pytest.raises(ValueError):
         pr.Trainer(None, entropy_coef=float("nan"))
+
+
+def test_the_command_line(capsys):
+    """One small round with everything by choice."""
+    pr.main(["--rounds", "1", "--population", "64", "--fused", "--int8"])
+    out = capsys.readouterr().out
+    assert "round 0" in out and ("best loss" in out or "no program" in out)
