@@ -19,25 +19,26 @@ inline int group_log(int64_t parts) {
 }
 
 // 2^g threads a token, a part of its row each at a time
-template <typename T, int W>
+template <typename T, bool ANY>
 __global__ __launch_bounds__(256) void embed_rows(SeqEmbedding p, int g) {
     const int64_t t = (int64_t)block_number() * (256 >> g) + (threadIdx.x >> g);
     if (t >= p.tokens) return;
-    const int parts = (int)(p.width / W), lane = threadIdx.x & ((1 << g) - 1);
+    const int parts = (int)((p.width + 7) / 8), lane = threadIdx.x & ((1 << g) - 1);
     const int64_t id = get_id(p.ids, p.ids_64, t);
     const bool in = id >= 0 && id < p.rows;
     const T *row = (const T *)p.table + (in ? id : 0) * p.table_row;
     const float scale = in ? p.scale : __builtin_nanf("");
 #pragma unroll 4
     for (int at = lane; at < parts; at += 1 << g) {
-        Cells<T, W> v;
+        const int n = cells_of<ANY>(p.width, at);
+        Cells<T, ANY> v;
         v.zero();
-        if (in) v.load(row + at * W);            // a table may have no row at all
-        float f[W];
+        if (in) v.load(row + at * 8, n);         // a table may have no row at all
+        float f[8];
         v.get(f);
 #pragma unroll
-        for (int j = 0; j < W; j++) f[j] *= scale;
-        put_cells<W>(p.out, p.out_dtype, t * p.out_row + at * W, f);
+        for (int j = 0; j < 8; j++) f[j] *= scale;
+        put_cells<ANY>(p.out, p.out_dtype, t * p.out_row + at * 8, f, n);
     }
 }
 
@@ -318,33 +319,36 @@ __device__ inline bool has_token(const uint32_t *keys, uint32_t n, uint32_t v) {
     return lo < n && keys[lo] == v;
 }
 
-// Zeros in those of `rows` rows from v0 on that are not present: 16 bytes or a value a thread,
-// several rows at a time where they are narrow
-template <int W>
+// Zeros in those of `rows` rows from v0 on that are not present: 16 bytes a thread, several
+// rows at a time where they are narrow, past the caches, which hold what is added
+template <bool ANY>
 __device__ inline void zero_absent(const SeqEmbeddingGrad &p, int64_t v0, int rows,
                                    const bool *present) {
-    const int e = p.out_dtype == SEQ_FP32 ? 4 : 2;
-    const int parts = (int)(W == 8 ? p.width * e / 16 : p.width);
+    const int e = p.out_dtype == SEQ_FP32 ? 4 : 2, bytes = (int)p.width * e;
+    const int parts = (bytes + 15) / 16;
     int g = 0;
     while (g < 8 && (1 << g) < parts) g++;
     for (int row = threadIdx.x >> g; row < rows; row += 256 >> g) {
         if (present[row]) continue;
+        char *to = (char *)p.dtable + (v0 + row) * p.dtable_row * e;
         for (int i = threadIdx.x & ((1 << g) - 1); i < parts; i += 1 << g) {
-            if constexpr (W == 8)                // past the caches, which hold what is added
-                __builtin_nontemporal_store(
-                    uint4v{0, 0, 0, 0},
-                    (uint4v *)((char *)p.dtable + (v0 + row) * p.dtable_row * e) + i);
-            else
-                put1(p.dtable, p.out_dtype, (v0 + row) * p.dtable_row + i, 0.0f);
+            const uint4v zero = {0, 0, 0, 0};
+            if (!ANY) {
+                __builtin_nontemporal_store(zero, (uint4v *)to + i);
+            } else if (i * 16 + 16 <= bytes) {
+                __builtin_memcpy(to + i * 16, &zero, 16);
+            } else {
+                for (int b = i * 16; b < bytes; b += 2) *(uint16_t *)(to + b) = 0;
+            }
         }
     }
 }
 
 // The first blocks: 2^g threads add a chunk's rows, a slab of columns at a time. The
 // others write zeros where a row of the table has no token.
-template <typename T, int W>
+template <typename T, bool ANY>
 __global__ __launch_bounds__(256) void embed_sum(SeqEmbeddingGrad p, Runs r) {
-    constexpr int AHEAD = 8;                     // rows on their way
+    constexpr int AHEAD = 8, W = 8;              // rows on their way
     __shared__ bool present[256];
     const uint32_t n = (uint32_t)p.tokens, V = (uint32_t)p.rows;
     const int64_t block = block_number();
@@ -355,7 +359,7 @@ __global__ __launch_bounds__(256) void embed_sum(SeqEmbeddingGrad p, Runs r) {
         if ((int)threadIdx.x < rows)
             present[threadIdx.x] = has_token(r.keys, n, (uint32_t)(v0 + threadIdx.x));
         __syncthreads();
-        zero_absent<W>(p, v0, rows, present);
+        zero_absent<ANY>(p, v0, rows, present);
         return;
     }
     const int groups = 256 >> r.g, lane = threadIdx.x & ((1 << r.g) - 1);
@@ -363,6 +367,7 @@ __global__ __launch_bounds__(256) void embed_sum(SeqEmbeddingGrad p, Runs r) {
     const int64_t c = block / r.slabs * groups + (threadIdx.x >> r.g);
     const int64_t col = ((int64_t)slab * (1 << r.g) + lane) * W;
     if (c >= r.chunks || col >= p.width) return;
+    const int cells = ANY && p.width - col < 8 ? (int)(p.width - col) : 8;
     const uint32_t a = (uint32_t)(c * r.chunk);
     const uint32_t b = n - a < (uint32_t)r.chunk ? n : a + r.chunk;
     const uint32_t last = a ? r.keys[a - 1] : 0xffffffffu, next = b < n ? r.keys[b] : 0xffffffffu;
@@ -373,22 +378,22 @@ __global__ __launch_bounds__(256) void embed_sum(SeqEmbeddingGrad p, Runs r) {
     auto flush = [&](bool goes_on) {
         if (run >= V) return;
         if (from_before || goes_on) {
-            Cells<float, W>::put(r.slots + (2 * c + !from_before) * r.pitch + col, sum);
+            Eight<float>::put(r.slots + (2 * c + !from_before) * r.pitch + col, sum);
         } else {
             float f[W];
 #pragma unroll
             for (int j = 0; j < W; j++) f[j] = sum[j] * p.scale;
-            put_cells<W>(p.dtable, p.out_dtype, run * p.dtable_row + col, f);
+            put_cells<ANY>(p.dtable, p.out_dtype, run * p.dtable_row + col, f, cells);
         }
     };
     for (uint32_t at = a; at < b; at += AHEAD) {
         uint32_t key[AHEAD];
-        Cells<T, W> v[AHEAD];
+        Cells<T, ANY> v[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             key[i] = at + i < b ? r.keys[at + i] : V;
             v[i].zero();
-            if (key[i] < V) v[i].load(x + r.places[at + i] * p.dout_row);
+            if (key[i] < V) v[i].load(x + r.places[at + i] * p.dout_row, cells);
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
@@ -488,9 +493,9 @@ __global__ __launch_bounds__(256) void embed_join(SeqEmbeddingGrad p, Runs r) {
 // call of 256 tokens and 32,001 rows of 1,024 in fp32 takes 23 us, sorted 41, of one token and
 // 131,071 rows of 64 9 and 23.
 constexpr int kFewTokens = 256;
-template <typename T, int W>
+template <typename T, bool ANY>
 __global__ __launch_bounds__(256) void embed_few(SeqEmbeddingGrad p, int slabs, int zero_rows) {
-    constexpr int AHEAD = 8;                     // rows on their way
+    constexpr int AHEAD = 8, W = 8;              // rows on their way
     __shared__ __align__(16) uint32_t keys[kFewTokens];
     __shared__ uint64_t like[kFewTokens / 64];
     const int tid = threadIdx.x, n = (int)p.tokens;
@@ -515,7 +520,7 @@ __global__ __launch_bounds__(256) void embed_few(SeqEmbeddingGrad p, int slabs, 
             present[tid] = is;
         }
         __syncthreads();
-        zero_absent<W>(p, v0, rows, present);
+        zero_absent<ANY>(p, v0, rows, present);
         return;
     }
     const int t = (int)(block / slabs);
@@ -528,12 +533,13 @@ __global__ __launch_bounds__(256) void embed_few(SeqEmbeddingGrad p, int slabs, 
     __syncthreads();
     const int64_t col = ((int64_t)(block % slabs) * 256 + tid) * W;
     if (col >= p.width) return;
+    const int cells = ANY && p.width - col < 8 ? (int)(p.width - col) : 8;
     const T *x = (const T *)p.d_out + col;
     float sum[W] = {};
     for (int w = 0; w < (n + 63) / 64; w++) {
         uint64_t left = like[w];
         while (left) {
-            Cells<T, W> v[AHEAD];
+            Cells<T, ANY> v[AHEAD];
             bool is[AHEAD];
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) {
@@ -542,7 +548,7 @@ __global__ __launch_bounds__(256) void embed_few(SeqEmbeddingGrad p, int slabs, 
                 if (!is[i]) continue;
                 const int u = w * 64 + __ffsll((unsigned long long)left) - 1;
                 left &= left - 1;
-                v[i].load(x + u * p.dout_row);
+                v[i].load(x + u * p.dout_row, cells);
             }
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) {
@@ -556,7 +562,7 @@ __global__ __launch_bounds__(256) void embed_few(SeqEmbeddingGrad p, int slabs, 
     }
 #pragma unroll
     for (int j = 0; j < W; j++) sum[j] *= p.scale;
-    put_cells<W>(p.dtable, p.out_dtype, (int64_t)mine * p.dtable_row + col, sum);
+    put_cells<ANY>(p.dtable, p.out_dtype, (int64_t)mine * p.dtable_row + col, sum, cells);
 }
 
 __global__ __launch_bounds__(256) void embed_zero(SeqEmbeddingGrad p) {
@@ -651,8 +657,9 @@ GradPlan grad_plan(const SeqEmbeddingGrad &p) {
     return r;
 }
 
-template <typename T, int W> void launch_sum(const SeqEmbeddingGrad &p, Runs r, hipStream_t s) {
-    const int64_t parts = p.width / W;
+template <typename T, bool ANY>
+void launch_sum(const SeqEmbeddingGrad &p, Runs r, hipStream_t s) {
+    const int64_t parts = (p.width + 7) / 8;
     r.g = group_log(parts);
     r.slabs = (int)((parts + (1 << r.g) - 1) >> r.g);
     const int groups = 256 >> r.g;
@@ -660,37 +667,37 @@ template <typename T, int W> void launch_sum(const SeqEmbeddingGrad &p, Runs r, 
     const int64_t zero = 65536 / p.width;        // rows that make a block's worth of zeros
     r.zero_rows = (int)(zero < 4 ? 4 : (zero > 256 ? 256 : zero));
     const int64_t blocks = r.sum_blocks + (p.rows + r.zero_rows - 1) / r.zero_rows;
-    embed_sum<T, W><<<grid_of(blocks, 256), 256, 0, s>>>(p, r);
+    embed_sum<T, ANY><<<grid_of(blocks, 256), 256, 0, s>>>(p, r);
 }
 template <typename T> void launch_sum(const SeqEmbeddingGrad &p, const Runs &r, hipStream_t s) {
     const bool eights = p.width % 8 == 0 && in_eights(p.d_out, p.dout_row) &&
                         in_eights(p.dtable, p.dtable_row);
-    if (eights) launch_sum<T, 8>(p, r, s);
-    else launch_sum<T, 1>(p, r, s);
+    if (eights) launch_sum<T, false>(p, r, s);
+    else launch_sum<T, true>(p, r, s);
 }
 
-template <typename T, int W> void launch_few(const SeqEmbeddingGrad &p, hipStream_t s) {
-    const int slabs = (int)((p.width / W + 255) / 256);
+template <typename T, bool ANY> void launch_few(const SeqEmbeddingGrad &p, hipStream_t s) {
+    const int slabs = (int)((p.width + 2047) / 2048);
     const int64_t zero = 65536 / p.width;
     const int zero_rows = (int)(zero < 4 ? 4 : (zero > 256 ? 256 : zero));
     const int64_t blocks = p.tokens * slabs + (p.rows + zero_rows - 1) / zero_rows;
-    embed_few<T, W><<<grid_of(blocks, 256), 256, 0, s>>>(p, slabs, zero_rows);
+    embed_few<T, ANY><<<grid_of(blocks, 256), 256, 0, s>>>(p, slabs, zero_rows);
 }
 template <typename T> void launch_few(const SeqEmbeddingGrad &p, hipStream_t s) {
     const bool eights = p.width % 8 == 0 && in_eights(p.d_out, p.dout_row) &&
                         in_eights(p.dtable, p.dtable_row);
-    if (eights) launch_few<T, 8>(p, s);
-    else launch_few<T, 1>(p, s);
+    if (eights) launch_few<T, false>(p, s);
+    else launch_few<T, true>(p, s);
 }
 
 template <typename T> void launch_embed(const SeqEmbedding &p, hipStream_t s) {
     const bool eights = p.width % 8 == 0 && in_eights(p.table, p.table_row) &&
                         in_eights(p.out, p.out_row);
-    const int g = group_log(p.width / (eights ? 8 : 1));
+    const int g = group_log((p.width + 7) / 8);
     const int rows = 256 >> g;
     const dim3 grid = grid_of((p.tokens + rows - 1) / rows, 256);
-    if (eights) embed_rows<T, 8><<<grid, 256, 0, s>>>(p, g);
-    else embed_rows<T, 1><<<grid, 256, 0, s>>>(p, g);
+    if (eights) embed_rows<T, false><<<grid, 256, 0, s>>>(p, g);
+    else embed_rows<T, true><<<grid, 256, 0, s>>>(p, g);
 }
 
 }  // namespace seq

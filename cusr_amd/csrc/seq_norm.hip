@@ -37,23 +37,25 @@ struct Bits8 {
     }
 };
 
-// A row per group of G threads, NV parts of W values a thread.
-template <typename X, typename H, bool RES, int W, int G, int NV>
+// A row per group of G threads, NV parts of 8 values a thread.
+template <typename X, typename H, bool RES, bool ANY, int G, int NV>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
     constexpr int THREADS = G < 256 ? 256 : G, ROWS = THREADS / G;
     __shared__ float red[16];
     const int64_t t = (int64_t)block_number() * ROWS + threadIdx.x / G;
     if (t >= p.tokens) return;                   // the whole group, and a block of one group
     const int lane = threadIdx.x % G;
-    const int parts = (int)(p.width / W);
+    constexpr int W = 8;
+    const int parts = (int)((p.width + 7) / 8);
+    auto n_of = [&](int at) { return cells_of<ANY>(p.width, at); };
     const X *x = (const X *)p.x + t * p.x_row;
-    Cells<X, W> xs[NV];
-    Cells<H, W> rs[RES ? NV : 1];
+    Cells<X, ANY> xs[NV];
+    Cells<H, ANY> rs[RES ? NV : 1];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int at = i * G + lane;
         xs[i].zero();
-        if (at < parts) xs[i].load(x + at * W);
+        if (at < parts) xs[i].load(x + at * W, n_of(at));
     }
     if constexpr (RES) {
         const H *r = (const H *)p.residual + t * p.residual_row;
@@ -61,7 +63,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
         for (int i = 0; i < NV; i++) {
             const int at = i * G + lane;
             rs[i].zero();
-            if (at < parts) rs[i].load(r + at * W);
+            if (at < parts) rs[i].load(r + at * W, n_of(at));
         }
     }
     float f[NV][W], sum = 0.0f;
@@ -74,7 +76,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
 #pragma unroll
             for (int j = 0; j < W; j++) f[i][j] = stream_sum<H>(f[i][j], r[j]);
             const int at = i * G + lane;
-            if (at < parts) Cells<H, W>::put((H *)p.h + t * p.h_row + at * W, f[i]);
+            if (at < parts) Cells<H, ANY>::put((H *)p.h + t * p.h_row + at * W, f[i], n_of(at));
         }
 #pragma unroll
         for (int j = 0; j < W; j++) sum += f[i][j] * f[i][j];
@@ -85,7 +87,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const int at = i * G + lane;
-                if (at < parts) get_cells<W>(p.gain, p.gain_dtype, at * W, g[i]);
+                if (at < parts) get_cells<ANY>(p.gain, p.gain_dtype, at * W, g[i], n_of(at));
             }
         }
         const float rho = rms_factor(over_group<Add, G>(sum, red), p.width, p.eps);
@@ -104,7 +106,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int at = i * G + lane;
-            if (at < parts) put_cells<W>(p.y, p.y_dtype, t * p.y_row + at * W, f[i]);
+            if (at < parts) put_cells<ANY>(p.y, p.y_dtype, t * p.y_row + at * W, f[i], n_of(at));
         }
         return;
     }
@@ -121,14 +123,17 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
     for (int i = 0; i < NV; i++) {
         const int at = i * G + lane;
         if (at >= parts) continue;
-        if constexpr (W == 8) {
-            uint2v v = {0, 0};
+        uint2v v = {0, 0};
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                v[j / 4] |= (uint32_t)(bits.of(f[i][j]) & 0xff) << (8 * (j % 4));
+        for (int j = 0; j < 8; j++)
+            v[j / 4] |= (uint32_t)(bits.of(f[i][j]) & 0xff) << (8 * (j % 4));
+        if (!ANY) {
             *(uint2v *)(y + at * 8) = v;
+        } else if (n_of(at) == 8) {
+            __builtin_memcpy(y + at * 8, &v, 8);
         } else {
-            y[at] = (int8_t)bits.of(f[i][0]);
+            for (int j = 0; j < n_of(at); j++)
+                y[at * 8 + j] = (int8_t)(v[j / 4] >> (8 * (j % 4)));
         }
     }
 }
@@ -177,38 +182,48 @@ __global__ __launch_bounds__(1024) void norm_long(SeqNorm p) {
 
 // A group's rows one after the other; the gain's gradient stays in registers and is
 // left as one row of partial sums a block.
-template <typename Y, typename H, int W, int G, int NV>
+template <typename Y, typename H, bool ANY, int G, int NV>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_grad_rows(SeqNormGrad p,
                                                                     float *partial) {
-    constexpr int THREADS = G < 256 ? 256 : G, ROWS = THREADS / G;
+    constexpr int THREADS = G < 256 ? 256 : G, ROWS = THREADS / G, W = 8;
     __shared__ float red[16];
     __shared__ float columns[ROWS > 1 ? ROWS * G * NV * W : 1];
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
-    const int parts = (int)(p.width / W);
-    float dgain[NV][W];
+    const int parts = (int)((p.width + 7) / 8);
+    auto n_of = [&](int at) { return cells_of<ANY>(p.width, at); };
+    float dgain[NV][W], gain[NV][W];             // the gain is read once
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
-        for (int j = 0; j < W; j++) dgain[i][j] = 0.0f;
+        for (int j = 0; j < W; j++) {
+            dgain[i][j] = 0.0f;
+            gain[i][j] = 1.0f;
+        }
+    if (p.gain)
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int at = i * G + lane;
+            if (at < parts) get_cells<ANY>(p.gain, p.gain_dtype, at * W, gain[i], n_of(at));
+        }
     const int64_t step = (int64_t)gridDim.x * gridDim.z * ROWS;
     for (int64_t t = (int64_t)block_number() * ROWS + group; t < p.tokens; t += step) {
-        Cells<Y, W> ys[NV];
-        Cells<H, W> hs[NV], es[NV];
+        Cells<Y, ANY> ys[NV];
+        Cells<H, ANY> hs[NV], es[NV];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int at = i * G + lane;
             ys[i].zero();
             hs[i].zero();
             if (at < parts) {
-                ys[i].load((const Y *)p.dy + t * p.dy_row + at * W);
-                hs[i].load((const H *)p.h + t * p.h_row + at * W);
+                ys[i].load((const Y *)p.dy + t * p.dy_row + at * W, n_of(at));
+                hs[i].load((const H *)p.h + t * p.h_row + at * W, n_of(at));
             }
         }
         if (p.dh) {
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const int at = i * G + lane;
-                if (at < parts) es[i].load((const H *)p.dh + t * p.dh_row + at * W);
+                if (at < parts) es[i].load((const H *)p.dh + t * p.dh_row + at * W, n_of(at));
             }
         }
         float sum = 0.0f, dot = 0.0f;
@@ -217,14 +232,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_grad_rows(SeqNormGrad 
             float h[W], u[W];
             hs[i].get(h);
             ys[i].get(u);
-            if (p.gain) {
-                float g[W];
 #pragma unroll
-                for (int j = 0; j < W; j++) g[j] = 0.0f;
-                if (i * G + lane < parts) get_cells<W>(p.gain, p.gain_dtype, (i * G + lane) * W, g);
-#pragma unroll
-                for (int j = 0; j < W; j++) u[j] *= g[j];
-            }
+            for (int j = 0; j < W; j++) u[j] *= gain[i][j];
 #pragma unroll
             for (int j = 0; j < W; j++) { sum += h[j] * h[j]; dot += u[j] * h[j]; }
         }
@@ -241,12 +250,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_grad_rows(SeqNormGrad 
 #pragma unroll
             for (int j = 0; j < W; j++) dgain[i][j] += u[j] * (h[j] * rho);
             if (at >= parts) continue;
-            if (p.gain) {
-                float g[W];
-                get_cells<W>(p.gain, p.gain_dtype, at * W, g);
 #pragma unroll
-                for (int j = 0; j < W; j++) u[j] *= g[j];
-            }
+            for (int j = 0; j < W; j++) u[j] *= gain[i][j];
 #pragma unroll
             for (int j = 0; j < W; j++) d[j] = (u[j] - h[j] * pull) * rho;
             if (p.dh) {
@@ -255,16 +260,18 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_grad_rows(SeqNormGrad 
 #pragma unroll
                 for (int j = 0; j < W; j++) d[j] += e[j];
             }
-            Cells<H, W>::put((H *)p.d + t * p.d_row + at * W, d);
-            if (p.dx) put_cells<W>(p.dx, p.x_dtype, t * p.dx_row + at * W, d);
+            Cells<H, ANY>::put((H *)p.d + t * p.d_row + at * W, d, n_of(at));
+            if (p.dx) put_cells<ANY>(p.dx, p.x_dtype, t * p.dx_row + at * W, d, n_of(at));
         }
     }
     if (!partial) return;
     float *out = partial + block_number() * p.width;
     if constexpr (ROWS == 1) {
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (i * G + lane < parts) Cells<float, W>::put(out + (i * G + lane) * W, dgain[i]);
+        for (int i = 0; i < NV; i++) {
+            const int at = i * G + lane;
+            if (at < parts) Cells<float, ANY>::put(out + at * W, dgain[i], n_of(at));
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < NV; i++)
@@ -343,35 +350,27 @@ __global__ __launch_bounds__(1024) void norm_columns(const float *partial, int r
 
 // ------------------------------------------------------------------- launches
 
-// Calls f(Const<G>, Const<NV>) with the threads and parts of a row of `parts` parts of W
-// values; false where registers do not hold it.
-template <int W, typename F> bool row_shape(int64_t parts, F f) {
-    if constexpr (W == 8) {
-        if (parts <= 16) f(Const<16>(), Const<1>());
-        else if (parts <= 32) f(Const<32>(), Const<1>());
-        else if (parts <= 64) f(Const<64>(), Const<1>());
-        else if (parts <= 128) f(Const<64>(), Const<2>());
-        else if (parts <= 256) f(Const<256>(), Const<1>());
-        else if (parts <= 512) f(Const<256>(), Const<2>());
-        else if (parts <= 1024) f(Const<256>(), Const<4>());
-        else if (parts <= 2048) f(Const<1024>(), Const<2>());
-        else return false;
-    } else {
-        if (parts <= 128) f(Const<16>(), Const<8>());
-        else if (parts <= 512) f(Const<64>(), Const<8>());
-        else if (parts <= 2048) f(Const<256>(), Const<8>());
-        else if (parts <= 16384) f(Const<1024>(), Const<16>());
-        else return false;
-    }
+// Calls f(Const<G>, Const<NV>) with the threads of a row of `parts` parts and the parts of
+// each; false where registers do not hold it.
+template <typename F> bool row_shape(int64_t parts, F f) {
+    if (parts <= 16) f(Const<16>(), Const<1>());
+    else if (parts <= 32) f(Const<32>(), Const<1>());
+    else if (parts <= 64) f(Const<64>(), Const<1>());
+    else if (parts <= 128) f(Const<64>(), Const<2>());
+    else if (parts <= 256) f(Const<256>(), Const<1>());
+    else if (parts <= 512) f(Const<256>(), Const<2>());
+    else if (parts <= 1024) f(Const<256>(), Const<4>());
+    else if (parts <= 2048) f(Const<1024>(), Const<2>());
+    else return false;
     return true;
 }
 
-template <typename X, typename H, bool RES, int W>
+template <typename X, typename H, bool RES, bool ANY>
 bool launch_norm(const SeqNorm &p, hipStream_t s) {
-    return row_shape<W>(p.width / W, [&](auto g, auto nv) {
+    return row_shape((p.width + 7) / 8, [&](auto g, auto nv) {
         constexpr int G = g.value, NV = nv.value, THREADS = G < 256 ? 256 : G;
         constexpr int ROWS = THREADS / G;
-        norm_rows<X, H, RES, W, G, NV>
+        norm_rows<X, H, RES, ANY, G, NV>
             <<<grid_of((p.tokens + ROWS - 1) / ROWS, THREADS), THREADS, 0, s>>>(p);
     });
 }
@@ -379,7 +378,7 @@ template <typename X, typename H, bool RES> bool launch_norm(const SeqNorm &p, h
     const bool eights = p.width % 8 == 0 && in_eights(p.x, p.x_row) &&
                         in_eights(p.residual, p.residual_row) && in_eights(p.h, p.h_row) &&
                         in_eights(p.gain, 0) && in_eights(p.y, p.y_row);
-    return eights ? launch_norm<X, H, RES, 8>(p, s) : launch_norm<X, H, RES, 1>(p, s);
+    return eights ? launch_norm<X, H, RES, false>(p, s) : launch_norm<X, H, RES, true>(p, s);
 }
 template <typename X> bool launch_norm(const SeqNorm &p, hipStream_t s) {
     if (!p.residual) return launch_norm<X, X, false>(p, s);
@@ -423,17 +422,17 @@ int64_t norm_grad_bytes(const SeqNormGrad &p) {
 }
 
 // Launches the rows' kernel; returns the rows of partial sums that it leaves.
-template <typename Y, typename H, int W>
+template <typename Y, typename H, bool ANY>
 int launch_norm_grad(const SeqNormGrad &p, float *partial, hipStream_t s) {
     int rows = 0;
-    row_shape<W>(p.width / W, [&](auto g, auto nv) {
+    row_shape((p.width + 7) / 8, [&](auto g, auto nv) {
         constexpr int G = g.value, NV = nv.value, THREADS = G < 256 ? 256 : G;
         constexpr int ROWS = THREADS / G;
         int64_t blocks = (p.tokens + ROWS - 1) / ROWS;
         const int64_t most = kGradBlocks * 256 / THREADS;
         if (partial && blocks > most) blocks = most;
         rows = partial ? (int)blocks : 0;
-        norm_grad_rows<Y, H, W, G, NV><<<grid_of(blocks, THREADS), THREADS, 0, s>>>(p, partial);
+        norm_grad_rows<Y, H, ANY, G, NV><<<grid_of(blocks, THREADS), THREADS, 0, s>>>(p, partial);
     });
     return rows;
 }
@@ -443,8 +442,8 @@ int launch_norm_grad(const SeqNormGrad &p, float *partial, hipStream_t s) {
                         in_eights(p.h, p.h_row) && in_eights(p.gain, 0) &&
                         in_eights(p.dh, p.dh_row) && in_eights(p.d, p.d_row) &&
                         in_eights(p.dx, p.dx_row);
-    return eights ? launch_norm_grad<Y, H, 8>(p, partial, s)
-                  : launch_norm_grad<Y, H, 1>(p, partial, s);
+    return eights ? launch_norm_grad<Y, H, false>(p, partial, s)
+                  : launch_norm_grad<Y, H, true>(p, partial, s);
 }
 template <typename Y> int launch_norm_grad(const SeqNormGrad &p, float *partial, hipStream_t s) {
     switch (p.h_dtype) {
