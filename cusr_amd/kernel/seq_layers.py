@@ -175,10 +175,10 @@ def _embedding(tokens, table, scale, dtype):
     T, (V, D) = tokens.shape[0], table.shape
     out = table.new_empty((T, D)) if dtype is table.dtype else table.new_empty((T, D), dtype=dtype)
     if T:
-        table = _rows(table)
+        table, tokens = _rows(table), tokens.contiguous()    # kept until the launch
         _run(load_library().seq_embedding, "seq_embedding", table.get_device(), _pack_embedding(
             _SIZE_EMBEDDING, _DTYPES[table.dtype], _DTYPES[dtype], tokens.dtype is torch.int64, T,
-            V, D, table.stride(0), D, scale, 0, tokens.contiguous().data_ptr(), table.data_ptr(),
+            V, D, table.stride(0), D, scale, 0, tokens.data_ptr(), table.data_ptr(),
             out.data_ptr()))
     return out
 

@@ -755,3 +755,35 @@ def test_far_offsets(ops):
     g = ops.token_logprobs_grad(x, at, lp[4], lp[1], one, one)
     assert torch.equal(g[-40:], ops.token_logprobs_grad(tail, at[:40], small[4], small[1],
                                                         one[:40], one[:40]))
+
+
+def test_copies_of_operands_live_until_the_launch(ops, monkeypatch):
+    """Operands that a call copies first are kept until its kernels are queued: memory that
+    another thread allocates and fills in between is not theirs."""
+    T, D, V = 3000, 96, 200
+    tokens, x, gain = ids(2 * T, V, 1)[::2], normal((T, 2 * D), BF, 2)[:, ::2], normal((2 * D,), F32, 3)
+    table, dy, dh = (normal((n, 2 * D), F32, 4 + n)[:, ::2] for n in (V, T, T + 1))
+    logits, g = normal((T, 2 * V), F32, 5)[:, ::2], normal((2 * T,), F32, 6)[::2]
+    a, w = int8s((T, 2 * D), 7)[:, ::2], int8s((V, 2 * D), 8)[:, ::2]
+
+    def calls():
+        _, entropy, *_, stats = ops.token_logprobs(logits, tokens, top=3, return_stats=True)
+        return (ops.embedding(tokens, table), ops.embedding_grad(dy, tokens, V),
+                *ops.rms_norm(x, gain[::2], residual=dy), *ops.rms_norm_int8(x, gain[::2]),
+                *ops.rms_norm_grad(x, dy, gain[::2], dh=dh[:T]),
+                ops.int8_product(a, g.abs(), w, gain[:1].expand(V)),
+                *ops.token_logprobs(logits, tokens, top=3),
+                ops.token_logprobs_grad(logits, tokens, stats, entropy, g, g))
+
+    want = calls()
+    real = ops._run
+
+    def run(*args):
+        taken = [torch.zeros(n, dtype=torch.uint8, device=DEV)
+                 for n in 4 * [8 * T, 4 * T, 2 * T * D, 4 * T * D, 4 * V * D, 4 * T * V, T * D, V * D,
+                               4 * D, 4 * V]]
+        real(*args)
+        del taken
+
+    monkeypatch.setattr(ops, "_run", run)
+    assert same(want, calls())
