@@ -322,7 +322,7 @@ def search(X, y, *, rounds=10, population=1024, max_iter=10, seed=0, proposer=No
     rng = np.random.default_rng(seed)
     best, history = (math.inf, None, None), []
     for i in range(rounds):
-        pop = p.sample(population, generator=g, int8=int8)
+        pop = p.sample(population, generator=g, **({"int8": True} if int8 else {}))
         native = p.programs(pop)
         inits = [rng.normal(size=int(np.sum(n[0] == popio.NODE_CONST))) for n in native]
         fits = lm.fit_batch(None, inits, X, y, native=native)

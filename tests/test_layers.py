@@ -5,12 +5,14 @@ from __future__ import annotations
 import ctypes
 import subprocess
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import layer_reference as ref
+from cusr_amd.benchmark import popio
 from cusr_amd.kernel import seq_layers as ops
 from cusr_amd.kernel import seq_ops
 from cusr_amd.kernel.co_inproc import CO_ERR_BOUNDS, CO_ERR_DATA, CO_ERR_NULLARG, CO_OK
@@ -271,3 +273,36 @@ def test_logprobs_gradient_against_differences():
     d, _ = ref.logprobs_grad(ref.logprobs(x, tokens, 0.7), tokens, gl, gh, 0.7, F)
     slope, want = (f(step) - f(-step)) / (2 * step), float((d * v).sum())
     assert abs(slope - want) < 1e-7 * (1 + abs(want))
+
+
+def test_a_search_with_a_proposer_of_its_own():
+    """A proposer that is given may know nothing of 8-bit products; it is asked for them only
+    where the search is."""
+    import numpy as np
+
+    from cusr_amd.demonstrator import proposer as pr
+    asked = []
+
+    class Fixed:
+        device = torch.device("cpu")
+
+        def sample(self, M, generator=None, **how):
+            asked.append(how)
+            return SimpleNamespace(lengths=torch.ones(M))
+
+        def programs(self, pop):
+            leaf = (np.array([popio.NODE_CONST]), np.array([0]), np.array([0]))
+            return [leaf] * len(pop.lengths)
+
+    class Still:
+        def step(self, pop, rewards):
+            return [0.0]
+
+    class Fits:
+        def fit_batch(self, _, inits, X, y, native):
+            return [SimpleNamespace(final_loss=1.0, constants=x) for x in inits]
+
+    for int8 in (False, True):
+        pr.search(np.zeros((3, 1)), np.ones(3), rounds=1, population=2, proposer=Fixed(),
+                  trainer=Still(), backend=Fits(), log=None, int8=int8)
+    assert asked == [{}, {"int8": True}]
