@@ -37,7 +37,11 @@ struct Bits8 {
     }
 };
 
-// A row per group of G threads, NV parts of 8 values a thread.
+// A row per group of G threads, NV parts of 8 values a thread: every load of a row is on its
+// way before the first sum, and the row is read once. Memory bounds it: 1.3 M rows of 128 in
+// bf16 into a stream in fp32 (2.0 GB) take 336 us at best, 5.9 TB/s, 16,383 of 4,096 into one
+// in bf16 (537 MB) 87, 6.2 TB/s, 24 of 4,096 3.4 us, which are three trips to memory and two
+// barriers. The gain is asked for before the first sum is joined.
 template <typename X, typename H, bool RES, bool ANY, int G, int NV>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_rows(SeqNorm p) {
     constexpr int THREADS = G < 256 ? 256 : G, ROWS = THREADS / G;
@@ -181,7 +185,9 @@ __global__ __launch_bounds__(1024) void norm_long(SeqNorm p) {
 // ------------------------------------------------------------------- gradient
 
 // A group's rows one after the other; the gain's gradient stays in registers and is
-// left as one row of partial sums a block.
+// left as one row of partial sums a block. Memory bounds it: 16,383 rows of 4,096 in bf16
+// with the stream's gradient (537 MB) take 115 us, 4.7 TB/s, the next row's loads waiting for
+// this one's sums; four such blocks a compute unit cover for each other.
 template <typename Y, typename H, bool ANY, int G, int NV>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_grad_rows(SeqNormGrad p,
                                                                     float *partial) {
@@ -328,7 +334,7 @@ __global__ __launch_bounds__(256) void norm_gain_long(SeqNormGrad p, const float
 }
 
 // The blocks' partial sums, column by column in one order: 32 columns a block, each the
-// sum of 32 threads' sums.
+// sum of 32 threads' sums. 1,024 rows of 4,096 take 5.0 us.
 __global__ __launch_bounds__(1024) void norm_columns(const float *partial, int rows,
                                                      int64_t width, float *dgain) {
     __shared__ float part[32][33];
@@ -351,7 +357,10 @@ __global__ __launch_bounds__(1024) void norm_columns(const float *partial, int r
 // ------------------------------------------------------------------- launches
 
 // Calls f(Const<G>, Const<NV>) with the threads of a row of `parts` parts and the parts of
-// each; false where registers do not hold it.
+// each; false where registers do not hold it. Up to 128 parts a row is a wave's at most, which
+// needs no barrier; beyond, a wave's registers would hold so much of a row that few waves
+// find room (the gradient of 16,383 rows of 4,096 in bf16: 147 us with a wave a row, 92 with
+// four).
 template <typename F> bool row_shape(int64_t parts, F f) {
     if (parts <= 16) f(Const<16>(), Const<1>());
     else if (parts <= 32) f(Const<32>(), Const<1>());
@@ -400,7 +409,8 @@ int check_norm(const SeqNorm *p) {
 }
 
 // Blocks of the gain's partial sums: enough to fill the chip, few enough that the sums
-// are small beside the rows.
+// are small beside the rows (16,383 rows of 4,096 in bf16: 94 us with 1,024, with 512 105,
+// with 2,048 98; h in dh's place too).
 constexpr int kGradBlocks = 1024;
 constexpr int64_t kLongChunks = 64;
 bool grad_is_long(const SeqNormGrad &p) { return p.width > 16384; }

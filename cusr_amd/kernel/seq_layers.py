@@ -312,7 +312,8 @@ def rms_norm(x, gain=None, *, residual=None, eps=1e-6, dtype=None):
     float32; gain [D] or None (1). The stream h = x + residual is rounded to residual's
     type (h = x without one), and y = gain * h / sqrt(mean(h**2) + eps), formed in
     float32, to `dtype` (x's by default). Returns y, or (y, h) with a residual. Gradients
-    go to x, residual and gain."""
+    go to x, residual and gain. A row of zeros with eps 0 gives NaN; one whose sum of squares
+    passes float32's largest number gives 0, and its gradient says nothing."""
     eps, dtype = _check_norm(x, gain, residual, eps), _type(dtype, x.dtype)
     if torch.is_grad_enabled() and (x.requires_grad
                                     or (gain is not None and gain.requires_grad)
