@@ -34,9 +34,10 @@ __device__ inline uint4v row_piece(const int8_t *row, int64_t l, int64_t inner) 
 // through LDS to leave as whole rows: stores of 32 bytes a row took 156 us for 8,192 x
 // 16,384 outputs of 128 terms. Those of large tiles pass the caches by, which hold operands
 // that are read again: 8,192 x 4,096 x 16,384 in 513 us rather than 565. WIDE: every 8
-// channels lie on a boundary of 16 bytes and are all inside or all outside.
+// channels lie on a boundary of 16 bytes and are all inside or all outside. RAW: the sums as
+// they are, in a float's place.
 template <typename O, int F> constexpr int slab_pitch() { return F * 32 + 16 / (int)sizeof(O); }
-template <typename O, bool WIDE, int F>
+template <typename O, bool WIDE, int F, bool RAW>
 __device__ inline void put_sums(const SeqInt8Product &p, int64_t i0, int64_t j0,
                                 const int16v (&acc)[F][F], const float *a_scale,
                                 const float *w_scale, O *slab) {
@@ -59,8 +60,13 @@ __device__ inline void put_sums(const SeqInt8Product &p, int64_t i0, int64_t j0,
                 for (int e = 0; e < 4; e++) {
                     const auto s = __builtin_amdgcn_permlane32_swap(
                         (uint32_t)acc[x][y][g * 8 + e], (uint32_t)acc[x][y][g * 8 + 4 + e], false, false);
-                    f[e] = (float)(int)s[0] * sa * lo[e];
-                    f[4 + e] = (float)(int)s[1] * sa * hi[e];
+                    if constexpr (RAW) {
+                        f[e] = __uint_as_float(s[0]);
+                        f[4 + e] = __uint_as_float(s[1]);
+                    } else {
+                        f[e] = (float)(int)s[0] * sa * lo[e];
+                        f[4 + e] = (float)(int)s[1] * sa * hi[e];
+                    }
                 }
                 Eight<O>::put(slab + lane % 32 * PITCH + col, f);
             }
@@ -112,11 +118,14 @@ __device__ inline bool tile_of(int64_t block, int64_t rows, int64_t columns, int
 // x 8,192 x 16,384 the products alone take 578 us (3.8 POP/s at the clock that the card
 // falls to), with the reads from LDS 718, with the copies into it 718, with both 941: LDS
 // bounds it.
-constexpr int kStep = 64, kStages = 5;
+constexpr int kStep = 64, kStages = 5, kMostCuts = 32;
 template <int T> constexpr int tile_bytes() { return 2 * T * kStep; }
 
-template <typename O, bool WIDE, int T>
-__global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Product p) {
+// RAW: a tile's terms are cut among `cuts` blocks, `terms` each, which leave their sums in
+// `parts` [cuts, m, n rounded up to 8] for int8_join.
+template <typename O, bool WIDE, int T, bool RAW>
+__global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Product p, int cuts,
+                                                                    int terms, float *parts) {
     constexpr int W = T / 2, F = W / 32;         // a wave's side, in products
     constexpr int COPIES = tile_bytes<T>() / 4096;           // a wave's copies of a step
     constexpr uint32_t BYTES = tile_bytes<T>(), ALL = kStages * BYTES;
@@ -124,11 +133,18 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Produ
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int64_t ti, tj;
-    if (!tile_of(block_number(), (p.m + T - 1) / T, (p.n + T - 1) / T, ti, tj)) return;
+    int64_t block = block_number(), cut = 0;
+    if constexpr (RAW) {                         // a cut's blocks are a multiple of eight
+        const int64_t each = (((p.m + T - 1) / T) * ((p.n + T - 1) / T) + 7) / 8 * 8;
+        cut = block / each;
+        block %= each;
+        if (cut >= cuts) return;                 // the launch's last numbers
+    }
+    if (!tile_of(block, (p.m + T - 1) / T, (p.n + T - 1) / T, ti, tj)) return;
     const int64_t i0 = ti * T, j0 = tj * T;
     float a_scale = 0.0f, w_scale = 0.0f;        // of row and column tid
-    if (tid < T && i0 + tid < p.m) a_scale = p.a_scale[i0 + tid];
-    if (tid < T && j0 + tid < p.n) w_scale = p.w_scale[j0 + tid];
+    if (!RAW && tid < T && i0 + tid < p.m) a_scale = p.a_scale[i0 + tid];
+    if (!RAW && tid < T && j0 + tid < p.n) w_scale = p.w_scale[j0 + tid];
     const uint32_t base = lds_address(lds);
     // Waves 0 and 1 bring a, waves 2 and 3 w. Copy x fills 16 rows, this lane row lane / 4,
     // place lane % 4; rows past the last are the last.
@@ -136,6 +152,12 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Produ
     const int64_t row_bytes = is_a ? p.a_row : p.w_row, first = is_a ? i0 : j0;
     const int64_t left = (is_a ? p.m : p.n) - 1 - first;
     const int8_t *from = (is_a ? p.a : p.w) + first * row_bytes;
+    int inner = (int)p.inner;
+    if constexpr (RAW) {
+        from += cut * terms;
+        inner -= (int)cut * terms;
+        if (inner > terms) inner = terms;
+    }
     uint32_t offset[COPIES];                     // below 2^32: the launch sees to it
     int piece[COPIES];
 #pragma unroll
@@ -151,7 +173,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Produ
         if constexpr (cut.value) {
             uint32_t o = offset[x];
             asm volatile("" : "+v"(o));          // no addresses kept over steps
-            copy_to_lds16(piece[x] < (int)p.inner - l ? (const void *)(from + l + o) : kZeros, to);
+            copy_to_lds16(piece[x] < inner - l ? (const void *)(from + l + o) : kZeros, to);
         } else {
             copy_to_lds16(from + l, offset[x], to);
         }
@@ -219,7 +241,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Produ
         copy(x / COPIES * kStep, x / COPIES * BYTES, x % COPIES, Const<1>());
     wait(Const<kStages - 2>());
     read(here, 0, a0, w0);
-    const int inner = (int)p.inner, whole = inner - kStages * kStep;
+    const int whole = inner - kStages * kStep;
     while (l <= whole) step(Const<0>());
     while (l < inner) step(Const<1>());
     wait(Const<0>());                            // the last step's reads are done
@@ -230,9 +252,38 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void int8_tiles(SeqInt8Produ
         scales[T + tid] = w_scale;
     }
     __syncthreads();
-    put_sums<O, WIDE, F>(p, i0 + wave / 2 * W, j0 + wave % 2 * W, acc, scales + wave / 2 * W,
-                         scales + T + wave % 2 * W,
-                         (O *)(scales + 2 * T) + wave * 32 * slab_pitch<O, F>());
+    if constexpr (RAW) {                         // whole eights of columns, those past n too
+        const int64_t pitch = (p.n + 7) / 8 * 8;
+        p.o = parts + cut * p.m * pitch;
+        p.o_row = p.n = pitch;
+    }
+    put_sums<O, WIDE, F, RAW>(p, i0 + wave / 2 * W, j0 + wave % 2 * W, acc, scales + wave / 2 * W,
+                              scales + T + wave % 2 * W,
+                              (O *)(scales + 2 * T) + wave * 32 * slab_pitch<O, F>());
+}
+
+// Adds up the cuts' sums, which are exact in any order: eight columns a thread. A launch more
+// and the way of the sums through the last cache: 5 us with 16 cuts of 24 x 1,024, 8 with
+// four of 64 x 4,096.
+__global__ __launch_bounds__(256) void int8_join(SeqInt8Product p, int cuts, const int *parts) {
+    const int64_t eights = (p.n + 7) / 8, at = (int64_t)block_number() * 256 + threadIdx.x;
+    const int64_t i = at / eights, j = at % eights * 8;
+    if (i >= p.m) return;
+    const int4v *from = (const int4v *)(parts + at * 8);
+    const int64_t step = p.m * eights * 2;
+    int4v lo = {0, 0, 0, 0}, hi = lo;
+#pragma unroll 8
+    for (int c = 0; c < cuts; c++) {
+        lo += from[c * step];
+        hi += from[c * step + 1];
+    }
+    const int n = cells_of<true>(p.n, (int)(j / 8));
+    const float sa = p.a_scale[i];
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        f[e] = e < n ? (float)(e < 4 ? lo[e % 4] : hi[e % 4]) * sa * p.w_scale[j + e] : 0.0f;
+    put_cells<true>(p.o, p.out_dtype, i * p.o_row + j, f, n);
 }
 
 // Rows off 16-byte boundaries, or that no whole number of pieces fills, are laid out anew
@@ -250,8 +301,8 @@ __global__ __launch_bounds__(256) void int8_pack(const int8_t *from, int64_t row
 
 // Few tokens: 16 channels a block and up to 16 M tokens, the terms cut among eight waves,
 // which read both operands from memory as the 16x16x64 product takes them and join their
-// sums in LDS. The weights are read once; the way to memory bounds it where blocks are fewer
-// than compute units (16 x 16,384 x 4,096, 67 MB, in 20 us with the call, 3.4 TB/s).
+// sums in LDS. The weights are read once. 1 x 4,096 x 4,096 takes 4.4 us, 3.8 TB/s of what the
+// caches hold, 24 x 4,096 x 4,096 7.5: the steps of a wave wait for the way to memory.
 template <int M>
 __global__ __launch_bounds__(512) void int8_few(SeqInt8Product p) {
     constexpr int WAVES = 8;
@@ -325,10 +376,65 @@ int64_t packed_row(const SeqInt8Product &p) { return (p.inner + 15) / 16 * 16; }
 int64_t packed_bytes(int64_t rows, const SeqInt8Product &p) {
     return (rows * packed_row(p) + 255) / 256 * 256;
 }
+
+// How a product is made: by int8_few<few>, or tiles of `side`, their terms in `cuts`.
+struct Int8Plan { int few, side, cuts, terms; };
+
+// Tiles first, those that take the least time: 256 of them, one to a compute unit, take 9, 21
+// and 46 us for 4,096 terms (sides of 64, 128 and 256), and more take as many times as long
+// (512 x 4,096 x 4,096: 19, 19, 48 us; 1,024: 36, 24, 52; 3,000: 97, 61, 58; 4,096: 122, 80,
+// 66). Then the same with the terms cut, whose sums are written and joined, and few tokens'
+// own kernel, by the times in ns that these come to. Tiles, their terms in 2, 4, 8 and 16,
+// few tokens' kernel, in us:
+//   24 x 4,096 x 4,096    10.0  10.5   9.6   9.7  12.5    7.6
+//   24 x 4,096 x 6,144    10.1  10.8  10.9  12.3  15.2   12.1
+//   24 x 16,384 x 1,024   31.0  21.1  14.4  10.7  10.1   20.5
+//   16 x 16,384 x 4,096   31.4  22.3  16.7  16.9  17.9   16.9
+//   64 x 4,096 x 4,096    10.1  11.2  10.8  13.3  18.6
+//   64 x 16,384 x 4,096   34.0  24.1  18.3  19.6  21.8
+//   512 x 16,384 x 4,096  58.0  48.8  55.1  61.9  77.0
+// What is taken is the least of a row, or within 1 in 20 of it.
+Int8Plan int8_plan(const SeqInt8Product &p) {
+    const int64_t inner = packed_row(p);
+    auto rounds = [](int64_t blocks) { return (blocks + 255) / 256; };
+    const int64_t t64 = rounds(tiles_of(p, 64)), t128 = rounds(tiles_of(p, 128)),
+                  t256 = rounds(tiles_of(p, 256));
+    Int8Plan r = {0, 256, 1, 0};
+    if (9 * t64 <= 21 * t128 && 9 * t64 <= 46 * t256) r.side = 64;
+    else if (21 * t128 <= 46 * t256) r.side = 128;
+    int64_t best = r.side == 64 ? 2600 + t64 * 7500 * inner / 4096
+                 : r.side == 128 ? 3000 + t128 * 18000 * inner / 4096
+                                 : 4000 + t256 * 42000 * inner / 4096;
+    auto cut = [&](int side, int64_t base, int64_t each, int cuts) {
+        const int64_t time = base + rounds(tiles_of(p, side) * cuts) * each * (inner / cuts) / 4096 +
+                             4500 + p.m * p.n / 600 * cuts;
+        if (time < best) {
+            best = time;
+            r.side = side;
+            r.cuts = cuts;
+        }
+    };
+    const int64_t tiles = tiles_of(p, 64);       // enough of them leave nothing to cut for
+    for (int cuts = 2; cuts <= kMostCuts && inner / cuts >= 512 && tiles * cuts <= 2048; cuts++) {
+        cut(64, 2600, 7500, cuts);
+        cut(128, 3000, 18000, cuts);
+    }
+    const int64_t channels = rounds((p.n + 15) / 16);
+    if (p.m <= 16 && 2500 + channels * 3500 * inner / 4096 < best) r = {1, 0, 1, 0};
+    else if (p.m > 16 && p.m <= 32 && 2700 + channels * 4500 * inner / 4096 < best) r = {2, 0, 1, 0};
+    if (r.cuts > 1) {
+        r.terms = (int)((inner + r.cuts - 1) / r.cuts + kStep - 1) / kStep * kStep;
+        r.cuts = (int)((inner + r.terms - 1) / r.terms);
+    }
+    return r;
+}
+int64_t parts_bytes(const SeqInt8Product &p, const Int8Plan &r) {
+    return r.cuts > 1 ? 4 * r.cuts * p.m * ((p.n + 7) / 8 * 8) : 0;
+}
 int64_t int8_bytes(const SeqInt8Product &p) {
     if (p.m == 0 || p.n == 0 || p.inner == 0) return 0;
     return (needs_pack(p, p.a, p.a_row) ? packed_bytes(p.m, p) : 0) +
-           (needs_pack(p, p.w, p.w_row) ? packed_bytes(p.n, p) : 0);
+           (needs_pack(p, p.w, p.w_row) ? packed_bytes(p.n, p) : 0) + parts_bytes(p, int8_plan(p));
 }
 void pack(const int8_t *&x, int64_t &row, int64_t rows, const SeqInt8Product &p, char *&ws,
           hipStream_t s) {
@@ -349,21 +455,26 @@ template <int M> void launch_few(const SeqInt8Product &p, hipStream_t s) {
 }
 template <typename O, bool WIDE, int T> void launch_tiles(const SeqInt8Product &p, hipStream_t s) {
     const int64_t blocks = (tiles_of(p, T) + 7) / 8 * 8;
-    int8_tiles<O, WIDE, T><<<grid_of(blocks, 256), 256, kStages * tile_bytes<T>(), s>>>(p);
+    int8_tiles<O, WIDE, T, false><<<grid_of(blocks, 256), 256, kStages * tile_bytes<T>(), s>>>(
+        p, 1, 0, nullptr);
 }
-// The tiles that take the least time: 256 of them, one to a compute unit, take 9, 21 and 46
-// us for 4,096 terms (sides of 64, 128 and 256), and more take as many times as long
-// (512 x 4,096 x 4,096: 19, 19, 48 us; 1,024: 36, 24, 52; 3,000: 97, 61, 58; 4,096: 122, 80, 66).
-template <typename O, bool WIDE> void launch_tiles(const SeqInt8Product &p, hipStream_t s) {
-    auto time = [&](int64_t t, int64_t each) { return (tiles_of(p, t) + 255) / 256 * each; };
-    const int64_t t64 = time(64, 9), t128 = time(128, 21), t256 = time(256, 46);
-    if (t64 <= t128 && t64 <= t256) launch_tiles<O, WIDE, 64>(p, s);
-    else if (t128 <= t256) launch_tiles<O, WIDE, 128>(p, s);
+template <int T> void launch_cuts(const SeqInt8Product &p, const Int8Plan &r, void *parts,
+                                  hipStream_t s) {
+    const int64_t blocks = (tiles_of(p, T) + 7) / 8 * 8 * r.cuts;
+    int8_tiles<float, true, T, true><<<grid_of(blocks, 256), 256, kStages * tile_bytes<T>(), s>>>(
+        p, r.cuts, r.terms, (float *)parts);
+    const int64_t threads = p.m * ((p.n + 7) / 8);
+    int8_join<<<grid_of((threads + 255) / 256, 256), 256, 0, s>>>(p, r.cuts, (const int *)parts);
+}
+template <typename O, bool WIDE>
+void launch_tiles(const SeqInt8Product &p, const Int8Plan &r, hipStream_t s) {
+    if (r.side == 64) launch_tiles<O, WIDE, 64>(p, s);
+    else if (r.side == 128) launch_tiles<O, WIDE, 128>(p, s);
     else launch_tiles<O, WIDE, 256>(p, s);
 }
-template <typename O> void launch_tiles(const SeqInt8Product &p, hipStream_t s) {
-    if (in_eights(p.o, p.o_row) && p.n % 8 == 0) launch_tiles<O, true>(p, s);
-    else launch_tiles<O, false>(p, s);
+template <typename O> void launch_tiles(const SeqInt8Product &p, const Int8Plan &r, hipStream_t s) {
+    if (in_eights(p.o, p.o_row) && p.n % 8 == 0) launch_tiles<O, true>(p, r, s);
+    else launch_tiles<O, false>(p, r, s);
 }
 
 }  // namespace seq
@@ -385,27 +496,27 @@ extern "C" int seq_int8_product(const SeqInt8Product *p, void *stream) {
     if (p->workspace_bytes < bytes || (bytes && ((uintptr_t)p->workspace & 255))) return CO_ERR_DATA;
     hipStream_t s = (hipStream_t)stream;
     SeqInt8Product q = *p;
+    const seq::Int8Plan plan = seq::int8_plan(q);
+    char *ws = (char *)q.workspace;
     if (q.inner) {
-        char *ws = (char *)q.workspace;
         seq::pack(q.a, q.a_row, q.m, *p, ws, s);
         seq::pack(q.w, q.w_row, q.n, *p, ws, s);
         q.inner = seq::packed_row(*p);           // zeros beyond it, or nothing
     } else {
         q.a_row = q.w_row = 0;                   // no row is read
     }
-    // Few tokens and so few channels that tiles would not fill the chip: the terms are cut
-    // (24 x 16,384 x 1,024: 21 against 31 us, 16 x 16,384 x 4,096: 20 against 32; but 16 x
-    // 4,096 x 16,384: 18 against 12, and 32 x 4,096 x 6,144: 14 against 10).
-    const int64_t sixteens = (q.m + 15) / 16, channels = (q.n + 15) / 16;
-    if (sixteens == 1 && channels <= 512) {
+    if (plan.few == 1) {
         seq::launch_few<1>(q, s);
-    } else if (sixteens == 2 && channels <= 128) {
+    } else if (plan.few) {
         seq::launch_few<2>(q, s);
+    } else if (plan.cuts > 1) {
+        if (plan.side == 64) seq::launch_cuts<64>(q, plan, ws, s);
+        else seq::launch_cuts<128>(q, plan, ws, s);
     } else {
         switch (q.out_dtype) {
-            case SEQ_FP32: seq::launch_tiles<float>(q, s); break;
-            case SEQ_BF16: seq::launch_tiles<__bf16>(q, s); break;
-            default: seq::launch_tiles<_Float16>(q, s); break;
+            case SEQ_FP32: seq::launch_tiles<float>(q, plan, s); break;
+            case SEQ_BF16: seq::launch_tiles<__bf16>(q, plan, s); break;
+            default: seq::launch_tiles<_Float16>(q, plan, s); break;
         }
     }
     return seq::launch_status();

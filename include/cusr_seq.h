@@ -242,7 +242,8 @@ int seq_norm_grad(const SeqNormGrad *n, void *stream);
 /* Product of 8-bit integers: o[i, j] = a_scale[i] w_scale[j] * sum over l of
  * a[i, l] w[j, l], the sum exact, the rest in fp32, rounded once to out_dtype.
  * a [m, inner], w [n, inner] (a row holds what one output takes). Operands whose address,
- * rows or inner size are no multiples of 16 are copied into the workspace first. */
+ * rows or inner size are no multiples of 16 are copied into the workspace first; long
+ * sums of few outputs are cut, and joined from there. */
 typedef struct SeqInt8Product {
     int32_t struct_size;
     int32_t out_dtype;

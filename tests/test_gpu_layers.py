@@ -349,6 +349,31 @@ def test_int8_product(ops, M, K, N):
             first = got
 
 
+# long sums of few outputs, which are cut among blocks: sides of 64 and 128, odd and ragged
+CUT = [(40, 16384, 72), (33, 8208, 1001), (100, 12000, 255), (17, 65536, 9), (3, 70001, 50),
+       (512, 16384, 136), (64, 131071, 8), (1, 131071, 1), (130, 4112, 7), (700, 20480, 1500)]
+
+
+@pytest.mark.parametrize("M,K,N", CUT)
+def test_int8_product_of_long_sums(ops, M, K, N):
+    _say("int8_product, cut", M, K, N)
+    a, sa, w, sw, want = product_case(M, K, N)
+    for dt in (F32, BF):
+        tol = ref.rounded(want, dt, 3.1 * E32 * want.abs())
+        got = ops.int8_product(a, sa, w, sw, dtype=dt)
+        check("o", got, want, tol)
+        assert torch.equal(got, ops.int8_product(layouts(a)[1], sa, w, sw, dtype=dt))
+    stream, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        out = ops.int8_product(a, sa, w, sw)
+    for seed in range(2):
+        a.copy_(int8s((M, K), 10 + seed))
+        got = ops.int8_product(a, sa, w, sw)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, got)
+
+
 def test_int8_product_extremes(ops):
     """The largest sums there are, of one sign and the other."""
     K = ops.SEQ_MAX_INNER

@@ -306,3 +306,21 @@ def test_a_search_with_a_proposer_of_its_own():
         pr.search(np.zeros((3, 1)), np.ones(3), rounds=1, population=2, proposer=Fixed(),
                   trainer=Still(), backend=Fits(), log=None, int8=int8)
     assert asked == [{}, {"int8": True}]
+
+
+def test_workspace_of_a_product():
+    """None where operands lie as they are read and the sums are short; room for every cut's
+    sums where they are long and few, in any layout."""
+    lib = seq_ops.load_library()
+
+    def need(m, inner, n, row=None):
+        c = ops.SeqInt8Product(struct_size=ctypes.sizeof(ops.SeqInt8Product), m=m, n=n, inner=inner,
+                               a_row=row or inner, w_row=inner, o_row=n, a=4096, w=4096)
+        return lib.seq_int8_product_workspace(ctypes.string_at(ctypes.byref(c), ctypes.sizeof(c)))
+
+    for shape in ((1, 4096, 4096), (24, 4096, 6144), (8192, 4096, 16384), (300, 256, 300)):
+        assert need(*shape) == 0
+    # a whole number of cuts, at least two, of 64 by 1,001 sums in rows of 1,008
+    cuts, rest = divmod(need(64, 16384, 1001), 4 * 64 * 1008)
+    assert cuts >= 2 and rest == 0
+    assert need(64, 16384, 1001, 16385) == need(64, 16384, 1001) + 64 * 16384
