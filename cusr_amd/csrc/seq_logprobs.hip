@@ -132,17 +132,19 @@ __device__ inline void put_row(const SeqLogprobs &p, const Warmth &w, int64_t t,
 }
 
 // Alternatives are ordered by keys: a value's place among floats, NaN the largest, then
-// the lower column before the higher. 0 is below every key.
+// the lower column before the higher. 0 is below every key and ~0 above: a NaN's place is not
+// the last one, so that its key in column 0 is none either.
 typedef unsigned long long Key;
+constexpr uint32_t kNanPlace = 0xfffffffeu;
 __device__ inline Key key_of(float x, uint32_t col) {
     const uint32_t b = __float_as_uint(x + 0.0f);             // -0 as +0
-    const uint32_t o = x != x ? 0xffffffffu : (b >> 31 ? ~b : b | 0x80000000u);
+    const uint32_t o = x != x ? kNanPlace : (b >> 31 ? ~b : b | 0x80000000u);
     return ((Key)o << 32) | (uint32_t)~col;
 }
 __device__ inline uint32_t col_of(Key k) { return ~(uint32_t)k; }
 __device__ inline float value_of(Key k) {
     const uint32_t o = (uint32_t)(k >> 32);
-    if (o == 0xffffffffu) return __builtin_nanf("");
+    if (o == kNanPlace) return __builtin_nanf("");
     return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o);
 }
 __device__ inline Key larger(Key a, Key b) { return a > b ? a : b; }

@@ -506,7 +506,8 @@ def token_logprobs(logits, tokens, *, temperature=1.0, top=0, return_stats=False
     token_logprobs_grad takes.
 
     A row whose logits are all -inf has logp -inf, entropy 0 and the alternatives 0, 1, ..
-    at -inf; one with NaN or +inf gives NaN; a token outside the vocabulary gives logp NaN.
+    at -inf; one with NaN or +inf gives NaN, a NaN coming before every number among its
+    alternatives; a token outside the vocabulary gives logp NaN.
     Gradients of logp and entropy go to the logits; the alternatives carry none. Sums are
     held in float32; a row of nearly all weight on one symbol keeps the precision of
     the little that is left."""

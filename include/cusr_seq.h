@@ -262,8 +262,8 @@ int seq_int8_product(const SeqInt8Product *p, void *stream);
  * temperature: logp = z[id] - logsumexp z, entropy = -sum p log p (0 log 0 = 0), and
  * the `top` largest log-probabilities of each row with their columns, the lower column
  * first among equals. A row whose logits are all -inf has logp -inf, entropy 0 and
- * the alternatives 0, 1, .. at -inf; one with NaN or +inf gives NaN (its columns are
- * some of the row's); a token outside the vocabulary gives logp NaN.
+ * the alternatives 0, 1, .. at -inf; one with NaN or +inf gives NaN (its columns have
+ * NaN before the numbers); a token outside the vocabulary gives logp NaN.
  * stats [tokens, 2], for the gradient: the row's largest logit and the sum of
  * exp(z - largest z) over the others (both 0 where all are -inf): what rounding
  * would take from logsumexp, or from the sum with its 1, is in every p. */
