@@ -234,9 +234,10 @@ class Proposer:
     def alternatives(self, pop, top=3, temperature=1.0):
         """What the present policy makes of each of the population's symbols: (log-probability
         [T], entropy [T], the `top` likeliest symbols' log-probabilities [T, top], those
-        symbols [T, top]). A symbol that is not allowed there comes last, at -inf."""
+        symbols [T, top]); top: as many as there are symbols, and 64, at most. A symbol that is
+        not allowed there comes last, at -inf."""
         return seq_layers.token_logprobs(self.logits(pop), pop.symbols, temperature=temperature,
-                                         top=min(top, self.symbols.size))
+                                         top=min(top, self.symbols.size, seq_layers.SEQ_MAX_TOP))
 
     @torch.no_grad()
     def log_probabilities(self, pop):

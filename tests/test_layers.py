@@ -308,6 +308,18 @@ def test_a_search_with_a_proposer_of_its_own():
     assert asked == [{}, {"int8": True}]
 
 
+def test_alternatives_of_a_large_vocabulary(monkeypatch):
+    """As many alternatives as there are symbols, and as token_logprobs gives at most."""
+    from cusr_amd.demonstrator import proposer as pr
+    monkeypatch.setattr(pr.seq_layers, "token_logprobs", lambda logits, tokens, **how: how["top"])
+    for n_vars in (2, 300):
+        p = pr.Proposer(n_vars, device="cpu")
+        monkeypatch.setattr(p, "logits", lambda pop: None)
+        for top in (0, 3, 99, 1000):
+            got = p.alternatives(SimpleNamespace(symbols=None), top=top)
+            assert got == min(top, p.symbols.size, ops.SEQ_MAX_TOP)
+
+
 def test_workspace_of_a_product():
     """None where operands lie as they are read and the sums are short; room for every cut's
     sums where they are long and few, in any layout."""
