@@ -241,6 +241,7 @@ int seq_norm_grad(const SeqNormGrad *n, void *stream);
 
 /* Product of 8-bit integers: o[i, j] = a_scale[i] w_scale[j] * sum over l of
  * a[i, l] w[j, l], the sum exact, the rest in fp32, rounded once to out_dtype.
+ * No intermediate passes fp32's largest number where the product does not.
  * a [m, inner], w [n, inner] (a row holds what one output takes). Operands whose address,
  * rows or inner size are no multiples of 16 are copied into the workspace first; long
  * sums of few outputs are cut, and joined from there. */

@@ -5,8 +5,10 @@ from __future__ import annotations
 import pytest
 import torch
 
+import layer_reference as ref
+from seq_reference import E32
 from test_gpu_layers import ids, layouts
-from test_gpu_seq import BF, DEV, F32, _say
+from test_gpu_seq import BF, DEV, F32, _say, check
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +56,42 @@ def test_alternatives_of_rows_with_nan(ops, V, T, top, dt):
         odd = x.isnan().any(1)
         assert bool(top_logp[odd].isnan().all()) and bool(logp[odd].isnan().all())
         assert not bool(top_logp[~odd].isnan().any())
+
+
+# --------------------------------------------------- scales far from each other
+
+# few tokens' kernel, tiles of 64, 128 and 256, terms cut among blocks, rows laid out anew,
+# columns that no eights fill
+PRODUCTS = [(1, 64, 33), (20, 128, 96), (70, 96, 100), (700, 64, 520), (3000, 64, 2056),
+            (2048, 128, 4096), (24, 16384, 96), (64, 16384, 1001), (33, 77, 40)]
+
+
+@pytest.mark.parametrize("out", [F32, BF])
+@pytest.mark.parametrize("M,K,N", PRODUCTS)
+def test_int8_product_of_scales_far_apart(ops, M, K, N, out):
+    """A sum times one scale may pass float32 where the whole product does not; the rows
+    beside such a one keep their bits."""
+    _say("scales", M, K, N, out)
+    g = torch.Generator().manual_seed(M + N)
+    a, w = (torch.randint(-127, 128, s, generator=g).to(torch.int8).to(DEV) for s in ((M, K), (N, K)))
+    a[:, 0], w[:, 0] = 127, 127
+    usual = torch.rand(M, generator=g).to(DEV) + 0.5
+    sa, sw = usual.clone(), (torch.rand(N, generator=g) + 0.5).to(DEV) * 1e-36
+    far = torch.arange(M, device=DEV) % 3 == 0
+    sa[far] *= 2e38
+    sums = a.cpu().double() @ w.cpu().double().t()
+    want = sums * sa.cpu().double()[:, None] * sw.cpu().double()
+    got = ops.int8_product(a, sa, w, sw, dtype=out)
+    assert bool(got.isfinite().all())
+    # an integer's rounding to float32 and two products', and the output's
+    least = torch.full_like(want, 2.0 ** -149 if out is F32 else 2.0 ** -133)
+    check("o", got, want, ref.rounded(want, out, 4 * E32 * want.abs()) + least)
+    plain = ops.int8_product(a, usual, w, sw, dtype=out)
+    assert torch.equal(got[~far], plain[~far])
+    # the whole product passes float32: infinite, and 0 where the sum is 0
+    a[:, 1:], w[:, 1:] = 0, 0
+    w[::2, 0] = 0
+    got = ops.int8_product(a, torch.full_like(sa, 3e38), w, sw * 1e36, dtype=out)
+    assert bool(got[:, 1::2].isinf().all()) and not bool(got[:, ::2].any())
+    got = ops.int8_product(a, sa * float("inf"), w, sw, dtype=out)
+    assert bool(got[:, 1::2].isinf().all()) and bool(got[:, ::2].isnan().all())
