@@ -161,13 +161,15 @@ __global__ __launch_bounds__(256) void embed_symbols(SeqEmbeddingGrad p, int sla
 }
 
 // The chunks' sums in their order: 32 places of the table a block, each by 32 threads (4.3 us
-// for 768 chunks of 22 rows of 128).
+// for 768 chunks of 22 rows of 128). S: float where 1,024 chunks make 32 of a thread's at most,
+// else double (which takes 2 us more for 12 rows of 4,096).
+template <typename S>
 __global__ __launch_bounds__(1024) void embed_chunks(SeqEmbeddingGrad p, int64_t chunks,
                                                      const float *partial) {
-    __shared__ float part[32][33];
+    __shared__ S part[32][33];
     const int x = threadIdx.x % 32, g = threadIdx.x / 32;
     const int64_t all = p.rows * p.width, at = blockIdx.x * 32ll + x;
-    float s = 0.0f;
+    S s = 0;
     if (at < all)
 #pragma unroll 8
         for (int64_t c = g; c < chunks; c += 32) s += partial[c * all + at];
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(1024) void embed_chunks(SeqEmbeddingGrad p, int64_t
         s = part[0][x];
 #pragma unroll
         for (int i = 1; i < 32; i++) s += part[i][x];
-        put1(p.dtable, p.out_dtype, at / p.width * p.dtable_row + at % p.width, s * p.scale);
+        put1(p.dtable, p.out_dtype, at / p.width * p.dtable_row + at % p.width, (float)s * p.scale);
     }
 }
 
@@ -609,7 +611,12 @@ int64_t chunk_of(int64_t tokens) {
 int64_t aligned256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // Slabs of columns and chunks of tokens of the symbols' kernel; chunks fill the chip and
-// have 16 tokens a wave at least.
+// have 16 tokens a wave at least, and 4,096 at most: those are added one after the other in
+// 32 bits, so that a sum's error does not grow with the tokens. (1,024 at most cost 3 to 5 in
+// 100 of the time, in more blocks.) The chunks' sums are some rows / 8,192 of a gradient in
+// 16 bits; where more rows than memory holds lie on each other, chunks are as long as a
+// workspace of 4 GiB makes them.
+constexpr int64_t kSymbolChunk = 4096 * kSymbolWaves, kSymbolBytes = 1ll << 32;
 struct SymbolPlan { int slabs; int64_t chunk, chunks; };
 bool few_symbols(const SeqEmbeddingGrad &p) { return p.rows <= kSymbolRows; }
 int64_t symbol_lds(const SeqEmbeddingGrad &p) { return kSymbolWaves * (p.rows + 1) * kSymbolCols * 4; }
@@ -620,6 +627,11 @@ SymbolPlan symbol_plan(const SeqEmbeddingGrad &p) {
     int64_t chunks = 256 * (fit < 8 ? fit : 8) / r.slabs;
     const int64_t most = (p.tokens + least - 1) / least;
     if (chunks < 1) chunks = 1;
+    // as many times over as chunks of that length need, so that the chip stays full to the end
+    const int64_t turn = chunks * kSymbolChunk;
+    const int64_t turns = (p.tokens + turn - 1) / turn;
+    const int64_t room = kSymbolBytes / (4 * p.rows * p.width * chunks);
+    chunks *= turns < room ? turns : room;       // room: 400 turns at least
     if (chunks > most) chunks = most;
     r.chunk = (p.tokens + chunks - 1) / chunks;
     r.chunks = (p.tokens + r.chunk - 1) / r.chunk;
@@ -632,7 +644,9 @@ template <typename T> void launch_symbols(const SeqEmbeddingGrad &p, float *part
     const bool pairs = !((uintptr_t)p.d_out % (2 * sizeof(T))) && p.dout_row % 2 == 0 && p.width % 2 == 0;
     if (pairs) embed_symbols<T, true><<<grid, 256, lds, s>>>(p, r.slabs, r.chunk, partial);
     else embed_symbols<T, false><<<grid, 256, lds, s>>>(p, r.slabs, r.chunk, partial);
-    embed_chunks<<<(unsigned)((p.rows * p.width + 31) / 32), 1024, 0, s>>>(p, r.chunks, partial);
+    const unsigned places = (unsigned)((p.rows * p.width + 31) / 32);
+    if (r.chunks <= 1024) embed_chunks<float><<<places, 1024, 0, s>>>(p, r.chunks, partial);
+    else embed_chunks<double><<<places, 1024, 0, s>>>(p, r.chunks, partial);
 }
 
 struct GradPlan {

@@ -95,3 +95,29 @@ def test_int8_product_of_scales_far_apart(ops, M, K, N, out):
     assert bool(got[:, 1::2].isinf().all()) and not bool(got[:, ::2].any())
     got = ops.int8_product(a, sa * float("inf"), w, sw, dtype=out)
     assert bool(got[:, 1::2].isinf().all()) and bool(got[:, ::2].isnan().all())
+
+
+# --------------------------------------------------- long sums of one sign
+
+def one_row(D, dt, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.rand(1, D, generator=g) * 0.5 + 0.5).to(dt).to(DEV)
+
+
+# what follows one another in float32: a wave's or a chunk's additions, 4,096 at most, and the
+# few that join them
+DEPTH = 4096 + 64
+
+
+@pytest.mark.parametrize("T,V,D", [(1200000, 32, 16384), (1200000, 20, 1027), (9000000, 7, 128),
+                                   (3000000, 5, 40000), (70000000, 32, 120)])
+def test_embedding_grad_of_one_sign(ops, T, V, D):
+    """One row's gradient over and over, whose roundings do not cancel: the error does not grow
+    with the tokens."""
+    _say("one sign", T, V, D)
+    d = one_row(D, F32, 1)
+    tokens = torch.full((T,), 3, dtype=torch.int32, device=DEV)
+    tokens[::7] = torch.arange(len(tokens[::7]), device=DEV, dtype=torch.int32) % V
+    got = ops.embedding_grad(d.expand(T, D), tokens, V)
+    want = torch.bincount(tokens.long(), minlength=V).double()[:, None] * d.double()
+    check("dtable", got, want.cpu(), want.cpu() * DEPTH * E32)
