@@ -424,8 +424,10 @@ __global__ __launch_bounds__(256) void embed_sum(SeqEmbeddingGrad p, Runs r) {
 
 // Joins the slots of a run that begins in a chunk and goes on, 128 columns at a time, 4 to a
 // thread. A block looks at eight chunks, 32 threads each, and those join a run of up to
-// eight more chunks by themselves; a longer one is the whole block's, in eight parts. 512
-// chunks of 32 words of 4,096 take 11 us, most of them the search for runs.
+// eight more chunks by themselves; a longer one is the whole block's, in eight parts, each
+// added in 64 bits, for it may have any number of chunks. 512 chunks of 32 words of 4,096 take
+// 11 us, most of them the search for runs.
+typedef double double4v __attribute__((ext_vector_type(4)));
 __global__ __launch_bounds__(256) void embed_join(SeqEmbeddingGrad p, Runs r) {
     __shared__ float4v part[8][33];
     __shared__ bool longer[8];
@@ -478,17 +480,18 @@ __global__ __launch_bounds__(256) void embed_join(SeqEmbeddingGrad p, Runs r) {
         }
         for (int64_t col0 = blockIdx.y * 128ll; col0 < p.width; col0 += gridDim.y * 128ll) {
             const int64_t col = col0 + x * 4;
-            float4v s = {0, 0, 0, 0};
+            double4v sum = {0, 0, 0, 0};
             if (col < p.width) {
-                if (g == 0) s = slot(2 * from + 1, col);
+                if (g == 0) sum = __builtin_convertvector(slot(2 * from + 1, col), double4v);
 #pragma unroll 8
-                for (int64_t at = from + 1 + g; at < end; at += 8) s += slot(2 * at, col);
+                for (int64_t at = from + 1 + g; at < end; at += 8)
+                    sum += __builtin_convertvector(slot(2 * at, col), double4v);
             }
             __syncthreads();
-            part[g][x] = s;
+            part[g][x] = __builtin_convertvector(sum, float4v);
             __syncthreads();
             if (g == 0 && col < p.width) {
-                s = part[0][x];
+                float4v s = part[0][x];
 #pragma unroll
                 for (int o = 1; o < 8; o++) s += part[o][x];
                 put(row, col, s);

@@ -110,7 +110,8 @@ DEPTH = 4096 + 64
 
 
 @pytest.mark.parametrize("T,V,D", [(1200000, 32, 16384), (1200000, 20, 1027), (9000000, 7, 128),
-                                   (3000000, 5, 40000), (70000000, 32, 120)])
+                                   (3000000, 5, 40000), (70000000, 32, 120),
+                                   (4000000, 33, 136), (6000000, 40, 24), (60000000, 33, 24)])
 def test_embedding_grad_of_one_sign(ops, T, V, D):
     """One row's gradient over and over, whose roundings do not cancel: the error does not grow
     with the tokens."""
