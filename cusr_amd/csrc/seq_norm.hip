@@ -326,21 +326,22 @@ __global__ __launch_bounds__(256) void norm_gain_long(SeqNormGrad p, const float
     const int64_t j = blockIdx.x * 256ll + threadIdx.x;
     if (j >= p.width) return;
     const int64_t a = blockIdx.y * chunk, b = a + chunk < p.tokens ? a + chunk : p.tokens;
-    float s = 0.0f;
+    double s = 0.0;                              // a chunk may have any number of rows
     for (int64_t t = a; t < b; t++)
         s += get1(p.dy, p.dy_dtype, t * p.dy_row + j) *
              (get1(p.h, p.h_dtype, t * p.h_row + j) * rhos[t]);
-    partial[blockIdx.y * p.width + j] = s;
+    partial[blockIdx.y * p.width + j] = (float)s;
 }
 
 // The blocks' partial sums, column by column in one order: 32 columns a block, each the
-// sum of 32 threads' sums. 1,024 rows of 4,096 take 5.0 us.
+// sum of 32 threads' sums. 1,024 rows of 4,096 take 5.0 us. S: float up to those, else double.
+template <typename S>
 __global__ __launch_bounds__(1024) void norm_columns(const float *partial, int rows,
                                                      int64_t width, float *dgain) {
-    __shared__ float part[32][33];
+    __shared__ S part[32][33];
     const int c = threadIdx.x % 32, g = threadIdx.x / 32;
     const int64_t j = blockIdx.x * 32ll + c;
-    float s = 0.0f;
+    S s = 0;
     if (j < width)
 #pragma unroll 4
         for (int r = g; r < rows; r += 32) s += partial[r * width + j];
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(1024) void norm_columns(const float *partial, int r
         s = part[0][c];
 #pragma unroll
         for (int i = 1; i < 32; i++) s += part[i][c];
-        dgain[j] = s;
+        dgain[j] = (float)s;
     }
 }
 
@@ -410,8 +411,10 @@ int check_norm(const SeqNorm *p) {
 
 // Blocks of the gain's partial sums: enough to fill the chip, few enough that the sums
 // are small beside the rows (16,383 rows of 4,096 in bf16: 94 us with 1,024, with 512 105,
-// with 2,048 98; h in dh's place too).
-constexpr int kGradBlocks = 1024;
+// with 2,048 98; h in dh's place too). A group adds 2,048 rows at most one after the other in
+// 32 bits, so that the error of many rows does not grow with them: beyond, there are as many
+// blocks more.
+constexpr int kGradBlocks = 1024, kGradRows = 2048;
 constexpr int64_t kLongChunks = 64;
 bool grad_is_long(const SeqNormGrad &p) { return p.width > 16384; }
 
@@ -425,10 +428,21 @@ int check_norm_grad(const SeqNormGrad *p) {
         return CO_ERR_DATA;
     return CO_OK;
 }
+// blocks of `threads` threads and `rows` rows each at a time that leave partial sums
+int64_t grad_blocks(int64_t tokens, int threads, int rows) {
+    const int64_t blocks = (tokens + rows - 1) / rows, most = kGradBlocks * 256 / threads;
+    const int64_t turn = most * rows * kGradRows, all = most * ((tokens + turn - 1) / turn);
+    return blocks < all ? blocks : all;
+}
 int64_t norm_grad_bytes(const SeqNormGrad &p) {
     if (!p.dgain || p.tokens == 0) return 0;
     if (grad_is_long(p)) return 4 * (p.tokens + kLongChunks * p.width);
-    return 4ll * kGradBlocks * p.width;
+    int64_t blocks = 0;
+    row_shape((p.width + 7) / 8, [&](auto g, auto) {
+        constexpr int G = g.value, THREADS = G < 256 ? 256 : G;
+        blocks = grad_blocks(p.tokens, THREADS, THREADS / G);
+    });
+    return 4 * blocks * p.width;
 }
 
 // Launches the rows' kernel; returns the rows of partial sums that it leaves.
@@ -438,9 +452,8 @@ int launch_norm_grad(const SeqNormGrad &p, float *partial, hipStream_t s) {
     row_shape((p.width + 7) / 8, [&](auto g, auto nv) {
         constexpr int G = g.value, NV = nv.value, THREADS = G < 256 ? 256 : G;
         constexpr int ROWS = THREADS / G;
-        int64_t blocks = (p.tokens + ROWS - 1) / ROWS;
-        const int64_t most = kGradBlocks * 256 / THREADS;
-        if (partial && blocks > most) blocks = most;
+        const int64_t blocks = partial ? grad_blocks(p.tokens, THREADS, ROWS)
+                                       : (p.tokens + ROWS - 1) / ROWS;
         rows = partial ? (int)blocks : 0;
         norm_grad_rows<Y, H, ANY, G, NV><<<grid_of(blocks, THREADS), THREADS, 0, s>>>(p, partial);
     });
@@ -495,7 +508,7 @@ extern "C" int seq_norm_grad(const SeqNormGrad *p, void *stream) {
     const unsigned blocks = (unsigned)((p->width + 31) / 32);
     if (p->tokens == 0) {
         if (!p->dgain) return CO_OK;
-        seq::norm_columns<<<blocks, 1024, 0, s>>>(nullptr, 0, p->width, p->dgain);
+        seq::norm_columns<float><<<blocks, 1024, 0, s>>>(nullptr, 0, p->width, p->dgain);
         return seq::launch_status();
     }
     if (!p->dy || !p->h || !p->d) return CO_ERR_NULLARG;
@@ -523,6 +536,9 @@ extern "C" int seq_norm_grad(const SeqNormGrad *p, void *stream) {
     }
     rc = seq::launch_status();
     if (rc != CO_OK || !p->dgain) return rc;
-    seq::norm_columns<<<blocks, 1024, 0, s>>>(ws, rows, p->width, p->dgain);
+    if (rows <= seq::kGradBlocks)
+        seq::norm_columns<float><<<blocks, 1024, 0, s>>>(ws, rows, p->width, p->dgain);
+    else
+        seq::norm_columns<double><<<blocks, 1024, 0, s>>>(ws, rows, p->width, p->dgain);
     return seq::launch_status();
 }

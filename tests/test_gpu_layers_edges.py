@@ -122,3 +122,15 @@ def test_embedding_grad_of_one_sign(ops, T, V, D):
     got = ops.embedding_grad(d.expand(T, D), tokens, V)
     want = torch.bincount(tokens.long(), minlength=V).double()[:, None] * d.double()
     check("dtable", got, want.cpu(), want.cpu() * DEPTH * E32)
+
+
+@pytest.mark.parametrize("T,D", [(3000000, 8200), (1000000, 16392), (12000000, 1032)])
+def test_norm_gain_grad_of_one_sign(ops, T, D):
+    """The same of the gain's gradient, whose groups add 2,048 rows at most."""
+    _say("one sign", T, D)
+    h, dy, gain = one_row(D, BF, 1), one_row(D, F32, 2), torch.ones(D, device=DEV)
+    got = ops.rms_norm_grad(dy.expand(T, D), h.expand(T, D), gain)[2]
+    n = h.double() * (h.double().square().mean(1, keepdim=True) + 1e-6) ** -0.5
+    want = (T * dy.double() * n)[0].cpu()
+    # the norm of a row: half the relative error of its sum of squares, and some products
+    check("dgain", got, want, want * (2048 + 64 + 0.5 * (D / 64 + 16) + 8) * E32)
