@@ -8,7 +8,7 @@ import torch
 import layer_reference as ref
 from seq_reference import E32
 from test_gpu_layers import ids, layouts
-from test_gpu_seq import BF, DEV, F32, _say, check
+from test_gpu_seq import BF, DEV, F32, FP, _say, check
 
 pytestmark = pytest.mark.gpu
 
@@ -95,6 +95,53 @@ def test_int8_product_of_scales_far_apart(ops, M, K, N, out):
     assert bool(got[:, 1::2].isinf().all()) and not bool(got[:, ::2].any())
     got = ops.int8_product(a, sa * float("inf"), w, sw, dtype=out)
     assert bool(got[:, 1::2].isinf().all()) and bool(got[:, ::2].isnan().all())
+
+
+# ----------------------------------------------------------- sums that are exact
+
+EXACT = [
+    # tokens, rows, width, type
+    (300, 22, 128, F32), (2049, 511, 64, BF), (66000, 22, 40, BF), (70001, 9, 8, F32),
+    (600000, 1000, 1, F32), (530000, 2, 16, BF), (40000, 128, 130, BF), (33000, 32, 257, FP),
+    (33000, 33, 257, FP), (33000, 5000, 264, F32), (32768, 513, 9, BF), (80000, 200, 136, BF),
+    (256, 1, 2056, BF), (257, 700, 40, FP), (20000, 31, 2056, BF), (700, 40, 2056, BF),
+    (100000, 3, 1160, FP),
+]
+
+
+@pytest.mark.parametrize("T,V,D,dt", EXACT)
+def test_embedding_grad_of_whole_numbers(ops, T, V, D, dt):
+    """Sums of small whole numbers are exact in float32 in any order: every token counts,
+    once."""
+    _say("whole", T, V, D, dt)
+    g = torch.Generator().manual_seed(T)
+    d = torch.randint(1, 4, (T, D), generator=g).to(dt).to(DEV)
+    tokens = ids(T, V + 2, 4) - 1                    # a few outside the table
+    tokens[T // 3:T // 2] = V // 2
+    inside = (tokens >= 0) & (tokens < V)
+    want = torch.zeros(V, D, dtype=torch.float64, device=DEV)
+    want.index_add_(0, tokens[inside], d[inside].double())
+    for x in layouts(d):
+        got = ops.embedding_grad(x, tokens, V, scale=0.5)
+        assert torch.equal(got.double(), want * 0.5)
+
+
+@pytest.mark.parametrize("T,D,dt", [(1, 8, F32), (301, 1, BF), (20001, 96, BF), (40003, 128, F32),
+                                    (30001, 250, FP), (9001, 512, BF), (5003, 1024, F32),
+                                    (20001, 2048, BF), (4099, 4096, FP), (2051, 8192, BF),
+                                    (1501, 16384, F32), (700, 16400, BF)])
+def test_norm_gain_grad_of_whole_numbers(ops, T, D, dt):
+    """Rows of ones of either sign are their own norm, and the gain's gradient a sum of whole
+    numbers: every row counts, once."""
+    _say("whole", T, D, dt)
+    g = torch.Generator().manual_seed(T)
+    h = (torch.randint(0, 2, (T, D), generator=g) * 2 - 1).to(dt).to(DEV)
+    dy = torch.randint(-3, 6, (T, D), generator=g).to(dt).to(DEV)
+    gain = torch.ones(D, device=DEV)
+    want = (dy.double() * h.double()).sum(0)
+    for x, y in zip(layouts(h), layouts(dy)):
+        got = ops.rms_norm_grad(y, x, gain, eps=0.0)[2]
+        assert torch.equal(got.double(), want)
 
 
 # --------------------------------------------------- long sums of one sign
