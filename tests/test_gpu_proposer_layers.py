@@ -85,6 +85,44 @@ def test_training_with_an_entropy_term():
         pr.Trainer(None, entropy_coef=float("nan"))
 
 
+def test_gradient_of_the_entropy_term():
+    """What the term adds to the parameters' gradients is its own gradient, formed by torch from
+    the same logits, with the sign that raises the entropy."""
+    coef = 4.0
+
+    def fresh():
+        p = pr.Proposer(2, longest=15, seed=1, fused=True)
+        return p, p.sample(128, generator=torch.Generator(device="cuda").manual_seed(3))
+
+    def gradients(p):
+        return {n: v.grad.double() for n, v in p.parameters.items()}
+
+    def entropy_of(p, pop):
+        lp = p.logits(pop).log_softmax(1)
+        h = -(lp.exp() * lp.masked_fill(~pop.allowed, 0.0)).sum(1)
+        weights = (1.0 / pop.lengths.float() / len(pop.lengths))[pop.sequence]
+        return (weights * h).sum()
+
+    grads, after = [], []
+    for c in (0.0, coef):
+        p, pop = fresh()
+        rewards = torch.rand(128, generator=torch.Generator().manual_seed(2))
+        pr.Trainer(p, entropy_coef=c, epochs=1, rate=1e-3).step(pop, rewards)
+        grads.append(gradients(p))
+        with torch.no_grad():
+            after.append(float(entropy_of(p, pop)))
+    p, pop = fresh()
+    before = entropy_of(p, pop)
+    (-coef * before).backward()
+    for n, own in gradients(p).items():
+        a, b = grads[0][n], grads[1][n]
+        # three passes back, each with sixteen roundings of 2^-8
+        tol = 16 * 2.0 ** -8 * float(a.norm() + b.norm() + own.norm())
+        assert tol < 0.5 * float(own.norm()), n      # a gradient that is not there would show
+        assert float((b - a - own).norm()) <= tol, n
+    assert after[1] > before.item() and after[1] > after[0]
+
+
 def test_the_command_line(capsys):
     """One small round with everything by choice."""
     pr.main(["--rounds", "1", "--population", "64", "--fused", "--int8"])
