@@ -48,7 +48,7 @@ __device__ inline uint4v row_piece(const int8_t *row, int64_t l, int64_t inner) 
 // wave; two groups g change halves, and it has 8 channels side by side. 32 tokens' go
 // through LDS to leave as whole rows: stores of 32 bytes a row took 156 us for 8,192 x
 // 16,384 outputs of 128 terms. Those of large tiles pass the caches by, which hold operands
-// that are read again: 8,192 x 4,096 x 16,384 in 513 us rather than 565. WIDE: every 8
+// that are read again: 8,192 x 4,096 x 16,384 took 9 in 100 less time. WIDE: every 8
 // channels lie on a boundary of 16 bytes and are all inside or all outside. RAW: the sums as
 // they are, in a float's place. w_scale holds the N channels' scales and, a tile's side
 // behind, the `raised` ones for tokens with a large scale: a lane's address says which (a branch
@@ -137,8 +137,10 @@ __device__ inline bool tile_of(int64_t block, int64_t rows, int64_t columns, int
 // multiplied, and the next one's first with its second. Row r of a buffer holds its four
 // pieces of 16 bytes turned by r / 4, so that 16 lanes' reads meet every bank once. At 8,192
 // x 8,192 x 16,384 the products alone take 578 us (3.8 POP/s at the clock that the card
-// falls to), with the reads from LDS 718, with the copies into it 718, with both 941: LDS
-// bounds it.
+// falls to), with the reads from LDS 718, with the copies into it 718, with both 941. LDS has
+// time for both (some 770 clocks a step, the products 1,024): what is lost is their overlap, with
+// one wave a SIMD, a barrier a step and the matrix unit busy 58 in 100 of the time. 8,192 x 4,096
+// x 16,384 take 490 to 690 us by the clock that the card is at, 530 to 570 from a cool start.
 constexpr int kStep = 64, kStages = 5, kMostCuts = 32;
 template <int T> constexpr int tile_bytes() { return 2 * T * kStep; }
 

@@ -5,7 +5,8 @@
 // With m the largest logit, t = x - m and e = exp(t / temperature), a row needs
 // S = sum e and U = sum t e: logp = t_id / temperature - log S, and the entropy is
 // log S - U / (S temperature), a sum of two terms of one sign. The bound is memory: a
-// forward pass reads a row once, the gradient reads and writes it once.
+// forward pass reads a row once, or twice where its largest value has nearly all the weight
+// and a block has the row (logprob_rows), the gradient reads and writes it once.
 #include "seq_rows.h"
 
 namespace seq {
@@ -103,8 +104,8 @@ template <int WAVES> __device__ inline Sums over_block(Sums a, const Warmth &w, 
     return r;
 }
 
-// Below this much beside the largest value, 1 + the rest has lost too much of the rest:
-// the rest is summed again without it.
+// Below this much beside the largest value (a weight above 98.5 %), 1 + the rest has lost too
+// much of the rest: the rest is summed again without it, from a second reading of the row.
 constexpr float kPeak = 0x1p-6f;
 
 struct Row { float m, rest, log_sum, entropy; }; // S = 1 + rest
@@ -166,8 +167,10 @@ __device__ inline void put_top(const SeqLogprobs &p, const Warmth &w, int64_t t,
 // the place of its largest value; the largest of all is taken out `top` times, and the
 // wave that owned it looks through that thread's values for the next below it. Memory bounds
 // it, with the exponentials close behind: 8,192 rows of 131,071 in bf16 (2.15 GB) take 363
-// us, 5.9 TB/s, the vector instructions some 90 in 100 of that time. Few rows wait for the
-// rounds of alternatives: 64 of 32,001 in fp32 with five take 12 us.
+// us, 5.9 TB/s, the vector instructions some 90 in 100 of that time, and 710 us at least where
+// the largest value has nearly all the weight of each row; 2,048 of 32,001 in fp32 43 and 77.
+// Few rows wait for a row's way to four waves, eight trips one after the other (64 of 32,001 in
+// fp32 8.3 us), and for a round an alternative: 9.1 with one, 12.1 with five, 22 with twenty.
 template <typename T, int THREADS, bool TOP>
 __global__ __launch_bounds__(THREADS) void logprob_rows(SeqLogprobs p, Warmth w) {
     constexpr int N = Sixteen<T>::n, WAVES = THREADS / 64;

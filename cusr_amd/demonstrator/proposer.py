@@ -187,7 +187,9 @@ class Proposer:
     @torch.no_grad()
     def sample(self, M, generator=None, int8=False):
         """M programs, one symbol a step for all of them. int8: with 8-bit products, whose
-        weights are made from the present parameters at the start."""
+        weights are made from the present parameters at the start. Programs come from
+        that model's probabilities then, while Trainer and alternatives() take those of
+        the bfloat16 one."""
         weights = self.int8_weights() if int8 else None
         dev, V, cap = self.device, self.symbols.size, self.longest
         shape = (self.layers, M, cap, self.kv_heads, self.d)
@@ -254,7 +256,10 @@ class Trainer:
     few, by how far they pass the last of them; 1 learns from all, by how far
     they pass the mean.
     entropy_coef: weight of the policy's mean entropy over the symbols that are learnt
-    from, which is added to what is reinforced."""
+    from, which is added to what is reinforced.
+    The ratio that is clipped is to the parameters' own log-probabilities before the step,
+    formed with bfloat16 products: for programs that 8-bit products sampled it starts at 1
+    too, and what the two models differ by is not made up for."""
 
     def __init__(self, proposer, *, rate=3e-3, clip=0.2, kl_coef=0.01, epochs=4, top=1.0,
                  entropy_coef=0.0):
